@@ -319,6 +319,95 @@ int rh_rec_preprocess_device(rh_ctx *ctx, int slot, const uint8_t *d_rgb, int64_
                              uint32_t max_w, float *d_out, int64_t out_len, uint32_t *out_widths, uint32_t *out_wmax,
                              void *stream);
 
+/* ------------------------------------------------------------------- training losses
+ *
+ * Softmax cross entropy over the vocabulary, and distillation from a teacher's top logits, of the
+ * head's projection z = a w^T + bias, computed in pieces of the vocabulary: the [rows][n] logits
+ * are never in memory. No counterpart in the reference, which only infers: they serve a program
+ * that fine-tunes or distils the head it then packs, and one that rates transcripts under it.
+ *
+ * Cross entropy: loss[r] = lse[r] - z[r][target[r]], lse[r] = log sum_j exp z[r][j]. A row whose
+ * target is negative is ignored: loss 0, lse 0, no gradient; its features are not used (they may
+ * hold anything, NaN included).
+ *
+ * Distillation: row r holds the teacher's entries (top_idx[r][i], top_logits[r][i]), i < n_top
+ * <= 64, in any order; an entry with a negative class is absent, a class named twice counts
+ * twice. With T = temperature, q = softmax(top_logits / T) over the row's entries and
+ * p = softmax(z / T) over every class,
+ *     loss[r] = T^2 sum_i q_i (log q_i - log p[top_idx[r][i]]),  lse[r] = log sum_j exp(z[r][j] / T).
+ * A row with no entry is ignored, as above.
+ *
+ * Features are [rows][k] (t_len = 0) or the SVTR tail's [rows / t_len][k][t_len] (t_len > 0), as
+ * in rh_head_decode and rh_head_decode_kt; rows are in (line, timestep) order. A bias of -inf
+ * masks its class; a row with every class masked has lse -inf and loss NaN.
+ *
+ * A class at or above n: host calls refuse it (RH_ERR_INVALID_ARG). On the device the row
+ * (cross entropy) or the entry (distillation) is taken as absent and the next rh_sync reports
+ * RH_ERR_INVALID_ARG.
+ *
+ * Device forms take a workspace of device memory (any alignment) of at least the bytes that
+ * rh_head_score_workspace_bytes / rh_head_grad_workspace_bytes name; it holds nothing between
+ * calls, and calls whose work may overlap need one each. They allocate nothing and can be captured
+ * into a CUDA graph. They leave the caller's current device as it was. Results do not depend on
+ * what else runs: sums are taken in a fixed order, without atomics.
+ */
+#define RH_DTYPE_F32 0
+#define RH_DTYPE_BF16 1
+
+/* Scores under a packed head (int8, compact int8 or FP32 weights; f32 features): loss [rows] and
+ * lse [rows], either may be NULL. Host memory, on the context's first device; k must equal the
+ * weight's K. */
+int rh_head_cross_entropy(rh_ctx *ctx, const rh_weight *w, const float *a, int64_t rows, int64_t k, int64_t t_len,
+                          const int32_t *target, float *loss, float *lse);
+int rh_head_distill(rh_ctx *ctx, const rh_weight *w, const float *a, int64_t rows, int64_t k, int64_t t_len,
+                    const int32_t *top_idx, const float *top_logits, int64_t n_top, float temperature, float *loss,
+                    float *lse);
+
+/* The same on device memory of `slot`'s device, enqueued on `stream`. Workspace bytes: -1 on bad
+ * arguments. */
+int64_t rh_head_score_workspace_bytes(rh_ctx *ctx, const rh_weight *w, int slot, int64_t rows);
+int rh_head_cross_entropy_device(rh_ctx *ctx, const rh_weight *w, int slot, const float *d_a, int64_t rows,
+                                 int64_t t_len, const int32_t *d_target, float *d_loss, float *d_lse,
+                                 void *d_workspace, int64_t workspace_bytes, void *stream);
+int rh_head_distill_device(rh_ctx *ctx, const rh_weight *w, int slot, const float *d_a, int64_t rows, int64_t t_len,
+                           const int32_t *d_top_idx, const float *d_top_logits, int64_t n_top, float temperature,
+                           float *d_loss, float *d_lse, void *d_workspace, int64_t workspace_bytes, void *stream);
+
+/* A training step: the losses and their gradients for a weight w [n][k] and bias [n] (NULL: none),
+ * k <= 128, n <= 262,144. row_grad [rows] is d total / d loss[r] (NULL: 1 each; 1 / count for a
+ * mean). With f[r] = row_grad[r] (times T for distillation) and the row's distribution q over its
+ * labels, dz = f (p - q), and
+ *     da = dz w (laid out as a),  dw = dz^T a [n][k],  dbias[j] = sum_r dz[r][j].
+ * loss, lse, da, dw and dbias may each be NULL (dbias needs dw); what is not asked for is not
+ * computed (da NULL: a frozen backbone; dw NULL: a frozen head). rows == 0 clears dw and dbias.
+ * Host form: f32, on the context's first device. */
+int rh_head_cross_entropy_grad(rh_ctx *ctx, const float *a, int64_t rows, int64_t k, int64_t t_len, const float *w,
+                               int64_t n, const float *bias, const int32_t *target, const float *row_grad, float *loss,
+                               float *lse, float *da, float *dw, float *dbias);
+int rh_head_distill_grad(rh_ctx *ctx, const float *a, int64_t rows, int64_t k, int64_t t_len, const float *w, int64_t n,
+                         const float *bias, const int32_t *top_idx, const float *top_logits, int64_t n_top,
+                         float temperature, const float *row_grad, float *loss, float *lse, float *da, float *dw,
+                         float *dbias);
+
+/* The same on device memory of `slot`'s device, enqueued on `stream`. dtype (RH_DTYPE_F32 or
+ * RH_DTYPE_BF16) is that of a, w, da and dw; bias, dbias, row_grad, loss and lse are f32.
+ * bf16: products of bf16 operands in f32, with the probabilities rounded to bf16 for the second
+ * product. f32: operands split into two fp16 parts (~22 bits below the largest of 128 rows), so
+ * results are as those of f32 arithmetic. n_top: entries per row (0 or 1 for cross entropy);
+ * workspace bytes: -1 on bad arguments. */
+int64_t rh_head_grad_workspace_bytes(rh_ctx *ctx, int slot, int dtype, int64_t rows, int64_t k, int64_t n,
+                                     int64_t n_top);
+int rh_head_cross_entropy_grad_device(rh_ctx *ctx, int slot, int dtype, const void *d_a, int64_t rows, int64_t k,
+                                      int64_t t_len, const void *d_w, int64_t n, const float *d_bias,
+                                      const int32_t *d_target, const float *d_row_grad, float *d_loss, float *d_lse,
+                                      void *d_da, void *d_dw, float *d_dbias, void *d_workspace,
+                                      int64_t workspace_bytes, void *stream);
+int rh_head_distill_grad_device(rh_ctx *ctx, int slot, int dtype, const void *d_a, int64_t rows, int64_t k,
+                                int64_t t_len, const void *d_w, int64_t n, const float *d_bias,
+                                const int32_t *d_top_idx, const float *d_top_logits, int64_t n_top, float temperature,
+                                const float *d_row_grad, float *d_loss, float *d_lse, void *d_da, void *d_dw,
+                                float *d_dbias, void *d_workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

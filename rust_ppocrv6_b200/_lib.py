@@ -23,7 +23,7 @@ RH_ERR_DEVICE_FAULT = 6
 
 _c_int, _c_i64, _vp = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p
 _i64p = ctypes.POINTER(ctypes.c_int64)
-_u32 = ctypes.c_uint32
+_u32, _f32 = ctypes.c_uint32, ctypes.c_float
 
 # name -> (restype, argtypes)
 SIGNATURES = {
@@ -59,6 +59,20 @@ SIGNATURES = {
     "rh_ctc_collapse_device": (_c_int, [_vp, _c_int, _vp, _vp, _vp, _c_i64, _vp, _vp, _vp, _vp]),
     "rh_head_decode_ctc": (_c_int, [_vp, _vp, _vp, _vp, _c_i64, _c_i64, _vp, _vp, _vp]),
     "rh_head_decode_kt_ctc": (_c_int, [_vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _vp, _vp, _vp, _vp]),
+    "rh_head_cross_entropy": (_c_int, [_vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _vp, _vp, _vp]),
+    "rh_head_distill": (_c_int, [_vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _vp, _vp, _c_i64, _f32, _vp, _vp]),
+    "rh_head_score_workspace_bytes": (_c_i64, [_vp, _vp, _c_int, _c_i64]),
+    "rh_head_cross_entropy_device": (_c_int, [_vp, _vp, _c_int, _vp, _c_i64, _c_i64, _vp, _vp, _vp, _vp, _c_i64, _vp]),
+    "rh_head_distill_device": (_c_int, [_vp, _vp, _c_int, _vp, _c_i64, _c_i64, _vp, _vp, _c_i64, _f32, _vp, _vp, _vp,
+                                        _c_i64, _vp]),
+    "rh_head_cross_entropy_grad": (_c_int, [_vp, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64] + [_vp] * 8),
+    "rh_head_distill_grad": (_c_int, [_vp, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _vp, _vp, _vp, _c_i64, _f32]
+                             + [_vp] * 6),
+    "rh_head_grad_workspace_bytes": (_c_i64, [_vp, _c_int, _c_int, _c_i64, _c_i64, _c_i64, _c_i64]),
+    "rh_head_cross_entropy_grad_device": (_c_int, [_vp, _c_int, _c_int, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64]
+                                          + [_vp] * 9 + [_c_i64, _vp]),
+    "rh_head_distill_grad_device": (_c_int, [_vp, _c_int, _c_int, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _vp, _vp,
+                                             _vp, _c_i64, _f32] + [_vp] * 7 + [_c_i64, _vp]),
     "rh_rec_resized_width": (_u32, [_u32, _u32, _u32, _u32]),
     "rh_rec_batch_shape": (_c_int, [_vp, _vp, _c_i64, _u32, _u32, _vp, _vp, _vp]),
     "rh_rec_preprocess": (_c_int, [_vp, _vp, _c_i64, _vp, _vp, _vp, _c_i64, _u32, _u32, _vp, _c_i64, _vp, _vp]),

@@ -1,0 +1,1346 @@
+// sm_100a kernels of the recognition head's training losses: softmax cross entropy over the CTC
+// vocabulary and distillation from a teacher's top logits, without the [rows][classes] logits in
+// memory. Both hold the row's softmax p = softmax(z / T), z = x W^T + b, against a sparse
+// distribution q (one class, or the teacher's entries), so they share every kernel:
+//
+//   loss_r = T^2 sum_i q_i (log q_i - log p[c_i]),   dz_r = T g_r (p - q),
+//   dx = dz W,  dW = dz^T x,  db = sum_r dz_r        (cross entropy: q = 1 at the target, T = 1)
+//
+//  loss_pack_kernel    operand tiles of 128 rows as tensor-core images, labels sorted by class tile
+//  loss_main_kernel    the dense work, in one of two directions that mirror each other:
+//                        row pass    own = 128 rows of x, streamed = W tiles: running (max, sum) of
+//                                    the softmax and the mean weight row sum_j p_j W_j
+//                        weight pass own = 128 classes, streamed = x tiles: dz^T x with p from the
+//                                    rows' lse
+//  loss_rows_kernel    joins a row's class ranges: loss, lse, dx = T g (sum_j p_j W_j - sum_i q_i W_ci)
+//  loss_reduce_kernel  joins a class's row ranges: dW, db
+//  loss_score_kernel   loss and lse of a packed head from the decode kernel's (argmax, probability)
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <math_constants.h>
+
+#include "head_params.h"
+#include "loss_params.h"
+#include "loss_ptx.cuh"
+
+namespace rh {
+
+namespace {
+
+constexpr float kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+template <bool F32>
+struct Elem {
+    using type = float;
+};
+template <>
+struct Elem<false> {
+    using type = __nv_bfloat16;
+};
+
+// Byte offset of 16-byte chunk `ch` (8 K slots) of row r in a 128 x 128 16-bit tile image: two
+// halves of 64 K slots, rows of 128 bytes, chunks XOR-swizzled by the row (the tensor core's
+// 128-byte swizzle).
+__device__ __forceinline__ uint32_t image_chunk(int r, int ch) {
+    return (uint32_t)(ch >> 3) * 16384u + (uint32_t)r * 128u + (uint32_t)(((ch & 7) ^ (r & 7)) << 4);
+}
+
+// Where element (row, kk) of the features lies: rows of k, or the SVTR tail's [b][k][t_len].
+__device__ __forceinline__ long long x_base(long long row, int k, long long t_len) {
+    return t_len > 0 ? (row / t_len) * (long long)k * t_len + row % t_len : row * (long long)k;
+}
+
+// Exponent of the power of two that brings `top` (> 0, finite) into [2^target, 2^(target + 1)).
+__device__ __forceinline__ int shift_to(float top, int target) {
+    if (!(top > 0.0f) || top > 3.4028235e38f) return 0;
+    const int e = (int)((__float_as_uint(top) >> 23) & 0xFFu) - 127;
+    return min(max(target - e, -126), 126);
+}
+__device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// A row's distribution q over its labels, in one warp: lane l holds entries l and l + 32 (class c
+// or -1, q, log q). False when the row has no label (it is then ignored).
+struct RowLabels {
+    int c[2];
+    float q[2], log_q[2];
+};
+__device__ __forceinline__ bool row_labels(const LossLabels& L, long long row, int lane, RowLabels& r) {
+    r.c[0] = r.c[1] = -1;
+    r.q[0] = r.q[1] = 0.0f;
+    r.log_q[0] = r.log_q[1] = 0.0f;
+    if (L.target) {
+        const int t = L.target[row];
+        if (lane == 0 && t >= 0 && t < L.n) {
+            r.c[0] = t;
+            r.q[0] = 1.0f;
+        }
+        return t >= 0 && t < L.n;
+    }
+    float u[2], top = -CUDART_INF_F;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        const int e = lane + 32 * s;
+        u[s] = -CUDART_INF_F;
+        if (e < L.n_top) {
+            const int c = L.top_idx[row * L.n_top + e];
+            if (c >= 0 && c < L.n) {
+                r.c[s] = c;
+                u[s] = L.top_logits[row * L.n_top + e] * L.inv_temp;
+            }
+        }
+        top = fmaxf(top, u[s]);
+    }
+    if (!__any_sync(0xffffffffu, r.c[0] >= 0 || r.c[1] >= 0)) return false;
+    top = warp_max(top);
+    float sum = 0.0f;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        u[s] -= top;
+        r.q[s] = r.c[s] >= 0 ? expf(u[s]) : 0.0f;
+        sum += r.q[s];
+    }
+    sum = warp_sum(sum);
+    const float log_sum = logf(sum);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        r.q[s] = r.c[s] >= 0 ? r.q[s] / sum : 0.0f;
+        r.log_q[s] = u[s] - log_sum;
+    }
+    return true;
+}
+
+}  // namespace
+
+// ------------------------------------------------------------------------------------ pack
+// One block per tile: w_tiles weight tiles, then x_tiles feature tiles. f32 values are scaled by
+// the tile's power of two into [2^14, 2^15) and split into fp16 hi + lo (~22 bits below the
+// tile's maximum, which an image of fp16 alone or of bf16 parts would not hold); bf16 values are
+// copied. A row that is ignored is zero in the image, so whatever its features hold (NaN
+// included) reaches nothing. The labels of a feature tile are sorted by class tile, rows
+// ascending within each: every warp counts its 16 rows' entries per class tile, a scan turns the
+// counts into positions, and a second walk places them (no atomics: the order is fixed).
+template <bool F32>
+__global__ void __launch_bounds__(256) loss_pack_kernel(const __grid_constant__ LossPackParams p) {
+    using T = typename Elem<F32>::type;
+    extern __shared__ int bins[];  // [8 warps][w_tiles] counts, then [w_tiles] starts
+    __shared__ float red[8];
+    __shared__ float s_g[128];
+    __shared__ uint8_t s_valid[128];
+    __shared__ int s_scan[8];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const bool is_w = (int)blockIdx.x < p.w_tiles;
+    const int tile = is_w ? (int)blockIdx.x : (int)blockIdx.x - p.w_tiles;
+    const long long row0 = (long long)tile * kLossTile;
+    const long long n_rows = is_w ? p.lab.n : p.rows;
+
+    float gs = 1.0f;  // scale of this tile's gradient factors
+    if (!is_w) {
+        float f = 0.0f;
+        if (tid < 128) {
+            const long long row = row0 + tid;
+            bool valid = false, bad = false;
+            if (row < p.rows) {
+                const int* c = p.lab.target ? p.lab.target + row : p.lab.top_idx + row * p.lab.n_top;
+                for (int e = 0; e < p.lab.n_top; ++e) {
+                    valid |= c[e] >= 0 && c[e] < p.lab.n;
+                    bad |= c[e] >= p.lab.n;
+                }
+            }
+            if (bad) atomicOr(p.status, kDevBadClass);
+            s_valid[tid] = valid ? 1 : 0;
+            if (valid) f = p.lab.temp * (p.row_grad ? p.row_grad[row] : 1.0f);
+        }
+        if (F32) {
+            const float m = warp_max(fabsf(f));
+            if (lane == 0) red[warp] = m;
+            __syncthreads();
+            float top = red[0];
+#pragma unroll
+            for (int i = 1; i < 4; ++i) top = fmaxf(top, red[i]);
+            const int sh = shift_to(top, 13);
+            gs = pow2i(sh);
+            if (tid == 0) p.g_scale[tile] = pow2i(-sh);
+        }
+        if (tid < 128) {
+            s_g[tid] = f * gs;
+            p.row_tab[(size_t)tile * 256 + 128 + tid] = f * gs;
+        }
+        __syncthreads();
+    } else if (tid < 128) {
+        const long long j = row0 + tid;
+        p.class_e[(size_t)tile * 128 + tid] =
+            j < p.lab.n ? (p.bias ? p.bias[j] * p.logit_scale : 0.0f) : -CUDART_INF_F;
+    }
+
+    // 2,048 chunks of 8 K slots, 8 per thread: row-major operands with neighbouring threads on
+    // neighbouring chunks, the [b][k][t] layout with neighbouring threads on neighbouring rows.
+    const long long t_len = is_w ? 0 : p.t_len;
+    const T* src = static_cast<const T*>(is_w ? p.w : p.x);
+    const bool vec = t_len == 0 && (reinterpret_cast<uintptr_t>(src) & 15u) == 0 && p.k % (F32 ? 4 : 8) == 0;
+    float v[8][8];
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int item = i * 256 + tid;
+        const int r = t_len > 0 ? item & 127 : item >> 4, ch = t_len > 0 ? item >> 7 : item & 15;
+        const long long row = row0 + r;
+        const bool ok = row < n_rows && (is_w || s_valid[r]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+        if (ok && 8 * ch < p.k) {
+            const T* a = src + x_base(row, p.k, t_len) + (t_len > 0 ? 8 * ch * t_len : 8 * ch);
+            if (vec && 8 * ch + 8 <= p.k) {
+                if constexpr (F32) {
+                    const float4 lo = *reinterpret_cast<const float4*>(a), hi = *reinterpret_cast<const float4*>(a + 4);
+                    v[i][0] = lo.x, v[i][1] = lo.y, v[i][2] = lo.z, v[i][3] = lo.w;
+                    v[i][4] = hi.x, v[i][5] = hi.y, v[i][6] = hi.z, v[i][7] = hi.w;
+                } else {
+                    const uint4 u = *reinterpret_cast<const uint4*>(a);
+                    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        v[i][2 * j] = __uint_as_float(w[j] << 16);
+                        v[i][2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+                    }
+                }
+            } else {
+                const long long step = t_len > 0 ? t_len : 1;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (8 * ch + j < p.k) v[i][j] = to_f32(a[j * step]);
+            }
+        }
+        if (F32) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[i][j]));
+        }
+    }
+    float up = 1.0f;
+    if (F32) {
+        top = warp_max(top);
+        __syncthreads();  // red is read above
+        if (lane == 0) red[warp] = top;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, red[i]);
+        const int sh = shift_to(top, 14);
+        up = pow2i(sh);
+        if (tid == 0) (is_w ? p.w_scale : p.x_scale)[tile] = pow2i(-sh);
+    }
+    uint8_t* img = (is_w ? p.w_img : p.x_img) + (size_t)tile * (F32 ? 2 * kLossImage : kLossImage);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int item = i * 256 + tid;
+        const int r = t_len > 0 ? item & 127 : item >> 4, ch = t_len > 0 ? item >> 7 : item & 15;
+        const uint32_t off = image_chunk(r, ch);
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (F32) {
+                const float a = v[i][2 * j] * up, b = v[i][2 * j + 1] * up;
+                const __half2 hv = __floats2half2_rn(a, b);
+                const float2 hf = __half22float2(hv);
+                const __half2 lv = __floats2half2_rn(a - hf.x, b - hf.y);
+                h[j] = *reinterpret_cast<const uint32_t*>(&hv);
+                l[j] = *reinterpret_cast<const uint32_t*>(&lv);
+            } else {
+                const __nv_bfloat162 hv = __floats2bfloat162_rn(v[i][2 * j], v[i][2 * j + 1]);
+                h[j] = *reinterpret_cast<const uint32_t*>(&hv);
+            }
+        }
+        *reinterpret_cast<uint4*>(img + off) = make_uint4(h[0], h[1], h[2], h[3]);
+        if constexpr (F32) *reinterpret_cast<uint4*>(img + kLossImage + off) = make_uint4(l[0], l[1], l[2], l[3]);
+    }
+    if (is_w || !p.sort_labels) return;
+
+    // ------------------------------------------------------------ labels by class tile
+    const int nb = p.w_tiles;
+    int* start = bins + 8 * nb;
+    for (int i = tid; i < 8 * nb; i += 256) bins[i] = 0;
+    __syncthreads();
+    int* mine = bins + warp * nb;
+    int2* ent = p.sp_ent + (size_t)tile * 128 * p.lab.n_top;
+    for (int pass = 0; pass < 2; ++pass) {
+        for (int rr = 0; rr < 16; ++rr) {
+            const int r = warp * 16 + rr;
+            if (!s_valid[r]) continue;
+            RowLabels lab;
+            row_labels(p.lab, row0 + r, lane, lab);
+            if (p.lab.n_top > 1) {  // a class named twice: one entry with both shares
+                float q[2] = {lab.q[0], lab.q[1]};
+                bool dup[2] = {false, false};
+                for (int j = 0; j < p.lab.n_top; ++j) {
+                    const int cj = __shfl_sync(0xffffffffu, j < 32 ? lab.c[0] : lab.c[1], j & 31);
+                    const float qj = __shfl_sync(0xffffffffu, j < 32 ? lab.q[0] : lab.q[1], j & 31);
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        const int e = lane + 32 * s;
+                        if (cj >= 0 && cj == lab.c[s] && j != e) {
+                            if (j < e)
+                                dup[s] = true;
+                            else
+                                q[s] += qj;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    lab.q[s] = q[s];
+                    if (dup[s]) lab.c[s] = -1;
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                if (32 * s >= p.lab.n_top) break;
+                const int bin = lab.c[s] >= 0 ? lab.c[s] >> 7 : -1;
+                const uint32_t same = __match_any_sync(0xffffffffu, bin);
+                const int rank = __popc(same & ((1u << lane) - 1u));
+                if (bin >= 0) {
+                    const int at = mine[bin];
+                    if (pass == 1)
+                        ent[start[bin] + at + rank] =
+                            make_int2((r << 7) | (lab.c[s] & 127), __float_as_int(-lab.q[s] * s_g[r]));
+                    __syncwarp(same);
+                    if (rank == 0) mine[bin] = at + __popc(same);
+                }
+                __syncwarp();
+            }
+        }
+        if (pass == 1) break;
+        __syncthreads();
+        // counts -> each warp's first position within its bin, and the bins' starts
+        const int per = (nb + 255) / 256, b0 = tid * per, b1 = min(nb, b0 + per);
+        int sum = 0;
+        for (int b = b0; b < b1; ++b) {
+            int tot = 0;
+            for (int w = 0; w < 8; ++w) {
+                const int c = bins[w * nb + b];
+                bins[w * nb + b] = tot;
+                tot += c;
+            }
+            start[b] = sum;
+            sum += tot;
+        }
+        int incl = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        if (lane == 31) s_scan[warp] = incl;
+        __syncthreads();
+        int base = incl - sum;
+        for (int w = 0; w < warp; ++w) base += s_scan[w];
+        int32_t* off = p.sp_off + (size_t)tile * (nb + 1);
+        for (int b = b0; b < b1; ++b) {
+            start[b] += base;
+            off[b] = start[b];
+        }
+        if (tid == 255) off[nb] = base + sum;
+        __syncthreads();
+    }
+}
+
+// ------------------------------------------------------------------------------- main pass
+namespace {
+
+// Warps: 0 producer, 1 tensor-core issuer (and TMEM), 2-3 idle, 4-7 and 8-11 two softmax
+// warpgroups that take the streamed tiles in turn (tile i of a unit: warpgroup i % 2, score
+// buffer i % 2).
+constexpr int kMainThreads = 384;
+constexpr int kCtrlRegs = 56, kSoftRegs = 224;  // 128 x 72 + 256 x 216 = 384 x 168: the launch's own registers
+static_assert(128 * kCtrlRegs + 256 * kSoftRegs <= kMainThreads * 168, "register split");
+
+template <bool F32>
+struct Ring {
+    static constexpr uint32_t kStage = F32 ? 2u * kLossImage : kLossImage;
+    static constexpr uint32_t kStages = F32 ? 3u : 6u;
+};
+constexpr uint32_t kMOffTab = 196608;             // per stage 1 KB: the tile's column table
+constexpr uint32_t kMOffBars = kMOffTab + 6 * 1024;
+constexpr uint32_t kMOffMisc = kMOffBars + 256;   // [0] TMEM base, [1] abort flag
+constexpr uint32_t kMOffMs = kMOffMisc + 64;      // [128] float2: warpgroup 1's row state
+constexpr uint32_t kPatchRow = 20;                // floats per class row of a label patch (16 used:
+                                                  // the 16-byte rows then fall on distinct banks)
+constexpr uint32_t kMOffPatch = kMOffMs + 1024;   // [8 warps][32][kPatchRow] f32
+constexpr uint32_t kMSmemUsed = kMOffPatch + 8 * 32 * kPatchRow * 4;
+constexpr uint32_t kMSmemBytes = kMSmemUsed + 1024;
+static_assert(Ring<true>::kStage * Ring<true>::kStages <= kMOffTab && Ring<false>::kStage * Ring<false>::kStages <= kMOffTab,
+              "stages fit");
+static_assert(kMSmemBytes <= 227 * 1024, "shared memory per CTA");
+
+constexpr int kLBarFull = 0;               // [6] tile and column table landed
+constexpr int kLBarEmpty = 6;              // [6] the tile's products done, its warpgroup done with the table
+constexpr int kLBarAFull = 12;             // own operand in TMEM
+constexpr int kLBarAEmpty = 13;            // the unit's products done with it
+constexpr int kLBarSFull = 14;             // [2] scores of a tile in TMEM
+constexpr int kLBarPFull = 16;             // [2] its probabilities in their place
+constexpr int kLBarOFull = 18;             // [2] (by warpgroup) the tile's second product in TMEM
+constexpr int kLBarOEmpty = 20;            // [2] added up, the buffer free
+constexpr int kLBarMerge = 22;             // warpgroup 1's state of a unit staged
+constexpr int kLBarDone = 23;              // every product retired (teardown)
+static_assert(kLBarDone < 32, "barrier area");
+
+// TMEM columns: own operand (hi | lo), score buffers, second product
+constexpr uint32_t kTOwn = 0, kTS = 128, kTO = 384;
+constexpr uint32_t kLSleepNs = 20000;
+
+struct Waiter {
+    volatile uint32_t* abort_flag;
+    int* status;
+    unsigned long long timeout_ns;
+};
+
+// Bounded wait: gives up when another role has, or after the time limit (device status set);
+// every role then leaves its loop and the kernel ends normally.
+__device__ __forceinline__ bool loss_wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, int* status,
+                                            unsigned long long timeout_ns, int where) {
+    const uint64_t t0 = globaltimer_ns();
+    while (true) {
+        if (mbar_try_wait_sleep(bar, parity, kLSleepNs)) return true;
+        if (*abort_flag) return false;
+        if (globaltimer_ns() - t0 > timeout_ns) {
+            *abort_flag = 1u;
+            atomicOr(status, kDevTimeout);
+            atomicExch(status + 1, where);
+            return false;
+        }
+    }
+}
+// Uniform over the (converged) warp.
+__device__ __forceinline__ bool loss_wait(uint32_t bar, uint32_t parity, const Waiter& w, int where) {
+    bool ok = mbar_try_wait(bar, parity);
+    if (__all_sync(0xffffffffu, ok)) return true;
+    if (!ok) ok = loss_wait_slow(bar, parity, w.abort_flag, w.status, w.timeout_ns, where);
+    return __all_sync(0xffffffffu, ok);
+}
+__device__ __forceinline__ void loss_drain(uint32_t bar, uint32_t parity, const Waiter& w) {
+    const uint64_t t0 = globaltimer_ns();
+    while (!mbar_try_wait_sleep(bar, parity, kLSleepNs)) {
+        if (globaltimer_ns() - t0 > w.timeout_ns) {
+            atomicOr(w.status, kDevTimeout);
+            return;
+        }
+    }
+}
+
+struct LUnit {
+    int own, c0, c1;
+};
+__device__ __forceinline__ bool lunit_exists(int u, const LossMainParams& p) {
+    return u < p.whole_units + (p.own_tiles - p.whole_units) * p.n_splits;
+}
+__device__ __forceinline__ LUnit lunit(int u, const LossMainParams& p) {
+    if (u < p.whole_units) return {u, 0, p.str_tiles};
+    const int v = u - p.whole_units, b = v / p.n_splits, s = v - b * p.n_splits;
+    const int c0 = s * p.tiles_per_split;
+    return {p.whole_units + b, c0, min(c0 + p.tiles_per_split, p.str_tiles)};
+}
+
+// 16 columns' values (8 pairs) as 16-bit tensor-core operands, over the 16 score columns they come
+// from: f32 as fp16 hi (8 columns) and lo (8 columns), whose sum holds ~22 bits and whose products
+// are exact in the f32 accumulator; bf16 by one rounding (half a step of the operand type, as the
+// features' own).
+template <bool F32>
+__device__ __forceinline__ void store_probs(uint32_t taddr, const float2 (&g)[8]) {
+    if constexpr (F32) {
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const __half2 h = __floats2half2_rn(g[i].x, g[i].y);
+            const float2 hf = __half22float2(h);
+            const float2 d = __fadd2_rn(g[i], make_float2(-hf.x, -hf.y));
+            const __half2 l = __floats2half2_rn(d.x, d.y);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            w[8 + i] = *reinterpret_cast<const uint32_t*>(&l);
+        }
+        tmem_st32x32b_x16(taddr, w);
+    } else {
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(g[i].x, g[i].y);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        tmem_st32x32b_x8(taddr, w);
+    }
+}
+
+// The tile's labels (weight pass), a window of 32 at a time: each lane holds one entry.
+struct LabelWindow {
+    int2 e;       // (row << 7 | class, factor); consumed or absent: row beyond the tile
+    int next, end;
+};
+constexpr int kNoLabel = 0x7fffffff;
+__device__ __forceinline__ void window_load(LabelWindow& w, const int2* ent, int lane) {
+    w.e = w.next + lane < w.end ? __ldg(ent + w.next + lane) : make_int2(kNoLabel, 0);
+    w.next += 32;
+}
+
+}  // namespace
+
+// Units (own tile, range of streamed tiles), persistent over the grid. Per streamed tile: scores
+// S = own . tile^T (tensor core, own operand in TMEM), the softmax warpgroup turns them into
+// probabilities (row pass: against the running maximum; weight pass: 2^(s - lse) times the rows'
+// gradient factors, less the labels' shares) in the same TMEM columns, and a second product
+// O = P . tile reads the same tile the other way round. O is added to registers tile by tile: the
+// tensor core's f32 accumulator rounds toward zero, which over thousands of steps would bias the
+// sums; over one tile's steps it stays below the operands' own error.
+// f32: three products each (hi.lo, lo.hi, hi.hi).
+template <bool F32, bool WPASS>
+__global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid_constant__ LossMainParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    uint8_t* gbase = smem_raw + (base - raw);
+    uint32_t* misc = reinterpret_cast<uint32_t*>(gbase + kMOffMisc);
+    constexpr uint32_t kStage = Ring<F32>::kStage, kStages = Ring<F32>::kStages;
+    constexpr uint32_t kTabBytes = WPASS ? 1024u : 512u;
+    auto bar = [&](int i) -> uint32_t { return base + kMOffBars + 8u * (uint32_t)i; };
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Waiter wt{misc + 1, p.status, p.timeout_ns};
+    const bool with_o = p.part_o != nullptr;
+
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < 6; ++s) {
+            mbar_init(bar(kLBarFull + s), 1);
+            mbar_init(bar(kLBarEmpty + s), 5);  // the product's commit, four warps
+        }
+        mbar_init(bar(kLBarAFull), 256);
+        mbar_init(bar(kLBarAEmpty), 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(bar(kLBarSFull + i), 1);
+            mbar_init(bar(kLBarPFull + i), 4);
+            mbar_init(bar(kLBarOFull + i), 1);
+            mbar_init(bar(kLBarOEmpty + i), 4);
+        }
+        mbar_init(bar(kLBarMerge), 128);
+        mbar_init(bar(kLBarDone), 1);
+        misc[1] = 0u;
+        fence_mbar_init();
+    }
+    for (uint32_t i = threadIdx.x; i < 8 * 32 * kPatchRow; i += kMainThreads)
+        reinterpret_cast<float*>(gbase + kMOffPatch)[i] = 0.0f;
+    if (warp == 1) {
+        tmem_alloc(base + kMOffMisc, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = misc[0];
+
+    if (warp < 4) {
+        setmaxnreg_dec<kCtrlRegs>();
+        if (warp == 0) {
+            // ------------------------------------------------------------ producer
+            uint32_t cc = 0, issued = 0;
+            bool ok = true;
+            for (int u = blockIdx.x; ok && lunit_exists(u, p); u += gridDim.x) {
+                const LUnit U = lunit(u, p);
+                for (int c = U.c0; c < U.c1; ++c, ++cc) {
+                    const uint32_t s = cc % kStages;
+                    ok = loss_wait(bar(kLBarEmpty + s), ((cc / kStages) & 1u) ^ 1u, wt, 101);
+                    if (!ok) break;
+                    if (elect_one()) {
+                        mbar_arrive_expect_tx(bar(kLBarFull + s), kStage + kTabBytes);
+                        bulk_copy_g2s(base + s * kStage, p.str + (size_t)c * kStage, kStage, bar(kLBarFull + s));
+                        bulk_copy_g2s(base + kMOffTab + s * 1024u, p.col_tab + (size_t)c * (kTabBytes / 4), kTabBytes,
+                                      bar(kLBarFull + s));
+                    }
+                    __syncwarp();
+                    issued = cc + 1;
+                }
+            }
+            for (uint32_t s = 0; s < kStages && s < issued; ++s)  // no copy outlives the CTA
+                loss_drain(bar(kLBarFull + s), ((issued - 1 - s) / kStages) & 1u, wt);
+        } else if (warp == 1) {
+            // ---------------------------------------------------------- tensor-core issuer
+            const uint32_t id_s = idesc_16b(!F32, false, 128, 128);
+            const uint32_t id_o = idesc_16b(!F32, true, 128, 16u * (uint32_t)p.ksteps);
+            const uint64_t k_desc = smem_desc_k_sw128(base), mn_desc = smem_desc_mn_sw128(base);
+            uint32_t cc = 0, uc = 0, pu[2] = {0, 0}, du[2] = {0, 0};
+            auto scores = [&](uint32_t i) -> bool {  // S of the unit's tile i
+                const uint32_t g = cc + i, s = g % kStages;
+                if (!loss_wait(bar(kLBarFull + s), (g / kStages) & 1u, wt, 102)) return false;
+                tc_fence_after();
+                const uint32_t d = tmem + kTS + 128u * (i & 1u);
+                const uint64_t b = k_desc + (uint64_t)(s * (kStage >> 4));
+                uint32_t acc = 0;
+                auto run = [&](uint32_t a_col, uint32_t b_off) {
+                    for (int st = 0; st < p.ksteps; ++st) {
+                        mma_f16_ts_warp(d, tmem + kTOwn + a_col + 8u * st,
+                                        b + ((b_off + (uint32_t)(st >> 2) * 16384u + (uint32_t)(st & 3) * 32u) >> 4),
+                                        id_s, acc);
+                        acc = 1;
+                    }
+                };
+                if (F32) {
+                    run(64, 0);
+                    run(0, kLossImage);
+                }
+                run(0, 0);
+                mma_commit_warp(bar(kLBarSFull + (int)(i & 1u)));
+                return true;
+            };
+            bool ok = true;
+            for (int u = blockIdx.x; ok && lunit_exists(u, p); u += gridDim.x, ++uc) {
+                const LUnit U = lunit(u, p);
+                const uint32_t n = (uint32_t)(U.c1 - U.c0);
+                ok = loss_wait(bar(kLBarAFull), uc & 1u, wt, 103);
+                if (!ok) break;
+                tc_fence_after();
+                ok = scores(0) && (n < 2 || scores(1));
+                for (uint32_t i = 0; ok && i < n; ++i) {
+                    const uint32_t w = i & 1u, s = (cc + i) % kStages;
+                    ok = loss_wait(bar(kLBarPFull + (int)w), pu[w]++ & 1u, wt, 104);
+                    if (!ok) break;
+                    if (with_o) {
+                        if (i > 0) {  // the other warpgroup has added the previous tile's product up
+                            ok = loss_wait(bar(kLBarOEmpty + (int)(w ^ 1u)), (du[w ^ 1u] - 1u) & 1u, wt, 105);
+                            if (!ok) break;
+                        }
+                        tc_fence_after();
+                        const uint64_t b = mn_desc + (uint64_t)(s * (kStage >> 4));
+                        const uint32_t a = tmem + kTS + 128u * w;
+                        uint32_t acc = 0;
+                        auto run = [&](uint32_t a_col, uint32_t b_off) {
+#pragma unroll
+                            for (uint32_t j = 0; j < 8; ++j) {  // 16 rows of the tile a step
+                                mma_f16_ts_warp(tmem + kTO, a + a_col + 16u * j,
+                                                b + ((b_off + 2048u * j) >> 4), id_o, acc);
+                                acc = 1;
+                            }
+                        };
+                        if (F32) {
+                            run(8, 0);
+                            run(0, kLossImage);
+                        }
+                        run(0, 0);
+                        mma_commit_warp(bar(kLBarOFull + (int)w));
+                        ++du[w];
+                    }
+                    mma_commit_warp(bar(kLBarEmpty + (int)s));
+                    // Tile i + 2 takes the score buffer of tile i, whose probabilities the product
+                    // above reads: the tensor core runs one thread's products in order.
+                    if (i + 2 < n) ok = scores(i + 2);
+                }
+                if (!ok) break;
+                cc += n;
+                mma_commit_warp(bar(kLBarAEmpty));
+            }
+            mma_commit_warp(bar(kLBarDone));
+            loss_drain(bar(kLBarDone), 0u, wt);
+        }
+    } else {
+        setmaxnreg_inc<kSoftRegs>();
+        // ------------------------------------------------------------- softmax warpgroups
+        const uint32_t g = (uint32_t)(warp - 4) >> 2;
+        const int quad = warp & 3, r = quad * 32 + lane;
+        const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+        float2* ms = reinterpret_cast<float2*>(gbase + kMOffMs);
+        const uint32_t patch = base + kMOffPatch + (uint32_t)(warp - 4) * 32u * kPatchRow * 4u;
+        const int feat = 16 * p.ksteps;
+        uint32_t cc = 0, uc = 0, uses = 0;
+        bool ok = true;
+        for (int u = blockIdx.x; ok && lunit_exists(u, p); u += gridDim.x, ++uc) {
+            const LUnit U = lunit(u, p);
+            const uint32_t n = (uint32_t)(U.c1 - U.c0);
+            // own operand -> TMEM: warpgroup g takes K slots 64 g .. 64 g + 63 of the lane's row
+            ok = loss_wait(bar(kLBarAEmpty), (uc & 1u) ^ 1u, wt, 106);
+            if (!ok) break;
+            tc_fence_after();
+            if ((int)(4 * g) < p.ksteps) {
+                const uint8_t* img = p.own + (size_t)U.own * kStage;
+#pragma unroll
+                for (int part = 0; part < (F32 ? 2 : 1); ++part) {
+                    uint32_t w[32];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(img + part * kLossImage + image_chunk(r, 8 * g + j));
+                        w[4 * j] = x.x, w[4 * j + 1] = x.y, w[4 * j + 2] = x.z, w[4 * j + 3] = x.w;
+                    }
+                    tmem_st32x32b_x32(tmem + lanes + kTOwn + 64u * part + 32u * g, w);
+                }
+                tmem_st_wait();
+            }
+            tc_fence_before();
+            mbar_arrive(bar(kLBarAFull));
+
+            const float own_mul = F32 ? p.logit_scale * __ldg(p.own_scale + U.own) : p.logit_scale;
+            const float lane_e = WPASS ? __ldg(p.lane_e + (size_t)U.own * 128 + r) : 0.0f;
+            float off = -CUDART_INF_F, sum = 0.0f, carry = 0.0f;  // weight pass: sum + carry = bias gradient
+            float2 acc[64];
+#pragma unroll
+            for (int i = 0; i < 64; ++i) acc[i] = make_float2(0.f, 0.f);
+
+            for (uint32_t i = g; i < n; i += 2, ++uses) {
+                const int c = U.c0 + (int)i;
+                const uint32_t s = (cc + i) % kStages;
+                const uint32_t tab = base + kMOffTab + s * 1024u;
+                const float str_s = F32 ? __ldg(p.str_scale + c) : 1.0f;
+                float o_mul = str_s;  // value of one unit of the second product
+                LabelWindow lw{make_int2(kNoLabel, 0), 0, 0};
+                const int2* ent = nullptr;
+                if (WPASS) {
+                    if (F32) o_mul *= __ldg(p.g_scale + c);
+                    const int32_t* o = p.sp_off + (size_t)c * (p.own_tiles + 1) + U.own;
+                    ent = p.sp_ent + (size_t)c * 128 * p.n_top;
+                    lw.next = __ldg(o);
+                    lw.end = __ldg(o + 1);
+                    if (lw.next < lw.end) window_load(lw, ent, lane);
+                } else if (F32) {
+                    o_mul *= 1.0f / 16384.0f;  // probabilities are stored times 2^14
+                }
+                const float2 mul = make_float2(own_mul * str_s, own_mul * str_s);
+                const uint32_t t_s = tmem + lanes + kTS + 128u * g;
+                ok = loss_wait(bar(kLBarSFull + (int)g), uses & 1u, wt, 107);
+                // the column table came with the tile: its barrier has passed, but this warp has to
+                // observe it before it reads what the copy wrote
+                ok = ok && loss_wait(bar(kLBarFull + s), ((cc + i) / kStages) & 1u, wt, 108);
+                if (!ok) break;
+                tc_fence_after();
+                float corr = 1.0f;
+                if constexpr (!WPASS) {
+                    float top = -CUDART_INF_F;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t v[32];
+                        tmem_ld32x32b_x32_wait(t_s + 32u * q, v);
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            const float4 e = lds128(tab + 4u * (32 * q + j));
+                            const float2 a = __ffma2_rn(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), mul,
+                                                        make_float2(e.x, e.y));
+                            const float2 b = __ffma2_rn(make_float2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])),
+                                                        mul, make_float2(e.z, e.w));
+                            top = max3f(top, a.x, a.y);
+                            top = max3f(top, b.x, b.y);
+                        }
+                    }
+                    const float m = fmaxf(off, top);
+                    // nothing visible yet (every class masked): any finite offset gives 2^-inf = 0
+                    const float m0 = m == -CUDART_INF_F ? 0.0f : m;
+                    corr = off == -CUDART_INF_F ? 0.0f : ex2_approx(off - m0);
+                    off = m;
+                    const float sub = F32 ? 14.0f - m0 : -m0;
+                    const float2 sub2 = make_float2(sub, sub);
+                    float2 ts = make_float2(0.f, 0.f);
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) {
+                        uint32_t v[16];
+                        float2 pr[8];
+                        tmem_ld32x32b_x16_wait(t_s + 16u * q, v);
+#pragma unroll
+                        for (int j = 0; j < 16; j += 4) {
+                            const float4 e = lds128(tab + 4u * (16 * q + j));
+                            float2 a = __ffma2_rn(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), mul,
+                                                  make_float2(e.x, e.y));
+                            float2 b = __ffma2_rn(make_float2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])), mul,
+                                                  make_float2(e.z, e.w));
+                            a = __fadd2_rn(a, sub2);
+                            b = __fadd2_rn(b, sub2);
+                            pr[j / 2] = make_float2(ex2_approx(a.x), ex2_approx(a.y));
+                            pr[j / 2 + 1] = make_float2(ex2_approx(b.x), ex2_approx(b.y));
+                            ts = __fadd2_rn(ts, __fadd2_rn(pr[j / 2], pr[j / 2 + 1]));
+                        }
+                        if (with_o) store_probs<F32>(t_s + 16u * q, pr);
+                    }
+                    const float t = F32 ? (ts.x + ts.y) * (1.0f / 16384.0f) : ts.x + ts.y;
+                    sum = fmaf(sum, corr, t);
+                } else {
+                    const float2 le = make_float2(lane_e, lane_e);
+                    float2 ts = make_float2(0.f, 0.f);
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) {
+                        uint32_t v[16];
+                        float2 pr[8];
+                        tmem_ld32x32b_x16_wait(t_s + 16u * q, v);
+#pragma unroll
+                        for (int j = 0; j < 16; j += 4) {
+                            const float4 e = lds128(tab + 4u * (16 * q + j));
+                            const float4 f = lds128(tab + 512u + 4u * (16 * q + j));
+                            float2 a = __ffma2_rn(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), mul,
+                                                  make_float2(e.x, e.y));
+                            float2 b = __ffma2_rn(make_float2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])), mul,
+                                                  make_float2(e.z, e.w));
+                            a = __fadd2_rn(a, le);
+                            b = __fadd2_rn(b, le);
+                            pr[j / 2] = __fmul2_rn(make_float2(ex2_approx(a.x), ex2_approx(a.y)), make_float2(f.x, f.y));
+                            pr[j / 2 + 1] =
+                                __fmul2_rn(make_float2(ex2_approx(b.x), ex2_approx(b.y)), make_float2(f.z, f.w));
+                        }
+                        // the labels' shares, 16 columns (rows of x) at a time through a patch of
+                        // shared memory: entries scatter into it, each lane then adds its class's row
+                        const int lo = 16 * q;
+                        bool any = false;
+                        while (true) {
+                            const bool in = (lw.e.x >> 7) < lo + 16;
+                            const uint32_t b = __ballot_sync(0xffffffffu, in);
+                            if (b == 0u) break;
+                            const bool hit = in && ((lw.e.x & 127) >> 5) == quad;
+                            if (hit)
+                                *reinterpret_cast<volatile float*>(
+                                    gbase + (patch - base) +
+                                    4u * ((uint32_t)(lw.e.x & 31) * kPatchRow + (uint32_t)((lw.e.x >> 7) - lo))) =
+                                    __int_as_float(lw.e.y);
+                            any |= __any_sync(0xffffffffu, hit);
+                            if (in) lw.e.x = kNoLabel;
+                            if (!(b >> 31) || lw.next >= lw.end) break;
+                            window_load(lw, ent, lane);
+                        }
+                        if (any) {
+                            __syncwarp();
+                            const uint32_t row = patch + 4u * (uint32_t)lane * kPatchRow;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const float4 d = lds128(row + 16u * j);
+                                pr[2 * j] = __fadd2_rn(pr[2 * j], make_float2(d.x, d.y));
+                                pr[2 * j + 1] = __fadd2_rn(pr[2 * j + 1], make_float2(d.z, d.w));
+                                sts128(row + 16u * j, make_float4(0.f, 0.f, 0.f, 0.f));
+                            }
+                            __syncwarp();
+                        }
+#pragma unroll
+                        for (int j = 0; j < 8; j += 2) ts = __fadd2_rn(ts, __fadd2_rn(pr[j], pr[j + 1]));
+                        store_probs<F32>(t_s + 16u * q, pr);
+                    }
+                    // bias gradient with the rounding error carried (up to thousands of tiles)
+                    const float t = fmaf(ts.x + ts.y, F32 ? __ldg(p.g_scale + c) : 1.0f, carry);
+                    const float nsum = sum + t;
+                    carry = t - (nsum - sum);
+                    sum = nsum;
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(bar(kLBarPFull + (int)g));
+                    mbar_arrive(bar(kLBarEmpty + (int)s));
+                }
+                if (with_o) {
+                    ok = loss_wait(bar(kLBarOFull + (int)g), uses & 1u, wt, 109);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (!WPASS && !__all_sync(0xffffffffu, corr == 1.0f)) {
+                        const float2 c2 = make_float2(corr, corr);
+#pragma unroll
+                        for (int j = 0; j < 64; ++j) acc[j] = __fmul2_rn(acc[j], c2);
+                    }
+                    const float2 om = make_float2(o_mul, o_mul);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        if (32 * q < feat) {
+                            uint32_t v[32];
+                            tmem_ld32x32b_x32_wait(tmem + lanes + kTO + 32u * q, v);
+#pragma unroll
+                            for (int j = 0; j < 16; ++j)
+                                acc[16 * q + j] = __ffma2_rn(make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])),
+                                                             om, acc[16 * q + j]);
+                        }
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(kLBarOEmpty + (int)g));
+                }
+            }
+            if (!ok) break;
+            cc += n;
+            // Join the two warpgroups' states: warpgroup 1 leaves its sums in its own score buffer
+            // (free: its last product is done, and the next unit's scores need warpgroup 0, which
+            // reads them first, to have passed the own operand's barrier).
+            if (g == 1) {
+                ok = loss_wait(bar(kLBarAFull), uc & 1u, wt, 110);
+                if (!ok) break;
+                if (with_o) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        if (32 * q < feat) {
+                            uint32_t v[32];
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                v[2 * j] = __float_as_uint(acc[16 * q + j].x);
+                                v[2 * j + 1] = __float_as_uint(acc[16 * q + j].y);
+                            }
+                            tmem_st32x32b_x32(tmem + lanes + kTS + 128u + 32u * q, v);
+                        }
+                    }
+                    tmem_st_wait();
+                }
+                ms[r] = WPASS ? make_float2(sum, carry) : make_float2(off, sum);
+                tc_fence_before();
+                mbar_arrive(bar(kLBarMerge));
+            } else {
+                ok = loss_wait(bar(kLBarMerge), uc & 1u, wt, 111);
+                if (!ok) break;
+                tc_fence_after();
+                const float2 o = ms[r];
+                float k0 = 1.0f, k1 = 1.0f;
+                float2 out;
+                if (WPASS) {
+                    out = make_float2((sum + o.x) + (carry + o.y), 0.0f);
+                } else {
+                    const float m = fmaxf(off, o.x);
+                    k0 = off == -CUDART_INF_F ? 0.0f : ex2_approx(off - m);
+                    k1 = o.x == -CUDART_INF_F ? 0.0f : ex2_approx(o.x - m);
+                    out = make_float2(m, sum * k0 + o.y * k1);
+                }
+                p.part_ms[(size_t)u * 128 + r] = out;
+                if (with_o) {
+                    float* po = p.part_o + (size_t)u * feat * 128 + r;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        if (32 * q < feat) {
+                            uint32_t v[32];
+                            tmem_ld32x32b_x32_wait(tmem + lanes + kTS + 128u + 32u * q, v);
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                const int f = 32 * q + 2 * j;
+                                if (f < feat) {
+                                    po[(size_t)f * 128] = acc[16 * q + j].x * k0 + __uint_as_float(v[2 * j]) * k1;
+                                    po[(size_t)(f + 1) * 128] = acc[16 * q + j].y * k0 + __uint_as_float(v[2 * j + 1]) * k1;
+                                }
+                            }
+                        }
+                    }
+                }
+                tc_fence_before();
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// ---------------------------------------------------------------------------- row kernel
+namespace {
+
+// 4 values of row `c` of a row-major [.][k] matrix: K slots 4 lane .. 4 lane + 3 (zero past k).
+template <bool F32>
+__device__ __forceinline__ float4 row_quad(const void* w, long long c, int k, int lane, bool vec) {
+    using T = typename Elem<F32>::type;
+    const T* a = static_cast<const T*>(w) + c * k + 4 * lane;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (vec) {
+        if (4 * lane < k) {
+            if constexpr (F32) {
+                v = __ldg(reinterpret_cast<const float4*>(a));
+            } else {
+                const uint2 u = __ldg(reinterpret_cast<const uint2*>(a));
+                v = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                                __uint_as_float(u.y & 0xffff0000u));
+            }
+        }
+    } else {
+        if (4 * lane < k) v.x = to_f32(a[0]);
+        if (4 * lane + 1 < k) v.y = to_f32(a[1]);
+        if (4 * lane + 2 < k) v.z = to_f32(a[2]);
+        if (4 * lane + 3 < k) v.w = to_f32(a[3]);
+    }
+    return v;
+}
+
+__device__ __forceinline__ float4 smem_quad(const float* row, int k, int lane) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (4 * lane < k) v.x = row[4 * lane];
+    if (4 * lane + 1 < k) v.y = row[4 * lane + 1];
+    if (4 * lane + 2 < k) v.z = row[4 * lane + 2];
+    if (4 * lane + 3 < k) v.w = row[4 * lane + 3];
+    return v;
+}
+__device__ __forceinline__ float dot4(float4 a, float4 b) {
+    return fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, a.w * b.w)));
+}
+
+// R rows of the features into shared memory (row stride k + 1), coalesced along the layout's
+// contiguous direction.
+template <int R, class T>
+__device__ __forceinline__ void load_rows(const T* x, long long row0, long long rows, int k, long long t_len, float* xs) {
+    if (t_len > 0) {
+        for (int i = threadIdx.x; i < R * k; i += 256) {
+            const int r = i % R, kk = i / R;
+            const long long row = row0 + r;
+            xs[r * (k + 1) + kk] = row < rows ? to_f32(x[x_base(row, k, t_len) + kk * t_len]) : 0.0f;
+        }
+    } else {
+        for (int i = threadIdx.x; i < R * k; i += 256) {
+            const int r = i / k, kk = i - r * k;
+            xs[r * (k + 1) + kk] = row0 + r < rows ? to_f32(x[row0 * k + i]) : 0.0f;
+        }
+    }
+}
+
+// Rows l0 .. l0 + R - 1 of the units u0 .. u0 + ns - 1's partial tiles [feat][128], weighted and
+// added in the units' order, into os [R][feat + 1] times inv[row]. A thread owns one row and every
+// (256 / R)-th feature, and keeps all of its features' loads of a unit in flight: with few rows the
+// work is split over many units, and their latency is what this join costs.
+template <int R, bool WEIGHTED>
+__device__ __forceinline__ void join_units(const float* part_o, size_t u0, int ns, int feat, int l0, const float* wgt,
+                                           const float* inv, float* os) {
+    constexpr int kStep = 256 / R, kPer = 128 / kStep;
+    const int r = threadIdx.x % R, f0 = threadIdx.x / R;
+    float a[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) a[i] = 0.0f;
+    const float* po = part_o + u0 * feat * 128 + (size_t)f0 * 128 + l0 + r;
+#pragma unroll 4
+    for (int s = 0; s < ns; ++s, po += (size_t)feat * 128) {
+        const float w = WEIGHTED ? wgt[s * R + r] : 1.0f;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+            if (f0 + i * kStep < feat) a[i] = fmaf(__ldg(po + (size_t)i * kStep * 128), w, a[i]);
+    }
+    const float k = WEIGHTED ? inv[r] : 1.0f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+        if (f0 + i * kStep < feat) os[r * (feat + 1) + f0 + i * kStep] = a[i] * k;
+}
+
+}  // namespace
+
+// One block per R rows (32; 8 where that leaves most SMs idle). Joins the class ranges of a row
+// block (the largest offset, the sums and mean weight rows brought to it), then one warp per row:
+// the labels' logits as f32 products, the loss, and dx = T g (sum_j p_j W_j - sum_i q_i W_ci).
+template <bool F32, int R>
+__global__ void __launch_bounds__(256) loss_rows_kernel(const __grid_constant__ LossRowParams p) {
+    using T = typename Elem<F32>::type;
+    extern __shared__ float sm[];
+    float* xs = sm;                            // [R][k + 1]
+    float* os = xs + R * (p.k + 1);            // [R][feat + 1]
+    float* wgt = os + R * (p.feat + 1);        // [n_splits][R]
+    constexpr int kG = 256 / R;                // threads that share a row's ranges
+    __shared__ float red[kG][R];
+    __shared__ float s_lse2[R], s_inv[R];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const long long row0 = (long long)blockIdx.x * R;
+    const int mb = (int)(row0 >> 7), l0 = (int)(row0 & 127);
+    const int ns = mb < p.whole_units ? 1 : p.n_splits;
+    const size_t u0 = mb < p.whole_units ? (size_t)mb : (size_t)p.whole_units + (size_t)(mb - p.whole_units) * p.n_splits;
+
+    load_rows<R>(static_cast<const T*>(p.x), row0, p.rows, p.k, p.t_len, xs);
+    const int jr = tid % R, jg = tid / R;
+    float m = -CUDART_INF_F;
+    for (int s = jg; s < ns; s += kG) {
+        const float o = p.part_ms[(u0 + s) * 128 + l0 + jr].x;
+        wgt[s * R + jr] = o;
+        m = fmaxf(m, o);
+    }
+    red[jg][jr] = m;
+    __syncthreads();
+    for (int i = 0; i < kG; ++i) m = fmaxf(m, red[i][jr]);
+    const float m0 = m == -CUDART_INF_F ? 0.0f : m;
+    float sum = 0.0f;
+    __syncthreads();
+    for (int s = jg; s < ns; s += kG) {
+        const float k = ex2_approx(wgt[s * R + jr] - m0);
+        wgt[s * R + jr] = k;
+        sum = fmaf(p.part_ms[(u0 + s) * 128 + l0 + jr].y, k, sum);
+    }
+    red[jg][jr] = sum;
+    __syncthreads();
+    if (jg == 0) {
+        sum = 0.0f;
+        for (int i = 0; i < kG; ++i) sum += red[i][jr];
+        s_lse2[jr] = m0 + log2f(sum);
+        s_inv[jr] = 1.0f / sum;
+    }
+    __syncthreads();
+    if (p.dx) {
+        join_units<R, true>(p.part_o, u0, ns, p.feat, l0, wgt, s_inv, os);
+        __syncthreads();
+    }
+    const bool vec = p.k % 4 == 0 && (reinterpret_cast<uintptr_t>(p.w) & (F32 ? 15u : 7u)) == 0;
+    for (int rr = 0; rr < R / 8; ++rr) {
+        const int r = warp * (R / 8) + rr;
+        const long long row = row0 + r;
+        float* tab = p.row_tab + (size_t)(row >> 7) * 256 + (row & 127);
+        RowLabels lab;
+        const bool valid = row < p.rows && row_labels(p.lab, row, lane, lab);
+        const float lse2 = s_lse2[r], lse = lse2 * kLn2;
+        if (lane == 0) *tab = valid ? -lse2 : -CUDART_INF_F;
+        if (row >= p.rows) continue;
+        float* xr = xs + r * (p.k + 1);
+        if (!valid) {
+            if (lane == 0) {
+                if (p.loss) p.loss[row] = 0.0f;
+                if (p.lse) p.lse[row] = 0.0f;
+            }
+            for (int kk = lane; kk < p.k; kk += 32) xr[kk] = 0.0f;
+            continue;
+        }
+        const float4 x4 = smem_quad(xr, p.k, lane);
+        float4 d = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (p.dx) d = smem_quad(os + r * (p.feat + 1), p.k, lane);
+        float loss = 0.0f;
+        for (int e0 = 0; e0 < p.lab.n_top; e0 += 4) {
+            int c[4];
+            float q[4], lq[4], z[4];
+            float4 w4[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int e = e0 + j;  // n_top <= 64, so e < 64; entries past n_top hold class -1
+                c[j] = __shfl_sync(0xffffffffu, e < 32 ? lab.c[0] : lab.c[1], e & 31);
+                q[j] = __shfl_sync(0xffffffffu, e < 32 ? lab.q[0] : lab.q[1], e & 31);
+                lq[j] = __shfl_sync(0xffffffffu, e < 32 ? lab.log_q[0] : lab.log_q[1], e & 31);
+                w4[j] = c[j] >= 0 ? row_quad<F32>(p.w, c[j], p.k, lane, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) z[j] = dot4(x4, w4[j]);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) z[j] += __shfl_xor_sync(0xffffffffu, z[j], o);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                // an entry of no share (teacher logit -inf) holds the row to nothing
+                if (c[j] >= 0 && q[j] != 0.0f) {
+                    const float zz = (z[j] + (p.bias ? p.bias[c[j]] : 0.0f)) * p.lab.inv_temp;
+                    loss = fmaf(q[j], lq[j] - (zz - lse), loss);
+                    d.x = fmaf(-q[j], w4[j].x, d.x);
+                    d.y = fmaf(-q[j], w4[j].y, d.y);
+                    d.z = fmaf(-q[j], w4[j].z, d.z);
+                    d.w = fmaf(-q[j], w4[j].w, d.w);
+                }
+            }
+        }
+        if (lane == 0) {
+            if (p.loss) p.loss[row] = loss * p.lab.temp * p.lab.temp;
+            if (p.lse) p.lse[row] = lse;
+        }
+        if (p.dx) {
+            const float f = p.lab.temp * (p.row_grad ? p.row_grad[row] : 1.0f);
+            if (4 * lane < p.k) xr[4 * lane] = f * d.x;
+            if (4 * lane + 1 < p.k) xr[4 * lane + 1] = f * d.y;
+            if (4 * lane + 2 < p.k) xr[4 * lane + 2] = f * d.z;
+            if (4 * lane + 3 < p.k) xr[4 * lane + 3] = f * d.w;
+        }
+    }
+    if (!p.dx) return;
+    __syncthreads();
+    T* dx = static_cast<T*>(p.dx);
+    if (p.t_len > 0) {
+        for (int i = tid; i < R * p.k; i += 256) {
+            const int r = i % R, kk = i / R;
+            if (row0 + r < p.rows) dx[x_base(row0 + r, p.k, p.t_len) + kk * p.t_len] = (T)xs[r * (p.k + 1) + kk];
+        }
+    } else {
+        for (int i = tid; i < R * p.k; i += 256) {
+            const int r = i / p.k, kk = i - r * p.k;
+            if (row0 + r < p.rows) dx[row0 * p.k + i] = (T)xs[r * (p.k + 1) + kk];
+        }
+    }
+}
+
+// One block per R classes (32, or 8 as above): the row ranges' partial sums added in their order,
+// transposed through shared memory into dW [n][k].
+template <bool F32, int R>
+__global__ void __launch_bounds__(256) loss_reduce_kernel(const __grid_constant__ LossReduceParams p) {
+    using T = typename Elem<F32>::type;
+    extern __shared__ float sm[];  // [R][feat + 1]
+    const int j0 = (int)blockIdx.x * R, tile = j0 >> 7, l0 = j0 & 127;
+    const int ns = tile < p.whole_units ? 1 : p.n_splits;
+    const size_t u0 = tile < p.whole_units ? (size_t)tile : (size_t)p.whole_units + (size_t)(tile - p.whole_units) * p.n_splits;
+    join_units<R, false>(p.part_o, u0, ns, p.feat, l0, nullptr, nullptr, sm);
+    if (p.db && threadIdx.x < R && j0 + (int)threadIdx.x < p.n) {
+        float a = 0.0f;
+        for (int s = 0; s < ns; ++s) a += p.part_ms[(u0 + s) * 128 + l0 + threadIdx.x].x;
+        p.db[j0 + threadIdx.x] = a;
+    }
+    __syncthreads();
+    T* dw = static_cast<T*>(p.dw);
+    for (int i = threadIdx.x; i < R * p.k; i += 256) {
+        const int r = i / p.k, kk = i - r * p.k;
+        if (j0 + r < p.n) dw[(long long)j0 * p.k + i] = (T)sm[r * (p.feat + 1) + kk];
+    }
+}
+
+// ---------------------------------------------------------------------------- packed heads
+// Class table at temperature T: scale / T and bias / T (the decode kernel then decodes z / T).
+__global__ void __launch_bounds__(256) loss_table_kernel(const float* __restrict__ ctab, long long n, float inv_temp,
+                                                         float* __restrict__ out) {
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i < n) out[i] = ctab[i] * inv_temp;
+}
+
+namespace {
+
+// K slots 4 lane .. 4 lane + 3 of a packed weight's class c, in units of its class-table scale.
+__device__ __forceinline__ float4 packed_quad(const uint8_t* tiles, int form, int c, int lane) {
+    const int tile = c >> 7, r = c & 127, s = 4 * lane;
+    if (form == 1) {
+        const uint32_t w =
+            __ldg(reinterpret_cast<const uint32_t*>(tiles + (size_t)tile * kTile8Bytes + image8_offset(r, s)));
+        return make_float4((float)(int)(w & 255u) - 128.0f, (float)(int)((w >> 8) & 255u) - 128.0f,
+                           (float)(int)((w >> 16) & 255u) - 128.0f, (float)(int)(w >> 24) - 128.0f);
+    }
+    const uint8_t* a = tiles + (size_t)tile * (form == 2 ? 2 * kTileBytes : kTileBytes) + image_chunk(r, s >> 3) + 2 * (s & 7);
+    auto quad = [](const uint8_t* b) {
+        const uint2 u = __ldg(reinterpret_cast<const uint2*>(b));
+        const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
+        const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+        return make_float4(lo.x, lo.y, hi.x, hi.y);
+    };
+    float4 v = quad(a);
+    if (form == 2) {
+        const float4 l = quad(a + kTileBytes);
+        v = make_float4(v.x + l.x, v.y + l.y, v.z + l.z, v.w + l.w);
+    }
+    return v;
+}
+
+}  // namespace
+
+// One block per 32 rows, one warp per row: the logits of the row's labels and of its argmax as f32
+// products with the packed weight. lse = z[argmax] / T - log(probability of the argmax).
+__global__ void __launch_bounds__(256) loss_score_kernel(const __grid_constant__ LossScoreParams p) {
+    extern __shared__ float xs[];  // [32][k + 1]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long long row0 = (long long)blockIdx.x * kLossRows;
+    load_rows<kLossRows>(p.x, row0, p.rows, p.k, p.t_len, xs);
+    __syncthreads();
+    for (int rr = 0; rr < kLossRows / 8; ++rr) {
+        const int r = warp * (kLossRows / 8) + rr;
+        const long long row = row0 + r;
+        if (row >= p.rows) break;
+        const int* cls = p.lab.target ? p.lab.target + row : p.lab.top_idx + row * p.lab.n_top;
+        bool bad = false;
+        for (int e = lane; e < p.lab.n_top; e += 32) bad |= cls[e] >= p.lab.n;
+        if (bad) atomicOr(p.status, kDevBadClass);
+        RowLabels lab;
+        if (!row_labels(p.lab, row, lane, lab)) {
+            if (lane == 0) {
+                if (p.loss) p.loss[row] = 0.0f;
+                if (p.lse) p.lse[row] = 0.0f;
+            }
+            continue;
+        }
+        const float4 x4 = smem_quad(xs + r * (p.k + 1), p.k, lane);
+        auto logit = [&](int c) -> float {
+            const float s = warp_sum(dot4(x4, packed_quad(p.tiles, p.form, c, lane)));
+            const float* t = p.ctab + (size_t)(c >> 7) * kCtabFloats + (c & 127);
+            return fmaf(s, t[0], t[kBlockN]) * p.lab.inv_temp;
+        };
+        const int best = min(max(p.idx[row], 0), p.lab.n - 1);
+        const float lse = logit(best) - logf(p.prob[row]);
+        float loss = 0.0f;
+        for (int e = 0; e < p.lab.n_top; ++e) {
+            const int c = __shfl_sync(0xffffffffu, e < 32 ? lab.c[0] : lab.c[1], e & 31);
+            const float q = __shfl_sync(0xffffffffu, e < 32 ? lab.q[0] : lab.q[1], e & 31);
+            const float lq = __shfl_sync(0xffffffffu, e < 32 ? lab.log_q[0] : lab.log_q[1], e & 31);
+            if (c < 0 || q == 0.0f) continue;
+            loss = fmaf(q, lq - (logit(c) - lse), loss);
+        }
+        if (lane == 0) {
+            if (p.loss) p.loss[row] = loss * p.lab.temp * p.lab.temp;
+            if (p.lse) p.lse[row] = lse;
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------- launchers
+namespace {
+constexpr int kPackSmemMax = 9 * (kLossMaxClasses / 128) * 4;
+constexpr int kRowsSmemMax = (2 * 32 * 129 + 32 * kLossMaxSplits) * 4;
+// Blocks of 32 rows would leave SMs idle: four times as many of 8.
+bool few_blocks(int tiles, int sms) { return tiles * (kLossTile / 32) < 2 * sms; }
+template <class K>
+cudaError_t smem_attr(K* k, int bytes) {
+    return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+}  // namespace
+
+cudaError_t loss_kernel_setup() {
+    cudaError_t e;
+    if ((e = smem_attr(loss_main_kernel<true, false>, kMSmemBytes)) != cudaSuccess) return e;
+    if ((e = smem_attr(loss_main_kernel<true, true>, kMSmemBytes)) != cudaSuccess) return e;
+    if ((e = smem_attr(loss_main_kernel<false, false>, kMSmemBytes)) != cudaSuccess) return e;
+    if ((e = smem_attr(loss_main_kernel<false, true>, kMSmemBytes)) != cudaSuccess) return e;
+    if ((e = smem_attr(loss_pack_kernel<true>, kPackSmemMax)) != cudaSuccess) return e;
+    if ((e = smem_attr(loss_pack_kernel<false>, kPackSmemMax)) != cudaSuccess) return e;
+    if ((e = smem_attr(loss_rows_kernel<true, 32>, kRowsSmemMax)) != cudaSuccess) return e;
+    return smem_attr(loss_rows_kernel<false, 32>, kRowsSmemMax);
+}
+
+cudaError_t launch_loss_pack(const LossPackParams& p, bool f32, cudaStream_t stream) {
+    const int grid = p.w_tiles + p.x_tiles;
+    const int smem = p.sort_labels ? 9 * p.w_tiles * 4 : 0;
+    if (f32)
+        loss_pack_kernel<true><<<grid, 256, smem, stream>>>(p);
+    else
+        loss_pack_kernel<false><<<grid, 256, smem, stream>>>(p);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_loss_main(const LossMainParams& p, bool f32, bool weight_pass, int grid, cudaStream_t stream) {
+    if (f32 && !weight_pass)
+        loss_main_kernel<true, false><<<grid, kMainThreads, kMSmemBytes, stream>>>(p);
+    else if (f32)
+        loss_main_kernel<true, true><<<grid, kMainThreads, kMSmemBytes, stream>>>(p);
+    else if (!weight_pass)
+        loss_main_kernel<false, false><<<grid, kMainThreads, kMSmemBytes, stream>>>(p);
+    else
+        loss_main_kernel<false, true><<<grid, kMainThreads, kMSmemBytes, stream>>>(p);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_loss_rows(const LossRowParams& p, bool f32, int sms, cudaStream_t stream) {
+    const int tiles = (int)((p.rows + kLossTile - 1) / kLossTile);  // the last tile's padding rows too
+    const int r = few_blocks(tiles, sms) ? 8 : 32;
+    const int grid = tiles * (kLossTile / r);
+    const int smem = (r * (p.k + 1) + r * (p.feat + 1) + r * p.n_splits) * 4;
+    if (f32 && r == 32)
+        loss_rows_kernel<true, 32><<<grid, 256, smem, stream>>>(p);
+    else if (f32)
+        loss_rows_kernel<true, 8><<<grid, 256, smem, stream>>>(p);
+    else if (r == 32)
+        loss_rows_kernel<false, 32><<<grid, 256, smem, stream>>>(p);
+    else
+        loss_rows_kernel<false, 8><<<grid, 256, smem, stream>>>(p);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_loss_reduce(const LossReduceParams& p, bool f32, int sms, cudaStream_t stream) {
+    const int r = few_blocks((p.n + kLossTile - 1) / kLossTile, sms) ? 8 : 32;
+    const int grid = (p.n + r - 1) / r, smem = r * (p.feat + 1) * 4;
+    if (f32 && r == 32)
+        loss_reduce_kernel<true, 32><<<grid, 256, smem, stream>>>(p);
+    else if (f32)
+        loss_reduce_kernel<true, 8><<<grid, 256, smem, stream>>>(p);
+    else if (r == 32)
+        loss_reduce_kernel<false, 32><<<grid, 256, smem, stream>>>(p);
+    else
+        loss_reduce_kernel<false, 8><<<grid, 256, smem, stream>>>(p);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_loss_table(const float* ctab, long long n_floats, float inv_temp, float* out, cudaStream_t stream) {
+    loss_table_kernel<<<(int)((n_floats + 255) / 256), 256, 0, stream>>>(ctab, n_floats, inv_temp, out);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_loss_score(const LossScoreParams& p, cudaStream_t stream) {
+    const int grid = (int)((p.rows + kLossRows - 1) / kLossRows);
+    loss_score_kernel<<<grid, 256, kLossRows * (p.k + 1) * 4, stream>>>(p);
+    return cudaGetLastError();
+}
+
+}  // namespace rh

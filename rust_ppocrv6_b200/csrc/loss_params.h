@@ -1,0 +1,129 @@
+// Launch parameters of the training-loss kernels (loss_kernels.cu), shared with the host
+// dispatch (rechead_abi.cu). Plain C types only.
+#pragma once
+#include <cstdint>
+#include <cuda_runtime.h>
+
+namespace rh {
+
+constexpr int kLossTile = 128;            // rows (classes) per operand tile
+constexpr int kLossImage = 128 * 128 * 2;  // one 16-bit tile image: 128 rows x 128 K slots
+constexpr int kLossMaxTop = 64;           // teacher entries per row
+constexpr int kLossMaxClasses = 1 << 18;  // class tiles are counted in shared memory (2,048 bins)
+constexpr int kLossRows = 32;             // rows per block of the score kernel
+constexpr int kLossMaxSplits = 148;       // ranges that an own tile's work is split into at most
+// Device status bit (status[0], beside kDevTimeout and kDevRecPlan): a target or teacher class
+// at or above the class count; the row or entry was taken as absent.
+constexpr int kDevBadClass = 4;
+
+// What a row is held to: a target class, or a teacher's top logits. Exactly one of target and
+// top_idx is set.
+struct LossLabels {
+    const int32_t* target;     // [rows], negative: the row is ignored
+    const int32_t* top_idx;    // [rows][n_top], negative: the entry is absent
+    const float* top_logits;   // [rows][n_top]
+    int n_top;                 // 1 with target
+    int n;                     // classes
+    float temp;                // T
+    float inv_temp;            // 1 / T
+};
+
+// Operand tiles of a training step: features and weight as tensor-core images, the class table,
+// the rows' gradient factors and, for the weight's gradient, the labels sorted by class tile.
+struct LossPackParams {
+    const void* x;             // [rows][k], or [rows / t_len][k][t_len] (t_len > 0)
+    const void* w;             // [n][k]
+    const float* bias;         // [n] or null
+    const float* row_grad;     // [rows] d total / d loss_r, or null: 1
+    LossLabels lab;
+    long long rows, t_len;
+    int k, x_tiles, w_tiles;
+    float logit_scale;         // log2(e) / T
+    int sort_labels;           // fill sp_off / sp_ent (the weight's gradient is wanted)
+    uint8_t* x_img;            // x_tiles images (f32: high image, then low image)
+    uint8_t* w_img;
+    float* x_scale;            // [x_tiles] value of one unit of the image (f32; a power of two)
+    float* w_scale;            // [w_tiles]
+    float* class_e;            // [w_tiles][128] bias * log2(e) / T; padding classes -inf
+    float* row_tab;            // [x_tiles][256]: 128 x (-lse, log2 units; written by the row kernel),
+                               // 128 x gradient factor (f32: scaled by the tile's power of two)
+    float* g_scale;            // [x_tiles] value of one unit of the tile's gradient factors
+    int32_t* sp_off;           // [x_tiles][w_tiles + 1] label ranges by class tile
+    int2* sp_ent;              // [x_tiles][128 n_top]: (row << 7 | class within its tile, factor bits)
+    int* status;
+};
+
+// One pass over (own tile, streamed tiles): see loss_main_kernel.
+struct LossMainParams {
+    const uint8_t* own;        // images of the stationary operand
+    const uint8_t* str;        // images of the streamed operand
+    const float* own_scale;    // per tile (f32)
+    const float* str_scale;
+    const float* col_tab;      // per streamed tile: class_e (128 floats) or row_tab (256 floats)
+    const float* lane_e;       // weight pass: class_e of the own classes
+    const float* g_scale;      // weight pass: per streamed tile
+    const int32_t* sp_off;     // weight pass
+    const int2* sp_ent;
+    int n_top;
+    int own_tiles, str_tiles;
+    int ksteps;                // K steps of 16
+    int whole_units, n_splits, tiles_per_split;
+    float logit_scale;
+    float* part_o;             // [units][16 ksteps][128], or null: only (offset, sum) (row pass)
+    float2* part_ms;           // [units][128]: row pass (offset, sum); weight pass (bias gradient, 0)
+    int* status;
+    unsigned long long timeout_ns;
+};
+
+// Rows of a training step after the row pass: loss, lse, the feature gradient and the row table.
+struct LossRowParams {
+    const void* x;
+    const void* w;
+    const float* bias;
+    const float* row_grad;
+    LossLabels lab;
+    long long rows, t_len;
+    int k, feat;
+    int whole_units, n_splits;
+    const float* part_o;
+    const float2* part_ms;
+    float* row_tab;
+    float* loss;               // [rows] or null
+    float* lse;                // [rows] or null
+    void* dx;                  // as x, or null
+};
+
+struct LossReduceParams {      // weight and bias gradient from the units' partial tiles
+    const float* part_o;
+    const float2* part_ms;
+    int n, k, feat;
+    int whole_units, n_splits;
+    void* dw;                  // [n][k]
+    float* db;                 // [n] or null
+};
+
+// Scores of a packed head: (idx, prob) of the decode kernel at temperature T -> loss, lse.
+struct LossScoreParams {
+    const float* x;
+    long long rows, t_len;
+    int k;
+    LossLabels lab;
+    const uint8_t* tiles;      // packed weight
+    const float* ctab;         // class table (scale, bias), at T = 1
+    int form;                  // 0 fp16 image of int8, 1 compact int8, 2 FP32 (hi, lo)
+    const int32_t* idx;
+    const float* prob;
+    float* loss;
+    float* lse;
+    int* status;
+};
+
+cudaError_t loss_kernel_setup();
+cudaError_t launch_loss_pack(const LossPackParams& p, bool f32, cudaStream_t stream);
+cudaError_t launch_loss_main(const LossMainParams& p, bool f32, bool weight_pass, int grid, cudaStream_t stream);
+cudaError_t launch_loss_rows(const LossRowParams& p, bool f32, int sms, cudaStream_t stream);
+cudaError_t launch_loss_reduce(const LossReduceParams& p, bool f32, int sms, cudaStream_t stream);
+cudaError_t launch_loss_table(const float* ctab, long long n_floats, float inv_temp, float* out, cudaStream_t stream);
+cudaError_t launch_loss_score(const LossScoreParams& p, cudaStream_t stream);
+
+}  // namespace rh

@@ -16,6 +16,7 @@
 #include <cuda_runtime.h>
 
 #include "head_params.h"
+#include "loss_params.h"
 #include "recpre_params.h"
 #include "rechead.h"
 
@@ -68,6 +69,7 @@ struct Slot {
     DevBuf a, idx, prob, out, partial;
     DevBuf lines, tok_off, tokens, scores;  // CTC collapse on the device
     DevBuf pre_rgb, pre_lines, pre_coords, pre_wts, pre_out;  // recognition preprocessing
+    DevBuf loss_in, loss_out, loss_ws;  // training losses from host memory
     cudaEvent_t pre_done = nullptr;  // recorded after the last kernel that reads pre_lines/coords/wts
     cudaEvent_t part_done = nullptr;  // recorded after the last merge that reads `partial`
     std::mutex mu;
@@ -78,7 +80,7 @@ struct Slot {
         if (stream) cudaStreamSynchronize(stream);
         if (copy_stream) cudaStreamSynchronize(copy_stream);
         for (DevBuf* b : {&a, &idx, &prob, &out, &partial, &lines, &tok_off, &tokens, &scores, &pre_rgb, &pre_lines,
-                          &pre_coords, &pre_wts, &pre_out})
+                          &pre_coords, &pre_wts, &pre_out, &loss_in, &loss_out, &loss_ws})
             b->release();
         if (d_status) cudaFree(d_status);
         if (h_status) cudaFreeHost(h_status);
@@ -288,6 +290,9 @@ int status_error(Slot& s, const int* st) {
         if (st[0] & rh::kDevTimeout)
             return fail(RH_ERR_TIMEOUT, "device wait timed out (site " + std::to_string(st[1]) +
                                             "); the kernel gave up and the context is still usable");
+        if (st[0] & rh::kDevBadClass)
+            return fail(RH_ERR_INVALID_ARG,
+                        "a target or teacher class is not below the class count; its row or entry was taken as absent");
         return fail(RH_ERR_CUDA, "device status " + std::to_string(st[0]));
     }
     return RH_OK;
@@ -792,6 +797,488 @@ int rec_host_on_slot(rh_ctx* ctx, int slot, const uint8_t* rgb, const int64_t* o
     return sync_and_check(s);
 }
 
+// ------------------------------------------------------------------- training losses
+// The caller's current device again on the way out.
+struct DeviceGuard {
+    int prev = -1;
+    DeviceGuard() {
+        if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+    }
+    ~DeviceGuard() {
+        if (prev >= 0) cudaSetDevice(prev);
+    }
+};
+
+// No C++ exception leaves a C entry point (an allocation on the host is all that can throw).
+template <class F>
+int guarded(F&& f) {
+    try {
+        return f();
+    } catch (const std::exception& e) {
+        return fail(RH_ERR_CUDA, std::string("host error: ") + e.what());
+    }
+}
+
+// Work units of one pass: as many full waves of whole own tiles as there are, the rest split into
+// ranges of the streamed tiles. Cost of a split in streamed tiles: the last wave's length (its
+// tiles plus `overhead` for the unit's own operand, pipeline fill and hand-over), the reader's
+// join (about 1/20 tile a range) and the partial tiles' traffic (64 KB each, written and read:
+// about 1/100 tile each).
+struct LossPlan {
+    int own = 0, str = 0, whole = 0, splits = 1, per = 0, grid = 0;
+    int64_t units = 0;
+};
+LossPlan loss_plan(int64_t own, int64_t str, int sms, double overhead) {
+    LossPlan p;
+    p.own = (int)own;
+    p.str = (int)str;
+    p.whole = (int)(own / sms * sms);
+    p.per = p.str;
+    const int rest = p.own - p.whole;
+    double best = 1e300;
+    for (int s = 1; rest > 0 && s <= std::min(p.str, rh::kLossMaxSplits); ++s) {
+        const int per = (p.str + s - 1) / s, eff = (p.str + per - 1) / per;
+        const int64_t units = (int64_t)rest * eff, waves = (units + sms - 1) / sms;
+        if (units > 4 * (int64_t)sms && s > 1) break;  // bounds the partial tiles: 64 KB a unit
+        const double cost = (double)waves * (per + overhead) + 0.05 * eff + 0.01 * (double)units;
+        if (cost < best - 1e-9) {
+            best = cost;
+            p.splits = eff;
+            p.per = per;
+        }
+    }
+    p.units = (int64_t)p.whole + (int64_t)rest * p.splits;
+    p.grid = (int)std::min<int64_t>(p.units, sms);
+    return p;
+}
+
+// A training step's workspace: byte offsets of its parts. Partial tiles are shared: the row pass's
+// are read before the weight pass writes its own.
+struct LossLayout {
+    LossPlan row, cls;
+    int x_tiles = 0, w_tiles = 0, feat = 0;
+    size_t x_img, w_img, x_scale, w_scale, g_scale, class_e, row_tab, sp_off, sp_ent, part_o, part_ms, total;
+};
+LossLayout loss_layout(bool f32, int64_t rows, int64_t k, int64_t n, int64_t n_top, int sms) {
+    LossLayout L;
+    L.x_tiles = (int)((rows + 127) / 128);
+    L.w_tiles = (int)((n + 127) / 128);
+    L.feat = (int)((k + 15) / 16 * 16);
+    // a unit's fixed cost, in streamed tiles: about 2.5 us against 1.7 us (f32) and 0.7 us a tile
+    L.row = loss_plan(L.x_tiles, L.w_tiles, sms, f32 ? 1.5 : 3.5);
+    L.cls = loss_plan(L.w_tiles, L.x_tiles, sms, f32 ? 1.5 : 3.5);
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += (bytes + 255) / 256 * 256;
+        return here;
+    };
+    const size_t img = (size_t)rh::kLossImage * (f32 ? 2 : 1);
+    const size_t units = (size_t)std::max(L.row.units, L.cls.units);
+    L.x_img = take((size_t)L.x_tiles * img);
+    L.w_img = take((size_t)L.w_tiles * img);
+    L.x_scale = take((size_t)L.x_tiles * 4);
+    L.w_scale = take((size_t)L.w_tiles * 4);
+    L.g_scale = take((size_t)L.x_tiles * 4);
+    L.class_e = take((size_t)L.w_tiles * 512);
+    L.row_tab = take((size_t)L.x_tiles * 1024);
+    L.sp_off = take((size_t)L.x_tiles * (size_t)(L.w_tiles + 1) * 4);
+    L.sp_ent = take((size_t)L.x_tiles * 128 * (size_t)n_top * 8);
+    L.part_o = take(units * (size_t)L.feat * 512);
+    L.part_ms = take(units * 1024);
+    L.total = at + 256;  // the caller's pointer is brought to a 256-byte boundary
+    return L;
+}
+
+int check_labels(const void* target, const void* top_idx, const void* top_logits, int64_t n_top, float temperature) {
+    if (target) return RH_OK;
+    if (n_top < 1 || n_top > rh::kLossMaxTop)
+        return fail(RH_ERR_INVALID_ARG, "n_top = " + std::to_string(n_top) + " is outside [1, 64]");
+    if (!(temperature > 0.0f) || !std::isfinite(temperature) || !std::isfinite(1.0f / temperature))
+        return fail(RH_ERR_INVALID_ARG, "temperature must be positive and finite");
+    if (!top_idx || !top_logits) return fail(RH_ERR_INVALID_ARG, "null teacher entries");
+    return RH_OK;
+}
+
+rh::LossLabels loss_labels(const int32_t* target, const int32_t* top_idx, const float* top_logits, int64_t n_top,
+                           float temperature, int64_t n) {
+    rh::LossLabels l{};
+    l.target = target;
+    l.top_idx = target ? nullptr : top_idx;
+    l.top_logits = target ? nullptr : top_logits;
+    l.n_top = target ? 1 : (int)n_top;
+    l.n = (int)n;
+    l.temp = target ? 1.0f : temperature;
+    l.inv_temp = 1.0f / l.temp;
+    return l;
+}
+
+int check_rows(int64_t rows, int64_t t_len) {
+    if (rows < 0 || t_len < 0) return fail(RH_ERR_INVALID_ARG, "negative row count or sequence length");
+    if (rows > (int64_t)1 << 30) return fail(RH_ERR_UNSUPPORTED, "more than 2^30 rows; split the batch");
+    if (t_len > 0 && rows % t_len != 0)
+        return fail(RH_ERR_INVALID_ARG, "rows = " + std::to_string(rows) + " is not a multiple of t_len = " +
+                                            std::to_string(t_len));
+    return RH_OK;
+}
+
+int check_workspace(const void* ws, int64_t have, size_t need) {
+    if (!ws || have < (int64_t)need)
+        return fail(RH_ERR_INVALID_ARG, "workspace holds " + std::to_string(ws ? have : 0) + " bytes; the call needs " +
+                                            std::to_string(need));
+    return RH_OK;
+}
+uint8_t* aligned256(void* p) { return (uint8_t*)(((uintptr_t)p + 255) & ~(uintptr_t)255); }
+
+int check_grad_shape(int dtype, int64_t rows, int64_t k, int64_t n) {
+    if (dtype != RH_DTYPE_F32 && dtype != RH_DTYPE_BF16)
+        return fail(RH_ERR_INVALID_ARG, "dtype must be RH_DTYPE_F32 or RH_DTYPE_BF16");
+    if (int rc = check_rows(rows, 0)) return rc;
+    if (n < 1 || k < 1) return fail(RH_ERR_INVALID_ARG, "weight must be [n>=1][k>=1]");
+    if (k > rh::kPadK)
+        return fail(RH_ERR_UNSUPPORTED, "K = " + std::to_string(k) + " exceeds the supported maximum of 128");
+    if (n > rh::kLossMaxClasses) return fail(RH_ERR_UNSUPPORTED, "more than 262,144 classes");
+    return RH_OK;
+}
+
+// A training step on device memory, enqueued on `st`; the caller has made the device current.
+int enqueue_grad(rh_ctx* ctx, Slot& s, int dtype, const void* d_a, int64_t rows, int64_t k, int64_t t_len,
+                 const void* d_w, int64_t n, const float* d_bias, const rh::LossLabels& lab, const float* d_row_grad,
+                 float* d_loss, float* d_lse, void* d_da, void* d_dw, float* d_dbias, uint8_t* ws, const LossLayout& L,
+                 cudaStream_t st) {
+    const bool f32 = dtype == RH_DTYPE_F32;
+    const float logit_scale = 1.4426950408889634f / lab.temp;
+    rh::LossPackParams pk{};
+    pk.x = d_a;
+    pk.w = d_w;
+    pk.bias = d_bias;
+    pk.row_grad = d_row_grad;
+    pk.lab = lab;
+    pk.rows = rows;
+    pk.t_len = t_len;
+    pk.k = (int)k;
+    pk.x_tiles = L.x_tiles;
+    pk.w_tiles = L.w_tiles;
+    pk.logit_scale = logit_scale;
+    pk.sort_labels = d_dw ? 1 : 0;
+    pk.x_img = ws + L.x_img;
+    pk.w_img = ws + L.w_img;
+    pk.x_scale = (float*)(ws + L.x_scale);
+    pk.w_scale = (float*)(ws + L.w_scale);
+    pk.class_e = (float*)(ws + L.class_e);
+    pk.row_tab = (float*)(ws + L.row_tab);
+    pk.g_scale = (float*)(ws + L.g_scale);
+    pk.sp_off = (int32_t*)(ws + L.sp_off);
+    pk.sp_ent = (int2*)(ws + L.sp_ent);
+    pk.status = s.d_status;
+    RH_CUDA(rh::launch_loss_pack(pk, f32, st));
+    s.launches++;
+
+    rh::LossMainParams m{};
+    m.own = pk.x_img;
+    m.str = pk.w_img;
+    m.own_scale = pk.x_scale;
+    m.str_scale = pk.w_scale;
+    m.col_tab = pk.class_e;
+    m.own_tiles = L.x_tiles;
+    m.str_tiles = L.w_tiles;
+    m.n_top = lab.n_top;
+    m.ksteps = L.feat / 16;
+    m.whole_units = L.row.whole;
+    m.n_splits = L.row.splits;
+    m.tiles_per_split = L.row.per;
+    m.logit_scale = logit_scale;
+    m.part_o = d_da ? (float*)(ws + L.part_o) : nullptr;
+    m.part_ms = (float2*)(ws + L.part_ms);
+    m.status = s.d_status;
+    m.timeout_ns = ctx->timeout_ns;
+    RH_CUDA(rh::launch_loss_main(m, f32, false, L.row.grid, st));
+    s.launches++;
+
+    rh::LossRowParams r{};
+    r.x = d_a;
+    r.w = d_w;
+    r.bias = d_bias;
+    r.row_grad = d_row_grad;
+    r.lab = lab;
+    r.rows = rows;
+    r.t_len = t_len;
+    r.k = (int)k;
+    r.feat = L.feat;
+    r.whole_units = L.row.whole;
+    r.n_splits = L.row.splits;
+    r.part_o = m.part_o;
+    r.part_ms = m.part_ms;
+    r.row_tab = pk.row_tab;
+    r.loss = d_loss;
+    r.lse = d_lse;
+    r.dx = d_da;
+    RH_CUDA(rh::launch_loss_rows(r, f32, s.sms, st));
+    s.launches++;
+    if (!d_dw) return RH_OK;
+
+    m.own = pk.w_img;
+    m.str = pk.x_img;
+    m.own_scale = pk.w_scale;
+    m.str_scale = pk.x_scale;
+    m.col_tab = pk.row_tab;
+    m.lane_e = pk.class_e;
+    m.g_scale = pk.g_scale;
+    m.sp_off = pk.sp_off;
+    m.sp_ent = pk.sp_ent;
+    m.own_tiles = L.w_tiles;
+    m.str_tiles = L.x_tiles;
+    m.whole_units = L.cls.whole;
+    m.n_splits = L.cls.splits;
+    m.tiles_per_split = L.cls.per;
+    m.part_o = (float*)(ws + L.part_o);
+    RH_CUDA(rh::launch_loss_main(m, f32, true, L.cls.grid, st));
+    s.launches++;
+
+    rh::LossReduceParams d{};
+    d.part_o = m.part_o;
+    d.part_ms = m.part_ms;
+    d.n = (int)n;
+    d.k = (int)k;
+    d.feat = L.feat;
+    d.whole_units = L.cls.whole;
+    d.n_splits = L.cls.splits;
+    d.dw = d_dw;
+    d.db = d_dbias;
+    RH_CUDA(rh::launch_loss_reduce(d, f32, s.sms, st));
+    s.launches++;
+    return RH_OK;
+}
+
+// Both operators' device form; `target` null: distillation.
+int grad_device(rh_ctx* ctx, int slot, int dtype, const void* d_a, int64_t rows, int64_t k, int64_t t_len,
+                const void* d_w, int64_t n, const float* d_bias, const int32_t* d_target, const int32_t* d_top_idx,
+                const float* d_top_logits, int64_t n_top, float temperature, const float* d_row_grad, float* d_loss,
+                float* d_lse, void* d_da, void* d_dw, float* d_dbias, void* ws, int64_t ws_bytes, void* stream) {
+    if (int rc = check_ctx(ctx)) return rc;
+    if (slot < 0 || slot >= (int)ctx->slots.size()) return fail(RH_ERR_INVALID_ARG, "slot out of range");
+    if (int rc = check_grad_shape(dtype, rows, k, n)) return rc;
+    if (int rc = check_rows(rows, t_len)) return rc;
+    if (d_dbias && !d_dw) return fail(RH_ERR_INVALID_ARG, "the bias gradient comes with the weight's: d_dw is null");
+    const int cleared = dtype == RH_DTYPE_F32 ? 4 : 2;
+    Slot& s = *ctx->slots[slot];
+    cudaStream_t st = (cudaStream_t)stream;
+    if (rows == 0) {  // no row: the sums over rows are zero
+        std::lock_guard<std::mutex> lock(s.mu);
+        DeviceGuard guard;
+        RH_CUDA(cudaSetDevice(s.device));
+        if (d_dw) RH_CUDA(cudaMemsetAsync(d_dw, 0, (size_t)n * (size_t)k * cleared, st));
+        if (d_dbias) RH_CUDA(cudaMemsetAsync(d_dbias, 0, (size_t)n * 4, st));
+        return RH_OK;
+    }
+    if (int rc = check_labels(d_target, d_top_idx, d_top_logits, n_top, temperature)) return rc;
+    if (!d_a || !d_w) return fail(RH_ERR_INVALID_ARG, "null device pointer");
+    const rh::LossLabels lab = loss_labels(d_target, d_top_idx, d_top_logits, n_top, temperature, n);
+    const LossLayout L = loss_layout(dtype == RH_DTYPE_F32, rows, k, n, lab.n_top, s.sms);
+    if (int rc = check_workspace(ws, ws_bytes, L.total)) return rc;
+    std::lock_guard<std::mutex> lock(s.mu);
+    DeviceGuard guard;
+    RH_CUDA(cudaSetDevice(s.device));
+    return enqueue_grad(ctx, s, dtype, d_a, rows, k, t_len, d_w, n, d_bias, lab, d_row_grad, d_loss, d_lse, d_da, d_dw,
+                        d_dbias, aligned256(ws), L, st);
+}
+
+// Both operators' host form (f32): the slot's own buffers and stream, device 0 of the context.
+int grad_host(rh_ctx* ctx, const float* a, int64_t rows, int64_t k, int64_t t_len, const float* w, int64_t n,
+              const float* bias, const int32_t* target, const int32_t* top_idx, const float* top_logits, int64_t n_top,
+              float temperature, const float* row_grad, float* loss, float* lse, float* da, float* dw, float* dbias) {
+    if (int rc = check_ctx(ctx)) return rc;
+    if (int rc = check_grad_shape(RH_DTYPE_F32, rows, k, n)) return rc;
+    if (int rc = check_rows(rows, t_len)) return rc;
+    if (dbias && !dw) return fail(RH_ERR_INVALID_ARG, "the bias gradient comes with the weight's: dw is null");
+    if (rows == 0) {
+        if (dw) std::fill(dw, dw + (size_t)n * (size_t)k, 0.0f);
+        if (dbias) std::fill(dbias, dbias + (size_t)n, 0.0f);
+        return RH_OK;
+    }
+    if (int rc = check_labels(target, top_idx, top_logits, n_top, temperature)) return rc;
+    if (!a || !w) return fail(RH_ERR_INVALID_ARG, "null input");
+    const int64_t entries = rows * (target ? 1 : n_top);
+    const int32_t* cls = target ? target : top_idx;
+    for (int64_t i = 0; i < entries; ++i)
+        if (cls[i] >= n)
+            return fail(RH_ERR_INVALID_ARG, "class " + std::to_string(cls[i]) + " of row " +
+                                                std::to_string(i / (target ? 1 : n_top)) + " is not below n = " +
+                                                std::to_string(n));
+    Slot& s = *ctx->slots[0];
+    std::lock_guard<std::mutex> lock(s.mu);
+    DeviceGuard guard;
+    RH_CUDA(cudaSetDevice(s.device));
+    size_t at = 0;
+    auto take = [&](size_t floats) {
+        const size_t here = at;
+        at += (floats * 4 + 255) / 256 * 256;
+        return here;
+    };
+    const size_t xf = (size_t)rows * (size_t)k, wf = (size_t)n * (size_t)k;
+    const size_t o_x = take(xf), o_w = take(wf), o_b = take((size_t)n), o_c = take((size_t)entries),
+                 o_t = take(target ? 0 : (size_t)entries), o_g = take((size_t)rows);
+    RH_CUDA(s.loss_in.ensure(at));
+    at = 0;
+    const size_t r_l = take((size_t)rows), r_e = take((size_t)rows), r_x = take(da ? xf : 0), r_w = take(dw ? wf : 0),
+                 r_b = take((size_t)n);
+    RH_CUDA(s.loss_out.ensure(at));
+    uint8_t *in = (uint8_t*)s.loss_in.p, *out = (uint8_t*)s.loss_out.p;
+    auto up = [&](size_t o, const void* p, size_t count) {
+        return p && count ? cudaMemcpyAsync(in + o, p, count * 4, cudaMemcpyHostToDevice, s.stream) : cudaSuccess;
+    };
+    RH_CUDA(up(o_x, a, xf));
+    RH_CUDA(up(o_w, w, wf));
+    RH_CUDA(up(o_b, bias, (size_t)n));
+    RH_CUDA(up(o_c, cls, (size_t)entries));
+    RH_CUDA(up(o_t, target ? nullptr : top_logits, (size_t)entries));
+    RH_CUDA(up(o_g, row_grad, (size_t)rows));
+    const rh::LossLabels lab = loss_labels(target ? (const int32_t*)(in + o_c) : nullptr, (const int32_t*)(in + o_c),
+                                           (const float*)(in + o_t), n_top, temperature, n);
+    const LossLayout L = loss_layout(true, rows, k, n, lab.n_top, s.sms);
+    RH_CUDA(s.loss_ws.ensure(L.total));
+    if (int rc = enqueue_grad(ctx, s, RH_DTYPE_F32, in + o_x, rows, k, t_len, in + o_w, n,
+                              bias ? (const float*)(in + o_b) : nullptr, lab,
+                              row_grad ? (const float*)(in + o_g) : nullptr, (float*)(out + r_l), (float*)(out + r_e),
+                              da ? out + r_x : nullptr, dw ? out + r_w : nullptr, dbias ? (float*)(out + r_b) : nullptr,
+                              aligned256(s.loss_ws.p), L, s.stream))
+        return rc;
+    auto down = [&](void* p, size_t o, size_t count) {
+        return p ? cudaMemcpyAsync(p, out + o, count * 4, cudaMemcpyDeviceToHost, s.stream) : cudaSuccess;
+    };
+    RH_CUDA(down(loss, r_l, (size_t)rows));
+    RH_CUDA(down(lse, r_e, (size_t)rows));
+    RH_CUDA(down(da, r_x, xf));
+    RH_CUDA(down(dw, r_w, wf));
+    RH_CUDA(down(dbias, r_b, (size_t)n));
+    return sync_and_check(s);
+}
+
+// Scores of a packed head: the decode kernel's (argmax, probability) at temperature T, then the
+// labels' logits. Workspace: idx, prob, the split's partial rows and, for T != 1, a class table.
+struct ScoreLayout {
+    size_t idx, prob, table, partial, total;
+};
+ScoreLayout score_layout(const rh_weight* w, int64_t rows, int sms) {
+    ScoreLayout L;
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += (bytes + 255) / 256 * 256;
+        return here;
+    };
+    int n_mblocks, whole, splits, cps, grid;
+    plan(rows, w->g.n_chunks, sms, n_mblocks, whole, splits, cps, grid);
+    const int64_t split = splits > 1 ? rows - (int64_t)whole * rh::kBlockM : 0;
+    L.idx = take((size_t)rows * 4);
+    L.prob = take((size_t)rows * 4);
+    L.table = take((size_t)w->g.n_chunks * rh::kCtabFloats * 4);
+    L.partial = take((size_t)splits * (size_t)split * sizeof(float4));
+    L.total = at + 256;
+    return L;
+}
+
+int enqueue_score(rh_ctx* ctx, const rh_weight* w, Slot& s, const rh_weight::Per& pw, const float* d_a, int64_t rows,
+                  int64_t t_len, const rh::LossLabels& lab, float* d_loss, float* d_lse, uint8_t* ws,
+                  const ScoreLayout& L, cudaStream_t st) {
+    int grid;
+    rh::HeadParams p = head_params(ctx, w, s, pw, d_a, rows, t_len, (int32_t*)(ws + L.idx), (float*)(ws + L.prob), nullptr,
+                                   grid);
+    p.partial = (float4*)(ws + L.partial);
+    if (lab.temp != 1.0f) {
+        RH_CUDA(rh::launch_loss_table(pw.ctab, (long long)w->g.n_chunks * rh::kCtabFloats, lab.inv_temp,
+                                      (float*)(ws + L.table), st));
+        s.launches++;
+        p.ctab = (const float*)(ws + L.table);
+    }
+    if (int rc = launch_head_and_merge(s, p, false, grid, st)) return rc;
+    rh::LossScoreParams q{};
+    q.x = d_a;
+    q.rows = rows;
+    q.t_len = t_len;
+    q.k = (int)w->k;
+    q.lab = lab;
+    q.tiles = pw.tiles;
+    q.ctab = pw.ctab;
+    q.form = w->f32 ? 2 : w->compact ? 1 : 0;
+    q.idx = p.idx;
+    q.prob = p.prob;
+    q.loss = d_loss;
+    q.lse = d_lse;
+    q.status = s.d_status;
+    RH_CUDA(rh::launch_loss_score(q, st));
+    s.launches++;
+    return RH_OK;
+}
+
+int score_device(rh_ctx* ctx, const rh_weight* w, int slot, const float* d_a, int64_t rows, int64_t t_len,
+                 const int32_t* d_target, const int32_t* d_top_idx, const float* d_top_logits, int64_t n_top,
+                 float temperature, float* d_loss, float* d_lse, void* ws, int64_t ws_bytes, void* stream) {
+    if (int rc = check_ctx(ctx)) return rc;
+    if (!w) return fail(RH_ERR_INVALID_ARG, "null weight");
+    if (slot < 0 || slot >= (int)ctx->slots.size()) return fail(RH_ERR_INVALID_ARG, "slot out of range");
+    if (int rc = check_rows(rows, t_len)) return rc;
+    if (rows == 0) return RH_OK;
+    if (int rc = check_labels(d_target, d_top_idx, d_top_logits, n_top, temperature)) return rc;
+    if (!d_a) return fail(RH_ERR_INVALID_ARG, "null device pointer");
+    Slot& s = *ctx->slots[slot];
+    const ScoreLayout L = score_layout(w, rows, s.sms);
+    if (int rc = check_workspace(ws, ws_bytes, L.total)) return rc;
+    std::lock_guard<std::mutex> lock(s.mu);
+    DeviceGuard guard;
+    RH_CUDA(cudaSetDevice(s.device));
+    const rh_weight::Per* pw = weight_on(w, s.device);
+    if (!pw) return fail(RH_ERR_INVALID_ARG, "weight was not packed for this device");
+    return enqueue_score(ctx, w, s, *pw, d_a, rows, t_len,
+                         loss_labels(d_target, d_top_idx, d_top_logits, n_top, temperature, w->n), d_loss, d_lse,
+                         aligned256(ws), L, (cudaStream_t)stream);
+}
+
+int score_host(rh_ctx* ctx, const rh_weight* w, const float* a, int64_t rows, int64_t k, int64_t t_len,
+               const int32_t* target, const int32_t* top_idx, const float* top_logits, int64_t n_top, float temperature,
+               float* loss, float* lse) {
+    if (int rc = check_ctx(ctx)) return rc;
+    if (!w) return fail(RH_ERR_INVALID_ARG, "null weight");
+    if (k != w->k)
+        return fail(RH_ERR_INVALID_ARG,
+                    "Inner dimensions must match: " + std::to_string(k) + " != " + std::to_string(w->k));
+    if (int rc = check_rows(rows, t_len)) return rc;
+    if (rows == 0) return RH_OK;
+    if (int rc = check_labels(target, top_idx, top_logits, n_top, temperature)) return rc;
+    if (!a) return fail(RH_ERR_INVALID_ARG, "null input");
+    const int64_t per = target ? 1 : n_top, entries = rows * per;
+    const int32_t* cls = target ? target : top_idx;
+    for (int64_t i = 0; i < entries; ++i)
+        if (cls[i] >= w->n)
+            return fail(RH_ERR_INVALID_ARG, "class " + std::to_string(cls[i]) + " of row " + std::to_string(i / per) +
+                                                " is not below n = " + std::to_string(w->n));
+    Slot& s = *ctx->slots[0];
+    std::lock_guard<std::mutex> lock(s.mu);
+    DeviceGuard guard;
+    RH_CUDA(cudaSetDevice(s.device));
+    const rh_weight::Per* pw = weight_on(w, s.device);
+    if (!pw) return fail(RH_ERR_INVALID_ARG, "weight was not packed for this context's devices");
+    const ScoreLayout L = score_layout(w, rows, s.sms);
+    RH_CUDA(s.loss_ws.ensure(L.total));
+    const size_t x_bytes = (size_t)rows * (size_t)k * 4, e_bytes = ((size_t)entries * 4 + 255) / 256 * 256;
+    const size_t r_bytes = ((size_t)rows * 4 + 255) / 256 * 256;
+    RH_CUDA(s.loss_in.ensure(x_bytes + 256 + 2 * e_bytes));
+    RH_CUDA(s.loss_out.ensure(2 * r_bytes));
+    uint8_t *in = (uint8_t*)s.loss_in.p, *out = (uint8_t*)s.loss_out.p;
+    const size_t o_c = (x_bytes + 255) / 256 * 256, o_t = o_c + e_bytes;
+    RH_CUDA(cudaMemcpyAsync(in, a, x_bytes, cudaMemcpyHostToDevice, s.stream));
+    RH_CUDA(cudaMemcpyAsync(in + o_c, cls, (size_t)entries * 4, cudaMemcpyHostToDevice, s.stream));
+    if (!target) RH_CUDA(cudaMemcpyAsync(in + o_t, top_logits, (size_t)entries * 4, cudaMemcpyHostToDevice, s.stream));
+    const rh::LossLabels lab = loss_labels(target ? (const int32_t*)(in + o_c) : nullptr, (const int32_t*)(in + o_c),
+                                           (const float*)(in + o_t), n_top, temperature, w->n);
+    if (int rc = enqueue_score(ctx, w, s, *pw, (const float*)in, rows, t_len, lab, (float*)out, (float*)(out + r_bytes),
+                               aligned256(s.loss_ws.p), L, s.stream))
+        return rc;
+    if (loss) RH_CUDA(cudaMemcpyAsync(loss, out, (size_t)rows * 4, cudaMemcpyDeviceToHost, s.stream));
+    if (lse) RH_CUDA(cudaMemcpyAsync(lse, out + r_bytes, (size_t)rows * 4, cudaMemcpyDeviceToHost, s.stream));
+    return sync_and_check(s);
+}
+
 }  // namespace
 
 extern "C" {
@@ -837,6 +1324,7 @@ int rh_ctx_create(const int* devices, int n_devices, rh_ctx** out) {
         s->sms = prop.multiProcessorCount;
         RH_CUDA(cudaSetDevice(d));
         RH_CUDA(rh::head_kernel_setup());
+        RH_CUDA(rh::loss_kernel_setup());
         RH_CUDA(cudaStreamCreateWithFlags(&s->stream, cudaStreamNonBlocking));
         RH_CUDA(cudaStreamCreateWithFlags(&s->copy_stream, cudaStreamNonBlocking));
         RH_CUDA(cudaEventCreateWithFlags(&s->copied, cudaEventDisableTiming));
@@ -1467,6 +1955,111 @@ int rh_rec_preprocess_device(rh_ctx* ctx, int slot, const uint8_t* d_rgb, int64_
     RH_CUDA(cudaEventRecord(s.pre_done, st));
     s.launches += 2;
     return RH_OK;
+}
+
+// ------------------------------------------------------------------- training losses
+
+int64_t rh_head_score_workspace_bytes(rh_ctx* ctx, const rh_weight* w, int slot, int64_t rows) {
+    if (check_ctx(ctx)) return -1;
+    if (!w || slot < 0 || slot >= (int)ctx->slots.size() || check_rows(rows, 0)) {
+        fail(RH_ERR_INVALID_ARG, "null weight, slot out of range or bad row count");
+        return -1;
+    }
+    return (int64_t)score_layout(w, rows, ctx->slots[slot]->sms).total;
+}
+
+int rh_head_cross_entropy(rh_ctx* ctx, const rh_weight* w, const float* a, int64_t rows, int64_t k, int64_t t_len,
+                          const int32_t* target, float* loss, float* lse) {
+    return guarded([&]() -> int {
+        if (rows > 0 && !target) return fail(RH_ERR_INVALID_ARG, "null targets");
+        return score_host(ctx, w, a, rows, k, t_len, target, nullptr, nullptr, 1, 1.0f, loss, lse);
+    });
+}
+
+int rh_head_cross_entropy_device(rh_ctx* ctx, const rh_weight* w, int slot, const float* d_a, int64_t rows,
+                                 int64_t t_len, const int32_t* d_target, float* d_loss, float* d_lse,
+                                 void* d_workspace, int64_t workspace_bytes, void* stream) {
+    return guarded([&]() -> int {
+        if (rows > 0 && !d_target) return fail(RH_ERR_INVALID_ARG, "null targets");
+        return score_device(ctx, w, slot, d_a, rows, t_len, d_target, nullptr, nullptr, 1, 1.0f, d_loss, d_lse,
+                            d_workspace, workspace_bytes, stream);
+    });
+}
+
+int rh_head_distill(rh_ctx* ctx, const rh_weight* w, const float* a, int64_t rows, int64_t k, int64_t t_len,
+                    const int32_t* top_idx, const float* top_logits, int64_t n_top, float temperature, float* loss,
+                    float* lse) {
+    return guarded([&]() -> int {
+        return score_host(ctx, w, a, rows, k, t_len, nullptr, top_idx, top_logits, n_top, temperature, loss, lse);
+    });
+}
+
+int rh_head_distill_device(rh_ctx* ctx, const rh_weight* w, int slot, const float* d_a, int64_t rows, int64_t t_len,
+                           const int32_t* d_top_idx, const float* d_top_logits, int64_t n_top, float temperature,
+                           float* d_loss, float* d_lse, void* d_workspace, int64_t workspace_bytes, void* stream) {
+    return guarded([&]() -> int {
+        return score_device(ctx, w, slot, d_a, rows, t_len, nullptr, d_top_idx, d_top_logits, n_top, temperature, d_loss,
+                            d_lse, d_workspace, workspace_bytes, stream);
+    });
+}
+
+int64_t rh_head_grad_workspace_bytes(rh_ctx* ctx, int slot, int dtype, int64_t rows, int64_t k, int64_t n,
+                                     int64_t n_top) {
+    if (check_ctx(ctx)) return -1;
+    if (slot < 0 || slot >= (int)ctx->slots.size()) {
+        fail(RH_ERR_INVALID_ARG, "slot out of range");
+        return -1;
+    }
+    if (check_grad_shape(dtype, rows, k, n)) return -1;
+    if (n_top < 0 || n_top > rh::kLossMaxTop) {
+        fail(RH_ERR_INVALID_ARG, "n_top = " + std::to_string(n_top) + " is outside [0, 64]");
+        return -1;
+    }
+    return (int64_t)loss_layout(dtype == RH_DTYPE_F32, rows, k, n, std::max<int64_t>(n_top, 1), ctx->slots[slot]->sms).total;
+}
+
+int rh_head_cross_entropy_grad(rh_ctx* ctx, const float* a, int64_t rows, int64_t k, int64_t t_len, const float* w,
+                               int64_t n, const float* bias, const int32_t* target, const float* row_grad, float* loss,
+                               float* lse, float* da, float* dw, float* dbias) {
+    return guarded([&]() -> int {
+        if (rows > 0 && !target) return fail(RH_ERR_INVALID_ARG, "null targets");
+        return grad_host(ctx, a, rows, k, t_len, w, n, bias, target, nullptr, nullptr, 1, 1.0f, row_grad, loss, lse, da,
+                         dw, dbias);
+    });
+}
+
+int rh_head_cross_entropy_grad_device(rh_ctx* ctx, int slot, int dtype, const void* d_a, int64_t rows, int64_t k,
+                                      int64_t t_len, const void* d_w, int64_t n, const float* d_bias,
+                                      const int32_t* d_target, const float* d_row_grad, float* d_loss, float* d_lse,
+                                      void* d_da, void* d_dw, float* d_dbias, void* d_workspace,
+                                      int64_t workspace_bytes, void* stream) {
+    return guarded([&]() -> int {
+        if (rows > 0 && !d_target) return fail(RH_ERR_INVALID_ARG, "null targets");
+        return grad_device(ctx, slot, dtype, d_a, rows, k, t_len, d_w, n, d_bias, d_target, nullptr, nullptr, 1, 1.0f,
+                           d_row_grad, d_loss, d_lse, d_da, d_dw, d_dbias, d_workspace, workspace_bytes, stream);
+    });
+}
+
+int rh_head_distill_grad(rh_ctx* ctx, const float* a, int64_t rows, int64_t k, int64_t t_len, const float* w, int64_t n,
+                         const float* bias, const int32_t* top_idx, const float* top_logits, int64_t n_top,
+                         float temperature, const float* row_grad, float* loss, float* lse, float* da, float* dw,
+                         float* dbias) {
+    return guarded([&]() -> int {
+        return grad_host(ctx, a, rows, k, t_len, w, n, bias, nullptr, top_idx, top_logits, n_top, temperature, row_grad,
+                         loss, lse, da, dw, dbias);
+    });
+}
+
+int rh_head_distill_grad_device(rh_ctx* ctx, int slot, int dtype, const void* d_a, int64_t rows, int64_t k,
+                                int64_t t_len, const void* d_w, int64_t n, const float* d_bias,
+                                const int32_t* d_top_idx, const float* d_top_logits, int64_t n_top, float temperature,
+                                const float* d_row_grad, float* d_loss, float* d_lse, void* d_da, void* d_dw,
+                                float* d_dbias, void* d_workspace, int64_t workspace_bytes, void* stream) {
+    return guarded([&]() -> int {
+        return grad_device(ctx, slot, dtype, d_a, rows, k, t_len, d_w, n, d_bias, nullptr, d_top_idx, d_top_logits, n_top,
+                           temperature, d_row_grad, d_loss, d_lse, d_da, d_dw, d_dbias, d_workspace, workspace_bytes,
+                           stream);
+    });
 }
 
 }  // extern "C"
