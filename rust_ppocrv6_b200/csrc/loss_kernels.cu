@@ -358,12 +358,15 @@ __global__ void __launch_bounds__(256) loss_pack_kernel(const __grid_constant__ 
 // ------------------------------------------------------------------------------- main pass
 namespace {
 
-// Warps: 0 producer, 1 tensor-core issuer (and TMEM), 2-3 idle, 4-7 and 8-11 two softmax
-// warpgroups that take the streamed tiles in turn (tile i of a unit: warpgroup i % 2, score
-// buffer i % 2).
-constexpr int kMainThreads = 384;
-constexpr int kCtrlRegs = 56, kSoftRegs = 224;  // 128 x 72 + 256 x 216 = 384 x 168: the launch's own registers
-static_assert(128 * kCtrlRegs + 256 * kSoftRegs <= kMainThreads * 168, "register split");
+// Warps: 0 producer, 1 tensor-core issuer (and TMEM), 2-3 idle; two softmax warpgroups (warps 4-7
+// and 8-11) that take the streamed tiles in turn (tile i of a unit: warpgroup i % 2, score buffer
+// i % 2); two adding warpgroups (12-15 and 16-19), 64 features of every tile's second product each.
+// Softmax and adding are apart so that a softmax warpgroup goes on to its next tile without waiting
+// for the tensor core to use its last.
+constexpr int kMainThreads = 640;
+constexpr int kLaunchRegs = 96;  // 65,536 registers / 640 threads
+constexpr int kCtrlRegs = 48, kSoftRegs = 112, kAddRegs = 104;
+static_assert(128 * kCtrlRegs + 256 * kSoftRegs + 256 * kAddRegs <= kMainThreads * kLaunchRegs, "register split");
 
 template <bool F32>
 struct Ring {
@@ -373,10 +376,11 @@ struct Ring {
 constexpr uint32_t kMOffTab = 196608;             // per stage 1 KB: the tile's column table
 constexpr uint32_t kMOffBars = kMOffTab + 6 * 1024;
 constexpr uint32_t kMOffMisc = kMOffBars + 256;   // [0] TMEM base, [1] abort flag
-constexpr uint32_t kMOffMs = kMOffMisc + 64;      // [128] float2: warpgroup 1's row state
+constexpr uint32_t kMOffMs = kMOffMisc + 64;      // [2][128] float2: the softmax warpgroups' row state
+constexpr uint32_t kMOffRing = kMOffMs + 2048;    // [4 tiles][128] f32: offset of a tile's probabilities
 constexpr uint32_t kPatchRow = 20;                // floats per class row of a label patch (16 used:
                                                   // the 16-byte rows then fall on distinct banks)
-constexpr uint32_t kMOffPatch = kMOffMs + 1024;   // [8 warps][32][kPatchRow] f32
+constexpr uint32_t kMOffPatch = kMOffRing + 2048;  // [8 warps][32][kPatchRow] f32
 constexpr uint32_t kMSmemUsed = kMOffPatch + 8 * 32 * kPatchRow * 4;
 constexpr uint32_t kMSmemBytes = kMSmemUsed + 1024;
 static_assert(Ring<true>::kStage * Ring<true>::kStages <= kMOffTab && Ring<false>::kStage * Ring<false>::kStages <= kMOffTab,
@@ -384,15 +388,17 @@ static_assert(Ring<true>::kStage * Ring<true>::kStages <= kMOffTab && Ring<false
 static_assert(kMSmemBytes <= 227 * 1024, "shared memory per CTA");
 
 constexpr int kLBarFull = 0;               // [6] tile and column table landed
-constexpr int kLBarEmpty = 6;              // [6] the tile's products done, its warpgroup done with the table
+constexpr int kLBarEmpty = 6;              // [6] the tile's products done, its softmax warps done with the table
 constexpr int kLBarAFull = 12;             // own operand in TMEM
 constexpr int kLBarAEmpty = 13;            // the unit's products done with it
 constexpr int kLBarSFull = 14;             // [2] scores of a tile in TMEM
 constexpr int kLBarPFull = 16;             // [2] its probabilities in their place
-constexpr int kLBarOFull = 18;             // [2] (by warpgroup) the tile's second product in TMEM
-constexpr int kLBarOEmpty = 20;            // [2] added up, the buffer free
-constexpr int kLBarMerge = 22;             // warpgroup 1's state of a unit staged
-constexpr int kLBarDone = 23;              // every product retired (teardown)
+constexpr int kLBarOFull = 18;             // the tile's second product in TMEM
+constexpr int kLBarOEmpty = 19;            // added up, the buffer free
+constexpr int kLBarRing = 20;              // [4] a tile's offsets written
+constexpr int kLBarMsFull = 24;            // row states of a unit written
+constexpr int kLBarMsEmpty = 25;           // and read
+constexpr int kLBarDone = 26;              // every product retired (teardown)
 static_assert(kLBarDone < 32, "barrier area");
 
 // TMEM columns: own operand (hi | lo), score buffers, second product
@@ -494,7 +500,7 @@ __device__ __forceinline__ void window_load(LabelWindow& w, const int2* ent, int
 }  // namespace
 
 // Units (own tile, range of streamed tiles), persistent over the grid. Per streamed tile: scores
-// S = own . tile^T (tensor core, own operand in TMEM), the softmax warpgroup turns them into
+// S = own . tile^T (tensor core, own operand in TMEM), a softmax warpgroup turns them into
 // probabilities (row pass: against the running maximum; weight pass: 2^(s - lse) times the rows'
 // gradient factors, less the labels' shares) in the same TMEM columns, and a second product
 // O = P . tile reads the same tile the other way round. O is added to registers tile by tile: the
@@ -525,10 +531,12 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar(kLBarSFull + i), 1);
             mbar_init(bar(kLBarPFull + i), 4);
-            mbar_init(bar(kLBarOFull + i), 1);
-            mbar_init(bar(kLBarOEmpty + i), 4);
         }
-        mbar_init(bar(kLBarMerge), 128);
+        mbar_init(bar(kLBarOFull), 1);
+        mbar_init(bar(kLBarOEmpty), 8);
+        for (int i = 0; i < 4; ++i) mbar_init(bar(kLBarRing + i), 4);
+        mbar_init(bar(kLBarMsFull), 256);
+        mbar_init(bar(kLBarMsEmpty), 128);
         mbar_init(bar(kLBarDone), 1);
         misc[1] = 0u;
         fence_mbar_init();
@@ -543,6 +551,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = misc[0];
+    const int feat = 16 * p.ksteps;
 
     if (warp < 4) {
         setmaxnreg_dec<kCtrlRegs>();
@@ -570,31 +579,26 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                 loss_drain(bar(kLBarFull + s), ((issued - 1 - s) / kStages) & 1u, wt);
         } else if (warp == 1) {
             // ---------------------------------------------------------- tensor-core issuer
+            // Ring positions advance by increments: this loop is the tensor core's only feed.
             const uint32_t id_s = idesc_16b(!F32, false, 128, 128);
-            const uint32_t id_o = idesc_16b(!F32, true, 128, 16u * (uint32_t)p.ksteps);
+            const uint32_t id_o = idesc_16b(!F32, true, 128, (uint32_t)feat);
             const uint64_t k_desc = smem_desc_k_sw128(base), mn_desc = smem_desc_mn_sw128(base);
-            uint32_t cc = 0, uc = 0, pu[2] = {0, 0}, du[2] = {0, 0};
-            auto scores = [&](uint32_t i) -> bool {  // S of the unit's tile i
-                const uint32_t g = cc + i, s = g % kStages;
-                if (!loss_wait(bar(kLBarFull + s), (g / kStages) & 1u, wt, 102)) return false;
+            constexpr uint64_t kStageDesc = kStage >> 4, kLoDesc = kLossImage >> 4;
+            uint32_t ss = 0, sph = 0;   // stage (and phase) of the next scores
+            uint32_t os = 0, oph = 1;   // stage of the next second product; phase of its buffer's release
+            uint32_t pph = 0, uc = 0;   // bit w: phase of warpgroup w's next probabilities
+            auto scores = [&](uint32_t w) -> bool {
+                if (!loss_wait(bar(kLBarFull + ss), sph, wt, 102)) return false;
                 tc_fence_after();
-                const uint32_t d = tmem + kTS + 128u * (i & 1u);
-                const uint64_t b = k_desc + (uint64_t)(s * (kStage >> 4));
-                uint32_t acc = 0;
-                auto run = [&](uint32_t a_col, uint32_t b_off) {
-                    for (int st = 0; st < p.ksteps; ++st) {
-                        mma_f16_ts_warp(d, tmem + kTOwn + a_col + 8u * st,
-                                        b + ((b_off + (uint32_t)(st >> 2) * 16384u + (uint32_t)(st & 3) * 32u) >> 4),
-                                        id_s, acc);
-                        acc = 1;
-                    }
-                };
+                const uint32_t d = tmem + kTS + 128u * w, a = tmem + kTOwn;
+                const uint64_t b = k_desc + ss * kStageDesc;
                 if (F32) {
-                    run(64, 0);
-                    run(0, kLossImage);
+                    mma_k_steps_warp(d, a + 64u, b, id_s, 0u, p.ksteps);
+                    mma_k_steps_warp(d, a, b + kLoDesc, id_s, 1u, p.ksteps);
                 }
-                run(0, 0);
-                mma_commit_warp(bar(kLBarSFull + (int)(i & 1u)));
+                mma_k_steps_warp(d, a, b, id_s, F32 ? 1u : 0u, p.ksteps);
+                mma_commit_warp(bar(kLBarSFull + (int)w));
+                if (++ss == kStages) ss = 0u, sph ^= 1u;
                 return true;
             };
             bool ok = true;
@@ -606,60 +610,62 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                 tc_fence_after();
                 ok = scores(0) && (n < 2 || scores(1));
                 for (uint32_t i = 0; ok && i < n; ++i) {
-                    const uint32_t w = i & 1u, s = (cc + i) % kStages;
-                    ok = loss_wait(bar(kLBarPFull + (int)w), pu[w]++ & 1u, wt, 104);
+                    const uint32_t w = i & 1u;
+                    ok = loss_wait(bar(kLBarPFull + (int)w), (pph >> w) & 1u, wt, 104);
+                    pph ^= 1u << w;
                     if (!ok) break;
                     if (with_o) {
-                        if (i > 0) {  // the other warpgroup has added the previous tile's product up
-                            ok = loss_wait(bar(kLBarOEmpty + (int)(w ^ 1u)), (du[w ^ 1u] - 1u) & 1u, wt, 105);
-                            if (!ok) break;
-                        }
+                        ok = loss_wait(bar(kLBarOEmpty), oph, wt, 105);  // the previous tile's product is added up
+                        oph ^= 1u;
+                        if (!ok) break;
                         tc_fence_after();
-                        const uint64_t b = mn_desc + (uint64_t)(s * (kStage >> 4));
-                        const uint32_t a = tmem + kTS + 128u * w;
-                        uint32_t acc = 0;
-                        auto run = [&](uint32_t a_col, uint32_t b_off) {
-#pragma unroll
-                            for (uint32_t j = 0; j < 8; ++j) {  // 16 rows of the tile a step
-                                mma_f16_ts_warp(tmem + kTO, a + a_col + 16u * j,
-                                                b + ((b_off + 2048u * j) >> 4), id_o, acc);
-                                acc = 1;
-                            }
-                        };
+                        const uint64_t b = mn_desc + os * kStageDesc;
+                        const uint32_t a = tmem + kTS + 128u * w, d = tmem + kTO;
                         if (F32) {
-                            run(8, 0);
-                            run(0, kLossImage);
+                            mma_row_steps_warp(d, a + 8u, b, id_o, 0u);
+                            mma_row_steps_warp(d, a, b + kLoDesc, id_o, 1u);
                         }
-                        run(0, 0);
-                        mma_commit_warp(bar(kLBarOFull + (int)w));
-                        ++du[w];
+                        mma_row_steps_warp(d, a, b, id_o, F32 ? 1u : 0u);
+                        mma_commit_warp(bar(kLBarOFull));
                     }
-                    mma_commit_warp(bar(kLBarEmpty + (int)s));
+                    mma_commit_warp(bar(kLBarEmpty + (int)os));
+                    if (++os == kStages) os = 0u;
                     // Tile i + 2 takes the score buffer of tile i, whose probabilities the product
                     // above reads: the tensor core runs one thread's products in order.
-                    if (i + 2 < n) ok = scores(i + 2);
+                    if (i + 2 < n) ok = scores(w);
                 }
                 if (!ok) break;
-                cc += n;
                 mma_commit_warp(bar(kLBarAEmpty));
             }
             mma_commit_warp(bar(kLBarDone));
             loss_drain(bar(kLBarDone), 0u, wt);
         }
-    } else {
+    } else if (warp < 12) {
         setmaxnreg_inc<kSoftRegs>();
         // ------------------------------------------------------------- softmax warpgroups
         const uint32_t g = (uint32_t)(warp - 4) >> 2;
         const int quad = warp & 3, r = quad * 32 + lane;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-        float2* ms = reinterpret_cast<float2*>(gbase + kMOffMs);
         const uint32_t patch = base + kMOffPatch + (uint32_t)(warp - 4) * 32u * kPatchRow * 4u;
-        const int feat = 16 * p.ksteps;
+        const uint32_t t_s = tmem + lanes + kTS + 128u * g;
+        float* ring = reinterpret_cast<float*>(gbase + kMOffRing);
         uint32_t cc = 0, uc = 0, uses = 0;
         bool ok = true;
         for (int u = blockIdx.x; ok && lunit_exists(u, p); u += gridDim.x, ++uc) {
             const LUnit U = lunit(u, p);
             const uint32_t n = (uint32_t)(U.c1 - U.c0);
+            // labels of this warpgroup's first tile (weight pass): range, then entries
+            LabelWindow lw{make_int2(kNoLabel, 0), 0, 0};
+            auto label_range = [&](int c, int& a, int& b) {
+                const int32_t* o = p.sp_off + (size_t)c * (p.own_tiles + 1) + U.own;
+                a = __ldg(o);
+                b = __ldg(o + 1);
+            };
+            auto label_base = [&](int c) { return p.sp_ent + (size_t)c * 128 * p.n_top; };
+            if (WPASS && g < n) {
+                label_range(U.c0 + (int)g, lw.next, lw.end);
+                window_load(lw, label_base(U.c0 + (int)g), lane);
+            }
             // own operand -> TMEM: warpgroup g takes K slots 64 g .. 64 g + 63 of the lane's row
             ok = loss_wait(bar(kLBarAEmpty), (uc & 1u) ^ 1u, wt, 106);
             if (!ok) break;
@@ -684,49 +690,37 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
             const float own_mul = F32 ? p.logit_scale * __ldg(p.own_scale + U.own) : p.logit_scale;
             const float lane_e = WPASS ? __ldg(p.lane_e + (size_t)U.own * 128 + r) : 0.0f;
             float off = -CUDART_INF_F, sum = 0.0f, carry = 0.0f;  // weight pass: sum + carry = bias gradient
-            float2 acc[64];
-#pragma unroll
-            for (int i = 0; i < 64; ++i) acc[i] = make_float2(0.f, 0.f);
-
             for (uint32_t i = g; i < n; i += 2, ++uses) {
                 const int c = U.c0 + (int)i;
                 const uint32_t s = (cc + i) % kStages;
                 const uint32_t tab = base + kMOffTab + s * 1024u;
                 const float str_s = F32 ? __ldg(p.str_scale + c) : 1.0f;
-                float o_mul = str_s;  // value of one unit of the second product
-                LabelWindow lw{make_int2(kNoLabel, 0), 0, 0};
-                const int2* ent = nullptr;
-                if (WPASS) {
-                    if (F32) o_mul *= __ldg(p.g_scale + c);
-                    const int32_t* o = p.sp_off + (size_t)c * (p.own_tiles + 1) + U.own;
-                    ent = p.sp_ent + (size_t)c * 128 * p.n_top;
-                    lw.next = __ldg(o);
-                    lw.end = __ldg(o + 1);
-                    if (lw.next < lw.end) window_load(lw, ent, lane);
-                } else if (F32) {
-                    o_mul *= 1.0f / 16384.0f;  // probabilities are stored times 2^14
-                }
+                const float gs = WPASS && F32 ? __ldg(p.g_scale + c) : 1.0f;
+                // the next tile's label range is fetched under this tile, its entries at this tile's end
+                int next_a = 0, next_b = 0;
+                if (WPASS && i + 2 < n) label_range(c + 2, next_a, next_b);
                 const float2 mul = make_float2(own_mul * str_s, own_mul * str_s);
-                const uint32_t t_s = tmem + lanes + kTS + 128u * g;
                 ok = loss_wait(bar(kLBarSFull + (int)g), uses & 1u, wt, 107);
                 // the column table came with the tile: its barrier has passed, but this warp has to
                 // observe it before it reads what the copy wrote
                 ok = ok && loss_wait(bar(kLBarFull + s), ((cc + i) / kStages) & 1u, wt, 108);
                 if (!ok) break;
                 tc_fence_after();
-                float corr = 1.0f;
+                uint32_t v[2][16];
+                tmem_ld32x32b_x16(t_s, v[0]);
                 if constexpr (!WPASS) {
                     float top = -CUDART_INF_F;
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        uint32_t v[32];
-                        tmem_ld32x32b_x32_wait(t_s + 32u * q, v);
+                    for (int q = 0; q < 8; ++q) {
+                        tmem_ld_wait16(v[q & 1]);
+                        tmem_ld32x32b_x16(t_s + 16u * ((q + 1) & 7), v[(q + 1) & 1]);  // at the end: the first again
+                        const uint32_t(&x)[16] = v[q & 1];
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            const float4 e = lds128(tab + 4u * (32 * q + j));
-                            const float2 a = __ffma2_rn(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), mul,
+                        for (int j = 0; j < 16; j += 4) {
+                            const float4 e = lds128(tab + 4u * (16 * q + j));
+                            const float2 a = __ffma2_rn(make_float2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), mul,
                                                         make_float2(e.x, e.y));
-                            const float2 b = __ffma2_rn(make_float2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])),
+                            const float2 b = __ffma2_rn(make_float2(__uint_as_float(x[j + 2]), __uint_as_float(x[j + 3])),
                                                         mul, make_float2(e.z, e.w));
                             top = max3f(top, a.x, a.y);
                             top = max3f(top, b.x, b.y);
@@ -735,22 +729,24 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                     const float m = fmaxf(off, top);
                     // nothing visible yet (every class masked): any finite offset gives 2^-inf = 0
                     const float m0 = m == -CUDART_INF_F ? 0.0f : m;
-                    corr = off == -CUDART_INF_F ? 0.0f : ex2_approx(off - m0);
+                    const float corr = off == -CUDART_INF_F ? 0.0f : ex2_approx(off - m0);
                     off = m;
+                    if (with_o) ring[((cc + i) & 3u) * 128 + r] = m;
                     const float sub = F32 ? 14.0f - m0 : -m0;
                     const float2 sub2 = make_float2(sub, sub);
                     float2 ts = make_float2(0.f, 0.f);
 #pragma unroll
                     for (int q = 0; q < 8; ++q) {
-                        uint32_t v[16];
+                        tmem_ld_wait16(v[q & 1]);
+                        if (q < 7) tmem_ld32x32b_x16(t_s + 16u * (q + 1), v[(q + 1) & 1]);
+                        const uint32_t(&x)[16] = v[q & 1];
                         float2 pr[8];
-                        tmem_ld32x32b_x16_wait(t_s + 16u * q, v);
 #pragma unroll
                         for (int j = 0; j < 16; j += 4) {
                             const float4 e = lds128(tab + 4u * (16 * q + j));
-                            float2 a = __ffma2_rn(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), mul,
+                            float2 a = __ffma2_rn(make_float2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), mul,
                                                   make_float2(e.x, e.y));
-                            float2 b = __ffma2_rn(make_float2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])), mul,
+                            float2 b = __ffma2_rn(make_float2(__uint_as_float(x[j + 2]), __uint_as_float(x[j + 3])), mul,
                                                   make_float2(e.z, e.w));
                             a = __fadd2_rn(a, sub2);
                             b = __fadd2_rn(b, sub2);
@@ -764,19 +760,21 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                     sum = fmaf(sum, corr, t);
                 } else {
                     const float2 le = make_float2(lane_e, lane_e);
+                    const int2* ent = label_base(c);
                     float2 ts = make_float2(0.f, 0.f);
 #pragma unroll
                     for (int q = 0; q < 8; ++q) {
-                        uint32_t v[16];
+                        tmem_ld_wait16(v[q & 1]);
+                        if (q < 7) tmem_ld32x32b_x16(t_s + 16u * (q + 1), v[(q + 1) & 1]);
+                        const uint32_t(&x)[16] = v[q & 1];
                         float2 pr[8];
-                        tmem_ld32x32b_x16_wait(t_s + 16u * q, v);
 #pragma unroll
                         for (int j = 0; j < 16; j += 4) {
                             const float4 e = lds128(tab + 4u * (16 * q + j));
                             const float4 f = lds128(tab + 512u + 4u * (16 * q + j));
-                            float2 a = __ffma2_rn(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), mul,
+                            float2 a = __ffma2_rn(make_float2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), mul,
                                                   make_float2(e.x, e.y));
-                            float2 b = __ffma2_rn(make_float2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])), mul,
+                            float2 b = __ffma2_rn(make_float2(__uint_as_float(x[j + 2]), __uint_as_float(x[j + 3])), mul,
                                                   make_float2(e.z, e.w));
                             a = __fadd2_rn(a, le);
                             b = __fadd2_rn(b, le);
@@ -820,10 +818,13 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                         store_probs<F32>(t_s + 16u * q, pr);
                     }
                     // bias gradient with the rounding error carried (up to thousands of tiles)
-                    const float t = fmaf(ts.x + ts.y, F32 ? __ldg(p.g_scale + c) : 1.0f, carry);
+                    const float t = fmaf(ts.x + ts.y, gs, carry);
                     const float nsum = sum + t;
                     carry = t - (nsum - sum);
                     sum = nsum;
+                    lw.next = next_a;
+                    lw.end = next_b;
+                    window_load(lw, label_base(i + 2 < n ? c + 2 : c), lane);
                 }
                 tmem_st_wait();
                 tc_fence_before();
@@ -831,94 +832,102 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                 if (lane == 0) {
                     mbar_arrive(bar(kLBarPFull + (int)g));
                     mbar_arrive(bar(kLBarEmpty + (int)s));
-                }
-                if (with_o) {
-                    ok = loss_wait(bar(kLBarOFull + (int)g), uses & 1u, wt, 109);
-                    if (!ok) break;
-                    tc_fence_after();
-                    if (!WPASS && !__all_sync(0xffffffffu, corr == 1.0f)) {
-                        const float2 c2 = make_float2(corr, corr);
-#pragma unroll
-                        for (int j = 0; j < 64; ++j) acc[j] = __fmul2_rn(acc[j], c2);
-                    }
-                    const float2 om = make_float2(o_mul, o_mul);
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        if (32 * q < feat) {
-                            uint32_t v[32];
-                            tmem_ld32x32b_x32_wait(tmem + lanes + kTO + 32u * q, v);
-#pragma unroll
-                            for (int j = 0; j < 16; ++j)
-                                acc[16 * q + j] = __ffma2_rn(make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])),
-                                                             om, acc[16 * q + j]);
-                        }
-                    }
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(bar(kLBarOEmpty + (int)g));
+                    if (!WPASS && with_o) mbar_arrive(bar(kLBarRing + (int)((cc + i) & 3u)));
                 }
             }
             if (!ok) break;
             cc += n;
-            // Join the two warpgroups' states: warpgroup 1 leaves its sums in its own score buffer
-            // (free: its last product is done, and the next unit's scores need warpgroup 0, which
-            // reads them first, to have passed the own operand's barrier).
-            if (g == 1) {
-                ok = loss_wait(bar(kLBarAFull), uc & 1u, wt, 110);
-                if (!ok) break;
-                if (with_o) {
+            ok = loss_wait(bar(kLBarMsEmpty), (uc & 1u) ^ 1u, wt, 110);
+            if (!ok) break;
+            reinterpret_cast<float2*>(gbase + kMOffMs)[g * 128 + r] = WPASS ? make_float2(sum, carry) : make_float2(off, sum);
+            mbar_arrive(bar(kLBarMsFull));
+        }
+    } else {
+        setmaxnreg_inc<kAddRegs>();
+        // -------------------------------------------------------------- adding warpgroups
+        // acc is relative to `off`, the largest offset of the tiles so far (row pass; the two softmax
+        // warpgroups each keep their own running maximum).
+        const uint32_t g = (uint32_t)(warp - 12) >> 2;
+        const int quad = warp & 3, r = quad * 32 + lane;
+        const uint32_t t_o = tmem + ((uint32_t)(quad * 32) << 16) + kTO + 64u * g;
+        const volatile float* ring = reinterpret_cast<const volatile float*>(gbase + kMOffRing);
+        const int f0 = 64 * (int)g;
+        uint32_t cc = 0, uc = 0;
+        bool ok = true;
+        for (int u = blockIdx.x; ok && lunit_exists(u, p); u += gridDim.x, ++uc) {
+            const LUnit U = lunit(u, p);
+            float off = -CUDART_INF_F;
+            float2 acc[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) acc[i] = make_float2(0.f, 0.f);
+            if (with_o) {
+                for (int c = U.c0; c < U.c1; ++c, ++cc) {
+                    float om = F32 ? __ldg(p.str_scale + c) : 1.0f;  // value of one unit of the product
+                    if (F32) om *= WPASS ? __ldg(p.g_scale + c) : 1.0f / 16384.0f;
+                    float corr = 1.0f;
+                    if (!WPASS) {
+                        ok = loss_wait(bar(kLBarRing + (int)(cc & 3u)), (cc >> 2) & 1u, wt, 112);
+                        if (!ok) break;
+                        const float o = ring[(cc & 3u) * 128 + r];
+                        const float m = fmaxf(off, o);
+                        corr = off == m ? 1.0f : off == -CUDART_INF_F ? 0.0f : ex2_approx(off - m);
+                        if (o != m) om *= ex2_approx(o - m);
+                        off = m;
+                    }
+                    ok = loss_wait(bar(kLBarOFull), cc & 1u, wt, 109);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const bool grow = !WPASS && !__all_sync(0xffffffffu, corr == 1.0f);
+                    const float2 om2 = make_float2(om, om), c2 = make_float2(corr, corr);
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        if (32 * q < feat) {
-                            uint32_t v[32];
+                        if (f0 + 16 * q < feat) {
+                            uint32_t v[16];
+                            tmem_ld32x32b_x16(t_o + 16u * q, v);
+                            tmem_ld_wait16(v);
+                            if (grow) {
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) {
-                                v[2 * j] = __float_as_uint(acc[16 * q + j].x);
-                                v[2 * j + 1] = __float_as_uint(acc[16 * q + j].y);
+                                for (int j = 0; j < 8; ++j) acc[8 * q + j] = __fmul2_rn(acc[8 * q + j], c2);
                             }
-                            tmem_st32x32b_x32(tmem + lanes + kTS + 128u + 32u * q, v);
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                acc[8 * q + j] = __ffma2_rn(make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])),
+                                                            om2, acc[8 * q + j]);
                         }
                     }
-                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(kLBarOEmpty));
                 }
-                ms[r] = WPASS ? make_float2(sum, carry) : make_float2(off, sum);
-                tc_fence_before();
-                mbar_arrive(bar(kLBarMerge));
-            } else {
-                ok = loss_wait(bar(kLBarMerge), uc & 1u, wt, 111);
                 if (!ok) break;
-                tc_fence_after();
-                const float2 o = ms[r];
-                float k0 = 1.0f, k1 = 1.0f;
+                float* po = p.part_o + ((size_t)u * feat + f0) * 128 + r;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    if (f0 + 16 * q < feat) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            po[(size_t)(16 * q + 2 * j) * 128] = acc[8 * q + j].x;
+                            po[(size_t)(16 * q + 2 * j + 1) * 128] = acc[8 * q + j].y;
+                        }
+                    }
+                }
+            }
+            if (g == 0) {
+                ok = loss_wait(bar(kLBarMsFull), uc & 1u, wt, 111);
+                if (!ok) break;
+                const float2* ms = reinterpret_cast<const float2*>(gbase + kMOffMs);
+                const float2 a = ms[r], b = ms[128 + r];
+                mbar_arrive(bar(kLBarMsEmpty));
                 float2 out;
                 if (WPASS) {
-                    out = make_float2((sum + o.x) + (carry + o.y), 0.0f);
+                    out = make_float2((a.x + b.x) + (a.y + b.y), 0.0f);
                 } else {
-                    const float m = fmaxf(off, o.x);
-                    k0 = off == -CUDART_INF_F ? 0.0f : ex2_approx(off - m);
-                    k1 = o.x == -CUDART_INF_F ? 0.0f : ex2_approx(o.x - m);
-                    out = make_float2(m, sum * k0 + o.y * k1);
+                    const float m = fmaxf(a.x, b.x);
+                    const float k0 = a.x == -CUDART_INF_F ? 0.0f : ex2_approx(a.x - m);
+                    const float k1 = b.x == -CUDART_INF_F ? 0.0f : ex2_approx(b.x - m);
+                    out = make_float2(m, a.y * k0 + b.y * k1);
                 }
                 p.part_ms[(size_t)u * 128 + r] = out;
-                if (with_o) {
-                    float* po = p.part_o + (size_t)u * feat * 128 + r;
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        if (32 * q < feat) {
-                            uint32_t v[32];
-                            tmem_ld32x32b_x32_wait(tmem + lanes + kTS + 128u + 32u * q, v);
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) {
-                                const int f = 32 * q + 2 * j;
-                                if (f < feat) {
-                                    po[(size_t)f * 128] = acc[16 * q + j].x * k0 + __uint_as_float(v[2 * j]) * k1;
-                                    po[(size_t)(f + 1) * 128] = acc[16 * q + j].y * k0 + __uint_as_float(v[2 * j + 1]) * k1;
-                                }
-                            }
-                        }
-                    }
-                }
-                tc_fence_before();
             }
         }
     }

@@ -26,15 +26,23 @@ __device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t addr) {
     return d;
 }
 
-// 16 columns of the warp's 32 lanes, waited for in the same block (no use can move above the wait).
-__device__ __forceinline__ void tmem_ld32x32b_x16_wait(uint32_t taddr, uint32_t (&r)[16]) {
+// 16 columns of the warp's 32 lanes, in flight until tmem_ld_wait16 (which ties the registers, so no
+// use can move above the wait).
+__device__ __forceinline__ void tmem_ld32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+        "%15}, [%16];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
           "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr)
         : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait16(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
 }
 
 __device__ __forceinline__ void tmem_st32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
@@ -43,6 +51,68 @@ __device__ __forceinline__ void tmem_st32x32b_x16(uint32_t taddr, const uint32_t
         "%14, %15, %16};" ::"r"(taddr),
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+
+// Up to 8 K steps of a product whose K runs along the image's rows' bytes (32 bytes a step, the
+// second four steps in the image's other half); A K-major in TMEM, 8 columns a step. One elect.sync
+// and immediate offsets: the issuing warp spends as few slots as it can between instructions.
+__device__ __forceinline__ void mma_k_steps_warp(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate, int steps) {
+    asm volatile(
+        "{\n\t.reg .pred e, pa, pt, q1, q2, q3, q4, q5, q6, q7;\n\t.reg .b64 b<8>;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 pa, %4, 0;\n\t"
+        "setp.eq.b32 pt, 0, 0;\n\t"
+        "add.s64 b1, %2, 2;\n\t"
+        "setp.gt.and.s32 q1, %5, 1, e;\n\t"
+        "add.s64 b2, %2, 4;\n\t"
+        "setp.gt.and.s32 q2, %5, 2, e;\n\t"
+        "add.s64 b3, %2, 6;\n\t"
+        "setp.gt.and.s32 q3, %5, 3, e;\n\t"
+        "add.s64 b4, %2, 1024;\n\t"
+        "setp.gt.and.s32 q4, %5, 4, e;\n\t"
+        "add.s64 b5, %2, 1026;\n\t"
+        "setp.gt.and.s32 q5, %5, 5, e;\n\t"
+        "add.s64 b6, %2, 1028;\n\t"
+        "setp.gt.and.s32 q6, %5, 6, e;\n\t"
+        "add.s64 b7, %2, 1030;\n\t"
+        "setp.gt.and.s32 q7, %5, 7, e;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, pa;\n\t"
+        "@q1 tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+8], b1, %3, pt;\n\t"
+        "@q2 tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+16], b2, %3, pt;\n\t"
+        "@q3 tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+24], b3, %3, pt;\n\t"
+        "@q4 tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+32], b4, %3, pt;\n\t"
+        "@q5 tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+40], b5, %3, pt;\n\t"
+        "@q6 tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+48], b6, %3, pt;\n\t"
+        "@q7 tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+56], b7, %3, pt;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(steps)
+        : "memory");
+}
+
+// The 8 K steps of a product whose contraction runs along the image's 128 rows (2 KB a step); A in
+// TMEM, 16 columns a step (8 of them read).
+__device__ __forceinline__ void mma_row_steps_warp(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred e, pa, pt;\n\t.reg .b64 b<8>;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 pa, %4, 0;\n\t"
+        "setp.eq.b32 pt, 0, 0;\n\t"
+        "add.s64 b1, %2, 128;\n\t"
+        "add.s64 b2, %2, 256;\n\t"
+        "add.s64 b3, %2, 384;\n\t"
+        "add.s64 b4, %2, 512;\n\t"
+        "add.s64 b5, %2, 640;\n\t"
+        "add.s64 b6, %2, 768;\n\t"
+        "add.s64 b7, %2, 896;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, pa;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+16], b1, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+32], b2, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+48], b3, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+64], b4, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+80], b5, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+96], b6, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+112], b7, %3, pt;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 
