@@ -136,7 +136,7 @@ __device__ __forceinline__ bool row_labels(const LossLabels& L, long long row, i
 template <bool F32>
 __global__ void __launch_bounds__(256) loss_pack_kernel(const __grid_constant__ LossPackParams p) {
     using T = typename Elem<F32>::type;
-    extern __shared__ int bins[];  // [8 warps][w_tiles] counts, then [w_tiles] starts
+    extern __shared__ int bins[];  // [8 warps][2 w_tiles] counts, then [2 w_tiles] starts
     __shared__ float red[8];
     __shared__ float s_g[128];
     __shared__ uint8_t s_valid[128];
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(256) loss_pack_kernel(const __grid_constant__ 
     if (is_w || !p.sort_labels) return;
 
     // ------------------------------------------------------------ labels by class tile
-    const int nb = p.w_tiles;
+    const int nb = 2 * p.w_tiles;  // (class tile, rows below 64 or above): a softmax warpgroup's share each
     int* start = bins + 8 * nb;
     for (int i = tid; i < 8 * nb; i += 256) bins[i] = 0;
     __syncthreads();
@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(256) loss_pack_kernel(const __grid_constant__ 
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 if (32 * s >= p.lab.n_top) break;
-                const int bin = lab.c[s] >= 0 ? lab.c[s] >> 7 : -1;
+                const int bin = lab.c[s] >= 0 ? 2 * (lab.c[s] >> 7) + (r >> 6) : -1;
                 const uint32_t same = __match_any_sync(0xffffffffu, bin);
                 const int rank = __popc(same & ((1u << lane) - 1u));
                 if (bin >= 0) {
@@ -358,33 +358,38 @@ __global__ void __launch_bounds__(256) loss_pack_kernel(const __grid_constant__ 
 // ------------------------------------------------------------------------------- main pass
 namespace {
 
-// Warps: 0 producer, 1 tensor-core issuer (and TMEM), 2-3 idle; two softmax warpgroups (warps 4-7
-// and 8-11) that take the streamed tiles in turn (tile i of a unit: warpgroup i % 2, score buffer
-// i % 2); two adding warpgroups (12-15 and 16-19), 64 features of every tile's second product each.
+// Warps: 0 producer, 1 tensor-core issuer (and TMEM), 2-3 idle; four softmax warpgroups (warps
+// 4-19): two for the even and two for the odd streamed tiles of a unit, 64 columns each (score
+// buffer = parity); two adding warpgroups (20-27), 64 features of every tile's second product each.
 // Softmax and adding are apart so that a softmax warpgroup goes on to its next tile without waiting
-// for the tensor core to use its last.
-constexpr int kMainThreads = 640;
-constexpr int kLaunchRegs = 96;  // 65,536 registers / 640 threads
-constexpr int kCtrlRegs = 48, kSoftRegs = 112, kAddRegs = 104;
-static_assert(128 * kCtrlRegs + 256 * kSoftRegs + 256 * kAddRegs <= kMainThreads * kLaunchRegs, "register split");
+// for the tensor core to use its last; two warpgroups a tile halve the time from scores to
+// probabilities, which the tensor core waits for whenever it exceeds the two products it can run
+// meanwhile.
+constexpr int kMainThreads = 896;
+constexpr int kLaunchRegs = 72;  // 65,536 registers / 896 threads
+constexpr int kCtrlRegs = 40, kSoftRegs = 72, kAddRegs = 88;
+static_assert(128 * kCtrlRegs + 512 * kSoftRegs + 256 * kAddRegs <= kMainThreads * kLaunchRegs, "register split");
 
 template <bool F32>
 struct Ring {
     static constexpr uint32_t kStage = F32 ? 2u * kLossImage : kLossImage;
-    static constexpr uint32_t kStages = F32 ? 3u : 6u;
+    static constexpr uint32_t kStages = F32 ? 3u : 5u;
+    static constexpr uint32_t kTab = kStage * kStages;  // column tables, 1 KB a stage
 };
-constexpr uint32_t kMOffTab = 196608;             // per stage 1 KB: the tile's column table
-constexpr uint32_t kMOffBars = kMOffTab + 6 * 1024;
-constexpr uint32_t kMOffMisc = kMOffBars + 256;   // [0] TMEM base, [1] abort flag
-constexpr uint32_t kMOffMs = kMOffMisc + 64;      // [2][128] float2: the softmax warpgroups' row state
-constexpr uint32_t kMOffRing = kMOffMs + 2048;    // [4 tiles][128] f32: offset of a tile's probabilities
-constexpr uint32_t kPatchRow = 20;                // floats per class row of a label patch (16 used:
-                                                  // the 16-byte rows then fall on distinct banks)
-constexpr uint32_t kMOffPatch = kMOffRing + 2048;  // [8 warps][32][kPatchRow] f32
-constexpr uint32_t kMSmemUsed = kMOffPatch + 8 * 32 * kPatchRow * 4;
+constexpr uint32_t kMOffBars = 196608 + 3 * 1024;  // after the stages and their column tables
+constexpr uint32_t kMOffMisc = kMOffBars + 512;   // [0] TMEM base, [1] abort flag
+constexpr uint32_t kMOffMs = kMOffMisc + 64;      // [4][128] float2: the softmax warpgroups' row state
+constexpr uint32_t kMOffUnion = kMOffMs + 4096;
+constexpr uint32_t kMOffRing = kMOffUnion;         // row pass: [4 tiles][128] f32, offset of a tile's probabilities
+constexpr uint32_t kMOffTop = kMOffUnion + 2048;   // row pass: [4][128] f32, maxima of a tile's two halves
+constexpr uint32_t kPatchRow = 12;                 // floats per class row of a label patch (8 used:
+                                                   // the 16-byte rows then fall on distinct banks)
+constexpr uint32_t kMOffPatch = kMOffUnion;        // weight pass: [16 warps][32][kPatchRow] f32
+constexpr uint32_t kMSmemUsed = kMOffPatch + 16 * 32 * kPatchRow * 4;
 constexpr uint32_t kMSmemBytes = kMSmemUsed + 1024;
-static_assert(Ring<true>::kStage * Ring<true>::kStages <= kMOffTab && Ring<false>::kStage * Ring<false>::kStages <= kMOffTab,
-              "stages fit");
+static_assert(Ring<true>::kStages * (Ring<true>::kStage + 1024) <= kMOffBars &&
+                  Ring<false>::kStages * (Ring<false>::kStage + 1024) <= kMOffBars,
+              "stages and tables fit");
 static_assert(kMSmemBytes <= 227 * 1024, "shared memory per CTA");
 
 constexpr int kLBarFull = 0;               // [6] tile and column table landed
@@ -398,8 +403,9 @@ constexpr int kLBarOEmpty = 19;            // added up, the buffer free
 constexpr int kLBarRing = 20;              // [4] a tile's offsets written
 constexpr int kLBarMsFull = 24;            // row states of a unit written
 constexpr int kLBarMsEmpty = 25;           // and read
-constexpr int kLBarDone = 26;              // every product retired (teardown)
-static_assert(kLBarDone < 32, "barrier area");
+constexpr int kLBarTop = 26;               // [2 parities][4 quadrants] both halves' maxima written
+constexpr int kLBarDone = 34;              // every product retired (teardown)
+static_assert(8 * (kLBarDone + 1) <= 512, "barrier area");
 
 // TMEM columns: own operand (hi | lo), score buffers, second product
 constexpr uint32_t kTOwn = 0, kTS = 128, kTO = 384;
@@ -486,15 +492,25 @@ __device__ __forceinline__ void store_probs(uint32_t taddr, const float2 (&g)[8]
     }
 }
 
-// The tile's labels (weight pass), a window of 32 at a time: each lane holds one entry.
+// A tile's labels (weight pass), a window of 32 at a time: each lane holds one entry of the current
+// window and one of the next, which is in flight meanwhile.
 struct LabelWindow {
-    int2 e;       // (row << 7 | class, factor); consumed or absent: row beyond the tile
-    int next, end;
+    int2 e, n;      // (row << 7 | class, factor); consumed or absent: row beyond the tile
+    int next, end;  // first entry after the current window
 };
 constexpr int kNoLabel = 0x7fffffff;
-__device__ __forceinline__ void window_load(LabelWindow& w, const int2* ent, int lane) {
-    w.e = w.next + lane < w.end ? __ldg(ent + w.next + lane) : make_int2(kNoLabel, 0);
+__device__ __forceinline__ int2 window_entry(const LabelWindow& w, int at, const int2* ent) {
+    return at < w.end ? __ldg(ent + at) : make_int2(kNoLabel, 0);
+}
+__device__ __forceinline__ void window_open(LabelWindow& w, const int2* ent, int lane) {
+    w.e = window_entry(w, w.next + lane, ent);
     w.next += 32;
+    w.n = window_entry(w, w.next + lane, ent);
+}
+__device__ __forceinline__ void window_next(LabelWindow& w, const int2* ent, int lane) {
+    w.e = w.n;
+    w.next += 32;
+    w.n = window_entry(w, w.next + lane, ent);
 }
 
 }  // namespace
@@ -524,24 +540,25 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < 6; ++s) {
             mbar_init(bar(kLBarFull + s), 1);
-            mbar_init(bar(kLBarEmpty + s), 5);  // the product's commit, four warps
+            mbar_init(bar(kLBarEmpty + s), 9);  // the product's commit, eight warps
         }
-        mbar_init(bar(kLBarAFull), 256);
+        mbar_init(bar(kLBarAFull), 512);
         mbar_init(bar(kLBarAEmpty), 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar(kLBarSFull + i), 1);
-            mbar_init(bar(kLBarPFull + i), 4);
+            mbar_init(bar(kLBarPFull + i), 8);
         }
         mbar_init(bar(kLBarOFull), 1);
         mbar_init(bar(kLBarOEmpty), 8);
         for (int i = 0; i < 4; ++i) mbar_init(bar(kLBarRing + i), 4);
-        mbar_init(bar(kLBarMsFull), 256);
+        mbar_init(bar(kLBarMsFull), 512);
+        for (int i = 0; i < 8; ++i) mbar_init(bar(kLBarTop + i), 2);
         mbar_init(bar(kLBarMsEmpty), 128);
         mbar_init(bar(kLBarDone), 1);
         misc[1] = 0u;
         fence_mbar_init();
     }
-    for (uint32_t i = threadIdx.x; i < 8 * 32 * kPatchRow; i += kMainThreads)
+    for (uint32_t i = threadIdx.x; i < 16 * 32 * kPatchRow; i += kMainThreads)
         reinterpret_cast<float*>(gbase + kMOffPatch)[i] = 0.0f;
     if (warp == 1) {
         tmem_alloc(base + kMOffMisc, 512);
@@ -568,7 +585,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                     if (elect_one()) {
                         mbar_arrive_expect_tx(bar(kLBarFull + s), kStage + kTabBytes);
                         bulk_copy_g2s(base + s * kStage, p.str + (size_t)c * kStage, kStage, bar(kLBarFull + s));
-                        bulk_copy_g2s(base + kMOffTab + s * 1024u, p.col_tab + (size_t)c * (kTabBytes / 4), kTabBytes,
+                        bulk_copy_g2s(base + Ring<F32>::kTab + s * 1024u, p.col_tab + (size_t)c * (kTabBytes / 4), kTabBytes,
                                       bar(kLBarFull + s));
                     }
                     __syncwarp();
@@ -640,47 +657,49 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
             mma_commit_warp(bar(kLBarDone));
             loss_drain(bar(kLBarDone), 0u, wt);
         }
-    } else if (warp < 12) {
-        setmaxnreg_inc<kSoftRegs>();
+    } else if (warp < 20) {
+        // (kSoftRegs is what the kernel was launched with)
         // ------------------------------------------------------------- softmax warpgroups
-        const uint32_t g = (uint32_t)(warp - 4) >> 2;
+        const uint32_t wg = (uint32_t)(warp - 4) >> 2, g = wg >> 1, half = wg & 1u;
         const int quad = warp & 3, r = quad * 32 + lane;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         const uint32_t patch = base + kMOffPatch + (uint32_t)(warp - 4) * 32u * kPatchRow * 4u;
-        const uint32_t t_s = tmem + lanes + kTS + 128u * g;
+        const uint32_t t_s = tmem + lanes + kTS + 128u * g + 64u * half;
         float* ring = reinterpret_cast<float*>(gbase + kMOffRing);
+        volatile float* tops = reinterpret_cast<volatile float*>(gbase + kMOffTop);
         uint32_t cc = 0, uc = 0, uses = 0;
         bool ok = true;
         for (int u = blockIdx.x; ok && lunit_exists(u, p); u += gridDim.x, ++uc) {
             const LUnit U = lunit(u, p);
             const uint32_t n = (uint32_t)(U.c1 - U.c0);
             // labels of this warpgroup's first tile (weight pass): range, then entries
-            LabelWindow lw{make_int2(kNoLabel, 0), 0, 0};
+            LabelWindow lw{make_int2(kNoLabel, 0), make_int2(kNoLabel, 0), 0, 0};
             auto label_range = [&](int c, int& a, int& b) {
-                const int32_t* o = p.sp_off + (size_t)c * (p.own_tiles + 1) + U.own;
+                const int32_t* o = p.sp_off + (size_t)c * (2 * p.own_tiles + 1) + 2 * U.own + half;
                 a = __ldg(o);
                 b = __ldg(o + 1);
             };
             auto label_base = [&](int c) { return p.sp_ent + (size_t)c * 128 * p.n_top; };
             if (WPASS && g < n) {
                 label_range(U.c0 + (int)g, lw.next, lw.end);
-                window_load(lw, label_base(U.c0 + (int)g), lane);
+                window_open(lw, label_base(U.c0 + (int)g), lane);
             }
-            // own operand -> TMEM: warpgroup g takes K slots 64 g .. 64 g + 63 of the lane's row
+            // own operand -> TMEM: warpgroup wg takes K slots 64 half .. 64 half + 63 of the lane's
+            // row, of the high part (even tiles' warpgroups) or the low part (odd; f32)
             ok = loss_wait(bar(kLBarAEmpty), (uc & 1u) ^ 1u, wt, 106);
             if (!ok) break;
             tc_fence_after();
-            if ((int)(4 * g) < p.ksteps) {
-                const uint8_t* img = p.own + (size_t)U.own * kStage;
+            if ((int)(4 * half) < p.ksteps && (F32 || g == 0)) {
+                const uint8_t* img = p.own + (size_t)U.own * kStage + g * kLossImage;
 #pragma unroll
-                for (int part = 0; part < (F32 ? 2 : 1); ++part) {
-                    uint32_t w[32];
+                for (int hj = 0; hj < 2; ++hj) {
+                    uint32_t w[16];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(img + part * kLossImage + image_chunk(r, 8 * g + j));
+                    for (int j = 0; j < 4; ++j) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(img + image_chunk(r, 8 * half + 4 * hj + j));
                         w[4 * j] = x.x, w[4 * j + 1] = x.y, w[4 * j + 2] = x.z, w[4 * j + 3] = x.w;
                     }
-                    tmem_st32x32b_x32(tmem + lanes + kTOwn + 64u * part + 32u * g, w);
+                    tmem_st32x32b_x16(tmem + lanes + kTOwn + 64u * g + 32u * half + 16u * hj, w);
                 }
                 tmem_st_wait();
             }
@@ -693,7 +712,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
             for (uint32_t i = g; i < n; i += 2, ++uses) {
                 const int c = U.c0 + (int)i;
                 const uint32_t s = (cc + i) % kStages;
-                const uint32_t tab = base + kMOffTab + s * 1024u;
+                const uint32_t tab = base + Ring<F32>::kTab + s * 1024u + 256u * half;
                 const float str_s = F32 ? __ldg(p.str_scale + c) : 1.0f;
                 const float gs = WPASS && F32 ? __ldg(p.g_scale + c) : 1.0f;
                 // the next tile's label range is fetched under this tile, its entries at this tile's end
@@ -706,15 +725,13 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                 ok = ok && loss_wait(bar(kLBarFull + s), ((cc + i) / kStages) & 1u, wt, 108);
                 if (!ok) break;
                 tc_fence_after();
-                uint32_t v[2][16];
-                tmem_ld32x32b_x16(t_s, v[0]);
                 if constexpr (!WPASS) {
                     float top = -CUDART_INF_F;
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) {
-                        tmem_ld_wait16(v[q & 1]);
-                        tmem_ld32x32b_x16(t_s + 16u * ((q + 1) & 7), v[(q + 1) & 1]);  // at the end: the first again
-                        const uint32_t(&x)[16] = v[q & 1];
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t x[16];
+                        tmem_ld32x32b_x16(t_s + 16u * q, x);
+                        tmem_ld_wait16(x);
 #pragma unroll
                         for (int j = 0; j < 16; j += 4) {
                             const float4 e = lds128(tab + 4u * (16 * q + j));
@@ -726,20 +743,27 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                             top = max3f(top, b.x, b.y);
                         }
                     }
+                    // the row's maximum over both halves of the tile
+                    tops[wg * 128 + r] = top;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(kLBarTop + 4 * (int)g + quad));
+                    ok = loss_wait(bar(kLBarTop + 4 * (int)g + quad), uses & 1u, wt, 113);
+                    if (!ok) break;
+                    top = fmaxf(top, tops[(wg ^ 1u) * 128 + r]);
                     const float m = fmaxf(off, top);
                     // nothing visible yet (every class masked): any finite offset gives 2^-inf = 0
                     const float m0 = m == -CUDART_INF_F ? 0.0f : m;
                     const float corr = off == -CUDART_INF_F ? 0.0f : ex2_approx(off - m0);
                     off = m;
-                    if (with_o) ring[((cc + i) & 3u) * 128 + r] = m;
+                    if (with_o && half == 0) ring[((cc + i) & 3u) * 128 + r] = m;
                     const float sub = F32 ? 14.0f - m0 : -m0;
                     const float2 sub2 = make_float2(sub, sub);
                     float2 ts = make_float2(0.f, 0.f);
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) {
-                        tmem_ld_wait16(v[q & 1]);
-                        if (q < 7) tmem_ld32x32b_x16(t_s + 16u * (q + 1), v[(q + 1) & 1]);
-                        const uint32_t(&x)[16] = v[q & 1];
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t x[16];
+                        tmem_ld32x32b_x16(t_s + 16u * q, x);
+                        tmem_ld_wait16(x);
                         float2 pr[8];
 #pragma unroll
                         for (int j = 0; j < 16; j += 4) {
@@ -763,10 +787,10 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                     const int2* ent = label_base(c);
                     float2 ts = make_float2(0.f, 0.f);
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) {
-                        tmem_ld_wait16(v[q & 1]);
-                        if (q < 7) tmem_ld32x32b_x16(t_s + 16u * (q + 1), v[(q + 1) & 1]);
-                        const uint32_t(&x)[16] = v[q & 1];
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t x[16];
+                        tmem_ld32x32b_x16(t_s + 16u * q, x);
+                        tmem_ld_wait16(x);
                         float2 pr[8];
 #pragma unroll
                         for (int j = 0; j < 16; j += 4) {
@@ -782,36 +806,39 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                             pr[j / 2 + 1] =
                                 __fmul2_rn(make_float2(ex2_approx(b.x), ex2_approx(b.y)), make_float2(f.z, f.w));
                         }
-                        // the labels' shares, 16 columns (rows of x) at a time through a patch of
+                        // the labels' shares, 8 columns (rows of x) at a time through a patch of
                         // shared memory: entries scatter into it, each lane then adds its class's row
-                        const int lo = 16 * q;
-                        bool any = false;
-                        while (true) {
-                            const bool in = (lw.e.x >> 7) < lo + 16;
-                            const uint32_t b = __ballot_sync(0xffffffffu, in);
-                            if (b == 0u) break;
-                            const bool hit = in && ((lw.e.x & 127) >> 5) == quad;
-                            if (hit)
-                                *reinterpret_cast<volatile float*>(
-                                    gbase + (patch - base) +
-                                    4u * ((uint32_t)(lw.e.x & 31) * kPatchRow + (uint32_t)((lw.e.x >> 7) - lo))) =
-                                    __int_as_float(lw.e.y);
-                            any |= __any_sync(0xffffffffu, hit);
-                            if (in) lw.e.x = kNoLabel;
-                            if (!(b >> 31) || lw.next >= lw.end) break;
-                            window_load(lw, ent, lane);
-                        }
-                        if (any) {
-                            __syncwarp();
-                            const uint32_t row = patch + 4u * (uint32_t)lane * kPatchRow;
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const float4 d = lds128(row + 16u * j);
-                                pr[2 * j] = __fadd2_rn(pr[2 * j], make_float2(d.x, d.y));
-                                pr[2 * j + 1] = __fadd2_rn(pr[2 * j + 1], make_float2(d.z, d.w));
-                                sts128(row + 16u * j, make_float4(0.f, 0.f, 0.f, 0.f));
+                        for (int h = 0; h < 2; ++h) {
+                            const int lo = 64 * (int)half + 16 * q + 8 * h;
+                            bool any = false;
+                            while (true) {
+                                const bool in = (lw.e.x >> 7) < lo + 8;
+                                const uint32_t b = __ballot_sync(0xffffffffu, in);
+                                if (b == 0u) break;
+                                const bool hit = in && ((lw.e.x & 127) >> 5) == quad;
+                                if (hit)
+                                    *reinterpret_cast<volatile float*>(
+                                        gbase + (patch - base) +
+                                        4u * ((uint32_t)(lw.e.x & 31) * kPatchRow + (uint32_t)((lw.e.x >> 7) - lo))) =
+                                        __int_as_float(lw.e.y);
+                                any |= __any_sync(0xffffffffu, hit);
+                                if (in) lw.e.x = kNoLabel;
+                                if (!(b >> 31)) break;
+                                window_next(lw, ent, lane);
                             }
-                            __syncwarp();
+                            if (any) {
+                                __syncwarp();
+                                const uint32_t row = patch + 4u * (uint32_t)lane * kPatchRow;
+#pragma unroll
+                                for (int j = 0; j < 2; ++j) {
+                                    const float4 d = lds128(row + 16u * j);
+                                    pr[4 * h + 2 * j] = __fadd2_rn(pr[4 * h + 2 * j], make_float2(d.x, d.y));
+                                    pr[4 * h + 2 * j + 1] = __fadd2_rn(pr[4 * h + 2 * j + 1], make_float2(d.z, d.w));
+                                    sts128(row + 16u * j, make_float4(0.f, 0.f, 0.f, 0.f));
+                                }
+                                __syncwarp();
+                            }
                         }
 #pragma unroll
                         for (int j = 0; j < 8; j += 2) ts = __fadd2_rn(ts, __fadd2_rn(pr[j], pr[j + 1]));
@@ -824,7 +851,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                     sum = nsum;
                     lw.next = next_a;
                     lw.end = next_b;
-                    window_load(lw, label_base(i + 2 < n ? c + 2 : c), lane);
+                    window_open(lw, label_base(i + 2 < n ? c + 2 : c), lane);
                 }
                 tmem_st_wait();
                 tc_fence_before();
@@ -832,14 +859,14 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                 if (lane == 0) {
                     mbar_arrive(bar(kLBarPFull + (int)g));
                     mbar_arrive(bar(kLBarEmpty + (int)s));
-                    if (!WPASS && with_o) mbar_arrive(bar(kLBarRing + (int)((cc + i) & 3u)));
+                    if (!WPASS && with_o && half == 0) mbar_arrive(bar(kLBarRing + (int)((cc + i) & 3u)));
                 }
             }
             if (!ok) break;
             cc += n;
             ok = loss_wait(bar(kLBarMsEmpty), (uc & 1u) ^ 1u, wt, 110);
             if (!ok) break;
-            reinterpret_cast<float2*>(gbase + kMOffMs)[g * 128 + r] = WPASS ? make_float2(sum, carry) : make_float2(off, sum);
+            reinterpret_cast<float2*>(gbase + kMOffMs)[wg * 128 + r] = WPASS ? make_float2(sum, carry) : make_float2(off, sum);
             mbar_arrive(bar(kLBarMsFull));
         }
     } else {
@@ -847,7 +874,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
         // -------------------------------------------------------------- adding warpgroups
         // acc is relative to `off`, the largest offset of the tiles so far (row pass; the two softmax
         // warpgroups each keep their own running maximum).
-        const uint32_t g = (uint32_t)(warp - 12) >> 2;
+        const uint32_t g = (uint32_t)(warp - 20) >> 2;
         const int quad = warp & 3, r = quad * 32 + lane;
         const uint32_t t_o = tmem + ((uint32_t)(quad * 32) << 16) + kTO + 64u * g;
         const volatile float* ring = reinterpret_cast<const volatile float*>(gbase + kMOffRing);
@@ -916,16 +943,16 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                 ok = loss_wait(bar(kLBarMsFull), uc & 1u, wt, 111);
                 if (!ok) break;
                 const float2* ms = reinterpret_cast<const float2*>(gbase + kMOffMs);
-                const float2 a = ms[r], b = ms[128 + r];
+                const float2 a0 = ms[r], a1 = ms[128 + r], b0 = ms[256 + r], b1 = ms[384 + r];
                 mbar_arrive(bar(kLBarMsEmpty));
                 float2 out;
                 if (WPASS) {
-                    out = make_float2((a.x + b.x) + (a.y + b.y), 0.0f);
-                } else {
-                    const float m = fmaxf(a.x, b.x);
-                    const float k0 = a.x == -CUDART_INF_F ? 0.0f : ex2_approx(a.x - m);
-                    const float k1 = b.x == -CUDART_INF_F ? 0.0f : ex2_approx(b.x - m);
-                    out = make_float2(m, a.y * k0 + b.y * k1);
+                    out = make_float2(((a0.x + a1.x) + (b0.x + b1.x)) + ((a0.y + a1.y) + (b0.y + b1.y)), 0.0f);
+                } else {  // the halves of one parity share their offset
+                    const float m = fmaxf(a0.x, b0.x);
+                    const float k0 = a0.x == -CUDART_INF_F ? 0.0f : ex2_approx(a0.x - m);
+                    const float k1 = b0.x == -CUDART_INF_F ? 0.0f : ex2_approx(b0.x - m);
+                    out = make_float2(m, (a0.y + a1.y) * k0 + (b0.y + b1.y) * k1);
                 }
                 p.part_ms[(size_t)u * 128 + r] = out;
             }
@@ -1267,7 +1294,7 @@ __global__ void __launch_bounds__(256) loss_score_kernel(const __grid_constant__
 
 // ------------------------------------------------------------------------------- launchers
 namespace {
-constexpr int kPackSmemMax = 9 * (kLossMaxClasses / 128) * 4;
+constexpr int kPackSmemMax = 9 * 2 * (kLossMaxClasses / 128) * 4;
 constexpr int kRowsSmemMax = (2 * 32 * 129 + 32 * kLossMaxSplits) * 4;
 // Blocks of 32 rows would leave SMs idle: four times as many of 8.
 bool few_blocks(int tiles, int sms) { return tiles * (kLossTile / 32) < 2 * sms; }
@@ -1291,7 +1318,7 @@ cudaError_t loss_kernel_setup() {
 
 cudaError_t launch_loss_pack(const LossPackParams& p, bool f32, cudaStream_t stream) {
     const int grid = p.w_tiles + p.x_tiles;
-    const int smem = p.sort_labels ? 9 * p.w_tiles * 4 : 0;
+    const int smem = p.sort_labels ? 9 * 2 * p.w_tiles * 4 : 0;
     if (f32)
         loss_pack_kernel<true><<<grid, 256, smem, stream>>>(p);
     else

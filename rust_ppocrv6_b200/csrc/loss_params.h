@@ -9,7 +9,7 @@ namespace rh {
 constexpr int kLossTile = 128;            // rows (classes) per operand tile
 constexpr int kLossImage = 128 * 128 * 2;  // one 16-bit tile image: 128 rows x 128 K slots
 constexpr int kLossMaxTop = 64;           // teacher entries per row
-constexpr int kLossMaxClasses = 1 << 18;  // class tiles are counted in shared memory (2,048 bins)
+constexpr int kLossMaxClasses = 1 << 18;  // class tiles are counted in shared memory (2 x 2,048 bins)
 constexpr int kLossRows = 32;             // rows per block of the score kernel
 constexpr int kLossMaxSplits = 148;       // ranges that an own tile's work is split into at most
 // Device status bit (status[0], beside kDevTimeout and kDevRecPlan): a target or teacher class
@@ -48,7 +48,7 @@ struct LossPackParams {
     float* row_tab;            // [x_tiles][256]: 128 x (-lse, log2 units; written by the row kernel),
                                // 128 x gradient factor (f32: scaled by the tile's power of two)
     float* g_scale;            // [x_tiles] value of one unit of the tile's gradient factors
-    int32_t* sp_off;           // [x_tiles][w_tiles + 1] label ranges by class tile
+    int32_t* sp_off;           // [x_tiles][2 w_tiles + 1] label ranges by class tile and half of the rows
     int2* sp_ent;              // [x_tiles][128 n_top]: (row << 7 | class within its tile, factor bits)
     int* status;
 };

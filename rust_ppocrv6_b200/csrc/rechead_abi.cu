@@ -882,7 +882,7 @@ LossLayout loss_layout(bool f32, int64_t rows, int64_t k, int64_t n, int64_t n_t
     L.g_scale = take((size_t)L.x_tiles * 4);
     L.class_e = take((size_t)L.w_tiles * 512);
     L.row_tab = take((size_t)L.x_tiles * 1024);
-    L.sp_off = take((size_t)L.x_tiles * (size_t)(L.w_tiles + 1) * 4);
+    L.sp_off = take((size_t)L.x_tiles * (size_t)(2 * L.w_tiles + 1) * 4);
     L.sp_ent = take((size_t)L.x_tiles * 128 * (size_t)n_top * 8);
     L.part_o = take(units * (size_t)L.feat * 512);
     L.part_ms = take(units * 1024);
