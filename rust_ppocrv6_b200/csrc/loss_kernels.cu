@@ -137,8 +137,8 @@ template <bool F32>
 __global__ void __launch_bounds__(256) loss_pack_kernel(const __grid_constant__ LossPackParams p) {
     using T = typename Elem<F32>::type;
     extern __shared__ int bins[];  // [8 warps][2 w_tiles] counts, then [2 w_tiles] starts
-    __shared__ float red[8];
-    __shared__ float s_g[128];
+    __shared__ float red[8], red2[8];
+    __shared__ float s_g[128], s_norm[128];
     __shared__ uint8_t s_valid[128];
     __shared__ int s_scan[8];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -174,10 +174,13 @@ __global__ void __launch_bounds__(256) loss_pack_kernel(const __grid_constant__ 
             const int sh = shift_to(top, 13);
             gs = pow2i(sh);
             if (tid == 0) p.g_scale[tile] = pow2i(-sh);
+        } else {
+            const int neg = __syncthreads_or(f < 0.0f);
+            if (tid == 0) p.g_scale[tile] = neg ? 1.0f : 0.0f;
         }
         if (tid < 128) {
             s_g[tid] = f * gs;
-            p.row_tab[(size_t)tile * 256 + 128 + tid] = f * gs;
+            p.row_tab[(size_t)tile * 256 + 128 + tid] = F32 ? f * gs : copysignf(1.0f, f);
         }
         __syncthreads();
     } else if (tid < 128) {
@@ -227,6 +230,78 @@ __global__ void __launch_bounds__(256) loss_pack_kernel(const __grid_constant__ 
         if (F32) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[i][j]));
+        }
+    }
+    if (!F32 && p.slots) {
+        // |row|: row-major operands have a row's 16 chunks in 16 neighbouring lanes, the other layout
+        // has the even and the odd ones in two threads; both add them up in the same tree
+        float q[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            q[i] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) q[i] = fmaf(v[i][j], v[i][j], q[i]);
+        }
+        if (t_len > 0) {
+            const float sum = ((q[0] + q[4]) + (q[2] + q[6])) + ((q[1] + q[5]) + (q[3] + q[7]));
+            if (tid < 128) s_norm[tid] = sum;
+            __syncthreads();
+            if (tid >= 128) s_norm[tid - 128] += sum;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1) q[i] += __shfl_xor_sync(0xffffffffu, q[i], o);
+                if ((tid & 15) == 0) s_norm[i * 16 + (tid >> 4)] = q[i];
+            }
+        }
+        __syncthreads();
+        const float norm = tid < 128 ? sqrtf(s_norm[tid]) : 0.0f;
+        if (is_w) {
+            const long long j = row0 + tid;
+            const bool real = tid < 128 && j < p.lab.n;
+            const float e = real ? (p.bias ? p.bias[j] * p.logit_scale : 0.0f) : -CUDART_INF_F;
+            // (a NaN norm or bias has to survive the maximum: it then rules the bound out)
+            const float wn = warp_max(norm), we = warp_max(e);
+            const int bad = __syncthreads_or(real && (isnan(norm) || isnan(e)));
+            if (lane == 0) {
+                red[warp] = wn;
+                red2[warp] = we;
+            }
+            __syncthreads();
+            if (tid == 0) {
+                float a = red[0], b = red2[0];
+                for (int i = 1; i < 4; ++i) {
+                    a = fmaxf(a, red[i]);
+                    b = fmaxf(b, red2[i]);
+                }
+                p.w_bound[tile] = make_float2(bad ? CUDART_NAN_F : a, b);
+            }
+        } else if (tid < 128) {
+            p.x_norm[(size_t)tile * 128 + tid] = norm;
+        }
+        // the bias (natural units) in three bf16 parts, against ones in the features: the parts'
+        // products with 1 are exact, so a score carries its bias to 24 bits. Padding classes: -inf.
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int item = i * 256 + tid;
+            const int r = t_len > 0 ? item & 127 : item >> 4, ch = t_len > 0 ? item >> 7 : item & 15;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int part = 8 * ch + j - p.k;
+                if (part < 0 || part > 2) continue;
+                if (!is_w) {
+                    v[i][j] = 1.0f;
+                    continue;
+                }
+                float rest = row0 + r < p.lab.n ? (p.bias ? p.bias[row0 + r] : 0.0f) : -CUDART_INF_F;
+                float here = 0.0f;
+                for (int a = 0; a <= part; ++a) {
+                    here = __bfloat162float(__float2bfloat16_rn(rest));
+                    rest = isfinite(here) ? rest - here : 0.0f;
+                }
+                v[i][j] = here;
+            }
         }
     }
     float up = 1.0f;
@@ -523,7 +598,13 @@ __device__ __forceinline__ void window_next(LabelWindow& w, const int2* ent, int
 // tensor core's f32 accumulator rounds toward zero, which over thousands of steps would bias the
 // sums; over one tile's steps it stays below the operands' own error.
 // f32: three products each (hi.lo, lo.hi, hi.hi).
-template <bool F32, bool WPASS>
+// bf16 with slots: the scores come with their bias, so they need no column table in the row pass;
+// and as bf16 probabilities have f32's range, a row's offset need not follow its maximum: by
+// Cauchy-Schwarz every logit lies within |x_r| max|w| of the largest bias, so where that leaves a
+// spread of at most 80 binary orders the upper bound itself is the offset, every probability is at
+// most 1, and what underflows (below 2^-126) is 2^-46 of the largest. Rows beyond it (a warp at a
+// time) follow the running maximum as the others do.
+template <bool F32, bool WPASS, bool SLOTS>
 __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid_constant__ LossMainParams p) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
@@ -665,6 +746,19 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         const uint32_t patch = base + kMOffPatch + (uint32_t)(warp - 4) * 32u * kPatchRow * 4u;
         const uint32_t t_s = tmem + lanes + kTS + 128u * g + 64u * half;
+        float w_max = 0.0f, e_max = -CUDART_INF_F;
+        if (SLOTS && !WPASS) {
+            bool nan = false;
+            for (int t = lane; t < p.str_tiles; t += 32) {
+                const float2 b = __ldg(p.w_bound + t);
+                nan |= isnan(b.x);
+                w_max = fmaxf(w_max, b.x);
+                e_max = fmaxf(e_max, b.y);
+            }
+            w_max = warp_max(w_max);
+            e_max = warp_max(e_max);
+            if (__any_sync(0xffffffffu, nan)) w_max = CUDART_INF_F;
+        }
         float* ring = reinterpret_cast<float*>(gbase + kMOffRing);
         volatile float* tops = reinterpret_cast<volatile float*>(gbase + kMOffTop);
         uint32_t cc = 0, uc = 0, uses = 0;
@@ -707,14 +801,21 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
             mbar_arrive(bar(kLBarAFull));
 
             const float own_mul = F32 ? p.logit_scale * __ldg(p.own_scale + U.own) : p.logit_scale;
-            const float lane_e = WPASS ? __ldg(p.lane_e + (size_t)U.own * 128 + r) : 0.0f;
+            const float lane_e = WPASS && !SLOTS ? __ldg(p.lane_e + (size_t)U.own * 128 + r) : 0.0f;
+            bool bounded = false;
+            float upper = 0.0f;
+            if (SLOTS && !WPASS) {
+                const float reach = p.logit_scale * __ldg(p.x_norm + (size_t)U.own * 128 + r) * w_max * 1.001f;
+                upper = reach + e_max;
+                bounded = __all_sync(0xffffffffu, reach <= 40.0f && fabsf(upper) < 1e6f);
+            }
             float off = -CUDART_INF_F, sum = 0.0f, carry = 0.0f;  // weight pass: sum + carry = bias gradient
             for (uint32_t i = g; i < n; i += 2, ++uses) {
                 const int c = U.c0 + (int)i;
                 const uint32_t s = (cc + i) % kStages;
                 const uint32_t tab = base + Ring<F32>::kTab + s * 1024u + 256u * half;
                 const float str_s = F32 ? __ldg(p.str_scale + c) : 1.0f;
-                const float gs = WPASS && F32 ? __ldg(p.g_scale + c) : 1.0f;
+                const float gs = WPASS ? __ldg(p.g_scale + c) : 1.0f;
                 // the next tile's label range is fetched under this tile, its entries at this tile's end
                 int next_a = 0, next_b = 0;
                 if (WPASS && i + 2 < n) label_range(c + 2, next_a, next_b);
@@ -725,7 +826,28 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                 ok = ok && loss_wait(bar(kLBarFull + s), ((cc + i) / kStages) & 1u, wt, 108);
                 if (!ok) break;
                 tc_fence_after();
-                if constexpr (!WPASS) {
+                if (SLOTS && !WPASS && bounded) {
+                    off = upper;
+                    if (with_o && half == 0) ring[((cc + i) & 3u) * 128 + r] = off;
+                    const float2 sub2 = make_float2(-off, -off);
+                    float2 ts = make_float2(0.f, 0.f);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t x[16];
+                        tmem_ld32x32b_x16(t_s + 16u * q, x);
+                        tmem_ld_wait16(x);
+                        float2 pr[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float2 a = __ffma2_rn(make_float2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])),
+                                                        mul, sub2);
+                            pr[j] = make_float2(ex2_approx(a.x), ex2_approx(a.y));
+                            ts = __fadd2_rn(ts, pr[j]);
+                        }
+                        if (with_o) store_probs<F32>(t_s + 16u * q, pr);
+                    }
+                    sum += ts.x + ts.y;
+                } else if constexpr (!WPASS) {
                     float top = -CUDART_INF_F;
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
@@ -734,7 +856,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                         tmem_ld_wait16(x);
 #pragma unroll
                         for (int j = 0; j < 16; j += 4) {
-                            const float4 e = lds128(tab + 4u * (16 * q + j));
+                            const float4 e = SLOTS ? make_float4(0.f, 0.f, 0.f, 0.f) : lds128(tab + 4u * (16 * q + j));
                             const float2 a = __ffma2_rn(make_float2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), mul,
                                                         make_float2(e.x, e.y));
                             const float2 b = __ffma2_rn(make_float2(__uint_as_float(x[j + 2]), __uint_as_float(x[j + 3])),
@@ -767,7 +889,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                         float2 pr[8];
 #pragma unroll
                         for (int j = 0; j < 16; j += 4) {
-                            const float4 e = lds128(tab + 4u * (16 * q + j));
+                            const float4 e = SLOTS ? make_float4(0.f, 0.f, 0.f, 0.f) : lds128(tab + 4u * (16 * q + j));
                             float2 a = __ffma2_rn(make_float2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), mul,
                                                   make_float2(e.x, e.y));
                             float2 b = __ffma2_rn(make_float2(__uint_as_float(x[j + 2]), __uint_as_float(x[j + 3])), mul,
@@ -795,16 +917,21 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
 #pragma unroll
                         for (int j = 0; j < 16; j += 4) {
                             const float4 e = lds128(tab + 4u * (16 * q + j));
-                            const float4 f = lds128(tab + 512u + 4u * (16 * q + j));
                             float2 a = __ffma2_rn(make_float2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), mul,
                                                   make_float2(e.x, e.y));
                             float2 b = __ffma2_rn(make_float2(__uint_as_float(x[j + 2]), __uint_as_float(x[j + 3])), mul,
                                                   make_float2(e.z, e.w));
-                            a = __fadd2_rn(a, le);
-                            b = __fadd2_rn(b, le);
-                            pr[j / 2] = __fmul2_rn(make_float2(ex2_approx(a.x), ex2_approx(a.y)), make_float2(f.x, f.y));
-                            pr[j / 2 + 1] =
-                                __fmul2_rn(make_float2(ex2_approx(b.x), ex2_approx(b.y)), make_float2(f.z, f.w));
+                            if (!SLOTS) {
+                                a = __fadd2_rn(a, le);
+                                b = __fadd2_rn(b, le);
+                            }
+                            pr[j / 2] = make_float2(ex2_approx(a.x), ex2_approx(a.y));
+                            pr[j / 2 + 1] = make_float2(ex2_approx(b.x), ex2_approx(b.y));
+                            if (F32 || gs != 0.0f) {  // f32: the factors; bf16: their signs, where one is negative
+                                const float4 f = lds128(tab + 512u + 4u * (16 * q + j));
+                                pr[j / 2] = __fmul2_rn(pr[j / 2], make_float2(f.x, f.y));
+                                pr[j / 2 + 1] = __fmul2_rn(pr[j / 2 + 1], make_float2(f.z, f.w));
+                            }
                         }
                         // the labels' shares, 8 columns (rows of x) at a time through a patch of
                         // shared memory: entries scatter into it, each lane then adds its class's row
@@ -845,7 +972,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                         store_probs<F32>(t_s + 16u * q, pr);
                     }
                     // bias gradient with the rounding error carried (up to thousands of tiles)
-                    const float t = fmaf(ts.x + ts.y, gs, carry);
+                    const float t = fmaf(ts.x + ts.y, F32 ? gs : 1.0f, carry);
                     const float nsum = sum + t;
                     carry = t - (nsum - sum);
                     sum = nsum;
@@ -1111,7 +1238,11 @@ __global__ void __launch_bounds__(256) loss_rows_kernel(const __grid_constant__ 
         RowLabels lab;
         const bool valid = row < p.rows && row_labels(p.lab, row, lane, lab);
         const float lse2 = s_lse2[r], lse = lse2 * kLn2;
-        if (lane == 0) *tab = valid ? -lse2 : -CUDART_INF_F;
+        if (lane == 0) {
+            float e = -CUDART_INF_F;  // no share of anything
+            if (valid) e = F32 ? -lse2 : log2f(fabsf(p.lab.temp * (p.row_grad ? p.row_grad[row] : 1.0f))) - lse2;
+            *tab = e;
+        }
         if (row >= p.rows) continue;
         float* xr = xs + r * (p.k + 1);
         if (!valid) {
@@ -1306,10 +1437,12 @@ cudaError_t smem_attr(K* k, int bytes) {
 
 cudaError_t loss_kernel_setup() {
     cudaError_t e;
-    if ((e = smem_attr(loss_main_kernel<true, false>, kMSmemBytes)) != cudaSuccess) return e;
-    if ((e = smem_attr(loss_main_kernel<true, true>, kMSmemBytes)) != cudaSuccess) return e;
-    if ((e = smem_attr(loss_main_kernel<false, false>, kMSmemBytes)) != cudaSuccess) return e;
-    if ((e = smem_attr(loss_main_kernel<false, true>, kMSmemBytes)) != cudaSuccess) return e;
+    if ((e = smem_attr(loss_main_kernel<true, false, false>, kMSmemBytes)) != cudaSuccess) return e;
+    if ((e = smem_attr(loss_main_kernel<true, true, false>, kMSmemBytes)) != cudaSuccess) return e;
+    if ((e = smem_attr(loss_main_kernel<false, false, false>, kMSmemBytes)) != cudaSuccess) return e;
+    if ((e = smem_attr(loss_main_kernel<false, true, false>, kMSmemBytes)) != cudaSuccess) return e;
+    if ((e = smem_attr(loss_main_kernel<false, false, true>, kMSmemBytes)) != cudaSuccess) return e;
+    if ((e = smem_attr(loss_main_kernel<false, true, true>, kMSmemBytes)) != cudaSuccess) return e;
     if ((e = smem_attr(loss_pack_kernel<true>, kPackSmemMax)) != cudaSuccess) return e;
     if ((e = smem_attr(loss_pack_kernel<false>, kPackSmemMax)) != cudaSuccess) return e;
     if ((e = smem_attr(loss_rows_kernel<true, 32>, kRowsSmemMax)) != cudaSuccess) return e;
@@ -1326,15 +1459,21 @@ cudaError_t launch_loss_pack(const LossPackParams& p, bool f32, cudaStream_t str
     return cudaGetLastError();
 }
 
-cudaError_t launch_loss_main(const LossMainParams& p, bool f32, bool weight_pass, int grid, cudaStream_t stream) {
-    if (f32 && !weight_pass)
-        loss_main_kernel<true, false><<<grid, kMainThreads, kMSmemBytes, stream>>>(p);
-    else if (f32)
-        loss_main_kernel<true, true><<<grid, kMainThreads, kMSmemBytes, stream>>>(p);
-    else if (!weight_pass)
-        loss_main_kernel<false, false><<<grid, kMainThreads, kMSmemBytes, stream>>>(p);
+namespace {
+template <bool F32, bool WPASS, bool SLOTS>
+void main_kernel(const LossMainParams& p, int grid, cudaStream_t stream) {
+    loss_main_kernel<F32, WPASS, SLOTS><<<grid, kMainThreads, kMSmemBytes, stream>>>(p);
+}
+}  // namespace
+
+cudaError_t launch_loss_main(const LossMainParams& p, bool f32, bool slots, bool weight_pass, int grid,
+                             cudaStream_t stream) {
+    if (f32)
+        weight_pass ? main_kernel<true, true, false>(p, grid, stream) : main_kernel<true, false, false>(p, grid, stream);
+    else if (slots)
+        weight_pass ? main_kernel<false, true, true>(p, grid, stream) : main_kernel<false, false, true>(p, grid, stream);
     else
-        loss_main_kernel<false, true><<<grid, kMainThreads, kMSmemBytes, stream>>>(p);
+        weight_pass ? main_kernel<false, true, false>(p, grid, stream) : main_kernel<false, false, false>(p, grid, stream);
     return cudaGetLastError();
 }
 

@@ -45,9 +45,15 @@ struct LossPackParams {
     float* x_scale;            // [x_tiles] value of one unit of the image (f32; a power of two)
     float* w_scale;            // [w_tiles]
     float* class_e;            // [w_tiles][128] bias * log2(e) / T; padding classes -inf
-    float* row_tab;            // [x_tiles][256]: 128 x (-lse, log2 units; written by the row kernel),
-                               // 128 x gradient factor (f32: scaled by the tile's power of two)
-    float* g_scale;            // [x_tiles] value of one unit of the tile's gradient factors
+    float* row_tab;            // [x_tiles][256]. f32: 128 x (-lse, log2 units; written by the row kernel),
+                               // 128 x gradient factor scaled by the tile's power of two. bf16: 128 x
+                               // (log2 |factor| - lse; by the row kernel), 128 x the factor's sign
+    float* g_scale;            // [x_tiles] f32: value of one unit of the tile's gradient factors; bf16: 1
+                               // where a factor is negative, else 0
+    int slots;                 // bf16, k <= 125: K slots k..k+2 hold the bias in three parts (weight) and 1
+                               // (features), so that the scores come with their bias
+    float* x_norm;             // slots: [x_tiles][128] |x_r|
+    float2* w_bound;           // slots: [w_tiles] (largest |w_j|, largest bias in log2 units)
     int32_t* sp_off;           // [x_tiles][2 w_tiles + 1] label ranges by class tile and half of the rows
     int2* sp_ent;              // [x_tiles][128 n_top]: (row << 7 | class within its tile, factor bits)
     int* status;
@@ -60,7 +66,9 @@ struct LossMainParams {
     const float* own_scale;    // per tile (f32)
     const float* str_scale;
     const float* col_tab;      // per streamed tile: class_e (128 floats) or row_tab (256 floats)
-    const float* lane_e;       // weight pass: class_e of the own classes
+    const float* lane_e;       // weight pass: class_e of the own classes (not with slots)
+    const float* x_norm;       // row pass, slots
+    const float2* w_bound;
     const float* g_scale;      // weight pass: per streamed tile
     const int32_t* sp_off;     // weight pass
     const int2* sp_ent;
@@ -120,7 +128,8 @@ struct LossScoreParams {
 
 cudaError_t loss_kernel_setup();
 cudaError_t launch_loss_pack(const LossPackParams& p, bool f32, cudaStream_t stream);
-cudaError_t launch_loss_main(const LossMainParams& p, bool f32, bool weight_pass, int grid, cudaStream_t stream);
+cudaError_t launch_loss_main(const LossMainParams& p, bool f32, bool slots, bool weight_pass, int grid,
+                             cudaStream_t stream);
 cudaError_t launch_loss_rows(const LossRowParams& p, bool f32, int sms, cudaStream_t stream);
 cudaError_t launch_loss_reduce(const LossReduceParams& p, bool f32, int sms, cudaStream_t stream);
 cudaError_t launch_loss_table(const float* ctab, long long n_floats, float inv_temp, float* out, cudaStream_t stream);

@@ -823,12 +823,14 @@ int guarded(F&& f) {
 // ranges of the streamed tiles. Cost of a split in streamed tiles: the last wave's length (its
 // tiles plus `overhead` for the unit's own operand, pipeline fill and hand-over), the reader's
 // join (about 1/20 tile a range) and the partial tiles' traffic (64 KB each, written and read:
-// about 1/100 tile each).
+// about 1/100 tile each). `uneven`: how much longer than the others a unit may run; in the weight
+// pass the class tile that holds most rows' label (the blank's) takes up to 1.3 times as long, so
+// its rows are better spread over several units than left to one SM.
 struct LossPlan {
     int own = 0, str = 0, whole = 0, splits = 1, per = 0, grid = 0;
     int64_t units = 0;
 };
-LossPlan loss_plan(int64_t own, int64_t str, int sms, double overhead) {
+LossPlan loss_plan(int64_t own, int64_t str, int sms, double overhead, double uneven) {
     LossPlan p;
     p.own = (int)own;
     p.str = (int)str;
@@ -840,7 +842,7 @@ LossPlan loss_plan(int64_t own, int64_t str, int sms, double overhead) {
         const int per = (p.str + s - 1) / s, eff = (p.str + per - 1) / per;
         const int64_t units = (int64_t)rest * eff, waves = (units + sms - 1) / sms;
         if (units > 4 * (int64_t)sms && s > 1) break;  // bounds the partial tiles: 64 KB a unit
-        const double cost = (double)waves * (per + overhead) + 0.05 * eff + 0.01 * (double)units;
+        const double cost = (double)waves * (per + overhead) + uneven * per + 0.05 * eff + 0.01 * (double)units;
         if (cost < best - 1e-9) {
             best = cost;
             p.splits = eff;
@@ -857,16 +859,19 @@ LossPlan loss_plan(int64_t own, int64_t str, int sms, double overhead) {
 struct LossLayout {
     LossPlan row, cls;
     int x_tiles = 0, w_tiles = 0, feat = 0;
-    size_t x_img, w_img, x_scale, w_scale, g_scale, class_e, row_tab, sp_off, sp_ent, part_o, part_ms, total;
+    bool slots = false;  // the bias rides in three spare K slots
+    size_t x_img, w_img, x_scale, w_scale, g_scale, class_e, row_tab, x_norm, w_bound, sp_off, sp_ent, part_o, part_ms,
+        total;
 };
 LossLayout loss_layout(bool f32, int64_t rows, int64_t k, int64_t n, int64_t n_top, int sms) {
     LossLayout L;
     L.x_tiles = (int)((rows + 127) / 128);
     L.w_tiles = (int)((n + 127) / 128);
-    L.feat = (int)((k + 15) / 16 * 16);
+    L.slots = !f32 && k + 3 <= rh::kPadK;
+    L.feat = (int)((k + (L.slots ? 3 : 0) + 15) / 16 * 16);
     // a unit's fixed cost, in streamed tiles: about 2.5 us against 1.7 us (f32) and 0.7 us a tile
-    L.row = loss_plan(L.x_tiles, L.w_tiles, sms, f32 ? 1.5 : 3.5);
-    L.cls = loss_plan(L.w_tiles, L.x_tiles, sms, f32 ? 1.5 : 3.5);
+    L.row = loss_plan(L.x_tiles, L.w_tiles, sms, f32 ? 1.5 : 3.5, 0.0);
+    L.cls = loss_plan(L.w_tiles, L.x_tiles, sms, f32 ? 1.5 : 3.5, 0.3);
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t here = at;
@@ -882,6 +887,8 @@ LossLayout loss_layout(bool f32, int64_t rows, int64_t k, int64_t n, int64_t n_t
     L.g_scale = take((size_t)L.x_tiles * 4);
     L.class_e = take((size_t)L.w_tiles * 512);
     L.row_tab = take((size_t)L.x_tiles * 1024);
+    L.x_norm = take(L.slots ? (size_t)L.x_tiles * 512 : 0);
+    L.w_bound = take(L.slots ? (size_t)L.w_tiles * 8 : 0);
     L.sp_off = take((size_t)L.x_tiles * (size_t)(2 * L.w_tiles + 1) * 4);
     L.sp_ent = take((size_t)L.x_tiles * 128 * (size_t)n_top * 8);
     L.part_o = take(units * (size_t)L.feat * 512);
@@ -968,6 +975,9 @@ int enqueue_grad(rh_ctx* ctx, Slot& s, int dtype, const void* d_a, int64_t rows,
     pk.class_e = (float*)(ws + L.class_e);
     pk.row_tab = (float*)(ws + L.row_tab);
     pk.g_scale = (float*)(ws + L.g_scale);
+    pk.slots = L.slots ? 1 : 0;
+    pk.x_norm = (float*)(ws + L.x_norm);
+    pk.w_bound = (float2*)(ws + L.w_bound);
     pk.sp_off = (int32_t*)(ws + L.sp_off);
     pk.sp_ent = (int2*)(ws + L.sp_ent);
     pk.status = s.d_status;
@@ -980,6 +990,8 @@ int enqueue_grad(rh_ctx* ctx, Slot& s, int dtype, const void* d_a, int64_t rows,
     m.own_scale = pk.x_scale;
     m.str_scale = pk.w_scale;
     m.col_tab = pk.class_e;
+    m.x_norm = pk.x_norm;
+    m.w_bound = pk.w_bound;
     m.own_tiles = L.x_tiles;
     m.str_tiles = L.w_tiles;
     m.n_top = lab.n_top;
@@ -992,7 +1004,7 @@ int enqueue_grad(rh_ctx* ctx, Slot& s, int dtype, const void* d_a, int64_t rows,
     m.part_ms = (float2*)(ws + L.part_ms);
     m.status = s.d_status;
     m.timeout_ns = ctx->timeout_ns;
-    RH_CUDA(rh::launch_loss_main(m, f32, false, L.row.grid, st));
+    RH_CUDA(rh::launch_loss_main(m, f32, L.slots, false, L.row.grid, st));
     s.launches++;
 
     rh::LossRowParams r{};
@@ -1032,7 +1044,7 @@ int enqueue_grad(rh_ctx* ctx, Slot& s, int dtype, const void* d_a, int64_t rows,
     m.n_splits = L.cls.splits;
     m.tiles_per_split = L.cls.per;
     m.part_o = (float*)(ws + L.part_o);
-    RH_CUDA(rh::launch_loss_main(m, f32, true, L.cls.grid, st));
+    RH_CUDA(rh::launch_loss_main(m, f32, L.slots, true, L.cls.grid, st));
     s.launches++;
 
     rh::LossReduceParams d{};
