@@ -66,62 +66,8 @@ __device__ __forceinline__ float warp_max(float v) {
     for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-
-// A row's distribution q over its labels, in one warp: lane l holds entries l and l + 32 (class c
-// or -1, q, log q). False when the row has no label (it is then ignored).
-struct RowLabels {
-    int c[2];
-    float q[2], log_q[2];
-};
-__device__ __forceinline__ bool row_labels(const LossLabels& L, long long row, int lane, RowLabels& r) {
-    r.c[0] = r.c[1] = -1;
-    r.q[0] = r.q[1] = 0.0f;
-    r.log_q[0] = r.log_q[1] = 0.0f;
-    if (L.target) {
-        const int t = L.target[row];
-        if (lane == 0 && t >= 0 && t < L.n) {
-            r.c[0] = t;
-            r.q[0] = 1.0f;
-        }
-        return t >= 0 && t < L.n;
-    }
-    float u[2], top = -CUDART_INF_F;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        const int e = lane + 32 * s;
-        u[s] = -CUDART_INF_F;
-        if (e < L.n_top) {
-            const int c = L.top_idx[row * L.n_top + e];
-            if (c >= 0 && c < L.n) {
-                r.c[s] = c;
-                u[s] = L.top_logits[row * L.n_top + e] * L.inv_temp;
-            }
-        }
-        top = fmaxf(top, u[s]);
-    }
-    if (!__any_sync(0xffffffffu, r.c[0] >= 0 || r.c[1] >= 0)) return false;
-    top = warp_max(top);
-    float sum = 0.0f;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        u[s] -= top;
-        r.q[s] = r.c[s] >= 0 ? expf(u[s]) : 0.0f;
-        sum += r.q[s];
-    }
-    sum = warp_sum(sum);
-    const float log_sum = logf(sum);
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        r.q[s] = r.c[s] >= 0 ? r.q[s] / sum : 0.0f;
-        r.log_q[s] = u[s] - log_sum;
-    }
-    return true;
-}
+// Whether class c is one of a row's labels at all.
+__device__ __forceinline__ bool is_class(int c, int n) { return c >= 0 && c < n; }
 
 }  // namespace
 
@@ -130,82 +76,44 @@ __device__ __forceinline__ bool row_labels(const LossLabels& L, long long row, i
 // the tile's power of two into [2^14, 2^15) and split into fp16 hi + lo (~22 bits below the
 // tile's maximum, which an image of fp16 alone or of bf16 parts would not hold); bf16 values are
 // copied. A row that is ignored is zero in the image, so whatever its features hold (NaN
-// included) reaches nothing. The labels of a feature tile are sorted by class tile, rows
-// ascending within each: every warp counts its 16 rows' entries per class tile, a scan turns the
-// counts into positions, and a second walk places them (no atomics: the order is fixed).
+// included) reaches nothing.
+// The labels of a feature tile are sorted by (class tile, half of the rows), rows ascending: each
+// warp takes 8 rows, a group of lanes per row, and notes for every entry how many of its bin came
+// before it in the warp; a scan over warps and bins then gives every entry its place (no atomics:
+// the order is fixed).
+constexpr int kPackThreads = 512, kPackWarps = kPackThreads / 32, kPackItems = 2048 / kPackThreads;
+
 template <bool F32>
-__global__ void __launch_bounds__(256) loss_pack_kernel(const __grid_constant__ LossPackParams p) {
+__global__ void __launch_bounds__(kPackThreads) loss_pack_kernel(const __grid_constant__ LossPackParams p) {
     using T = typename Elem<F32>::type;
-    extern __shared__ int bins[];  // [8 warps][2 w_tiles] counts, then [2 w_tiles] starts
-    __shared__ float red[8], red2[8];
-    __shared__ float s_g[128], s_norm[128];
+    extern __shared__ __align__(16) uint8_t pack_smem[];
+    __shared__ float red[kPackWarps], red2[4];
+    __shared__ float s_norm[128];
     __shared__ uint8_t s_valid[128];
-    __shared__ int s_scan[8];
+    __shared__ int s_scan[kPackWarps];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const bool is_w = (int)blockIdx.x < p.w_tiles;
     const int tile = is_w ? (int)blockIdx.x : (int)blockIdx.x - p.w_tiles;
     const long long row0 = (long long)tile * kLossTile;
     const long long n_rows = is_w ? p.lab.n : p.rows;
 
-    float gs = 1.0f;  // scale of this tile's gradient factors
-    if (!is_w) {
-        float f = 0.0f;
-        if (tid < 128) {
-            const long long row = row0 + tid;
-            bool valid = false, bad = false;
-            if (row < p.rows) {
-                const int* c = p.lab.target ? p.lab.target + row : p.lab.top_idx + row * p.lab.n_top;
-                for (int e = 0; e < p.lab.n_top; ++e) {
-                    valid |= c[e] >= 0 && c[e] < p.lab.n;
-                    bad |= c[e] >= p.lab.n;
-                }
-            }
-            if (bad) atomicOr(p.status, kDevBadClass);
-            s_valid[tid] = valid ? 1 : 0;
-            if (valid) f = p.lab.temp * (p.row_grad ? p.row_grad[row] : 1.0f);
-        }
-        if (F32) {
-            const float m = warp_max(fabsf(f));
-            if (lane == 0) red[warp] = m;
-            __syncthreads();
-            float top = red[0];
-#pragma unroll
-            for (int i = 1; i < 4; ++i) top = fmaxf(top, red[i]);
-            const int sh = shift_to(top, 13);
-            gs = pow2i(sh);
-            if (tid == 0) p.g_scale[tile] = pow2i(-sh);
-        } else {
-            const int neg = __syncthreads_or(f < 0.0f);
-            if (tid == 0) p.g_scale[tile] = neg ? 1.0f : 0.0f;
-        }
-        if (tid < 128) {
-            s_g[tid] = f * gs;
-            p.row_tab[(size_t)tile * 256 + 128 + tid] = F32 ? f * gs : copysignf(1.0f, f);
-        }
-        __syncthreads();
-    } else if (tid < 128) {
-        const long long j = row0 + tid;
-        p.class_e[(size_t)tile * 128 + tid] =
-            j < p.lab.n ? (p.bias ? p.bias[j] * p.logit_scale : 0.0f) : -CUDART_INF_F;
-    }
-
-    // 2,048 chunks of 8 K slots, 8 per thread: row-major operands with neighbouring threads on
+    // 2,048 chunks of 8 K slots, 4 per thread: row-major operands with neighbouring threads on
     // neighbouring chunks, the [b][k][t] layout with neighbouring threads on neighbouring rows.
     const long long t_len = is_w ? 0 : p.t_len;
     const T* src = static_cast<const T*>(is_w ? p.w : p.x);
     const bool vec = t_len == 0 && (reinterpret_cast<uintptr_t>(src) & 15u) == 0 && p.k % (F32 ? 4 : 8) == 0;
-    float v[8][8];
-    float top = 0.0f;
+    auto item_row = [&](int i) { return t_len > 0 ? tid & 127 : i * (kPackThreads / 16) + (tid >> 4); };
+    auto item_chunk = [&](int i) { return t_len > 0 ? i * (kPackThreads / 128) + (tid >> 7) : tid & 15; };
+    const long long kt_base = t_len > 0 && row0 + (tid & 127) < n_rows ? x_base(row0 + (tid & 127), p.k, t_len) : 0;
+    float v[kPackItems][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int item = i * 256 + tid;
-        const int r = t_len > 0 ? item & 127 : item >> 4, ch = t_len > 0 ? item >> 7 : item & 15;
+    for (int i = 0; i < kPackItems; ++i) {
+        const int r = item_row(i), ch = item_chunk(i);
         const long long row = row0 + r;
-        const bool ok = row < n_rows && (is_w || s_valid[r]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
-        if (ok && 8 * ch < p.k) {
-            const T* a = src + x_base(row, p.k, t_len) + (t_len > 0 ? 8 * ch * t_len : 8 * ch);
+        if (row < n_rows && 8 * ch < p.k) {
+            const T* a = src + (t_len > 0 ? kt_base + 8 * ch * t_len : row * p.k + 8 * ch);
             if (vec && 8 * ch + 8 <= p.k) {
                 if constexpr (F32) {
                     const float4 lo = *reinterpret_cast<const float4*>(a), hi = *reinterpret_cast<const float4*>(a + 4);
@@ -227,32 +135,176 @@ __global__ void __launch_bounds__(256) loss_pack_kernel(const __grid_constant__ 
                     if (8 * ch + j < p.k) v[i][j] = to_f32(a[j * step]);
             }
         }
+    }
+
+    // ---- labels: which rows count, their factors, and (weight gradient) the entries with their
+    // place among the warp's own of the same bin
+    const int nb = 2 * p.w_tiles;                                  // (class tile, rows below 64 or above)
+    uint16_t* counts = reinterpret_cast<uint16_t*>(pack_smem);     // [16 warps][nb]
+    int* start = reinterpret_cast<int*>(pack_smem + kPackWarps * 2 * (size_t)nb);  // [nb]
+    int2* ents = reinterpret_cast<int2*>(start + nb);              // [128][n_top]: (class << 10 | place, factor)
+    const bool sort = !is_w && p.sort_labels;
+    if (sort) {
+        for (int i = tid; i < kPackWarps * nb / 2; i += kPackThreads) reinterpret_cast<uint32_t*>(counts)[i] = 0u;
+        __syncthreads();
+    }
+    if (!is_w) {
+        // lanes per row: the power of two that holds the entries (two each beyond 32)
+        const int width = p.lab.n_top > 16 ? 32 : p.lab.n_top > 8 ? 16 : p.lab.n_top > 4 ? 8 : p.lab.n_top > 1 ? 4 : 1;
+        const int per = min(8, 32 / width), sub = lane & (width - 1), grp = lane / width;
+        const int slots = p.lab.n_top > 32 ? 2 : 1;
+        uint16_t* mine = counts + (size_t)warp * nb;
+        for (int r0 = 0; r0 < 8; r0 += per) {
+            const int r = warp * 8 + r0 + grp;
+            const long long row = row0 + r;
+            const bool live = grp < per && row < p.rows;
+            int c[2] = {-1, -1};
+            float u[2] = {-CUDART_INF_F, -CUDART_INF_F}, q[2] = {0.0f, 0.0f};
+            bool bad = false;
+            float g = 0.0f;
+            if (live) {
+                for (int s = 0; s < slots; ++s) {
+                    const int e = sub + 32 * s;
+                    if (e < p.lab.n_top) {
+                        const int x = p.lab.target ? p.lab.target[row] : p.lab.top_idx[row * p.lab.n_top + e];
+                        bad |= x >= p.lab.n;
+                        if (is_class(x, p.lab.n)) {
+                            c[s] = x;
+                            u[s] = p.lab.target ? 0.0f : p.lab.top_logits[row * p.lab.n_top + e] * p.lab.inv_temp;
+                        }
+                    }
+                }
+                g = p.row_grad ? p.row_grad[row] : 1.0f;
+            }
+            if (bad) atomicOr(p.status, kDevBadClass);
+            const uint32_t have = __ballot_sync(0xffffffffu, c[0] >= 0 || c[1] >= 0);
+            const uint32_t gm = (width == 32 ? 0xffffffffu : ((1u << width) - 1u) << (grp * width));
+            const bool valid = (have & gm) != 0u;
+            const float f = valid ? p.lab.temp * g : 0.0f;
+            if (grp < per && sub == 0) {
+                s_valid[r] = valid ? 1 : 0;
+                s_norm[r] = f;  // the factors, until the norms need the place
+            }
+            if (!sort) continue;
+            float top = fmaxf(u[0], u[1]);
+            for (int o = width >> 1; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            float sum = 0.0f;
+            for (int s = 0; s < slots; ++s) {
+                q[s] = c[s] >= 0 ? expf(u[s] - top) : 0.0f;
+                sum += q[s];
+            }
+            for (int o = width >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            float share[2] = {c[0] >= 0 ? q[0] / sum : 0.0f, c[1] >= 0 ? q[1] / sum : 0.0f};
+            if (p.lab.n_top > 1) {  // a class named twice: one entry with both shares
+                bool dup[2] = {false, false};
+                float all[2] = {share[0], share[1]};
+                for (int j = 0; j < p.lab.n_top; ++j) {
+                    const int from = grp * width + (j & (width - 1));
+                    const int cj = __shfl_sync(0xffffffffu, j < 32 ? c[0] : c[1], from);
+                    const float qj = __shfl_sync(0xffffffffu, j < 32 ? share[0] : share[1], from);
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        const int e = sub + 32 * s;
+                        if (cj >= 0 && cj == c[s] && j != e) {
+                            if (j < e)
+                                dup[s] = true;
+                            else
+                                all[s] += qj;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    share[s] = all[s];
+                    if (dup[s]) c[s] = -1;
+                }
+            }
+            for (int s = 0; s < slots; ++s) {
+                const int e = sub + 32 * s;
+                const int bin = c[s] >= 0 ? 2 * (c[s] >> 7) + (r >> 6) : -1;
+                const uint32_t same = __match_any_sync(0xffffffffu, bin);
+                const int rank = __popc(same & ((1u << lane) - 1u));
+                int at = 0;
+                if (bin >= 0) {
+                    at = mine[bin];
+                    __syncwarp(same);
+                    if (rank == 0) mine[bin] = (uint16_t)(at + __popc(same));
+                }
+                __syncwarp();
+                if (live && e < p.lab.n_top)
+                    ents[r * p.lab.n_top + e] =
+                        make_int2(c[s] >= 0 ? (c[s] << 10) | (at + rank) : -1, __float_as_int(-share[s] * f));
+            }
+        }
+        __syncthreads();
+    }
+    float gs = 1.0f;  // scale of this tile's gradient factors
+    if (!is_w) {
+        const float f = tid < 128 ? s_norm[tid] : 0.0f;
         if (F32) {
+            const float m = warp_max(fabsf(f));
+            if (lane == 0) red[warp] = m;
+            __syncthreads();
+            const int sh = shift_to(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), 13);
+            gs = pow2i(sh);
+            if (tid == 0) p.g_scale[tile] = pow2i(-sh);
+        } else {
+            const int neg = __syncthreads_or(f < 0.0f);
+            if (tid == 0) p.g_scale[tile] = neg ? 1.0f : 0.0f;
+        }
+        if (tid < 128) p.row_tab[(size_t)tile * 256 + 128 + tid] = F32 ? f * gs : copysignf(1.0f, f);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kPackItems; ++i) {
+            if (row0 + item_row(i) < n_rows && !s_valid[item_row(i)]) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+            }
+        }
+    } else if (tid < 128) {
+        const long long j = row0 + tid;
+        p.class_e[(size_t)tile * 128 + tid] =
+            j < p.lab.n ? (p.bias ? p.bias[j] * p.logit_scale : 0.0f) : -CUDART_INF_F;
+    }
+
+    // ---- scale and images
+    float up = 1.0f;
+    if (F32) {
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kPackItems; ++i) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[i][j]));
         }
-    }
-    if (!F32 && p.slots) {
-        // |row|: row-major operands have a row's 16 chunks in 16 neighbouring lanes, the other layout
-        // has the even and the odd ones in two threads; both add them up in the same tree
-        float q[8];
+        top = warp_max(top);
+        if (lane == 0) red[warp] = top;
+        __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < kPackWarps; ++i) top = fmaxf(top, red[i]);
+        const int sh = shift_to(top, 14);
+        up = pow2i(sh);
+        if (tid == 0) (is_w ? p.w_scale : p.x_scale)[tile] = pow2i(-sh);
+    } else if (p.slots) {
+        // |row|: row-major operands have a row's 16 chunks in 16 neighbouring lanes, the other layout
+        // has every fourth one in each of four threads; both add them up in the same tree
+        float q[kPackItems];
+#pragma unroll
+        for (int i = 0; i < kPackItems; ++i) {
             q[i] = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) q[i] = fmaf(v[i][j], v[i][j], q[i]);
         }
         if (t_len > 0) {
-            const float sum = ((q[0] + q[4]) + (q[2] + q[6])) + ((q[1] + q[5]) + (q[3] + q[7]));
-            if (tid < 128) s_norm[tid] = sum;
+            float* part = reinterpret_cast<float*>(pack_smem) + p.norm_smem;  // [4][128]
+            part[tid] = (q[0] + q[2]) + (q[1] + q[3]);
             __syncthreads();
-            if (tid >= 128) s_norm[tid - 128] += sum;
+            if (tid < 128) s_norm[tid] = (part[tid] + part[256 + tid]) + (part[128 + tid] + part[384 + tid]);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < kPackItems; ++i) {
 #pragma unroll
                 for (int o = 8; o > 0; o >>= 1) q[i] += __shfl_xor_sync(0xffffffffu, q[i], o);
-                if ((tid & 15) == 0) s_norm[i * 16 + (tid >> 4)] = q[i];
+                if ((tid & 15) == 0) s_norm[item_row(i)] = q[i];
             }
         }
         __syncthreads();
@@ -264,64 +316,22 @@ __global__ void __launch_bounds__(256) loss_pack_kernel(const __grid_constant__ 
             // (a NaN norm or bias has to survive the maximum: it then rules the bound out)
             const float wn = warp_max(norm), we = warp_max(e);
             const int bad = __syncthreads_or(real && (isnan(norm) || isnan(e)));
-            if (lane == 0) {
+            if (lane == 0 && warp < 4) {
                 red[warp] = wn;
                 red2[warp] = we;
             }
             __syncthreads();
-            if (tid == 0) {
-                float a = red[0], b = red2[0];
-                for (int i = 1; i < 4; ++i) {
-                    a = fmaxf(a, red[i]);
-                    b = fmaxf(b, red2[i]);
-                }
-                p.w_bound[tile] = make_float2(bad ? CUDART_NAN_F : a, b);
-            }
+            if (tid == 0)
+                p.w_bound[tile] = make_float2(bad ? CUDART_NAN_F : fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])),
+                                              fmaxf(fmaxf(red2[0], red2[1]), fmaxf(red2[2], red2[3])));
         } else if (tid < 128) {
             p.x_norm[(size_t)tile * 128 + tid] = norm;
         }
-        // the bias (natural units) in three bf16 parts, against ones in the features: the parts'
-        // products with 1 are exact, so a score carries its bias to 24 bits. Padding classes: -inf.
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int item = i * 256 + tid;
-            const int r = t_len > 0 ? item & 127 : item >> 4, ch = t_len > 0 ? item >> 7 : item & 15;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int part = 8 * ch + j - p.k;
-                if (part < 0 || part > 2) continue;
-                if (!is_w) {
-                    v[i][j] = 1.0f;
-                    continue;
-                }
-                float rest = row0 + r < p.lab.n ? (p.bias ? p.bias[row0 + r] : 0.0f) : -CUDART_INF_F;
-                float here = 0.0f;
-                for (int a = 0; a <= part; ++a) {
-                    here = __bfloat162float(__float2bfloat16_rn(rest));
-                    rest = isfinite(here) ? rest - here : 0.0f;
-                }
-                v[i][j] = here;
-            }
-        }
-    }
-    float up = 1.0f;
-    if (F32) {
-        top = warp_max(top);
-        __syncthreads();  // red is read above
-        if (lane == 0) red[warp] = top;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, red[i]);
-        const int sh = shift_to(top, 14);
-        up = pow2i(sh);
-        if (tid == 0) (is_w ? p.w_scale : p.x_scale)[tile] = pow2i(-sh);
     }
     uint8_t* img = (is_w ? p.w_img : p.x_img) + (size_t)tile * (F32 ? 2 * kLossImage : kLossImage);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int item = i * 256 + tid;
-        const int r = t_len > 0 ? item & 127 : item >> 4, ch = t_len > 0 ? item >> 7 : item & 15;
-        const uint32_t off = image_chunk(r, ch);
+    for (int i = 0; i < kPackItems; ++i) {
+        const uint32_t off = image_chunk(item_row(i), item_chunk(i));
         uint32_t h[4], l[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -340,93 +350,60 @@ __global__ void __launch_bounds__(256) loss_pack_kernel(const __grid_constant__ 
         *reinterpret_cast<uint4*>(img + off) = make_uint4(h[0], h[1], h[2], h[3]);
         if constexpr (F32) *reinterpret_cast<uint4*>(img + kLossImage + off) = make_uint4(l[0], l[1], l[2], l[3]);
     }
-    if (is_w || !p.sort_labels) return;
+    if (!F32 && p.slots) {
+        // the bias (natural units) in three bf16 parts, against ones in the features: the parts'
+        // products with 1 are exact, so a score carries its bias to 24 bits. Padding classes: -inf.
+        __syncthreads();  // the chunks that hold the slots are written above, by other threads
+        if (tid < 128) {
+            float rest = row0 + tid < p.lab.n ? (is_w && p.bias ? p.bias[row0 + tid] : 0.0f) : -CUDART_INF_F;
+            for (int part = 0; part < 3; ++part) {
+                const __nv_bfloat16 here = __float2bfloat16_rn(is_w ? rest : 1.0f);
+                rest = isfinite(__bfloat162float(here)) ? rest - __bfloat162float(here) : 0.0f;
+                const int kk = p.k + part;
+                *reinterpret_cast<__nv_bfloat16*>(img + image_chunk(tid, kk >> 3) + 2 * (kk & 7)) = here;
+            }
+        }
+    }
+    if (!sort) return;
 
-    // ------------------------------------------------------------ labels by class tile
-    const int nb = 2 * p.w_tiles;  // (class tile, rows below 64 or above): a softmax warpgroup's share each
-    int* start = bins + 8 * nb;
-    for (int i = tid; i < 8 * nb; i += 256) bins[i] = 0;
+    // ---- the entries' places: counts -> each warp's first position within its bin, bins' starts
+    const int per = (nb + kPackThreads - 1) / kPackThreads, b0 = tid * per, b1 = min(nb, b0 + per);
+    int sum = 0;
+    for (int b = b0; b < b1; ++b) {
+        int tot = 0;
+        for (int w = 0; w < kPackWarps; ++w) {
+            const int c = counts[(size_t)w * nb + b];
+            counts[(size_t)w * nb + b] = (uint16_t)tot;
+            tot += c;
+        }
+        start[b] = sum;
+        sum += tot;
+    }
+    int incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+    }
+    if (lane == 31) s_scan[warp] = incl;
     __syncthreads();
-    int* mine = bins + warp * nb;
-    int2* ent = p.sp_ent + (size_t)tile * 128 * p.lab.n_top;
-    for (int pass = 0; pass < 2; ++pass) {
-        for (int rr = 0; rr < 16; ++rr) {
-            const int r = warp * 16 + rr;
-            if (!s_valid[r]) continue;
-            RowLabels lab;
-            row_labels(p.lab, row0 + r, lane, lab);
-            if (p.lab.n_top > 1) {  // a class named twice: one entry with both shares
-                float q[2] = {lab.q[0], lab.q[1]};
-                bool dup[2] = {false, false};
-                for (int j = 0; j < p.lab.n_top; ++j) {
-                    const int cj = __shfl_sync(0xffffffffu, j < 32 ? lab.c[0] : lab.c[1], j & 31);
-                    const float qj = __shfl_sync(0xffffffffu, j < 32 ? lab.q[0] : lab.q[1], j & 31);
-#pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        const int e = lane + 32 * s;
-                        if (cj >= 0 && cj == lab.c[s] && j != e) {
-                            if (j < e)
-                                dup[s] = true;
-                            else
-                                q[s] += qj;
-                        }
-                    }
-                }
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    lab.q[s] = q[s];
-                    if (dup[s]) lab.c[s] = -1;
-                }
-            }
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                if (32 * s >= p.lab.n_top) break;
-                const int bin = lab.c[s] >= 0 ? 2 * (lab.c[s] >> 7) + (r >> 6) : -1;
-                const uint32_t same = __match_any_sync(0xffffffffu, bin);
-                const int rank = __popc(same & ((1u << lane) - 1u));
-                if (bin >= 0) {
-                    const int at = mine[bin];
-                    if (pass == 1)
-                        ent[start[bin] + at + rank] =
-                            make_int2((r << 7) | (lab.c[s] & 127), __float_as_int(-lab.q[s] * s_g[r]));
-                    __syncwarp(same);
-                    if (rank == 0) mine[bin] = at + __popc(same);
-                }
-                __syncwarp();
-            }
-        }
-        if (pass == 1) break;
-        __syncthreads();
-        // counts -> each warp's first position within its bin, and the bins' starts
-        const int per = (nb + 255) / 256, b0 = tid * per, b1 = min(nb, b0 + per);
-        int sum = 0;
-        for (int b = b0; b < b1; ++b) {
-            int tot = 0;
-            for (int w = 0; w < 8; ++w) {
-                const int c = bins[w * nb + b];
-                bins[w * nb + b] = tot;
-                tot += c;
-            }
-            start[b] = sum;
-            sum += tot;
-        }
-        int incl = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += y;
-        }
-        if (lane == 31) s_scan[warp] = incl;
-        __syncthreads();
-        int base = incl - sum;
-        for (int w = 0; w < warp; ++w) base += s_scan[w];
-        int32_t* off = p.sp_off + (size_t)tile * (nb + 1);
-        for (int b = b0; b < b1; ++b) {
-            start[b] += base;
-            off[b] = start[b];
-        }
-        if (tid == 255) off[nb] = base + sum;
-        __syncthreads();
+    int base = incl - sum;
+    for (int w = 0; w < warp; ++w) base += s_scan[w];
+    int32_t* off = p.sp_off + (size_t)tile * (nb + 1);
+    for (int b = b0; b < b1; ++b) {
+        start[b] += base;
+        off[b] = start[b];
+    }
+    if (tid == kPackThreads - 1) off[nb] = base + sum;
+    __syncthreads();
+    int2* out = p.sp_ent + (size_t)tile * 128 * p.lab.n_top;
+    const int live = (int)min((long long)128, p.rows - row0) * p.lab.n_top;
+    for (int i = tid; i < live; i += kPackThreads) {
+        const int2 e = ents[i];
+        if (e.x < 0) continue;
+        const int r = i / p.lab.n_top, c = e.x >> 10, bin = 2 * (c >> 7) + (r >> 6);
+        out[start[bin] + counts[(size_t)(r >> 3) * nb + bin] + (e.x & 1023)] =
+            make_int2((r << 7) | (c & 127), __float_as_int(__int_as_float(e.y) * gs));
     }
 }
 
@@ -434,12 +411,14 @@ __global__ void __launch_bounds__(256) loss_pack_kernel(const __grid_constant__ 
 namespace {
 
 // Warps: 0 producer, 1 tensor-core issuer (and TMEM), 2-3 idle; four softmax warpgroups (warps
-// 4-19): two for the even and two for the odd streamed tiles of a unit, 64 columns each (score
-// buffer = parity); two adding warpgroups (20-27), 64 features of every tile's second product each.
-// Softmax and adding are apart so that a softmax warpgroup goes on to its next tile without waiting
-// for the tensor core to use its last; two warpgroups a tile halve the time from scores to
-// probabilities, which the tensor core waits for whenever it exceeds the two products it can run
-// meanwhile.
+// 4-19): two for the even and two for the odd streamed tiles of a unit, 64 columns each; two adding
+// warpgroups (20-27), 64 features of every tile's second product each. Softmax and adding are apart
+// so that a softmax warpgroup goes on to its next tile without waiting for the tensor core to use
+// its last. Scores live in a ring of 128-column buffers: two in f32, whose own operand (hi | lo)
+// takes 128 TMEM columns; three in bf16, whose own operand stays in shared memory, so that the next
+// scores are there when a softmax warpgroup comes for them. (An operand in TMEM costs the tensor
+// core less shared-memory bandwidth; f32 is bound by the tensor core, bf16 is not. Narrower buffers
+// are no way out: an instruction of 64 columns takes as long as one of 128.)
 constexpr int kMainThreads = 896;
 constexpr int kLaunchRegs = 72;  // 65,536 registers / 896 threads
 constexpr int kCtrlRegs = 40, kSoftRegs = 72, kAddRegs = 88;
@@ -448,42 +427,46 @@ static_assert(128 * kCtrlRegs + 512 * kSoftRegs + 256 * kAddRegs <= kMainThreads
 template <bool F32>
 struct Ring {
     static constexpr uint32_t kStage = F32 ? 2u * kLossImage : kLossImage;
-    static constexpr uint32_t kStages = F32 ? 3u : 5u;
-    static constexpr uint32_t kTab = kStage * kStages;  // column tables, 1 KB a stage
+    static constexpr uint32_t kStages = F32 ? 3u : 4u;
+    static constexpr uint32_t kTab = kStage * kStages;              // column tables, 1 KB a stage
+    static constexpr uint32_t kOwn = kTab + 1024u * kStages;        // bf16: two images of the own operand
+    static constexpr uint32_t kEnd = kOwn + (F32 ? 0u : 2u * kLossImage);
+    static constexpr uint32_t kBufs = F32 ? 2u : 3u;                // score buffers of 128 TMEM columns
+    static constexpr uint32_t kTS = F32 ? 128u : 0u;                // their first column (f32: after the own operand)
 };
-constexpr uint32_t kMOffBars = 196608 + 3 * 1024;  // after the stages and their column tables
+constexpr uint32_t kMOffBars = 200704;             // after the stages, their column tables and own images
 constexpr uint32_t kMOffMisc = kMOffBars + 512;   // [0] TMEM base, [1] abort flag
 constexpr uint32_t kMOffMs = kMOffMisc + 64;      // [4][128] float2: the softmax warpgroups' row state
 constexpr uint32_t kMOffUnion = kMOffMs + 4096;
 constexpr uint32_t kMOffRing = kMOffUnion;         // row pass: [4 tiles][128] f32, offset of a tile's probabilities
-constexpr uint32_t kMOffTop = kMOffUnion + 2048;   // row pass: [4][128] f32, maxima of a tile's two halves
+constexpr uint32_t kMOffTop = kMOffUnion + 2048;   // row pass: [2][4][128] f32, maxima of a tile's two halves
 constexpr uint32_t kPatchRow = 12;                 // floats per class row of a label patch (8 used:
                                                    // the 16-byte rows then fall on distinct banks)
 constexpr uint32_t kMOffPatch = kMOffUnion;        // weight pass: [16 warps][32][kPatchRow] f32
 constexpr uint32_t kMSmemUsed = kMOffPatch + 16 * 32 * kPatchRow * 4;
 constexpr uint32_t kMSmemBytes = kMSmemUsed + 1024;
-static_assert(Ring<true>::kStages * (Ring<true>::kStage + 1024) <= kMOffBars &&
-                  Ring<false>::kStages * (Ring<false>::kStage + 1024) <= kMOffBars,
-              "stages and tables fit");
+static_assert(Ring<true>::kEnd <= kMOffBars && Ring<false>::kEnd <= kMOffBars && Ring<false>::kOwn % 1024 == 0, "shared memory map");
 static_assert(kMSmemBytes <= 227 * 1024, "shared memory per CTA");
 
-constexpr int kLBarFull = 0;               // [6] tile and column table landed
-constexpr int kLBarEmpty = 6;              // [6] the tile's products done, its softmax warps done with the table
-constexpr int kLBarAFull = 12;             // own operand in TMEM
-constexpr int kLBarAEmpty = 13;            // the unit's products done with it
-constexpr int kLBarSFull = 14;             // [2] scores of a tile in TMEM
-constexpr int kLBarPFull = 16;             // [2] its probabilities in their place
-constexpr int kLBarOFull = 18;             // the tile's second product in TMEM
-constexpr int kLBarOEmpty = 19;            // added up, the buffer free
-constexpr int kLBarRing = 20;              // [4] a tile's offsets written
-constexpr int kLBarMsFull = 24;            // row states of a unit written
-constexpr int kLBarMsEmpty = 25;           // and read
-constexpr int kLBarTop = 26;               // [2 parities][4 quadrants] both halves' maxima written
-constexpr int kLBarDone = 34;              // every product retired (teardown)
+constexpr int kLBarFull = 0;               // [4] tile and column table landed
+constexpr int kLBarEmpty = 4;              // [4] the tile's products done, its softmax warps done with the table
+constexpr int kLBarAFull = 8;              // [2] own operand in place (f32: [0] only)
+constexpr int kLBarAEmpty = 10;            // [2] the unit's products done with it
+constexpr int kLBarSFull = 12;             // [3] scores of a buffer in TMEM
+constexpr int kLBarPFull = 15;             // [3][2 halves] its probabilities in their place
+constexpr int kLBarOFull = 21;             // the tile's second product in TMEM
+constexpr int kLBarOEmpty = 22;            // added up, the buffer free
+constexpr int kLBarRing = 23;              // [4] a tile's offsets written
+constexpr int kLBarMsFull = 27;            // row states of a unit written
+constexpr int kLBarMsEmpty = 28;           // and read
+constexpr int kLBarTop = 29;               // [2 parities][4 quadrants] both halves' maxima written
+constexpr int kLBarDone = 37;              // every product retired (teardown)
 static_assert(8 * (kLBarDone + 1) <= 512, "barrier area");
 
-// TMEM columns: own operand (hi | lo), score buffers, second product
-constexpr uint32_t kTOwn = 0, kTS = 128, kTO = 384;
+// TMEM columns: f32 own operand from 0, score buffers (Ring), second product
+constexpr uint32_t kTOwn = 0, kTO = 384;
+static_assert(Ring<true>::kTS + 128 * Ring<true>::kBufs <= kTO && Ring<false>::kTS + 128 * Ring<false>::kBufs <= kTO,
+              "TMEM columns");
 constexpr uint32_t kLSleepNs = 20000;
 
 struct Waiter {
@@ -507,6 +490,13 @@ __device__ __forceinline__ bool loss_wait_slow(uint32_t bar, uint32_t parity, vo
             return false;
         }
     }
+}
+// The issuer's wait polls a while before it sleeps: its wake-up is on every tile's critical path.
+__device__ __forceinline__ bool issuer_wait(uint32_t bar, uint32_t parity, const Waiter& w, int where) {
+    bool ok = false;
+    for (int i = 0; i < 64 && !ok; ++i) ok = mbar_try_wait(bar, parity);
+    if (!ok) ok = loss_wait_slow(bar, parity, w.abort_flag, w.status, w.timeout_ns, where);
+    return __all_sync(0xffffffffu, ok);
 }
 // Uniform over the (converged) warp.
 __device__ __forceinline__ bool loss_wait(uint32_t bar, uint32_t parity, const Waiter& w, int where) {
@@ -567,31 +557,42 @@ __device__ __forceinline__ void store_probs(uint32_t taddr, const float2 (&g)[8]
     }
 }
 
-// A tile's labels (weight pass), a window of 32 at a time: each lane holds one entry of the current
-// window and one of the next, which is in flight meanwhile.
+// A half tile's labels (weight pass), a window of 32 at a time, rows ascending: each lane holds one
+// entry of the current window and one of the next, which is in flight meanwhile.
 struct LabelWindow {
-    int2 e, n;      // (row << 7 | class, factor); consumed or absent: row beyond the tile
-    int next, end;  // first entry after the current window
+    int2 e, n;        // (row << 7 | class, factor)
+    int next, end;    // first entry after the current window
+    uint32_t groups;  // groups of 8 rows in which this warp's classes have an entry of the window
+    int last;         // group of the window's last entry where entries follow it, else beyond any group
+    bool hit;         // this lane's entry is one of this warp's classes'
 };
 constexpr int kNoLabel = 0x7fffffff;
 __device__ __forceinline__ int2 window_entry(const LabelWindow& w, int at, const int2* ent) {
     return at < w.end ? __ldg(ent + at) : make_int2(kNoLabel, 0);
 }
+// Both windows' loads; window_use then looks at the first, when it is needed.
 __device__ __forceinline__ void window_open(LabelWindow& w, const int2* ent, int lane) {
     w.e = window_entry(w, w.next + lane, ent);
     w.next += 32;
     w.n = window_entry(w, w.next + lane, ent);
 }
-__device__ __forceinline__ void window_next(LabelWindow& w, const int2* ent, int lane) {
+__device__ __forceinline__ void window_use(LabelWindow& w, int quad) {
+    w.hit = w.e.x != kNoLabel && ((w.e.x & 127) >> 5) == quad;
+    const int group = (w.e.x >> 10) & 7;
+    w.groups = __reduce_or_sync(0xffffffffu, w.hit ? 1u << group : 0u);
+    w.last = w.next < w.end ? __shfl_sync(0xffffffffu, group, 31) : 8;
+}
+__device__ __forceinline__ void window_next(LabelWindow& w, const int2* ent, int lane, int quad) {
     w.e = w.n;
     w.next += 32;
     w.n = window_entry(w, w.next + lane, ent);
+    window_use(w, quad);
 }
 
 }  // namespace
 
 // Units (own tile, range of streamed tiles), persistent over the grid. Per streamed tile: scores
-// S = own . tile^T (tensor core, own operand in TMEM), a softmax warpgroup turns them into
+// S = own . tile^T (tensor core), a softmax warpgroup turns them into
 // probabilities (row pass: against the running maximum; weight pass: 2^(s - lse) times the rows'
 // gradient factors, less the labels' shares) in the same TMEM columns, and a second product
 // O = P . tile reads the same tile the other way round. O is added to registers tile by tile: the
@@ -619,15 +620,18 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
     const bool with_o = p.part_o != nullptr;
 
     if (threadIdx.x == 0) {
-        for (uint32_t s = 0; s < 6; ++s) {
+        for (int s = 0; s < 4; ++s) {
             mbar_init(bar(kLBarFull + s), 1);
             mbar_init(bar(kLBarEmpty + s), 9);  // the product's commit, eight warps
         }
-        mbar_init(bar(kLBarAFull), 512);
-        mbar_init(bar(kLBarAEmpty), 1);
         for (int i = 0; i < 2; ++i) {
+            mbar_init(bar(kLBarAFull + i), F32 ? 512 : 1);  // bf16: one bulk copy
+            mbar_init(bar(kLBarAEmpty + i), 1);
+        }
+        for (int i = 0; i < 3; ++i) {
             mbar_init(bar(kLBarSFull + i), 1);
-            mbar_init(bar(kLBarPFull + i), 8);
+            mbar_init(bar(kLBarPFull + 2 * i), 4);
+            mbar_init(bar(kLBarPFull + 2 * i + 1), 4);
         }
         mbar_init(bar(kLBarOFull), 1);
         mbar_init(bar(kLBarOEmpty), 8);
@@ -655,10 +659,22 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
         setmaxnreg_dec<kCtrlRegs>();
         if (warp == 0) {
             // ------------------------------------------------------------ producer
-            uint32_t cc = 0, issued = 0;
+            uint32_t cc = 0, issued = 0, uc = 0, owns = 0;
             bool ok = true;
-            for (int u = blockIdx.x; ok && lunit_exists(u, p); u += gridDim.x) {
+            for (int u = blockIdx.x; ok && lunit_exists(u, p); u += gridDim.x, ++uc) {
                 const LUnit U = lunit(u, p);
+                if (!F32) {  // the unit's own image, in the slot that the unit before the last has left
+                    const uint32_t w = uc & 1u;
+                    ok = loss_wait(bar(kLBarAEmpty + w), ((uc >> 1) & 1u) ^ 1u, wt, 114);
+                    if (!ok) break;
+                    if (elect_one()) {
+                        mbar_arrive_expect_tx(bar(kLBarAFull + w), kLossImage);
+                        bulk_copy_g2s(base + Ring<F32>::kOwn + w * kLossImage, p.own + (size_t)U.own * kLossImage, kLossImage,
+                                      bar(kLBarAFull + w));
+                    }
+                    __syncwarp();
+                    owns = uc + 1;
+                }
                 for (int c = U.c0; c < U.c1; ++c, ++cc) {
                     const uint32_t s = cc % kStages;
                     ok = loss_wait(bar(kLBarEmpty + s), ((cc / kStages) & 1u) ^ 1u, wt, 101);
@@ -673,67 +689,80 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                     issued = cc + 1;
                 }
             }
-            for (uint32_t s = 0; s < kStages && s < issued; ++s)  // no copy outlives the CTA
+            // no copy outlives the CTA
+            for (uint32_t s = 0; s < kStages && s < issued; ++s)
                 loss_drain(bar(kLBarFull + s), ((issued - 1 - s) / kStages) & 1u, wt);
+            for (uint32_t w = 0; w < 2 && w < owns; ++w) loss_drain(bar(kLBarAFull + w), ((owns - 1 - w) / 2) & 1u, wt);
         } else if (warp == 1) {
             // ---------------------------------------------------------- tensor-core issuer
             // Ring positions advance by increments: this loop is the tensor core's only feed.
             const uint32_t id_s = idesc_16b(!F32, false, 128, 128);
             const uint32_t id_o = idesc_16b(!F32, true, 128, (uint32_t)feat);
             const uint64_t k_desc = smem_desc_k_sw128(base), mn_desc = smem_desc_mn_sw128(base);
-            constexpr uint64_t kStageDesc = kStage >> 4, kLoDesc = kLossImage >> 4;
-            uint32_t ss = 0, sph = 0;   // stage (and phase) of the next scores
-            uint32_t os = 0, oph = 1;   // stage of the next second product; phase of its buffer's release
-            uint32_t pph = 0, uc = 0;   // bit w: phase of warpgroup w's next probabilities
-            auto scores = [&](uint32_t w) -> bool {
-                if (!loss_wait(bar(kLBarFull + ss), sph, wt, 102)) return false;
+            constexpr uint64_t kStageDesc = kStage >> 4, kLoDesc = kLossImage >> 4, kHalfDesc = 8192 >> 4;  // 64 rows
+            constexpr uint32_t kBufs = Ring<F32>::kBufs;
+            uint32_t ss = 0, sph = 0, sb = 0;  // stage (and phase) and buffer of the next scores
+            uint32_t os = 0, oph = 1;          // stage of the next second product; phase of its buffer's release
+            uint32_t ob = 0, pph = 0;          // its next probabilities' buffer, and that buffer's phase
+            uint32_t uc = 0;
+            uint64_t own_desc = 0;
+            auto scores = [&]() -> bool {
+                if (!issuer_wait(bar(kLBarFull + ss), sph, wt, 102)) return false;
                 tc_fence_after();
-                const uint32_t d = tmem + kTS + 128u * w, a = tmem + kTOwn;
+                const uint32_t d = tmem + Ring<F32>::kTS + 128u * sb, a = tmem + kTOwn;
                 const uint64_t b = k_desc + ss * kStageDesc;
                 if (F32) {
                     mma_k_steps_warp(d, a + 64u, b, id_s, 0u, p.ksteps);
                     mma_k_steps_warp(d, a, b + kLoDesc, id_s, 1u, p.ksteps);
+                    mma_k_steps_warp(d, a, b, id_s, 1u, p.ksteps);
+                } else {
+                    mma_k_steps_ss_warp(d, own_desc, b, id_s, p.ksteps);
                 }
-                mma_k_steps_warp(d, a, b, id_s, F32 ? 1u : 0u, p.ksteps);
-                mma_commit_warp(bar(kLBarSFull + (int)w));
+                mma_commit_warp(bar(kLBarSFull + (int)sb));
+                if (++sb == kBufs) sb = 0u;
                 if (++ss == kStages) ss = 0u, sph ^= 1u;
                 return true;
             };
             bool ok = true;
             for (int u = blockIdx.x; ok && lunit_exists(u, p); u += gridDim.x, ++uc) {
                 const LUnit U = lunit(u, p);
-                const uint32_t n = (uint32_t)(U.c1 - U.c0);
-                ok = loss_wait(bar(kLBarAFull), uc & 1u, wt, 103);
+                const uint32_t n = (uint32_t)(U.c1 - U.c0), w = F32 ? 0u : uc & 1u;
+                ok = issuer_wait(bar(kLBarAFull + w), F32 ? uc & 1u : (uc >> 1) & 1u, wt, 103);
                 if (!ok) break;
                 tc_fence_after();
-                ok = scores(0) && (n < 2 || scores(1));
+                own_desc = k_desc + ((Ring<F32>::kOwn + w * kLossImage) >> 4);
+                for (uint32_t i = 0; ok && i < kBufs && i < n; ++i) ok = scores();
                 for (uint32_t i = 0; ok && i < n; ++i) {
-                    const uint32_t w = i & 1u;
-                    ok = loss_wait(bar(kLBarPFull + (int)w), (pph >> w) & 1u, wt, 104);
-                    pph ^= 1u << w;
-                    if (!ok) break;
-                    if (with_o) {
-                        ok = loss_wait(bar(kLBarOEmpty), oph, wt, 105);  // the previous tile's product is added up
-                        oph ^= 1u;
+#pragma unroll
+                    for (uint32_t half = 0; half < 2; ++half) {
+                        ok = ok && issuer_wait(bar(kLBarPFull + 2 * (int)ob + half), pph, wt, 104);
+                        if (half == 0 && with_o) {  // the previous tile's product is added up
+                            ok = ok && issuer_wait(bar(kLBarOEmpty), oph, wt, 105);
+                            oph ^= 1u;
+                        }
                         if (!ok) break;
                         tc_fence_after();
-                        const uint64_t b = mn_desc + os * kStageDesc;
-                        const uint32_t a = tmem + kTS + 128u * w, d = tmem + kTO;
-                        if (F32) {
-                            mma_row_steps_warp(d, a + 8u, b, id_o, 0u);
-                            mma_row_steps_warp(d, a, b + kLoDesc, id_o, 1u);
+                        if (with_o) {
+                            const uint64_t b = mn_desc + os * kStageDesc + half * kHalfDesc;
+                            const uint32_t a = tmem + Ring<F32>::kTS + 128u * ob + 64u * half, d = tmem + kTO;
+                            if (F32) {
+                                mma_row_steps_warp(d, a + 8u, b, id_o, half);
+                                mma_row_steps_warp(d, a, b + kLoDesc, id_o, 1u);
+                            }
+                            mma_row_steps_warp(d, a, b, id_o, F32 ? 1u : half);
                         }
-                        mma_row_steps_warp(d, a, b, id_o, F32 ? 1u : 0u);
-                        mma_commit_warp(bar(kLBarOFull));
                     }
+                    if (!ok) break;
+                    if (with_o) mma_commit_warp(bar(kLBarOFull));
                     mma_commit_warp(bar(kLBarEmpty + (int)os));
                     if (++os == kStages) os = 0u;
-                    // Tile i + 2 takes the score buffer of tile i, whose probabilities the product
-                    // above reads: the tensor core runs one thread's products in order.
-                    if (i + 2 < n) ok = scores(w);
+                    if (++ob == kBufs) ob = 0u, pph ^= 1u;
+                    // The buffer that the second product reads takes the scores of the tile kBufs further:
+                    // the tensor core runs one thread's products in order.
+                    if (i + kBufs < n) ok = scores();
                 }
                 if (!ok) break;
-                mma_commit_warp(bar(kLBarAEmpty));
+                mma_commit_warp(bar(kLBarAEmpty + w));
             }
             mma_commit_warp(bar(kLBarDone));
             loss_drain(bar(kLBarDone), 0u, wt);
@@ -745,7 +774,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
         const int quad = warp & 3, r = quad * 32 + lane;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         const uint32_t patch = base + kMOffPatch + (uint32_t)(warp - 4) * 32u * kPatchRow * 4u;
-        const uint32_t t_s = tmem + lanes + kTS + 128u * g + 64u * half;
+        const uint32_t t_bufs = tmem + lanes + Ring<F32>::kTS + 64u * half;
         float w_max = 0.0f, e_max = -CUDART_INF_F;
         if (SLOTS && !WPASS) {
             bool nan = false;
@@ -767,7 +796,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
             const LUnit U = lunit(u, p);
             const uint32_t n = (uint32_t)(U.c1 - U.c0);
             // labels of this warpgroup's first tile (weight pass): range, then entries
-            LabelWindow lw{make_int2(kNoLabel, 0), make_int2(kNoLabel, 0), 0, 0};
+            LabelWindow lw{};
             auto label_range = [&](int c, int& a, int& b) {
                 const int32_t* o = p.sp_off + (size_t)c * (2 * p.own_tiles + 1) + 2 * U.own + half;
                 a = __ldg(o);
@@ -778,27 +807,29 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                 label_range(U.c0 + (int)g, lw.next, lw.end);
                 window_open(lw, label_base(U.c0 + (int)g), lane);
             }
-            // own operand -> TMEM: warpgroup wg takes K slots 64 half .. 64 half + 63 of the lane's
-            // row, of the high part (even tiles' warpgroups) or the low part (odd; f32)
-            ok = loss_wait(bar(kLBarAEmpty), (uc & 1u) ^ 1u, wt, 106);
-            if (!ok) break;
-            tc_fence_after();
-            if ((int)(4 * half) < p.ksteps && (F32 || g == 0)) {
-                const uint8_t* img = p.own + (size_t)U.own * kStage + g * kLossImage;
+            if (F32) {
+                // own operand -> TMEM: warpgroup wg takes K slots 64 half .. 64 half + 63 of the lane's
+                // row, of the high part (even tiles' warpgroups) or the low part (odd)
+                ok = loss_wait(bar(kLBarAEmpty), (uc & 1u) ^ 1u, wt, 106);
+                if (!ok) break;
+                tc_fence_after();
+                if ((int)(4 * half) < p.ksteps) {
+                    const uint8_t* img = p.own + (size_t)U.own * kStage + g * kLossImage;
 #pragma unroll
-                for (int hj = 0; hj < 2; ++hj) {
-                    uint32_t w[16];
+                    for (int hj = 0; hj < 2; ++hj) {
+                        uint32_t w[16];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(img + image_chunk(r, 8 * half + 4 * hj + j));
-                        w[4 * j] = x.x, w[4 * j + 1] = x.y, w[4 * j + 2] = x.z, w[4 * j + 3] = x.w;
+                        for (int j = 0; j < 4; ++j) {
+                            const uint4 x = *reinterpret_cast<const uint4*>(img + image_chunk(r, 8 * half + 4 * hj + j));
+                            w[4 * j] = x.x, w[4 * j + 1] = x.y, w[4 * j + 2] = x.z, w[4 * j + 3] = x.w;
+                        }
+                        tmem_st32x32b_x16(tmem + lanes + kTOwn + 64u * g + 32u * half + 16u * hj, w);
                     }
-                    tmem_st32x32b_x16(tmem + lanes + kTOwn + 64u * g + 32u * half + 16u * hj, w);
+                    tmem_st_wait();
                 }
-                tmem_st_wait();
+                tc_fence_before();
+                mbar_arrive(bar(kLBarAFull));
             }
-            tc_fence_before();
-            mbar_arrive(bar(kLBarAFull));
 
             const float own_mul = F32 ? p.logit_scale * __ldg(p.own_scale + U.own) : p.logit_scale;
             const float lane_e = WPASS && !SLOTS ? __ldg(p.lane_e + (size_t)U.own * 128 + r) : 0.0f;
@@ -820,7 +851,9 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                 int next_a = 0, next_b = 0;
                 if (WPASS && i + 2 < n) label_range(c + 2, next_a, next_b);
                 const float2 mul = make_float2(own_mul * str_s, own_mul * str_s);
-                ok = loss_wait(bar(kLBarSFull + (int)g), uses & 1u, wt, 107);
+                const uint32_t buf = (cc + i) % Ring<F32>::kBufs;
+                const uint32_t t_s = t_bufs + 128u * buf;
+                ok = loss_wait(bar(kLBarSFull + (int)buf), ((cc + i) / Ring<F32>::kBufs) & 1u, wt, 107);
                 // the column table came with the tile: its barrier has passed, but this warp has to
                 // observe it before it reads what the copy wrote
                 ok = ok && loss_wait(bar(kLBarFull + s), ((cc + i) / kStages) & 1u, wt, 108);
@@ -831,7 +864,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                     if (with_o && half == 0) ring[((cc + i) & 3u) * 128 + r] = off;
                     const float2 sub2 = make_float2(-off, -off);
                     float2 ts = make_float2(0.f, 0.f);
-#pragma unroll
+#pragma unroll (F32 ? 1 : 4)
                     for (int q = 0; q < 4; ++q) {
                         uint32_t x[16];
                         tmem_ld32x32b_x16(t_s + 16u * q, x);
@@ -849,7 +882,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                     sum += ts.x + ts.y;
                 } else if constexpr (!WPASS) {
                     float top = -CUDART_INF_F;
-#pragma unroll
+#pragma unroll (F32 ? 1 : 4)
                     for (int q = 0; q < 4; ++q) {
                         uint32_t x[16];
                         tmem_ld32x32b_x16(t_s + 16u * q, x);
@@ -866,12 +899,13 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                         }
                     }
                     // the row's maximum over both halves of the tile
-                    tops[wg * 128 + r] = top;
+                    volatile float* t2 = tops + (uses & 1u) * 512;  // the partner may still read the last tile's
+                    t2[wg * 128 + r] = top;
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar(kLBarTop + 4 * (int)g + quad));
                     ok = loss_wait(bar(kLBarTop + 4 * (int)g + quad), uses & 1u, wt, 113);
                     if (!ok) break;
-                    top = fmaxf(top, tops[(wg ^ 1u) * 128 + r]);
+                    top = fmaxf(top, t2[(wg ^ 1u) * 128 + r]);
                     const float m = fmaxf(off, top);
                     // nothing visible yet (every class masked): any finite offset gives 2^-inf = 0
                     const float m0 = m == -CUDART_INF_F ? 0.0f : m;
@@ -881,7 +915,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                     const float sub = F32 ? 14.0f - m0 : -m0;
                     const float2 sub2 = make_float2(sub, sub);
                     float2 ts = make_float2(0.f, 0.f);
-#pragma unroll
+#pragma unroll (F32 ? 1 : 4)
                     for (int q = 0; q < 4; ++q) {
                         uint32_t x[16];
                         tmem_ld32x32b_x16(t_s + 16u * q, x);
@@ -907,8 +941,9 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                 } else {
                     const float2 le = make_float2(lane_e, lane_e);
                     const int2* ent = label_base(c);
+                    window_use(lw, quad);
                     float2 ts = make_float2(0.f, 0.f);
-#pragma unroll
+#pragma unroll (F32 ? 1 : 4)
                     for (int q = 0; q < 4; ++q) {
                         uint32_t x[16];
                         tmem_ld32x32b_x16(t_s + 16u * q, x);
@@ -937,22 +972,19 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                         // shared memory: entries scatter into it, each lane then adds its class's row
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const int lo = 64 * (int)half + 16 * q + 8 * h;
+                            const int group = 2 * q + h;
                             bool any = false;
                             while (true) {
-                                const bool in = (lw.e.x >> 7) < lo + 8;
-                                const uint32_t b = __ballot_sync(0xffffffffu, in);
-                                if (b == 0u) break;
-                                const bool hit = in && ((lw.e.x & 127) >> 5) == quad;
-                                if (hit)
-                                    *reinterpret_cast<volatile float*>(
-                                        gbase + (patch - base) +
-                                        4u * ((uint32_t)(lw.e.x & 31) * kPatchRow + (uint32_t)((lw.e.x >> 7) - lo))) =
-                                        __int_as_float(lw.e.y);
-                                any |= __any_sync(0xffffffffu, hit);
-                                if (in) lw.e.x = kNoLabel;
-                                if (!(b >> 31)) break;
-                                window_next(lw, ent, lane);
+                                if ((lw.groups >> group) & 1u) {
+                                    any = true;
+                                    if (lw.hit && (int)((lw.e.x >> 10) & 7) == group)
+                                        *reinterpret_cast<volatile float*>(
+                                            gbase + (patch - base) +
+                                            4u * ((uint32_t)(lw.e.x & 31) * kPatchRow + (uint32_t)((lw.e.x >> 7) & 7))) =
+                                            __int_as_float(lw.e.y);
+                                }
+                                if (group < lw.last) break;  // the window reaches beyond this group, or is the last
+                                window_next(lw, ent, lane, quad);
                             }
                             if (any) {
                                 __syncwarp();
@@ -984,7 +1016,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {
-                    mbar_arrive(bar(kLBarPFull + (int)g));
+                    mbar_arrive(bar(kLBarPFull + 2 * (int)buf + (int)half));
                     mbar_arrive(bar(kLBarEmpty + (int)s));
                     if (!WPASS && with_o && half == 0) mbar_arrive(bar(kLBarRing + (int)((cc + i) & 3u)));
                 }
@@ -1096,59 +1128,145 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
 // ---------------------------------------------------------------------------- row kernel
 namespace {
 
-// 4 values of row `c` of a row-major [.][k] matrix: K slots 4 lane .. 4 lane + 3 (zero past k).
+// A row's K slots over a group of 8 lanes: 16 per lane, in runs of kRun (one 16-byte load in the
+// element type E): lane s of the group holds slots kRun (s + 8 j) + i, j < 16 / kRun, i < kRun.
+template <int kRun>
+__device__ __forceinline__ int lane_slot(int s, int i) {
+    return kRun * (s + 8 * (i / kRun)) + i % kRun;
+}
+
+// A lane's 16 values of row `c` of a row-major [.][k] matrix (zero past k).
 template <bool F32>
-__device__ __forceinline__ float4 row_quad(const void* w, long long c, int k, int lane, bool vec) {
+__device__ __forceinline__ void weight_row(const void* w, long long c, int k, int s, bool vec, float (&v)[16]) {
     using T = typename Elem<F32>::type;
-    const T* a = static_cast<const T*>(w) + c * k + 4 * lane;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (vec) {
-        if (4 * lane < k) {
-            if constexpr (F32) {
-                v = __ldg(reinterpret_cast<const float4*>(a));
-            } else {
-                const uint2 u = __ldg(reinterpret_cast<const uint2*>(a));
-                v = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
-                                __uint_as_float(u.y & 0xffff0000u));
+    constexpr int kRun = F32 ? 4 : 8;
+    const T* a = static_cast<const T*>(w) + c * k;
+#pragma unroll
+    for (int j = 0; j < 16 / kRun; ++j) {
+        const int k0 = kRun * (s + 8 * j);
+        if (vec) {
+            uint4 u = make_uint4(0u, 0u, 0u, 0u);
+            if (k0 < k) u = __ldg(reinterpret_cast<const uint4*>(a + k0));
+            const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (F32) {
+                    v[4 * j + i] = __uint_as_float(x[i]);
+                } else {
+                    v[8 * j + 2 * i] = __uint_as_float(x[i] << 16);
+                    v[8 * j + 2 * i + 1] = __uint_as_float(x[i] & 0xffff0000u);
+                }
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kRun; ++i) v[kRun * j + i] = k0 + i < k ? to_f32(a[k0 + i]) : 0.0f;
         }
-    } else {
-        if (4 * lane < k) v.x = to_f32(a[0]);
-        if (4 * lane + 1 < k) v.y = to_f32(a[1]);
-        if (4 * lane + 2 < k) v.z = to_f32(a[2]);
-        if (4 * lane + 3 < k) v.w = to_f32(a[3]);
     }
+}
+template <int kRun>
+__device__ __forceinline__ void shared_row(const float* row, int k, int s, float (&v)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = lane_slot<kRun>(s, i) < k ? row[lane_slot<kRun>(s, i)] : 0.0f;
+}
+__device__ __forceinline__ float dot16(const float (&a)[16], const float (&b)[16]) {
+    float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+        s0 = fmaf(a[i], b[i], s0);
+        s1 = fmaf(a[i + 1], b[i + 1], s1);
+    }
+    return s0 + s1;
+}
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ float group_max(float v) {
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
 
-__device__ __forceinline__ float4 smem_quad(const float* row, int k, int lane) {
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (4 * lane < k) v.x = row[4 * lane];
-    if (4 * lane + 1 < k) v.y = row[4 * lane + 1];
-    if (4 * lane + 2 < k) v.z = row[4 * lane + 2];
-    if (4 * lane + 3 < k) v.w = row[4 * lane + 3];
-    return v;
-}
-__device__ __forceinline__ float dot4(float4 a, float4 b) {
-    return fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, a.w * b.w)));
-}
-
-// R rows of the features into shared memory (row stride k + 1), coalesced along the layout's
-// contiguous direction.
+// R rows of the features into shared memory (row stride k + 1), and back: coalesced along the
+// layout's contiguous direction.
 template <int R, class T>
 __device__ __forceinline__ void load_rows(const T* x, long long row0, long long rows, int k, long long t_len, float* xs) {
     if (t_len > 0) {
-        for (int i = threadIdx.x; i < R * k; i += 256) {
-            const int r = i % R, kk = i / R;
-            const long long row = row0 + r;
-            xs[r * (k + 1) + kk] = row < rows ? to_f32(x[x_base(row, k, t_len) + kk * t_len]) : 0.0f;
-        }
+        const int r = threadIdx.x % R;
+        const long long at = row0 + r < rows ? x_base(row0 + r, k, t_len) : 0;
+#pragma unroll 8
+        for (int kk = threadIdx.x / R; kk < k; kk += 256 / R)
+            xs[r * (k + 1) + kk] = row0 + r < rows ? to_f32(x[at + kk * t_len]) : 0.0f;
     } else {
-        for (int i = threadIdx.x; i < R * k; i += 256) {
-            const int r = i / k, kk = i - r * k;
-            xs[r * (k + 1) + kk] = row0 + r < rows ? to_f32(x[row0 * k + i]) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < R / 8; ++i) {
+            const int r = (threadIdx.x >> 5) + 8 * i;
+#pragma unroll 4
+            for (int kk = threadIdx.x & 31; kk < k; kk += 32)
+                xs[r * (k + 1) + kk] = row0 + r < rows ? to_f32(x[(row0 + r) * k + kk]) : 0.0f;
         }
     }
+}
+template <int R, class T>
+__device__ __forceinline__ void store_rows(T* x, long long row0, long long rows, int k, long long t_len, const float* xs) {
+    if (t_len > 0) {
+        const int r = threadIdx.x % R;
+        if (row0 + r >= rows) return;
+        T* at = x + x_base(row0 + r, k, t_len);
+#pragma unroll 4
+        for (int kk = threadIdx.x / R; kk < k; kk += 256 / R) at[kk * t_len] = (T)xs[r * (k + 1) + kk];
+    } else {
+#pragma unroll
+        for (int i = 0; i < R / 8; ++i) {
+            const int r = (threadIdx.x >> 5) + 8 * i;
+            if (row0 + r >= rows) return;
+#pragma unroll 4
+            for (int kk = threadIdx.x & 31; kk < k; kk += 32) x[(row0 + r) * k + kk] = (T)xs[r * (k + 1) + kk];
+        }
+    }
+}
+
+// A row's labels in a group of 8 lanes: their shares q into shared memory as (class or -1, q), and
+// sum_i q_i log q_i. False when the row has none (it is then ignored), or none is asked for.
+__device__ __forceinline__ bool group_labels(const LossLabels& L, long long row, bool live, int s, int2* ent, float& entropy) {
+    entropy = 0.0f;
+    if (L.target) {
+        const int t = live ? L.target[row] : -1;
+        const bool valid = is_class(t, L.n);
+        if (s == 0) ent[0] = make_int2(valid ? t : -1, __float_as_int(1.0f));
+        __syncwarp();
+        return valid;
+    }
+    const long long at = row * L.n_top;
+    float top = -CUDART_INF_F;
+    bool any = false;
+    for (int e = s; e < L.n_top; e += 8) {
+        int c = live ? L.top_idx[at + e] : -1;
+        c = is_class(c, L.n) ? c : -1;
+        const float u = c >= 0 ? L.top_logits[at + e] * L.inv_temp : -CUDART_INF_F;
+        ent[e] = make_int2(c, __float_as_int(u));
+        any |= c >= 0;
+        top = fmaxf(top, u);
+    }
+    top = group_max(top);
+    const bool valid = group_max(any ? 1.0f : 0.0f) > 0.0f;
+    float sum = 0.0f;
+    for (int e = s; e < L.n_top; e += 8)
+        if (ent[e].x >= 0) sum += expf(__int_as_float(ent[e].y) - top);
+    sum = group_sum(sum);
+    const float log_sum = logf(sum);
+    float h = 0.0f;
+    for (int e = s; e < L.n_top; e += 8) {
+        if (ent[e].x < 0) continue;
+        const float u = __int_as_float(ent[e].y) - top, q = expf(u) / sum;
+        // an entry of no share (teacher logit -inf) holds the row to nothing
+        if (q != 0.0f) h = fmaf(q, u - log_sum, h);
+        ent[e] = make_int2(q != 0.0f ? ent[e].x : -1, __float_as_int(q));
+    }
+    entropy = group_sum(h);
+    __syncwarp();
+    return valid;
 }
 
 // Rows l0 .. l0 + R - 1 of the units u0 .. u0 + ns - 1's partial tiles [feat][128], weighted and
@@ -1180,19 +1298,21 @@ __device__ __forceinline__ void join_units(const float* part_o, size_t u0, int n
 }  // namespace
 
 // One block per R rows (32; 8 where that leaves most SMs idle). Joins the class ranges of a row
-// block (the largest offset, the sums and mean weight rows brought to it), then one warp per row:
-// the labels' logits as f32 products, the loss, and dx = T g (sum_j p_j W_j - sum_i q_i W_ci).
+// block (the largest offset, the sums and mean weight rows brought to it); then 8 lanes per row: the
+// labels' logits as f32 products, the loss, and dx = T g (sum_j p_j W_j - sum_i q_i W_ci).
 template <bool F32, int R>
 __global__ void __launch_bounds__(256) loss_rows_kernel(const __grid_constant__ LossRowParams p) {
     using T = typename Elem<F32>::type;
-    extern __shared__ float sm[];
-    float* xs = sm;                            // [R][k + 1]
-    float* os = xs + R * (p.k + 1);            // [R][feat + 1]
-    float* wgt = os + R * (p.feat + 1);        // [n_splits][R]
+    extern __shared__ __align__(16) float sm[];
+    float* xs = sm;                                           // [R][k + 1]
+    float* os = xs + R * (p.k + 1);                           // [R][feat + 1]
+    float* wgt = os + R * (p.feat + 1);                       // [n_splits][R]
+    int2* ents = reinterpret_cast<int2*>(wgt + R * p.n_splits);  // [R][n_top] (R is even: 8-byte aligned)
     constexpr int kG = 256 / R;                // threads that share a row's ranges
+    constexpr int kRun = F32 ? 4 : 8;
     __shared__ float red[kG][R];
     __shared__ float s_lse2[R], s_inv[R];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x;
     const long long row0 = (long long)blockIdx.x * R;
     const int mb = (int)(row0 >> 7), l0 = (int)(row0 & 127);
     const int ns = mb < p.whole_units ? 1 : p.n_splits;
@@ -1208,6 +1328,7 @@ __global__ void __launch_bounds__(256) loss_rows_kernel(const __grid_constant__ 
     }
     red[jg][jr] = m;
     __syncthreads();
+#pragma unroll
     for (int i = 0; i < kG; ++i) m = fmaxf(m, red[i][jr]);
     const float m0 = m == -CUDART_INF_F ? 0.0f : m;
     float sum = 0.0f;
@@ -1221,6 +1342,7 @@ __global__ void __launch_bounds__(256) loss_rows_kernel(const __grid_constant__ 
     __syncthreads();
     if (jg == 0) {
         sum = 0.0f;
+#pragma unroll
         for (int i = 0; i < kG; ++i) sum += red[i][jr];
         s_lse2[jr] = m0 + log2f(sum);
         s_inv[jr] = 1.0f / sum;
@@ -1230,91 +1352,61 @@ __global__ void __launch_bounds__(256) loss_rows_kernel(const __grid_constant__ 
         join_units<R, true>(p.part_o, u0, ns, p.feat, l0, wgt, s_inv, os);
         __syncthreads();
     }
-    const bool vec = p.k % 4 == 0 && (reinterpret_cast<uintptr_t>(p.w) & (F32 ? 15u : 7u)) == 0;
-    for (int rr = 0; rr < R / 8; ++rr) {
-        const int r = warp * (R / 8) + rr;
+    if (tid < 8 * R) {  // (R = 8: two warps have rows)
+        const bool vec = p.k % kRun == 0 && (reinterpret_cast<uintptr_t>(p.w) & 15u) == 0;
+        const int r = tid >> 3, s = tid & 7;
         const long long row = row0 + r;
-        float* tab = p.row_tab + (size_t)(row >> 7) * 256 + (row & 127);
-        RowLabels lab;
-        const bool valid = row < p.rows && row_labels(p.lab, row, lane, lab);
+        const bool live = row < p.rows;
+        int2* ent = ents + r * p.lab.n_top;
+        float entropy;
+        const bool valid = group_labels(p.lab, row, live, s, ent, entropy);
+        const float f = live ? p.lab.temp * (p.row_grad ? p.row_grad[row] : 1.0f) : 0.0f;
         const float lse2 = s_lse2[r], lse = lse2 * kLn2;
-        if (lane == 0) {
+        if (s == 0) {
             float e = -CUDART_INF_F;  // no share of anything
-            if (valid) e = F32 ? -lse2 : log2f(fabsf(p.lab.temp * (p.row_grad ? p.row_grad[row] : 1.0f))) - lse2;
-            *tab = e;
+            if (valid) e = F32 ? -lse2 : log2f(fabsf(f)) - lse2;
+            p.row_tab[(size_t)(row >> 7) * 256 + (row & 127)] = e;
         }
-        if (row >= p.rows) continue;
         float* xr = xs + r * (p.k + 1);
-        if (!valid) {
-            if (lane == 0) {
-                if (p.loss) p.loss[row] = 0.0f;
-                if (p.lse) p.lse[row] = 0.0f;
+        float x[16], d[16];
+        shared_row<kRun>(xr, p.k, s, x);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) d[i] = 0.0f;
+        if (p.dx) shared_row<kRun>(os + r * (p.feat + 1), p.k, s, d);
+        float zq = 0.0f;  // sum_i q_i (z_i - lse)
+#pragma unroll 2
+        for (int e = 0; e < p.lab.n_top; ++e) {
+            const int2 c = ent[e];
+            const bool here = valid && c.x >= 0;
+            const float q = here ? __int_as_float(c.y) : 0.0f;
+            float w[16];
+            if (here) {
+                weight_row<F32>(p.w, c.x, p.k, s, vec, w);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) w[i] = 0.0f;
             }
-            for (int kk = lane; kk < p.k; kk += 32) xr[kk] = 0.0f;
-            continue;
-        }
-        const float4 x4 = smem_quad(xr, p.k, lane);
-        float4 d = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (p.dx) d = smem_quad(os + r * (p.feat + 1), p.k, lane);
-        float loss = 0.0f;
-        for (int e0 = 0; e0 < p.lab.n_top; e0 += 4) {
-            int c[4];
-            float q[4], lq[4], z[4];
-            float4 w4[4];
+            const float z = group_sum(dot16(x, w));
+            if (here) {
+                zq = fmaf(q, fmaf(z + (p.bias ? __ldg(p.bias + c.x) : 0.0f), p.lab.inv_temp, -lse), zq);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int e = e0 + j;  // n_top <= 64, so e < 64; entries past n_top hold class -1
-                c[j] = __shfl_sync(0xffffffffu, e < 32 ? lab.c[0] : lab.c[1], e & 31);
-                q[j] = __shfl_sync(0xffffffffu, e < 32 ? lab.q[0] : lab.q[1], e & 31);
-                lq[j] = __shfl_sync(0xffffffffu, e < 32 ? lab.log_q[0] : lab.log_q[1], e & 31);
-                w4[j] = c[j] >= 0 ? row_quad<F32>(p.w, c[j], p.k, lane, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) z[j] = dot4(x4, w4[j]);
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) z[j] += __shfl_xor_sync(0xffffffffu, z[j], o);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                // an entry of no share (teacher logit -inf) holds the row to nothing
-                if (c[j] >= 0 && q[j] != 0.0f) {
-                    const float zz = (z[j] + (p.bias ? p.bias[c[j]] : 0.0f)) * p.lab.inv_temp;
-                    loss = fmaf(q[j], lq[j] - (zz - lse), loss);
-                    d.x = fmaf(-q[j], w4[j].x, d.x);
-                    d.y = fmaf(-q[j], w4[j].y, d.y);
-                    d.z = fmaf(-q[j], w4[j].z, d.z);
-                    d.w = fmaf(-q[j], w4[j].w, d.w);
-                }
+                for (int i = 0; i < 16; ++i) d[i] = fmaf(-q, w[i], d[i]);
             }
         }
-        if (lane == 0) {
-            if (p.loss) p.loss[row] = loss * p.lab.temp * p.lab.temp;
-            if (p.lse) p.lse[row] = lse;
+        if (live && s == 0) {
+            if (p.loss) p.loss[row] = valid ? (entropy - zq) * p.lab.temp * p.lab.temp : 0.0f;
+            if (p.lse) p.lse[row] = valid ? lse : 0.0f;
         }
         if (p.dx) {
-            const float f = p.lab.temp * (p.row_grad ? p.row_grad[row] : 1.0f);
-            if (4 * lane < p.k) xr[4 * lane] = f * d.x;
-            if (4 * lane + 1 < p.k) xr[4 * lane + 1] = f * d.y;
-            if (4 * lane + 2 < p.k) xr[4 * lane + 2] = f * d.z;
-            if (4 * lane + 3 < p.k) xr[4 * lane + 3] = f * d.w;
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (lane_slot<kRun>(s, i) < p.k) xr[lane_slot<kRun>(s, i)] = valid ? f * d[i] : 0.0f;
         }
     }
     if (!p.dx) return;
     __syncthreads();
-    T* dx = static_cast<T*>(p.dx);
-    if (p.t_len > 0) {
-        for (int i = tid; i < R * p.k; i += 256) {
-            const int r = i % R, kk = i / R;
-            if (row0 + r < p.rows) dx[x_base(row0 + r, p.k, p.t_len) + kk * p.t_len] = (T)xs[r * (p.k + 1) + kk];
-        }
-    } else {
-        for (int i = tid; i < R * p.k; i += 256) {
-            const int r = i / p.k, kk = i - r * p.k;
-            if (row0 + r < p.rows) dx[row0 * p.k + i] = (T)xs[r * (p.k + 1) + kk];
-        }
-    }
+    store_rows<R>(static_cast<T*>(p.dx), row0, p.rows, p.k, p.t_len, xs);
 }
 
 // One block per R classes (32, or 8 as above): the row ranges' partial sums added in their order,
@@ -1334,9 +1426,12 @@ __global__ void __launch_bounds__(256) loss_reduce_kernel(const __grid_constant_
     }
     __syncthreads();
     T* dw = static_cast<T*>(p.dw);
-    for (int i = threadIdx.x; i < R * p.k; i += 256) {
-        const int r = i / p.k, kk = i - r * p.k;
-        if (j0 + r < p.n) dw[(long long)j0 * p.k + i] = (T)sm[r * (p.feat + 1) + kk];
+#pragma unroll
+    for (int i = 0; i < R / 8; ++i) {
+        const int r = (threadIdx.x >> 5) + 8 * i;
+        if (j0 + r < p.n) {
+            for (int kk = threadIdx.x & 31; kk < p.k; kk += 32) dw[(long long)(j0 + r) * p.k + kk] = (T)sm[r * (p.feat + 1) + kk];
+        }
     }
 }
 
@@ -1350,83 +1445,138 @@ __global__ void __launch_bounds__(256) loss_table_kernel(const float* __restrict
 
 namespace {
 
-// K slots 4 lane .. 4 lane + 3 of a packed weight's class c, in units of its class-table scale.
-__device__ __forceinline__ float4 packed_quad(const uint8_t* tiles, int form, int c, int lane) {
-    const int tile = c >> 7, r = c & 127, s = 4 * lane;
-    if (form == 1) {
-        const uint32_t w =
-            __ldg(reinterpret_cast<const uint32_t*>(tiles + (size_t)tile * kTile8Bytes + image8_offset(r, s)));
-        return make_float4((float)(int)(w & 255u) - 128.0f, (float)(int)((w >> 8) & 255u) - 128.0f,
-                           (float)(int)((w >> 16) & 255u) - 128.0f, (float)(int)(w >> 24) - 128.0f);
+// A lane's 16 K slots of a packed weight's class c, in units of its class-table scale: runs of 8
+// (fp16 images), or 16 in a row (compact).
+template <int FORM>
+__device__ __forceinline__ void packed_row(const uint8_t* tiles, int c, int s, float (&v)[16]) {
+    const int tile = c >> 7, r = c & 127;
+    if constexpr (FORM == 1) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(tiles + (size_t)tile * kTile8Bytes + image8_offset(r, 16 * s)));
+        const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = (float)(int)((x[i / 4] >> (8 * (i % 4))) & 255u) - 128.0f;
+    } else {
+        const uint8_t* a = tiles + (size_t)tile * (FORM == 2 ? 2 * kTileBytes : kTileBytes);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t off = image_chunk(r, s + 8 * j);
+#pragma unroll
+            for (int part = 0; part < (FORM == 2 ? 2 : 1); ++part) {
+                const uint4 u = __ldg(reinterpret_cast<const uint4*>(a + part * kTileBytes + off));
+                const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x[i]));
+                    v[8 * j + 2 * i] = part ? v[8 * j + 2 * i] + f.x : f.x;
+                    v[8 * j + 2 * i + 1] = part ? v[8 * j + 2 * i + 1] + f.y : f.y;
+                }
+            }
+        }
     }
-    const uint8_t* a = tiles + (size_t)tile * (form == 2 ? 2 * kTileBytes : kTileBytes) + image_chunk(r, s >> 3) + 2 * (s & 7);
-    auto quad = [](const uint8_t* b) {
-        const uint2 u = __ldg(reinterpret_cast<const uint2*>(b));
-        const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
-        const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
-        return make_float4(lo.x, lo.y, hi.x, hi.y);
-    };
-    float4 v = quad(a);
-    if (form == 2) {
-        const float4 l = quad(a + kTileBytes);
-        v = make_float4(v.x + l.x, v.y + l.y, v.z + l.z, v.w + l.w);
-    }
-    return v;
 }
 
 }  // namespace
 
-// One block per 32 rows, one warp per row: the logits of the row's labels and of its argmax as f32
-// products with the packed weight. lse = z[argmax] / T - log(probability of the argmax).
+// One block per 32 rows, 8 lanes per row: the logits of the row's labels and of its argmax as f32
+// products with the packed weight. lse = z[argmax] / T + log(sum of exponentials relative to it).
+// Rows whose class range was split are joined here, from the decode kernel's partial (maximum, sum,
+// argmax) rows.
+template <int FORM>
 __global__ void __launch_bounds__(256) loss_score_kernel(const __grid_constant__ LossScoreParams p) {
-    extern __shared__ float xs[];  // [32][k + 1]
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    extern __shared__ __align__(16) float xs[];  // [32][k + 1], then [32][n_top] int2
+    constexpr int kRun = FORM == 1 ? 16 : 8;
+    int2* ents = reinterpret_cast<int2*>(xs + kLossRows * (p.k + 1));
     const long long row0 = (long long)blockIdx.x * kLossRows;
+    const int r = threadIdx.x >> 3, s = threadIdx.x & 7;
+    const long long row = row0 + r;
+    const bool live = row < p.rows;
     load_rows<kLossRows>(p.x, row0, p.rows, p.k, p.t_len, xs);
+    int best = 0;
+    float sum = 1.0f;
+    if (row >= p.split_row0 && live) {
+        float m = -CUDART_INF_F;
+        sum = 0.0f;
+        best = 0x7fffffff;
+        for (int i = s; i < p.n_splits; i += 8) {
+            const float4 v = p.partial[(size_t)i * (size_t)(p.rows - p.split_row0) + (size_t)(row - p.split_row0)];
+            const int c = __float_as_int(v.z);
+            if (v.x > m) {
+                sum = (m == -CUDART_INF_F ? 0.0f : sum * ex2_approx(m - v.x)) + v.y;
+                m = v.x;
+                best = c;
+            } else if (v.x != -CUDART_INF_F) {
+                sum += v.y * ex2_approx(v.x - m);
+                if (v.x == m) best = min(best, c);
+            } else if (isnan(v.x) || isnan(v.y)) {
+                sum = CUDART_NAN_F;
+            }
+        }
+        // lanes of a group that had no range, or only masked classes, bring nothing
+        const uint32_t group = 0xffu << (threadIdx.x & 24);
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) {
+            const float om = __shfl_xor_sync(group, m, o), os = __shfl_xor_sync(group, sum, o);
+            const int ob = __shfl_xor_sync(group, best, o);
+            const float M = fmaxf(m, om);
+            if (M != -CUDART_INF_F) {
+                sum = (m == -CUDART_INF_F ? 0.0f : sum * ex2_approx(m - M)) + (om == -CUDART_INF_F ? 0.0f : os * ex2_approx(om - M));
+                best = m == om ? min(best, ob) : m > om ? best : ob;
+            } else {
+                sum += os;
+            }
+            m = M;
+        }
+    } else if (live) {
+        best = p.idx[row];
+        sum = 1.0f / p.prob[row];
+    }
+    best = min(max(best, 0), p.lab.n - 1);
     __syncthreads();
-    for (int rr = 0; rr < kLossRows / 8; ++rr) {
-        const int r = warp * (kLossRows / 8) + rr;
-        const long long row = row0 + r;
-        if (row >= p.rows) break;
+    int2* ent = ents + r * p.lab.n_top;
+    float entropy;
+    const bool valid = group_labels(p.lab, row, live, s, ent, entropy);
+    if (live) {
         const int* cls = p.lab.target ? p.lab.target + row : p.lab.top_idx + row * p.lab.n_top;
         bool bad = false;
-        for (int e = lane; e < p.lab.n_top; e += 32) bad |= cls[e] >= p.lab.n;
+        for (int e = s; e < p.lab.n_top; e += 8) bad |= cls[e] >= p.lab.n;
         if (bad) atomicOr(p.status, kDevBadClass);
-        RowLabels lab;
-        if (!row_labels(p.lab, row, lane, lab)) {
-            if (lane == 0) {
-                if (p.loss) p.loss[row] = 0.0f;
-                if (p.lse) p.lse[row] = 0.0f;
-            }
-            continue;
-        }
-        const float4 x4 = smem_quad(xs + r * (p.k + 1), p.k, lane);
-        auto logit = [&](int c) -> float {
-            const float s = warp_sum(dot4(x4, packed_quad(p.tiles, p.form, c, lane)));
-            const float* t = p.ctab + (size_t)(c >> 7) * kCtabFloats + (c & 127);
-            return fmaf(s, t[0], t[kBlockN]) * p.lab.inv_temp;
-        };
-        const int best = min(max(p.idx[row], 0), p.lab.n - 1);
-        const float lse = logit(best) - logf(p.prob[row]);
-        float loss = 0.0f;
-        for (int e = 0; e < p.lab.n_top; ++e) {
-            const int c = __shfl_sync(0xffffffffu, e < 32 ? lab.c[0] : lab.c[1], e & 31);
-            const float q = __shfl_sync(0xffffffffu, e < 32 ? lab.q[0] : lab.q[1], e & 31);
-            const float lq = __shfl_sync(0xffffffffu, e < 32 ? lab.log_q[0] : lab.log_q[1], e & 31);
-            if (c < 0 || q == 0.0f) continue;
-            loss = fmaf(q, lq - (logit(c) - lse), loss);
-        }
-        if (lane == 0) {
-            if (p.loss) p.loss[row] = loss * p.lab.temp * p.lab.temp;
-            if (p.lse) p.lse[row] = lse;
-        }
+    }
+    float x[16];
+    shared_row<kRun>(xs + r * (p.k + 1), p.k, s, x);
+    auto logit = [&](int c) -> float {
+        float w[16];
+        packed_row<FORM>(p.tiles, c, s, w);
+        const float* t = p.ctab + (size_t)(c >> 7) * kCtabFloats + (c & 127);
+        return fmaf(group_sum(dot16(x, w)), __ldg(t), __ldg(t + kBlockN)) * p.lab.inv_temp;
+    };
+    const float lse = logit(best) + logf(sum);
+    float zq = 0.0f;
+#pragma unroll 2
+    for (int e = 0; e < p.lab.n_top; ++e) {
+        const int2 c = ent[e];
+        const bool here = valid && c.x >= 0;
+        const float z = logit(here ? c.x : 0);
+        if (here) zq = fmaf(__int_as_float(c.y), z - lse, zq);
+    }
+    if (live && s == 0) {
+        if (p.loss) p.loss[row] = valid ? (entropy - zq) * p.lab.temp * p.lab.temp : 0.0f;
+        if (p.lse) p.lse[row] = valid ? lse : 0.0f;
     }
 }
 
 // ------------------------------------------------------------------------------- launchers
 namespace {
-constexpr int kPackSmemMax = 9 * 2 * (kLossMaxClasses / 128) * 4;
-constexpr int kRowsSmemMax = (2 * 32 * 129 + 32 * kLossMaxSplits) * 4;
+// (counts, starts, entries; the norms' four partial sums)
+constexpr int pack_smem_bytes(int w_tiles, int n_top) {
+    return 2 * w_tiles * (2 * kPackWarps + 4) + 128 * n_top * 8;
+}
+constexpr int kPackSmemMax = pack_smem_bytes(kLossMaxClasses / 128, kLossMaxTop) + 2048;
+static_assert(kPackSmemMax <= 226 * 1024, "shared memory per block");
+int rows_smem_bytes(int r, int k, int feat, int n_splits, int n_top) {
+    return r * ((k + 1 + feat + 1 + n_splits) * 4 + n_top * 8);
+}
+constexpr int kRowsSmemMax = 32 * ((2 * 129 + kLossMaxSplits) * 4 + kLossMaxTop * 8);
+int score_smem_bytes(int k, int n_top) { return kLossRows * ((k + 1) * 4 + n_top * 8); }
 // Blocks of 32 rows would leave SMs idle: four times as many of 8.
 bool few_blocks(int tiles, int sms) { return tiles * (kLossTile / 32) < 2 * sms; }
 template <class K>
@@ -1451,11 +1601,14 @@ cudaError_t loss_kernel_setup() {
 
 cudaError_t launch_loss_pack(const LossPackParams& p, bool f32, cudaStream_t stream) {
     const int grid = p.w_tiles + p.x_tiles;
-    const int smem = p.sort_labels ? 9 * 2 * p.w_tiles * 4 : 0;
+    const int labels = p.sort_labels ? pack_smem_bytes(p.w_tiles, p.lab.n_top) : 0;
+    LossPackParams q = p;
+    q.norm_smem = (labels + 3) / 4;
+    const int smem = 4 * q.norm_smem + (p.slots && p.t_len > 0 ? 2048 : 0);
     if (f32)
-        loss_pack_kernel<true><<<grid, 256, smem, stream>>>(p);
+        loss_pack_kernel<true><<<grid, kPackThreads, smem, stream>>>(q);
     else
-        loss_pack_kernel<false><<<grid, 256, smem, stream>>>(p);
+        loss_pack_kernel<false><<<grid, kPackThreads, smem, stream>>>(q);
     return cudaGetLastError();
 }
 
@@ -1481,7 +1634,7 @@ cudaError_t launch_loss_rows(const LossRowParams& p, bool f32, int sms, cudaStre
     const int tiles = (int)((p.rows + kLossTile - 1) / kLossTile);  // the last tile's padding rows too
     const int r = few_blocks(tiles, sms) ? 8 : 32;
     const int grid = tiles * (kLossTile / r);
-    const int smem = (r * (p.k + 1) + r * (p.feat + 1) + r * p.n_splits) * 4;
+    const int smem = rows_smem_bytes(r, p.k, p.feat, p.n_splits, p.lab.n_top);
     if (f32 && r == 32)
         loss_rows_kernel<true, 32><<<grid, 256, smem, stream>>>(p);
     else if (f32)
@@ -1513,8 +1666,13 @@ cudaError_t launch_loss_table(const float* ctab, long long n_floats, float inv_t
 }
 
 cudaError_t launch_loss_score(const LossScoreParams& p, cudaStream_t stream) {
-    const int grid = (int)((p.rows + kLossRows - 1) / kLossRows);
-    loss_score_kernel<<<grid, 256, kLossRows * (p.k + 1) * 4, stream>>>(p);
+    const int grid = (int)((p.rows + kLossRows - 1) / kLossRows), smem = score_smem_bytes(p.k, p.lab.n_top);
+    if (p.form == 0)
+        loss_score_kernel<0><<<grid, 256, smem, stream>>>(p);
+    else if (p.form == 1)
+        loss_score_kernel<1><<<grid, 256, smem, stream>>>(p);
+    else
+        loss_score_kernel<2><<<grid, 256, smem, stream>>>(p);
     return cudaGetLastError();
 }
 

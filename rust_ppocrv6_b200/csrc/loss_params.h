@@ -54,6 +54,7 @@ struct LossPackParams {
                                // (features), so that the scores come with their bias
     float* x_norm;             // slots: [x_tiles][128] |x_r|
     float2* w_bound;           // slots: [w_tiles] (largest |w_j|, largest bias in log2 units)
+    int norm_smem;             // set by the launcher: first float of the norms' shared memory
     int32_t* sp_off;           // [x_tiles][2 w_tiles + 1] label ranges by class tile and half of the rows
     int2* sp_ent;              // [x_tiles][128 n_top]: (row << 7 | class within its tile, factor bits)
     int* status;
@@ -119,8 +120,11 @@ struct LossScoreParams {
     const uint8_t* tiles;      // packed weight
     const float* ctab;         // class table (scale, bias), at T = 1
     int form;                  // 0 fp16 image of int8, 1 compact int8, 2 FP32 (hi, lo)
-    const int32_t* idx;
+    const int32_t* idx;        // rows below split_row0
     const float* prob;
+    const float4* partial;     // rows from split_row0 on: [n_splits][rows - split_row0], as HeadParams::partial
+    long long split_row0;
+    int n_splits;
     float* loss;
     float* lse;
     int* status;

@@ -89,29 +89,62 @@ __device__ __forceinline__ void mma_k_steps_warp(uint32_t d_tmem, uint32_t a_tme
         : "memory");
 }
 
-// The 8 K steps of a product whose contraction runs along the image's 128 rows (2 KB a step); A in
+// The same with A in shared memory too, an image like B's; the accumulator starts at zero.
+__device__ __forceinline__ void mma_k_steps_ss_warp(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                                    int steps) {
+    asm volatile(
+        "{\n\t.reg .pred e, pa, pt, q1, q2, q3, q4, q5, q6, q7;\n\t.reg .b64 a<8>, b<8>;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 pa, 0, 0;\n\t"
+        "setp.eq.b32 pt, 0, 0;\n\t"
+        "add.s64 a1, %1, 2;\n\t"
+        "add.s64 b1, %2, 2;\n\t"
+        "setp.gt.and.s32 q1, %4, 1, e;\n\t"
+        "add.s64 a2, %1, 4;\n\t"
+        "add.s64 b2, %2, 4;\n\t"
+        "setp.gt.and.s32 q2, %4, 2, e;\n\t"
+        "add.s64 a3, %1, 6;\n\t"
+        "add.s64 b3, %2, 6;\n\t"
+        "setp.gt.and.s32 q3, %4, 3, e;\n\t"
+        "add.s64 a4, %1, 1024;\n\t"
+        "add.s64 b4, %2, 1024;\n\t"
+        "setp.gt.and.s32 q4, %4, 4, e;\n\t"
+        "add.s64 a5, %1, 1026;\n\t"
+        "add.s64 b5, %2, 1026;\n\t"
+        "setp.gt.and.s32 q5, %4, 5, e;\n\t"
+        "add.s64 a6, %1, 1028;\n\t"
+        "add.s64 b6, %2, 1028;\n\t"
+        "setp.gt.and.s32 q6, %4, 6, e;\n\t"
+        "add.s64 a7, %1, 1030;\n\t"
+        "add.s64 b7, %2, 1030;\n\t"
+        "setp.gt.and.s32 q7, %4, 7, e;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, pa;\n\t"
+        "@q1 tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, pt;\n\t"
+        "@q2 tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, pt;\n\t"
+        "@q3 tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, pt;\n\t"
+        "@q4 tcgen05.mma.cta_group::1.kind::f16 [%0], a4, b4, %3, pt;\n\t"
+        "@q5 tcgen05.mma.cta_group::1.kind::f16 [%0], a5, b5, %3, pt;\n\t"
+        "@q6 tcgen05.mma.cta_group::1.kind::f16 [%0], a6, b6, %3, pt;\n\t"
+        "@q7 tcgen05.mma.cta_group::1.kind::f16 [%0], a7, b7, %3, pt;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(steps)
+        : "memory");
+}
+
+// The 4 K steps of a product whose contraction runs along 64 of the image's rows (2 KB a step); A in
 // TMEM, 16 columns a step (8 of them read).
 __device__ __forceinline__ void mma_row_steps_warp(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred e, pa, pt;\n\t.reg .b64 b<8>;\n\t"
+        "{\n\t.reg .pred e, pa, pt;\n\t.reg .b64 b<4>;\n\t"
         "elect.sync _|e, 0xffffffff;\n\t"
         "setp.ne.b32 pa, %4, 0;\n\t"
         "setp.eq.b32 pt, 0, 0;\n\t"
         "add.s64 b1, %2, 128;\n\t"
         "add.s64 b2, %2, 256;\n\t"
         "add.s64 b3, %2, 384;\n\t"
-        "add.s64 b4, %2, 512;\n\t"
-        "add.s64 b5, %2, 640;\n\t"
-        "add.s64 b6, %2, 768;\n\t"
-        "add.s64 b7, %2, 896;\n\t"
         "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, pa;\n\t"
         "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+16], b1, %3, pt;\n\t"
         "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+32], b2, %3, pt;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+48], b3, %3, pt;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+64], b4, %3, pt;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+80], b5, %3, pt;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+96], b6, %3, pt;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+112], b7, %3, pt;\n\t}"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+48], b3, %3, pt;\n\t}"
         ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }

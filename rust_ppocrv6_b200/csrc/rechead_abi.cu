@@ -1203,7 +1203,8 @@ int enqueue_score(rh_ctx* ctx, const rh_weight* w, Slot& s, const rh_weight::Per
         s.launches++;
         p.ctab = (const float*)(ws + L.table);
     }
-    if (int rc = launch_head_and_merge(s, p, false, grid, st)) return rc;
+    RH_CUDA(rh::launch_head(p, false, grid, st));
+    s.launches++;
     rh::LossScoreParams q{};
     q.x = d_a;
     q.rows = rows;
@@ -1215,6 +1216,9 @@ int enqueue_score(rh_ctx* ctx, const rh_weight* w, Slot& s, const rh_weight::Per
     q.form = w->f32 ? 2 : w->compact ? 1 : 0;
     q.idx = p.idx;
     q.prob = p.prob;
+    q.partial = p.partial;
+    q.split_row0 = rows - split_rows(p);
+    q.n_splits = p.n_splits;
     q.loss = d_loss;
     q.lse = d_lse;
     q.status = s.d_status;
