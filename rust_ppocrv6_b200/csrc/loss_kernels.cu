@@ -92,6 +92,7 @@ __global__ void __launch_bounds__(kPackThreads) loss_pack_kernel(const __grid_co
     __shared__ uint8_t s_valid[128];
     __shared__ int s_scan[kPackWarps];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    launch_next();
     const bool is_w = (int)blockIdx.x < p.w_tiles;
     const int tile = is_w ? (int)blockIdx.x : (int)blockIdx.x - p.w_tiles;
     const long long row0 = (long long)tile * kLossTile;
@@ -617,7 +618,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
     auto bar = [&](int i) -> uint32_t { return base + kMOffBars + 8u * (uint32_t)i; };
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Waiter wt{misc + 1, p.status, p.timeout_ns};
-    const bool with_o = p.part_o != nullptr;
+    const bool with_o = WPASS || p.part_o != nullptr;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < 4; ++s) {
@@ -654,6 +655,8 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
     tc_fence_after();
     const uint32_t tmem = misc[0];
     const int feat = 16 * p.ksteps;
+    launch_next();
+    wait_previous();
 
     if (warp < 4) {
         setmaxnreg_dec<kCtrlRegs>();
@@ -1086,10 +1089,32 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                     if (lane == 0) mbar_arrive(bar(kLBarOEmpty));
                 }
                 if (!ok) break;
+                const bool direct = WPASS && p.dw != nullptr;
+                if (direct && U.own * 128 + r < p.n) {
+                    // a thread's class row, 16 bytes at a time
+                    const size_t at = (size_t)(U.own * 128 + r) * p.k + f0;
+#pragma unroll
+                    for (int q = 0; q < (F32 ? 16 : 8); ++q) {
+                        if constexpr (F32) {
+                            if (f0 + 4 * q < p.k)
+                                *reinterpret_cast<float4*>(static_cast<float*>(p.dw) + at + 4 * q) =
+                                    make_float4(acc[2 * q].x, acc[2 * q].y, acc[2 * q + 1].x, acc[2 * q + 1].y);
+                        } else if (f0 + 8 * q < p.k) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const __nv_bfloat162 h = __floats2bfloat162_rn(acc[4 * q + j].x, acc[4 * q + j].y);
+                                w[j] = *reinterpret_cast<const uint32_t*>(&h);
+                            }
+                            *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.dw) + at + 8 * q) =
+                                make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    }
+                }
                 float* po = p.part_o + ((size_t)u * feat + f0) * 128 + r;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    if (f0 + 16 * q < feat) {
+                    if (!direct && f0 + 16 * q < feat) {
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
                             po[(size_t)(16 * q + 2 * j) * 128] = acc[8 * q + j].x;
@@ -1113,7 +1138,10 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                     const float k1 = b0.x == -CUDART_INF_F ? 0.0f : ex2_approx(b0.x - m);
                     out = make_float2(m, (a0.y + a1.y) * k0 + (b0.y + b1.y) * k1);
                 }
-                p.part_ms[(size_t)u * 128 + r] = out;
+                if (!WPASS || p.dw == nullptr)
+                    p.part_ms[(size_t)u * 128 + r] = out;
+                else if (p.db && U.own * 128 + r < p.n)
+                    p.db[U.own * 128 + r] = out.x;
             }
         }
     }
@@ -1282,7 +1310,7 @@ __device__ __forceinline__ void join_units(const float* part_o, size_t u0, int n
 #pragma unroll
     for (int i = 0; i < kPer; ++i) a[i] = 0.0f;
     const float* po = part_o + u0 * feat * 128 + (size_t)f0 * 128 + l0 + r;
-#pragma unroll 4
+#pragma unroll(R == 8 ? 8 : 2)
     for (int s = 0; s < ns; ++s, po += (size_t)feat * 128) {
         const float w = WEIGHTED ? wgt[s * R + r] : 1.0f;
 #pragma unroll
@@ -1313,6 +1341,8 @@ __global__ void __launch_bounds__(256) loss_rows_kernel(const __grid_constant__ 
     __shared__ float red[kG][R];
     __shared__ float s_lse2[R], s_inv[R];
     const int tid = threadIdx.x;
+    launch_next();
+    wait_previous();
     const long long row0 = (long long)blockIdx.x * R;
     const int mb = (int)(row0 >> 7), l0 = (int)(row0 & 127);
     const int ns = mb < p.whole_units ? 1 : p.n_splits;
@@ -1415,6 +1445,7 @@ template <bool F32, int R>
 __global__ void __launch_bounds__(256) loss_reduce_kernel(const __grid_constant__ LossReduceParams p) {
     using T = typename Elem<F32>::type;
     extern __shared__ float sm[];  // [R][feat + 1]
+    wait_previous();
     const int j0 = (int)blockIdx.x * R, tile = j0 >> 7, l0 = j0 & 127;
     const int ns = tile < p.whole_units ? 1 : p.n_splits;
     const size_t u0 = tile < p.whole_units ? (size_t)tile : (size_t)p.whole_units + (size_t)(tile - p.whole_units) * p.n_splits;
@@ -1497,18 +1528,28 @@ __global__ void __launch_bounds__(256) loss_score_kernel(const __grid_constant__
         float m = -CUDART_INF_F;
         sum = 0.0f;
         best = 0x7fffffff;
-        for (int i = s; i < p.n_splits; i += 8) {
-            const float4 v = p.partial[(size_t)i * (size_t)(p.rows - p.split_row0) + (size_t)(row - p.split_row0)];
-            const int c = __float_as_int(v.z);
-            if (v.x > m) {
-                sum = (m == -CUDART_INF_F ? 0.0f : sum * ex2_approx(m - v.x)) + v.y;
-                m = v.x;
-                best = c;
-            } else if (v.x != -CUDART_INF_F) {
-                sum += v.y * ex2_approx(v.x - m);
-                if (v.x == m) best = min(best, c);
-            } else if (isnan(v.x) || isnan(v.y)) {
-                sum = CUDART_NAN_F;
+        // eight ranges' entries in flight at a time: their latency is what this join costs
+        const float4* part = p.partial + (size_t)(row - p.split_row0);
+        const size_t step = (size_t)(p.rows - p.split_row0);
+        for (int i0 = s; i0 < p.n_splits; i0 += 64) {
+            float4 v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                v[j] = i0 + 8 * j < p.n_splits ? __ldg(part + (size_t)(i0 + 8 * j) * step)
+                                               : make_float4(-CUDART_INF_F, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int c = __float_as_int(v[j].z);
+                if (v[j].x > m) {
+                    sum = (m == -CUDART_INF_F ? 0.0f : sum * ex2_approx(m - v[j].x)) + v[j].y;
+                    m = v[j].x;
+                    best = c;
+                } else if (v[j].x != -CUDART_INF_F) {
+                    sum += v[j].y * ex2_approx(v[j].x - m);
+                    if (v[j].x == m) best = min(best, c);
+                } else if (isnan(v[j].y)) {
+                    sum = CUDART_NAN_F;
+                }
             }
         }
         // lanes of a group that had no range, or only masked classes, bring nothing
@@ -1599,6 +1640,25 @@ cudaError_t loss_kernel_setup() {
     return smem_attr(loss_rows_kernel<false, 32>, kRowsSmemMax);
 }
 
+namespace {
+// A launch that may start before the kernel ahead of it in the stream has ended (that kernel says
+// when; wait_previous() then waits for its end).
+template <class P>
+cudaError_t launch_chained(void (*kernel)(P), int grid, int threads, int smem, cudaStream_t stream, const P& p) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+}  // namespace
+
 cudaError_t launch_loss_pack(const LossPackParams& p, bool f32, cudaStream_t stream) {
     const int grid = p.w_tiles + p.x_tiles;
     const int labels = p.sort_labels ? pack_smem_bytes(p.w_tiles, p.lab.n_top) : 0;
@@ -1612,52 +1672,37 @@ cudaError_t launch_loss_pack(const LossPackParams& p, bool f32, cudaStream_t str
     return cudaGetLastError();
 }
 
-namespace {
-template <bool F32, bool WPASS, bool SLOTS>
-void main_kernel(const LossMainParams& p, int grid, cudaStream_t stream) {
-    loss_main_kernel<F32, WPASS, SLOTS><<<grid, kMainThreads, kMSmemBytes, stream>>>(p);
-}
-}  // namespace
-
 cudaError_t launch_loss_main(const LossMainParams& p, bool f32, bool slots, bool weight_pass, int grid,
                              cudaStream_t stream) {
+    void (*k)(LossMainParams);
     if (f32)
-        weight_pass ? main_kernel<true, true, false>(p, grid, stream) : main_kernel<true, false, false>(p, grid, stream);
+        k = weight_pass ? loss_main_kernel<true, true, false> : loss_main_kernel<true, false, false>;
     else if (slots)
-        weight_pass ? main_kernel<false, true, true>(p, grid, stream) : main_kernel<false, false, true>(p, grid, stream);
+        k = weight_pass ? loss_main_kernel<false, true, true> : loss_main_kernel<false, false, true>;
     else
-        weight_pass ? main_kernel<false, true, false>(p, grid, stream) : main_kernel<false, false, false>(p, grid, stream);
-    return cudaGetLastError();
+        k = weight_pass ? loss_main_kernel<false, true, false> : loss_main_kernel<false, false, false>;
+    return launch_chained(k, grid, kMainThreads, kMSmemBytes, stream, p);
 }
 
 cudaError_t launch_loss_rows(const LossRowParams& p, bool f32, int sms, cudaStream_t stream) {
     const int tiles = (int)((p.rows + kLossTile - 1) / kLossTile);  // the last tile's padding rows too
     const int r = few_blocks(tiles, sms) ? 8 : 32;
-    const int grid = tiles * (kLossTile / r);
-    const int smem = rows_smem_bytes(r, p.k, p.feat, p.n_splits, p.lab.n_top);
-    if (f32 && r == 32)
-        loss_rows_kernel<true, 32><<<grid, 256, smem, stream>>>(p);
-    else if (f32)
-        loss_rows_kernel<true, 8><<<grid, 256, smem, stream>>>(p);
-    else if (r == 32)
-        loss_rows_kernel<false, 32><<<grid, 256, smem, stream>>>(p);
+    void (*k)(LossRowParams);
+    if (f32)
+        k = r == 32 ? loss_rows_kernel<true, 32> : loss_rows_kernel<true, 8>;
     else
-        loss_rows_kernel<false, 8><<<grid, 256, smem, stream>>>(p);
-    return cudaGetLastError();
+        k = r == 32 ? loss_rows_kernel<false, 32> : loss_rows_kernel<false, 8>;
+    return launch_chained(k, tiles * (kLossTile / r), 256, rows_smem_bytes(r, p.k, p.feat, p.n_splits, p.lab.n_top), stream, p);
 }
 
 cudaError_t launch_loss_reduce(const LossReduceParams& p, bool f32, int sms, cudaStream_t stream) {
     const int r = few_blocks((p.n + kLossTile - 1) / kLossTile, sms) ? 8 : 32;
-    const int grid = (p.n + r - 1) / r, smem = r * (p.feat + 1) * 4;
-    if (f32 && r == 32)
-        loss_reduce_kernel<true, 32><<<grid, 256, smem, stream>>>(p);
-    else if (f32)
-        loss_reduce_kernel<true, 8><<<grid, 256, smem, stream>>>(p);
-    else if (r == 32)
-        loss_reduce_kernel<false, 32><<<grid, 256, smem, stream>>>(p);
+    void (*k)(LossReduceParams);
+    if (f32)
+        k = r == 32 ? loss_reduce_kernel<true, 32> : loss_reduce_kernel<true, 8>;
     else
-        loss_reduce_kernel<false, 8><<<grid, 256, smem, stream>>>(p);
-    return cudaGetLastError();
+        k = r == 32 ? loss_reduce_kernel<false, 32> : loss_reduce_kernel<false, 8>;
+    return launch_chained(k, (p.n + r - 1) / r, 256, r * (p.feat + 1) * 4, stream, p);
 }
 
 cudaError_t launch_loss_table(const float* ctab, long long n_floats, float inv_temp, float* out, cudaStream_t stream) {

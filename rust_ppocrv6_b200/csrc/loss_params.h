@@ -80,6 +80,11 @@ struct LossMainParams {
     float logit_scale;
     float* part_o;             // [units][16 ksteps][128], or null: only (offset, sum) (row pass)
     float2* part_ms;           // [units][128]: row pass (offset, sum); weight pass (bias gradient, 0)
+    // Weight pass of one unit per own tile: dW [n][k] and db [n] (or null) straight from the unit,
+    // instead of part_o / part_ms. 16-byte rows and pointer.
+    void* dw;
+    float* db;
+    int n, k;
     int* status;
     unsigned long long timeout_ns;
 };

@@ -1,6 +1,6 @@
 // PTX wrappers that only the training-loss kernels use, beside sm100_ptx.cuh: bf16 operands, a
-// shared-memory operand read along its rows (MN-major), 16-column TMEM accesses and the register
-// split between warpgroups.
+// shared-memory operand read along its rows (MN-major), 16-column TMEM accesses, the register
+// split between warpgroups and the programmatic launch order of a chain of kernels.
 #pragma once
 #include "sm100_ptx.cuh"
 
@@ -148,6 +148,11 @@ __device__ __forceinline__ void mma_row_steps_warp(uint32_t d_tmem, uint32_t a_t
         ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+
+// Programmatic launch order: the next kernel of the chain may start its own set-up now; nothing of
+// the one before may be read or overwritten before the wait, which sees it complete.
+__device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 template <int N>
 __device__ __forceinline__ void setmaxnreg_inc() {

@@ -1044,8 +1044,17 @@ int enqueue_grad(rh_ctx* ctx, Slot& s, int dtype, const void* d_a, int64_t rows,
     m.n_splits = L.cls.splits;
     m.tiles_per_split = L.cls.per;
     m.part_o = (float*)(ws + L.part_o);
+    // every class's sums end in one unit: no join, where the rows of dW can be written 16 bytes at a time
+    const size_t row_bytes = (size_t)k * (f32 ? 4 : 2);
+    if (L.cls.splits == 1 && row_bytes % 16 == 0 && ((uintptr_t)d_dw & 15) == 0) {
+        m.dw = d_dw;
+        m.db = d_dbias;
+        m.n = (int)n;
+        m.k = (int)k;
+    }
     RH_CUDA(rh::launch_loss_main(m, f32, L.slots, true, L.cls.grid, st));
     s.launches++;
+    if (m.dw) return RH_OK;
 
     rh::LossReduceParams d{};
     d.part_o = m.part_o;
