@@ -411,7 +411,8 @@ __global__ void __launch_bounds__(kPackThreads) loss_pack_kernel(const __grid_co
 // ------------------------------------------------------------------------------- main pass
 namespace {
 
-// Warps: 0 producer, 1 tensor-core issuer (and TMEM), 2-3 idle; four softmax warpgroups (warps
+// Warps: 0 producer, 1 issuer of the scores (and TMEM), 2 issuer of the second products, 3 idle; four
+// softmax warpgroups (warps
 // 4-19): two for the even and two for the odd streamed tiles of a unit, 64 columns each; two adding
 // warpgroups (20-27), 64 features of every tile's second product each. Softmax and adding are apart
 // so that a softmax warpgroup goes on to its next tile without waiting for the tensor core to use
@@ -461,8 +462,9 @@ constexpr int kLBarRing = 23;              // [4] a tile's offsets written
 constexpr int kLBarMsFull = 27;            // row states of a unit written
 constexpr int kLBarMsEmpty = 28;           // and read
 constexpr int kLBarTop = 29;               // [2 parities][4 quadrants] both halves' maxima written
-constexpr int kLBarDone = 37;              // every product retired (teardown)
-static_assert(8 * (kLBarDone + 1) <= 512, "barrier area");
+constexpr int kLBarSFree = 37;             // [3] a buffer's probabilities used up: it may take scores again
+constexpr int kLBarDone = 40;              // [2 issuers] every product retired (teardown)
+static_assert(8 * (kLBarDone + 2) <= 512, "barrier area");
 
 // TMEM columns: f32 own operand from 0, score buffers (Ring), second product
 constexpr uint32_t kTOwn = 0, kTO = 384;
@@ -492,11 +494,31 @@ __device__ __forceinline__ bool loss_wait_slow(uint32_t bar, uint32_t parity, vo
         }
     }
 }
-// The issuer's wait polls a while before it sleeps: its wake-up is on every tile's critical path.
+// The issuers' waits poll a while before they sleep (their wake-up is on every tile's critical path)
+// and look at all the barriers they need at once.
 __device__ __forceinline__ bool issuer_wait(uint32_t bar, uint32_t parity, const Waiter& w, int where) {
     bool ok = false;
     for (int i = 0; i < 64 && !ok; ++i) ok = mbar_try_wait(bar, parity);
     if (!ok) ok = loss_wait_slow(bar, parity, w.abort_flag, w.status, w.timeout_ns, where);
+    return __all_sync(0xffffffffu, ok);
+}
+__device__ __forceinline__ bool issuer_wait2(uint32_t bar0, uint32_t parity0, uint32_t bar1, uint32_t parity1,
+                                             const Waiter& w, int where) {
+    bool ok = false;
+    for (int i = 0; i < 64 && !ok; ++i) ok = mbar_try_wait2(bar0, parity0, bar1, parity1);
+    if (!ok)
+        ok = loss_wait_slow(bar0, parity0, w.abort_flag, w.status, w.timeout_ns, where) &&
+             loss_wait_slow(bar1, parity1, w.abort_flag, w.status, w.timeout_ns, where + 20);
+    return __all_sync(0xffffffffu, ok);
+}
+__device__ __forceinline__ bool issuer_wait3(uint32_t bar0, uint32_t parity0, uint32_t bar1, uint32_t parity1,
+                                             uint32_t bar2, uint32_t parity2, const Waiter& w, int where) {
+    bool ok = false;
+    for (int i = 0; i < 64 && !ok; ++i) ok = mbar_try_wait3(bar0, parity0, bar1, parity1, bar2, parity2);
+    if (!ok)
+        ok = loss_wait_slow(bar0, parity0, w.abort_flag, w.status, w.timeout_ns, where) &&
+             loss_wait_slow(bar1, parity1, w.abort_flag, w.status, w.timeout_ns, where) &&
+             loss_wait_slow(bar2, parity2, w.abort_flag, w.status, w.timeout_ns, where + 20);
     return __all_sync(0xffffffffu, ok);
 }
 // Uniform over the (converged) warp.
@@ -631,6 +653,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
         }
         for (int i = 0; i < 3; ++i) {
             mbar_init(bar(kLBarSFull + i), 1);
+            mbar_init(bar(kLBarSFree + i), 1);
             mbar_init(bar(kLBarPFull + 2 * i), 4);
             mbar_init(bar(kLBarPFull + 2 * i + 1), 4);
         }
@@ -641,6 +664,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
         for (int i = 0; i < 8; ++i) mbar_init(bar(kLBarTop + i), 2);
         mbar_init(bar(kLBarMsEmpty), 128);
         mbar_init(bar(kLBarDone), 1);
+        mbar_init(bar(kLBarDone + 1), 1);
         misc[1] = 0u;
         fence_mbar_init();
     }
@@ -697,78 +721,68 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                 loss_drain(bar(kLBarFull + s), ((issued - 1 - s) / kStages) & 1u, wt);
             for (uint32_t w = 0; w < 2 && w < owns; ++w) loss_drain(bar(kLBarAFull + w), ((owns - 1 - w) / 2) & 1u, wt);
         } else if (warp == 1) {
-            // ---------------------------------------------------------- tensor-core issuer
-            // Ring positions advance by increments: this loop is the tensor core's only feed.
+            // ------------------------------------------------------------ issuer of the scores
+            // Ring positions advance by increments: the issuers are the tensor core's only feed.
             const uint32_t id_s = idesc_16b(!F32, false, 128, 128);
-            const uint32_t id_o = idesc_16b(!F32, true, 128, (uint32_t)feat);
-            const uint64_t k_desc = smem_desc_k_sw128(base), mn_desc = smem_desc_mn_sw128(base);
-            constexpr uint64_t kStageDesc = kStage >> 4, kLoDesc = kLossImage >> 4, kHalfDesc = 8192 >> 4;  // 64 rows
-            constexpr uint32_t kBufs = Ring<F32>::kBufs;
-            uint32_t ss = 0, sph = 0, sb = 0;  // stage (and phase) and buffer of the next scores
-            uint32_t os = 0, oph = 1;          // stage of the next second product; phase of its buffer's release
-            uint32_t ob = 0, pph = 0;          // its next probabilities' buffer, and that buffer's phase
-            uint32_t uc = 0;
-            uint64_t own_desc = 0;
-            auto scores = [&]() -> bool {
-                if (!issuer_wait(bar(kLBarFull + ss), sph, wt, 102)) return false;
-                tc_fence_after();
-                const uint32_t d = tmem + Ring<F32>::kTS + 128u * sb, a = tmem + kTOwn;
-                const uint64_t b = k_desc + ss * kStageDesc;
-                if (F32) {
-                    mma_k_steps_warp(d, a + 64u, b, id_s, 0u, p.ksteps);
-                    mma_k_steps_warp(d, a, b + kLoDesc, id_s, 1u, p.ksteps);
-                    mma_k_steps_warp(d, a, b, id_s, 1u, p.ksteps);
-                } else {
-                    mma_k_steps_ss_warp(d, own_desc, b, id_s, p.ksteps);
-                }
-                mma_commit_warp(bar(kLBarSFull + (int)sb));
-                if (++sb == kBufs) sb = 0u;
-                if (++ss == kStages) ss = 0u, sph ^= 1u;
-                return true;
-            };
+            const uint64_t k_desc = smem_desc_k_sw128(base);
+            uint32_t st = 0, sph = 0, b = 0, fph = 1, uc = 0;  // stage, buffer, their phases (the buffer: freed)
             bool ok = true;
             for (int u = blockIdx.x; ok && lunit_exists(u, p); u += gridDim.x, ++uc) {
                 const LUnit U = lunit(u, p);
-                const uint32_t n = (uint32_t)(U.c1 - U.c0), w = F32 ? 0u : uc & 1u;
+                const uint32_t w = F32 ? 0u : uc & 1u;
                 ok = issuer_wait(bar(kLBarAFull + w), F32 ? uc & 1u : (uc >> 1) & 1u, wt, 103);
-                if (!ok) break;
-                tc_fence_after();
-                own_desc = k_desc + ((Ring<F32>::kOwn + w * kLossImage) >> 4);
-                for (uint32_t i = 0; ok && i < kBufs && i < n; ++i) ok = scores();
-                for (uint32_t i = 0; ok && i < n; ++i) {
-#pragma unroll
-                    for (uint32_t half = 0; half < 2; ++half) {
-                        ok = ok && issuer_wait(bar(kLBarPFull + 2 * (int)ob + half), pph, wt, 104);
-                        if (half == 0 && with_o) {  // the previous tile's product is added up
-                            ok = ok && issuer_wait(bar(kLBarOEmpty), oph, wt, 105);
-                            oph ^= 1u;
-                        }
-                        if (!ok) break;
-                        tc_fence_after();
-                        if (with_o) {
-                            const uint64_t b = mn_desc + os * kStageDesc + half * kHalfDesc;
-                            const uint32_t a = tmem + Ring<F32>::kTS + 128u * ob + 64u * half, d = tmem + kTO;
-                            if (F32) {
-                                mma_row_steps_warp(d, a + 8u, b, id_o, half);
-                                mma_row_steps_warp(d, a, b + kLoDesc, id_o, 1u);
-                            }
-                            mma_row_steps_warp(d, a, b, id_o, F32 ? 1u : half);
-                        }
-                    }
+                const uint64_t own_desc = k_desc + ((Ring<F32>::kOwn + w * kLossImage) >> 4);
+                for (int c = U.c0; ok && c < U.c1; ++c) {
+                    ok = issuer_wait2(bar(kLBarFull + st), sph, bar(kLBarSFree + b), fph, wt, 102);
                     if (!ok) break;
-                    if (with_o) mma_commit_warp(bar(kLBarOFull));
-                    mma_commit_warp(bar(kLBarEmpty + (int)os));
-                    if (++os == kStages) os = 0u;
-                    if (++ob == kBufs) ob = 0u, pph ^= 1u;
-                    // The buffer that the second product reads takes the scores of the tile kBufs further:
-                    // the tensor core runs one thread's products in order.
-                    if (i + kBufs < n) ok = scores();
+                    tc_fence_after();
+                    const uint64_t b_desc = k_desc + st * (uint64_t)(kStage >> 4);
+                    const uint32_t d = tmem + Ring<F32>::kTS + 128u * b;
+                    if (F32)
+                        mma_scores_f32_warp(d, tmem + kTOwn, b_desc, id_s, p.ksteps);
+                    else
+                        mma_scores_bf16_warp(d, own_desc, b_desc, id_s, p.ksteps);
+                    mma_commit_warp(bar(kLBarSFull + (int)b));
+                    if (++st == kStages) st = 0u, sph ^= 1u;
+                    if (++b == Ring<F32>::kBufs) b = 0u, fph ^= 1u;
                 }
                 if (!ok) break;
                 mma_commit_warp(bar(kLBarAEmpty + w));
             }
             mma_commit_warp(bar(kLBarDone));
             loss_drain(bar(kLBarDone), 0u, wt);
+        } else if (warp == 2) {
+            // -------------------------------------------------- issuer of the second products
+            const uint32_t id_o = idesc_16b(!F32, true, 128, (uint32_t)feat);
+            const uint64_t mn_desc = smem_desc_mn_sw128(base);
+            uint32_t st = 0, b = 0, pph = 0, oph = 1;  // stage, buffer and phase of its probabilities; O's release
+            bool ok = true;
+            for (int u = blockIdx.x; ok && lunit_exists(u, p); u += gridDim.x) {
+                const LUnit U = lunit(u, p);
+                for (int c = U.c0; ok && c < U.c1; ++c) {
+                    // both halves' probabilities, and the previous tile's product added up
+                    ok = issuer_wait3(bar(kLBarPFull + 2 * (int)b), pph, bar(kLBarPFull + 2 * (int)b + 1), pph,
+                                      bar(kLBarOEmpty), with_o ? oph : 1u, wt, 104);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (with_o) {
+                        const uint64_t b_desc = mn_desc + st * (uint64_t)(kStage >> 4);
+                        const uint32_t a = tmem + Ring<F32>::kTS + 128u * b;
+                        if (F32)
+                            mma_rows_f32_warp(tmem + kTO, a, b_desc, id_o);
+                        else
+                            mma_rows_bf16_warp(tmem + kTO, a, b_desc, id_o);
+                        mma_commit_warp(bar(kLBarOFull));
+                        oph ^= 1u;
+                    }
+                    mma_commit_warp(bar(kLBarSFree + (int)b));
+                    mma_commit_warp(bar(kLBarEmpty + (int)st));
+                    if (++st == kStages) st = 0u;
+                    if (++b == Ring<F32>::kBufs) b = 0u, pph ^= 1u;
+                }
+            }
+            mma_commit_warp(bar(kLBarDone + 1));
+            loss_drain(bar(kLBarDone + 1), 0u, wt);
         }
     } else if (warp < 20) {
         // (kSoftRegs is what the kernel was launched with)
@@ -1310,7 +1324,7 @@ __device__ __forceinline__ void join_units(const float* part_o, size_t u0, int n
 #pragma unroll
     for (int i = 0; i < kPer; ++i) a[i] = 0.0f;
     const float* po = part_o + u0 * feat * 128 + (size_t)f0 * 128 + l0 + r;
-#pragma unroll(R == 8 ? 8 : 2)
+#pragma unroll(R == 8 ? 8 : 4)
     for (int s = 0; s < ns; ++s, po += (size_t)feat * 128) {
         const float w = WEIGHTED ? wgt[s * R + r] : 1.0f;
 #pragma unroll

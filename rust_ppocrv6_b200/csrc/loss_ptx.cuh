@@ -54,30 +54,56 @@ __device__ __forceinline__ void tmem_st32x32b_x16(uint32_t taddr, const uint32_t
         : "memory");
 }
 
-// Up to 8 K steps of a product whose K runs along the image's rows' bytes (32 bytes a step, the
-// second four steps in the image's other half); A K-major in TMEM, 8 columns a step. One elect.sync
-// and immediate offsets: the issuing warp spends as few slots as it can between instructions.
-__device__ __forceinline__ void mma_k_steps_warp(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate, int steps) {
+// Scores of a tile, f32: the products lo.hi, hi.lo and hi.hi of up to 8 K steps each. K runs along
+// the image's rows' bytes (32 bytes a step, the second four steps in the image's other half; the low
+// image 32 KB further); A in TMEM, 8 columns a step, the low part 64 columns further. One elect.sync
+// and immediate offsets: the tensor core queues only a few instructions, so what the issuing warp
+// spends between them is time it stands still.
+__device__ __forceinline__ void mma_scores_f32_warp(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, int steps) {
     asm volatile(
-        "{\n\t.reg .pred e, pa, pt, q1, q2, q3, q4, q5, q6, q7;\n\t.reg .b64 b<8>;\n\t"
+        "{\n\t.reg .pred e, pf, pt, q1, q2, q3, q4, q5, q6, q7;\n\t.reg .b64 b<8>, c<8>;\n\t"
         "elect.sync _|e, 0xffffffff;\n\t"
-        "setp.ne.b32 pa, %4, 0;\n\t"
+        "setp.ne.b32 pf, 0, 0;\n\t"
         "setp.eq.b32 pt, 0, 0;\n\t"
+        "setp.gt.and.s32 q1, %4, 1, e;\n\t"
         "add.s64 b1, %2, 2;\n\t"
-        "setp.gt.and.s32 q1, %5, 1, e;\n\t"
+        "setp.gt.and.s32 q2, %4, 2, e;\n\t"
         "add.s64 b2, %2, 4;\n\t"
-        "setp.gt.and.s32 q2, %5, 2, e;\n\t"
+        "setp.gt.and.s32 q3, %4, 3, e;\n\t"
         "add.s64 b3, %2, 6;\n\t"
-        "setp.gt.and.s32 q3, %5, 3, e;\n\t"
+        "setp.gt.and.s32 q4, %4, 4, e;\n\t"
         "add.s64 b4, %2, 1024;\n\t"
-        "setp.gt.and.s32 q4, %5, 4, e;\n\t"
+        "setp.gt.and.s32 q5, %4, 5, e;\n\t"
         "add.s64 b5, %2, 1026;\n\t"
-        "setp.gt.and.s32 q5, %5, 5, e;\n\t"
+        "setp.gt.and.s32 q6, %4, 6, e;\n\t"
         "add.s64 b6, %2, 1028;\n\t"
-        "setp.gt.and.s32 q6, %5, 6, e;\n\t"
+        "setp.gt.and.s32 q7, %4, 7, e;\n\t"
         "add.s64 b7, %2, 1030;\n\t"
-        "setp.gt.and.s32 q7, %5, 7, e;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, pa;\n\t"
+        "add.s64 c0, %2, 2048;\n\t"
+        "add.s64 c1, %2, 2050;\n\t"
+        "add.s64 c2, %2, 2052;\n\t"
+        "add.s64 c3, %2, 2054;\n\t"
+        "add.s64 c4, %2, 3072;\n\t"
+        "add.s64 c5, %2, 3074;\n\t"
+        "add.s64 c6, %2, 3076;\n\t"
+        "add.s64 c7, %2, 3078;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+64], %2, %3, pf;\n\t"
+        "@q1 tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+72], b1, %3, pt;\n\t"
+        "@q2 tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+80], b2, %3, pt;\n\t"
+        "@q3 tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+88], b3, %3, pt;\n\t"
+        "@q4 tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+96], b4, %3, pt;\n\t"
+        "@q5 tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+104], b5, %3, pt;\n\t"
+        "@q6 tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+112], b6, %3, pt;\n\t"
+        "@q7 tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+120], b7, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+0], c0, %3, pt;\n\t"
+        "@q1 tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+8], c1, %3, pt;\n\t"
+        "@q2 tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+16], c2, %3, pt;\n\t"
+        "@q3 tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+24], c3, %3, pt;\n\t"
+        "@q4 tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+32], c4, %3, pt;\n\t"
+        "@q5 tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+40], c5, %3, pt;\n\t"
+        "@q6 tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+48], c6, %3, pt;\n\t"
+        "@q7 tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+56], c7, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+0], %2, %3, pt;\n\t"
         "@q1 tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+8], b1, %3, pt;\n\t"
         "@q2 tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+16], b2, %3, pt;\n\t"
         "@q3 tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+24], b3, %3, pt;\n\t"
@@ -85,40 +111,39 @@ __device__ __forceinline__ void mma_k_steps_warp(uint32_t d_tmem, uint32_t a_tme
         "@q5 tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+40], b5, %3, pt;\n\t"
         "@q6 tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+48], b6, %3, pt;\n\t"
         "@q7 tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+56], b7, %3, pt;\n\t}"
-        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(steps)
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(steps)
         : "memory");
 }
 
-// The same with A in shared memory too, an image like B's; the accumulator starts at zero.
-__device__ __forceinline__ void mma_k_steps_ss_warp(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                                    int steps) {
+// Scores of a tile, bf16: up to 8 K steps, A in shared memory, an image like B's.
+__device__ __forceinline__ void mma_scores_bf16_warp(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, int steps) {
     asm volatile(
-        "{\n\t.reg .pred e, pa, pt, q1, q2, q3, q4, q5, q6, q7;\n\t.reg .b64 a<8>, b<8>;\n\t"
+        "{\n\t.reg .pred e, pf, pt, q1, q2, q3, q4, q5, q6, q7;\n\t.reg .b64 a<8>, b<8>;\n\t"
         "elect.sync _|e, 0xffffffff;\n\t"
-        "setp.ne.b32 pa, 0, 0;\n\t"
+        "setp.ne.b32 pf, 0, 0;\n\t"
         "setp.eq.b32 pt, 0, 0;\n\t"
-        "add.s64 a1, %1, 2;\n\t"
-        "add.s64 b1, %2, 2;\n\t"
         "setp.gt.and.s32 q1, %4, 1, e;\n\t"
-        "add.s64 a2, %1, 4;\n\t"
-        "add.s64 b2, %2, 4;\n\t"
+        "add.s64 b1, %2, 2;\n\t"
+        "add.s64 a1, %1, 2;\n\t"
         "setp.gt.and.s32 q2, %4, 2, e;\n\t"
-        "add.s64 a3, %1, 6;\n\t"
-        "add.s64 b3, %2, 6;\n\t"
+        "add.s64 b2, %2, 4;\n\t"
+        "add.s64 a2, %1, 4;\n\t"
         "setp.gt.and.s32 q3, %4, 3, e;\n\t"
-        "add.s64 a4, %1, 1024;\n\t"
-        "add.s64 b4, %2, 1024;\n\t"
+        "add.s64 b3, %2, 6;\n\t"
+        "add.s64 a3, %1, 6;\n\t"
         "setp.gt.and.s32 q4, %4, 4, e;\n\t"
-        "add.s64 a5, %1, 1026;\n\t"
-        "add.s64 b5, %2, 1026;\n\t"
+        "add.s64 b4, %2, 1024;\n\t"
+        "add.s64 a4, %1, 1024;\n\t"
         "setp.gt.and.s32 q5, %4, 5, e;\n\t"
-        "add.s64 a6, %1, 1028;\n\t"
-        "add.s64 b6, %2, 1028;\n\t"
+        "add.s64 b5, %2, 1026;\n\t"
+        "add.s64 a5, %1, 1026;\n\t"
         "setp.gt.and.s32 q6, %4, 6, e;\n\t"
-        "add.s64 a7, %1, 1030;\n\t"
-        "add.s64 b7, %2, 1030;\n\t"
+        "add.s64 b6, %2, 1028;\n\t"
+        "add.s64 a6, %1, 1028;\n\t"
         "setp.gt.and.s32 q7, %4, 7, e;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, pa;\n\t"
+        "add.s64 b7, %2, 1030;\n\t"
+        "add.s64 a7, %1, 1030;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, pf;\n\t"
         "@q1 tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, pt;\n\t"
         "@q2 tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, pt;\n\t"
         "@q3 tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, pt;\n\t"
@@ -130,23 +155,99 @@ __device__ __forceinline__ void mma_k_steps_ss_warp(uint32_t d_tmem, uint64_t a_
         : "memory");
 }
 
-// The 4 K steps of a product whose contraction runs along 64 of the image's rows (2 KB a step); A in
-// TMEM, 16 columns a step (8 of them read).
-__device__ __forceinline__ void mma_row_steps_warp(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+// The second product of a tile, f32 (lo.hi, hi.lo, hi.hi): the contraction runs along the image's 128
+// rows (2 KB a step); A in TMEM, 16 columns a step: 8 of the high part, then 8 of the low part.
+__device__ __forceinline__ void mma_rows_f32_warp(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc) {
     asm volatile(
-        "{\n\t.reg .pred e, pa, pt;\n\t.reg .b64 b<4>;\n\t"
+        "{\n\t.reg .pred e, pf, pt;\n\t.reg .b64 b<8>, c<8>;\n\t"
         "elect.sync _|e, 0xffffffff;\n\t"
-        "setp.ne.b32 pa, %4, 0;\n\t"
+        "setp.ne.b32 pf, 0, 0;\n\t"
         "setp.eq.b32 pt, 0, 0;\n\t"
         "add.s64 b1, %2, 128;\n\t"
         "add.s64 b2, %2, 256;\n\t"
         "add.s64 b3, %2, 384;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, pa;\n\t"
+        "add.s64 b4, %2, 512;\n\t"
+        "add.s64 b5, %2, 640;\n\t"
+        "add.s64 b6, %2, 768;\n\t"
+        "add.s64 b7, %2, 896;\n\t"
+        "add.s64 c0, %2, 2048;\n\t"
+        "add.s64 c1, %2, 2176;\n\t"
+        "add.s64 c2, %2, 2304;\n\t"
+        "add.s64 c3, %2, 2432;\n\t"
+        "add.s64 c4, %2, 2560;\n\t"
+        "add.s64 c5, %2, 2688;\n\t"
+        "add.s64 c6, %2, 2816;\n\t"
+        "add.s64 c7, %2, 2944;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+8], %2, %3, pf;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+24], b1, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+40], b2, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+56], b3, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+72], b4, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+88], b5, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+104], b6, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+120], b7, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+0], c0, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+16], c1, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+32], c2, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+48], c3, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+64], c4, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+80], c5, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+96], c6, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+112], c7, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+0], %2, %3, pt;\n\t"
         "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+16], b1, %3, pt;\n\t"
         "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+32], b2, %3, pt;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+48], b3, %3, pt;\n\t}"
-        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+48], b3, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+64], b4, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+80], b5, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+96], b6, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+112], b7, %3, pt;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc)
         : "memory");
+}
+
+// The same in bf16 (8 of a step's 16 columns).
+__device__ __forceinline__ void mma_rows_bf16_warp(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred e, pf, pt;\n\t.reg .b64 b<8>;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 pf, 0, 0;\n\t"
+        "setp.eq.b32 pt, 0, 0;\n\t"
+        "add.s64 b1, %2, 128;\n\t"
+        "add.s64 b2, %2, 256;\n\t"
+        "add.s64 b3, %2, 384;\n\t"
+        "add.s64 b4, %2, 512;\n\t"
+        "add.s64 b5, %2, 640;\n\t"
+        "add.s64 b6, %2, 768;\n\t"
+        "add.s64 b7, %2, 896;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+0], %2, %3, pf;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+16], b1, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+32], b2, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+48], b3, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+64], b4, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+80], b5, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+96], b6, %3, pt;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+112], b7, %3, pt;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc)
+        : "memory");
+}
+
+// All phases complete? The try_waits issue back to back, so their latencies overlap.
+__device__ __forceinline__ bool mbar_try_wait3(uint32_t bar0, uint32_t parity0, uint32_t bar1, uint32_t parity1,
+                                               uint32_t bar2, uint32_t parity2) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p0, p1, p2;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p0, [%1], %2;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p1, [%3], %4;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p2, [%5], %6;\n\t"
+        "and.pred p0, p0, p1;\n\t"
+        "and.pred p0, p0, p2;\n\t"
+        "selp.u32 %0, 1, 0, p0;\n\t}"
+        : "=r"(ok)
+        : "r"(bar0), "r"(parity0), "r"(bar1), "r"(parity1), "r"(bar2), "r"(parity2)
+        : "memory");
+    return ok != 0;
 }
 
 // Programmatic launch order: the next kernel of the chain may start its own set-up now; nothing of
