@@ -412,15 +412,18 @@ __global__ void __launch_bounds__(kPackThreads) loss_pack_kernel(const __grid_co
 namespace {
 
 // Warps: 0 producer, 1 issuer of the scores (and TMEM), 2 issuer of the second products, 3 idle; four
-// softmax warpgroups (warps
-// 4-19): two for the even and two for the odd streamed tiles of a unit, 64 columns each; two adding
-// warpgroups (20-27), 64 features of every tile's second product each. Softmax and adding are apart
-// so that a softmax warpgroup goes on to its next tile without waiting for the tensor core to use
-// its last. Scores live in a ring of 128-column buffers: two in f32, whose own operand (hi | lo)
-// takes 128 TMEM columns; three in bf16, whose own operand stays in shared memory, so that the next
-// scores are there when a softmax warpgroup comes for them. (An operand in TMEM costs the tensor
-// core less shared-memory bandwidth; f32 is bound by the tensor core, bf16 is not. Narrower buffers
-// are no way out: an instruction of 64 columns takes as long as one of 128.)
+// softmax warpgroups (warps 4-19): two for the even and two for the odd streamed tiles, 64 columns
+// each; two adding warpgroups (20-27), 64 features of the second products each.
+// Softmax and adding are apart so that a softmax warpgroup goes on to its next tile without waiting
+// for the tensor core to use its last. Two issuers, because the tensor core queues only a few
+// instructions: while one waits on its barriers the other's products run (with one issuer, its waits
+// and the products added up: f32 took 3,870 cycles a tile without any softmax work, of which 3,072
+// were products).
+// Scores live in buffers of 128 TMEM columns: two in f32, whose own operand (hi | lo) takes 128
+// columns; three in bf16, whose own operand stays in shared memory, so that the next scores are there
+// when a softmax warpgroup comes for them. (An operand in TMEM costs the tensor core less
+// shared-memory bandwidth; f32 is bound by the tensor core, bf16 is not. Buffers of half a tile's
+// scores are no way out: an instruction of 64 columns takes as long as one of 128.)
 constexpr int kMainThreads = 896;
 constexpr int kLaunchRegs = 72;  // 65,536 registers / 896 threads
 constexpr int kCtrlRegs = 40, kSoftRegs = 72, kAddRegs = 88;
@@ -614,13 +617,19 @@ __device__ __forceinline__ void window_next(LabelWindow& w, const int2* ent, int
 
 }  // namespace
 
+// Streamed tiles whose second products the tensor core adds up before the adding warps do.
+// The tensor core's f32 accumulator rounds toward zero, a bias of up to 2^-24 of the sum a step. In
+// f32 every tile's product is added in registers: 24 steps stay below the operands' own error. In
+// bf16 the 8 steps of 32 tiles leave at most 2^-16, a hundredth of the probabilities' rounding; that
+// takes the adding off every tile's path, where the offset does not move (the weight pass; the row
+// pass where every row of the own tile is bounded, see below).
+constexpr int kAddEvery = 32;
+
 // Units (own tile, range of streamed tiles), persistent over the grid. Per streamed tile: scores
 // S = own . tile^T (tensor core), a softmax warpgroup turns them into
 // probabilities (row pass: against the running maximum; weight pass: 2^(s - lse) times the rows'
 // gradient factors, less the labels' shares) in the same TMEM columns, and a second product
-// O = P . tile reads the same tile the other way round. O is added to registers tile by tile: the
-// tensor core's f32 accumulator rounds toward zero, which over thousands of steps would bias the
-// sums; over one tile's steps it stays below the operands' own error.
+// O = P . tile reads the same tile the other way round; the adding warps sum it in registers.
 // f32: three products each (hi.lo, lo.hi, hi.hi).
 // bf16 with slots: the scores come with their bias, so they need no column table in the row pass;
 // and as bf16 probabilities have f32's range, a row's offset need not follow its maximum: by
@@ -681,6 +690,32 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
     const int feat = 16 * p.ksteps;
     launch_next();
     wait_previous();
+    // slots, row pass: the reach of a row's logits around the largest bias is |x_r| max|w|
+    float w_max = 0.0f, e_max = -CUDART_INF_F;
+    if (SLOTS && !WPASS && warp >= 2) {
+        bool nan = false;
+        for (int t = lane; t < p.str_tiles; t += 32) {
+            const float2 b = __ldg(p.w_bound + t);
+            nan |= isnan(b.x);
+            w_max = fmaxf(w_max, b.x);
+            e_max = fmaxf(e_max, b.y);
+        }
+        w_max = warp_max(w_max);
+        e_max = warp_max(e_max);
+        if (__any_sync(0xffffffffu, nan)) w_max = CUDART_INF_F;
+    }
+    auto reach_of = [&](int own, int row) { return p.logit_scale * __ldg(p.x_norm + (size_t)own * 128 + row) * w_max * 1.001f; };
+    auto in_bounds = [&](float reach) { return reach <= 40.0f && fabsf(reach + e_max) < 1e6f; };
+    // tiles added up in TMEM at a time, for this own tile (every role that asks finds the same)
+    auto add_every = [&](int own) -> int {
+        if (F32) return 1;
+        if (WPASS) return kAddEvery;
+        if (!SLOTS) return 1;
+        bool all = true;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) all = all && in_bounds(reach_of(own, 32 * i + lane));
+        return __all_sync(0xffffffffu, all) ? kAddEvery : 1;
+    };
 
     if (warp < 4) {
         setmaxnreg_dec<kCtrlRegs>();
@@ -759,8 +794,10 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
             bool ok = true;
             for (int u = blockIdx.x; ok && lunit_exists(u, p); u += gridDim.x) {
                 const LUnit U = lunit(u, p);
+                const int every = with_o ? add_every(U.own) : 1;
+                int held = 0;  // products in O so far
                 for (int c = U.c0; ok && c < U.c1; ++c) {
-                    // both halves' probabilities, and the previous tile's product added up
+                    // both halves' probabilities, and what O held added up
                     ok = issuer_wait3(bar(kLBarPFull + 2 * (int)b), pph, bar(kLBarPFull + 2 * (int)b + 1), pph,
                                       bar(kLBarOEmpty), with_o ? oph : 1u, wt, 104);
                     if (!ok) break;
@@ -771,9 +808,12 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                         if (F32)
                             mma_rows_f32_warp(tmem + kTO, a, b_desc, id_o);
                         else
-                            mma_rows_bf16_warp(tmem + kTO, a, b_desc, id_o);
-                        mma_commit_warp(bar(kLBarOFull));
-                        oph ^= 1u;
+                            mma_rows_bf16_warp(tmem + kTO, a, b_desc, id_o, held > 0 ? 1u : 0u);
+                        if (++held == every || c + 1 == U.c1) {
+                            mma_commit_warp(bar(kLBarOFull));
+                            oph ^= 1u;
+                            held = 0;
+                        }
                     }
                     mma_commit_warp(bar(kLBarSFree + (int)b));
                     mma_commit_warp(bar(kLBarEmpty + (int)st));
@@ -792,27 +832,18 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         const uint32_t patch = base + kMOffPatch + (uint32_t)(warp - 4) * 32u * kPatchRow * 4u;
         const uint32_t t_bufs = tmem + lanes + Ring<F32>::kTS + 64u * half;
-        float w_max = 0.0f, e_max = -CUDART_INF_F;
-        if (SLOTS && !WPASS) {
-            bool nan = false;
-            for (int t = lane; t < p.str_tiles; t += 32) {
-                const float2 b = __ldg(p.w_bound + t);
-                nan |= isnan(b.x);
-                w_max = fmaxf(w_max, b.x);
-                e_max = fmaxf(e_max, b.y);
-            }
-            w_max = warp_max(w_max);
-            e_max = warp_max(e_max);
-            if (__any_sync(0xffffffffu, nan)) w_max = CUDART_INF_F;
-        }
         float* ring = reinterpret_cast<float*>(gbase + kMOffRing);
         volatile float* tops = reinterpret_cast<volatile float*>(gbase + kMOffTop);
-        uint32_t cc = 0, uc = 0, uses = 0;
+        uint32_t cc = 0, uc = 0, uses = 0, rc = 0;  // tiles, units, own tiles; tiles whose offsets were handed on
         bool ok = true;
         for (int u = blockIdx.x; ok && lunit_exists(u, p); u += gridDim.x, ++uc) {
             const LUnit U = lunit(u, p);
             const uint32_t n = (uint32_t)(U.c1 - U.c0);
-            // labels of this warpgroup's first tile (weight pass): range, then entries
+            // This pair of warpgroups takes every tile whose number in the CTA's whole sequence has its
+            // parity. Scores come in that order, so the phase before the one it waits for is over (a wait
+            // on a phase's parity is good only then), however units of odd length shift the buffers.
+            const uint32_t i0 = (g ^ cc) & 1u;
+            // labels of the first of them (weight pass): range, then entries
             LabelWindow lw{};
             auto label_range = [&](int c, int& a, int& b) {
                 const int32_t* o = p.sp_off + (size_t)c * (2 * p.own_tiles + 1) + 2 * U.own + half;
@@ -820,9 +851,9 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                 b = __ldg(o + 1);
             };
             auto label_base = [&](int c) { return p.sp_ent + (size_t)c * 128 * p.n_top; };
-            if (WPASS && g < n) {
-                label_range(U.c0 + (int)g, lw.next, lw.end);
-                window_open(lw, label_base(U.c0 + (int)g), lane);
+            if (WPASS && i0 < n) {
+                label_range(U.c0 + (int)i0, lw.next, lw.end);
+                window_open(lw, label_base(U.c0 + (int)i0), lane);
             }
             if (F32) {
                 // own operand -> TMEM: warpgroup wg takes K slots 64 half .. 64 half + 63 of the lane's
@@ -850,15 +881,17 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
 
             const float own_mul = F32 ? p.logit_scale * __ldg(p.own_scale + U.own) : p.logit_scale;
             const float lane_e = WPASS && !SLOTS ? __ldg(p.lane_e + (size_t)U.own * 128 + r) : 0.0f;
+            // the tiles' offsets go to the adding warps only where they move
+            const bool ringed = !WPASS && with_o && add_every(U.own) == 1;
             bool bounded = false;
             float upper = 0.0f;
             if (SLOTS && !WPASS) {
-                const float reach = p.logit_scale * __ldg(p.x_norm + (size_t)U.own * 128 + r) * w_max * 1.001f;
+                const float reach = reach_of(U.own, r);
                 upper = reach + e_max;
-                bounded = __all_sync(0xffffffffu, reach <= 40.0f && fabsf(upper) < 1e6f);
+                bounded = __all_sync(0xffffffffu, in_bounds(reach));
             }
             float off = -CUDART_INF_F, sum = 0.0f, carry = 0.0f;  // weight pass: sum + carry = bias gradient
-            for (uint32_t i = g; i < n; i += 2, ++uses) {
+            for (uint32_t i = i0; i < n; i += 2, ++uses) {
                 const int c = U.c0 + (int)i;
                 const uint32_t s = (cc + i) % kStages;
                 const uint32_t tab = base + Ring<F32>::kTab + s * 1024u + 256u * half;
@@ -878,7 +911,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                 tc_fence_after();
                 if (SLOTS && !WPASS && bounded) {
                     off = upper;
-                    if (with_o && half == 0) ring[((cc + i) & 3u) * 128 + r] = off;
+                    if (with_o && half == 0 && ringed) ring[((rc + i) & 3u) * 128 + r] = off;
                     const float2 sub2 = make_float2(-off, -off);
                     float2 ts = make_float2(0.f, 0.f);
 #pragma unroll (F32 ? 1 : 4)
@@ -928,7 +961,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                     const float m0 = m == -CUDART_INF_F ? 0.0f : m;
                     const float corr = off == -CUDART_INF_F ? 0.0f : ex2_approx(off - m0);
                     off = m;
-                    if (with_o && half == 0) ring[((cc + i) & 3u) * 128 + r] = m;
+                    if (with_o && half == 0 && ringed) ring[((rc + i) & 3u) * 128 + r] = m;
                     const float sub = F32 ? 14.0f - m0 : -m0;
                     const float2 sub2 = make_float2(sub, sub);
                     float2 ts = make_float2(0.f, 0.f);
@@ -1035,11 +1068,12 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                 if (lane == 0) {
                     mbar_arrive(bar(kLBarPFull + 2 * (int)buf + (int)half));
                     mbar_arrive(bar(kLBarEmpty + (int)s));
-                    if (!WPASS && with_o && half == 0) mbar_arrive(bar(kLBarRing + (int)((cc + i) & 3u)));
+                    if (!WPASS && with_o && half == 0 && ringed) mbar_arrive(bar(kLBarRing + (int)((rc + i) & 3u)));
                 }
             }
             if (!ok) break;
             cc += n;
+            if (ringed) rc += n;
             ok = loss_wait(bar(kLBarMsEmpty), (uc & 1u) ^ 1u, wt, 110);
             if (!ok) break;
             reinterpret_cast<float2*>(gbase + kMOffMs)[wg * 128 + r] = WPASS ? make_float2(sum, carry) : make_float2(off, sum);
@@ -1055,7 +1089,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
         const uint32_t t_o = tmem + ((uint32_t)(quad * 32) << 16) + kTO + 64u * g;
         const volatile float* ring = reinterpret_cast<const volatile float*>(gbase + kMOffRing);
         const int f0 = 64 * (int)g;
-        uint32_t cc = 0, uc = 0;
+        uint32_t fc = 0, rc = 0, uc = 0;  // products taken, of them with an offset; units
         bool ok = true;
         for (int u = blockIdx.x; ok && lunit_exists(u, p); u += gridDim.x, ++uc) {
             const LUnit U = lunit(u, p);
@@ -1064,23 +1098,25 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
 #pragma unroll
             for (int i = 0; i < 32; ++i) acc[i] = make_float2(0.f, 0.f);
             if (with_o) {
-                for (int c = U.c0; c < U.c1; ++c, ++cc) {
+                const int every = add_every(U.own);
+                for (int c = U.c0; c < U.c1; c += every, ++fc) {
                     float om = F32 ? __ldg(p.str_scale + c) : 1.0f;  // value of one unit of the product
                     if (F32) om *= WPASS ? __ldg(p.g_scale + c) : 1.0f / 16384.0f;
                     float corr = 1.0f;
-                    if (!WPASS) {
-                        ok = loss_wait(bar(kLBarRing + (int)(cc & 3u)), (cc >> 2) & 1u, wt, 112);
+                    if (!WPASS && every == 1) {
+                        ok = loss_wait(bar(kLBarRing + (int)(rc & 3u)), (rc >> 2) & 1u, wt, 112);
                         if (!ok) break;
-                        const float o = ring[(cc & 3u) * 128 + r];
+                        const float o = ring[(rc & 3u) * 128 + r];
                         const float m = fmaxf(off, o);
                         corr = off == m ? 1.0f : off == -CUDART_INF_F ? 0.0f : ex2_approx(off - m);
                         if (o != m) om *= ex2_approx(o - m);
                         off = m;
+                        ++rc;
                     }
-                    ok = loss_wait(bar(kLBarOFull), cc & 1u, wt, 109);
+                    const bool grow = !WPASS && !__all_sync(0xffffffffu, corr == 1.0f);
+                    ok = loss_wait(bar(kLBarOFull), fc & 1u, wt, 109);
                     if (!ok) break;
                     tc_fence_after();
-                    const bool grow = !WPASS && !__all_sync(0xffffffffu, corr == 1.0f);
                     const float2 om2 = make_float2(om, om), c2 = make_float2(corr, corr);
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {

@@ -206,12 +206,13 @@ __device__ __forceinline__ void mma_rows_f32_warp(uint32_t d_tmem, uint32_t a_tm
         : "memory");
 }
 
-// The same in bf16 (8 of a step's 16 columns).
-__device__ __forceinline__ void mma_rows_bf16_warp(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc) {
+// The same in bf16 (8 of a step's 16 columns), added to the accumulator where `accumulate` is set.
+__device__ __forceinline__ void mma_rows_bf16_warp(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                                   uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred e, pf, pt;\n\t.reg .b64 b<8>;\n\t"
         "elect.sync _|e, 0xffffffff;\n\t"
-        "setp.ne.b32 pf, 0, 0;\n\t"
+        "setp.ne.b32 pf, %4, 0;\n\t"
         "setp.eq.b32 pt, 0, 0;\n\t"
         "add.s64 b1, %2, 128;\n\t"
         "add.s64 b2, %2, 256;\n\t"
@@ -228,7 +229,7 @@ __device__ __forceinline__ void mma_rows_bf16_warp(uint32_t d_tmem, uint32_t a_t
         "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+80], b5, %3, pt;\n\t"
         "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+96], b6, %3, pt;\n\t"
         "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1+112], b7, %3, pt;\n\t}"
-        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc)
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 

@@ -203,10 +203,20 @@ def test_tail_layout_is_the_row_layout_transposed(rh, ctx, lines, t_len, k, n, d
         assert torch.equal(rows[i], tail[i]), i
 
 
-def test_full_vocabulary_batch_in_waves_and_ranges(rh, ctx):
-    """More row blocks than SMs (whole units, then split ones) on the full vocabulary."""
-    d = make(20_100, 120, 18710, seed=3)
-    check(grad(rh, ctx, d, "f32"), definition(d), False)
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [18_944, 20_100, 4_735])
+def test_full_vocabulary_batch_in_waves_and_ranges(rh, ctx, rows, dtype):
+    """Several units per SM, of odd and even numbers of tiles, whole and split, on the full vocabulary."""
+    d = make(rows, 120, 18710, seed=3)
+    check(grad(rh, ctx, d, dtype), definition(rounded(d, dtype)), dtype == "bf16")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,n", [(40_000, 300), (57_000, 129), (300, 40_000), (19_000, 6906)])
+def test_many_short_units(rh, ctx, rows, n, dtype):
+    """Long batches on small vocabularies and short ones on large: many units of few tiles each way."""
+    d = make(rows, 24, n, seed=4, n_top=3)
+    check(grad(rh, ctx, d, dtype, 2.0), definition(rounded(d, dtype), 2.0), dtype == "bf16")
 
 
 @pytest.mark.parametrize("op", ["ce", "distill"])
