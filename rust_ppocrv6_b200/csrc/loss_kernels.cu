@@ -992,6 +992,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                     const float2 le = make_float2(lane_e, lane_e);
                     const int2* ent = label_base(c);
                     window_use(lw, quad);
+                    const bool labelled = lw.groups != 0u || lw.last < 8;  // most tiles have none of a warp's classes
                     float2 ts = make_float2(0.f, 0.f);
 #pragma unroll (F32 ? 1 : 4)
                     for (int q = 0; q < 4; ++q) {
@@ -1021,7 +1022,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                         // the labels' shares, 8 columns (rows of x) at a time through a patch of
                         // shared memory: entries scatter into it, each lane then adds its class's row
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
+                        for (int h = 0; h < 2 && labelled; ++h) {
                             const int group = 2 * q + h;
                             bool any = false;
                             while (true) {
