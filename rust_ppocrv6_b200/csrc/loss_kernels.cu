@@ -84,7 +84,7 @@ __device__ __forceinline__ bool is_class(int c, int n) { return c >= 0 && c < n;
 constexpr int kPackThreads = 512, kPackWarps = kPackThreads / 32, kPackItems = 2048 / kPackThreads;
 
 template <bool F32>
-__global__ void __launch_bounds__(kPackThreads) loss_pack_kernel(const __grid_constant__ LossPackParams p) {
+__global__ void __launch_bounds__(kPackThreads, 2) loss_pack_kernel(const __grid_constant__ LossPackParams p) {
     using T = typename Elem<F32>::type;
     extern __shared__ __align__(16) uint8_t pack_smem[];
     __shared__ float red[kPackWarps], red2[4];
@@ -196,7 +196,10 @@ __global__ void __launch_bounds__(kPackThreads) loss_pack_kernel(const __grid_co
             }
             for (int o = width >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             float share[2] = {c[0] >= 0 ? q[0] / sum : 0.0f, c[1] >= 0 ? q[1] / sum : 0.0f};
-            if (p.lab.n_top > 1) {  // a class named twice: one entry with both shares
+            // a class named twice: one entry with both shares (rare; beyond 32 entries a lane holds two,
+            // which one match does not compare)
+            const uint32_t twice = __match_any_sync(0xffffffffu, c[0] >= 0 ? c[0] : ~lane) & gm;
+            if (slots == 2 || __any_sync(0xffffffffu, __popc(twice) > 1)) {
                 bool dup[2] = {false, false};
                 float all[2] = {share[0], share[1]};
                 for (int j = 0; j < p.lab.n_top; ++j) {
@@ -1214,47 +1217,59 @@ __device__ __forceinline__ int lane_slot(int s, int i) {
     return kRun * (s + 8 * (i / kRun)) + i % kRun;
 }
 
-// A lane's 16 values of row `c` of a row-major [.][k] matrix (zero past k).
+// A lane's 16 values of row `c` of a row-major [.][k] matrix (zero past k), as loaded: several rows'
+// loads are in flight before the first is used.
 template <bool F32>
-__device__ __forceinline__ void weight_row(const void* w, long long c, int k, int s, bool vec, float (&v)[16]) {
-    using T = typename Elem<F32>::type;
-    constexpr int kRun = F32 ? 4 : 8;
-    const T* a = static_cast<const T*>(w) + c * k;
+struct WeightRow {
+    static constexpr int kRun = F32 ? 4 : 8;
+    uint4 u[16 / kRun];
+    __device__ __forceinline__ void fetch(const void* w, long long c, int k, int s, bool vec) {
+        using T = typename Elem<F32>::type;
+        const T* a = static_cast<const T*>(w) + c * k;
 #pragma unroll
-    for (int j = 0; j < 16 / kRun; ++j) {
-        const int k0 = kRun * (s + 8 * j);
-        if (vec) {
-            uint4 u = make_uint4(0u, 0u, 0u, 0u);
-            if (k0 < k) u = __ldg(reinterpret_cast<const uint4*>(a + k0));
-            const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+        for (int j = 0; j < 16 / kRun; ++j) {
+            const int k0 = kRun * (s + 8 * j);
+            u[j] = make_uint4(0u, 0u, 0u, 0u);
+            if (vec) {
+                if (k0 < k) u[j] = __ldg(reinterpret_cast<const uint4*>(a + k0));
+            } else {
+                uint32_t x[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (F32) {
-                    v[4 * j + i] = __uint_as_float(x[i]);
-                } else {
-                    v[8 * j + 2 * i] = __uint_as_float(x[i] << 16);
-                    v[8 * j + 2 * i + 1] = __uint_as_float(x[i] & 0xffff0000u);
+                for (int i = 0; i < kRun; ++i) {
+                    if (k0 + i >= k) continue;
+                    if constexpr (F32)
+                        x[i] = __float_as_uint(a[k0 + i]);
+                    else
+                        x[i / 2] |= (uint32_t)__bfloat16_as_ushort(a[k0 + i]) << (16 * (i % 2));
                 }
+                u[j] = make_uint4(x[0], x[1], x[2], x[3]);
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kRun; ++i) v[kRun * j + i] = k0 + i < k ? to_f32(a[k0 + i]) : 0.0f;
         }
     }
-}
-template <int kRun>
-__device__ __forceinline__ void shared_row(const float* row, int k, int s, float (&v)[16]) {
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = lane_slot<kRun>(s, i) < k ? row[lane_slot<kRun>(s, i)] : 0.0f;
-}
-__device__ __forceinline__ float dot16(const float (&a)[16], const float (&b)[16]) {
-    float s0 = 0.0f, s1 = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 16; i += 2) {
-        s0 = fmaf(a[i], b[i], s0);
-        s1 = fmaf(a[i + 1], b[i + 1], s1);
+        for (int j = 0; j < 16 / kRun; ++j) u[j] = make_uint4(0u, 0u, 0u, 0u);
     }
-    return s0 + s1;
+    // values 2 i and 2 i + 1
+    __device__ __forceinline__ float2 pair(int i) const {
+        if constexpr (F32) {
+            const uint4 q = u[i / 2];
+            return i % 2 == 0 ? make_float2(__uint_as_float(q.x), __uint_as_float(q.y))
+                              : make_float2(__uint_as_float(q.z), __uint_as_float(q.w));
+        } else {
+            const uint4 q = u[i / 4];
+            const uint32_t x = i % 4 == 0 ? q.x : i % 4 == 1 ? q.y : i % 4 == 2 ? q.z : q.w;
+            return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+        }
+    }
+};
+template <int kRun>
+__device__ __forceinline__ void shared_row(const float* row, int k, int s, float2 (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int k0 = lane_slot<kRun>(s, 2 * i);
+        v[i] = make_float2(k0 < k ? row[k0] : 0.0f, k0 + 1 < k ? row[k0 + 1] : 0.0f);
+    }
 }
 __device__ __forceinline__ float group_sum(float v) {
 #pragma unroll
@@ -1268,25 +1283,37 @@ __device__ __forceinline__ float group_max(float v) {
 }
 
 // R rows of the features into shared memory (row stride k + 1), and back: coalesced along the
-// layout's contiguous direction.
+// layout's contiguous direction, every load of a thread in flight at once (k <= 128).
 template <int R, class T>
-__device__ __forceinline__ void load_rows(const T* x, long long row0, long long rows, int k, long long t_len, float* xs) {
-    if (t_len > 0) {
-        const int r = threadIdx.x % R;
-        const long long at = row0 + r < rows ? x_base(row0 + r, k, t_len) : 0;
-#pragma unroll 8
-        for (int kk = threadIdx.x / R; kk < k; kk += 256 / R)
-            xs[r * (k + 1) + kk] = row0 + r < rows ? to_f32(x[at + kk * t_len]) : 0.0f;
-    } else {
+struct RowLoad {
+    float v[R / 2];
+    __device__ __forceinline__ void fetch(const T* x, long long row0, long long rows, int k, long long t_len) {
+        if (t_len > 0) {
+            const int r = threadIdx.x % R;
+            const bool live = row0 + r < rows;
+            const T* at = x + (live ? x_base(row0 + r, k, t_len) : 0);
 #pragma unroll
-        for (int i = 0; i < R / 8; ++i) {
-            const int r = (threadIdx.x >> 5) + 8 * i;
-#pragma unroll 4
-            for (int kk = threadIdx.x & 31; kk < k; kk += 32)
-                xs[r * (k + 1) + kk] = row0 + r < rows ? to_f32(x[(row0 + r) * k + kk]) : 0.0f;
+            for (int i = 0; i < R / 2; ++i) {
+                const int kk = threadIdx.x / R + i * (256 / R);
+                v[i] = live && kk < k ? to_f32(at[kk * t_len]) : 0.0f;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < R / 2; ++i) {
+                const int r = (threadIdx.x >> 5) + 8 * (i / 4), kk = (threadIdx.x & 31) + 32 * (i % 4);
+                v[i] = row0 + r < rows && kk < k ? to_f32(x[(row0 + r) * k + kk]) : 0.0f;
+            }
         }
     }
-}
+    __device__ __forceinline__ void put(int k, long long t_len, float* xs) const {
+#pragma unroll
+        for (int i = 0; i < R / 2; ++i) {
+            const int r = t_len > 0 ? threadIdx.x % R : (threadIdx.x >> 5) + 8 * (i / 4);
+            const int kk = t_len > 0 ? threadIdx.x / R + i * (256 / R) : (threadIdx.x & 31) + 32 * (i % 4);
+            if (kk < k) xs[r * (k + 1) + kk] = v[i];
+        }
+    }
+};
 template <int R, class T>
 __device__ __forceinline__ void store_rows(T* x, long long row0, long long rows, int k, long long t_len, const float* xs) {
     if (t_len > 0) {
@@ -1380,7 +1407,7 @@ __device__ __forceinline__ void join_units(const float* part_o, size_t u0, int n
 // block (the largest offset, the sums and mean weight rows brought to it); then 8 lanes per row: the
 // labels' logits as f32 products, the loss, and dx = T g (sum_j p_j W_j - sum_i q_i W_ci).
 template <bool F32, int R>
-__global__ void __launch_bounds__(256) loss_rows_kernel(const __grid_constant__ LossRowParams p) {
+__global__ void __launch_bounds__(256, 3) loss_rows_kernel(const __grid_constant__ LossRowParams p) {
     using T = typename Elem<F32>::type;
     extern __shared__ __align__(16) float sm[];
     float* xs = sm;                                           // [R][k + 1]
@@ -1399,40 +1426,57 @@ __global__ void __launch_bounds__(256) loss_rows_kernel(const __grid_constant__ 
     const int ns = mb < p.whole_units ? 1 : p.n_splits;
     const size_t u0 = mb < p.whole_units ? (size_t)mb : (size_t)p.whole_units + (size_t)(mb - p.whole_units) * p.n_splits;
 
-    load_rows<R>(static_cast<const T*>(p.x), row0, p.rows, p.k, p.t_len, xs);
+    RowLoad<R, T> xv;
+    xv.fetch(static_cast<const T*>(p.x), row0, p.rows, p.k, p.t_len);
     const int jr = tid % R, jg = tid / R;
-    float m = -CUDART_INF_F;
-    for (int s = jg; s < ns; s += kG) {
-        const float o = p.part_ms[(u0 + s) * 128 + l0 + jr].x;
-        wgt[s * R + jr] = o;
-        m = fmaxf(m, o);
-    }
-    red[jg][jr] = m;
-    __syncthreads();
+    if (ns == 1) {
+        // one unit has the whole class range: nothing to join
+        const float2 ms = __ldg(p.part_ms + u0 * 128 + l0 + jr);
+        if (jg == 0) s_lse2[jr] = (ms.x == -CUDART_INF_F ? 0.0f : ms.x) + log2f(ms.y);
+        if (p.dx) {
+            constexpr int kPer = R / 2;
+            const float* po = p.part_o + u0 * p.feat * 128 + l0 + jr;
+            const float inv = 1.0f / ms.y;
+            float a[kPer];
 #pragma unroll
-    for (int i = 0; i < kG; ++i) m = fmaxf(m, red[i][jr]);
-    const float m0 = m == -CUDART_INF_F ? 0.0f : m;
-    float sum = 0.0f;
-    __syncthreads();
-    for (int s = jg; s < ns; s += kG) {
-        const float k = ex2_approx(wgt[s * R + jr] - m0);
-        wgt[s * R + jr] = k;
-        sum = fmaf(p.part_ms[(u0 + s) * 128 + l0 + jr].y, k, sum);
-    }
-    red[jg][jr] = sum;
-    __syncthreads();
-    if (jg == 0) {
-        sum = 0.0f;
+            for (int i = 0; i < kPer; ++i) a[i] = jg + i * kG < p.feat ? __ldg(po + (size_t)(jg + i * kG) * 128) : 0.0f;
 #pragma unroll
-        for (int i = 0; i < kG; ++i) sum += red[i][jr];
-        s_lse2[jr] = m0 + log2f(sum);
-        s_inv[jr] = 1.0f / sum;
-    }
-    __syncthreads();
-    if (p.dx) {
-        join_units<R, true>(p.part_o, u0, ns, p.feat, l0, wgt, s_inv, os);
+            for (int i = 0; i < kPer; ++i)
+                if (jg + i * kG < p.feat) os[jr * (p.feat + 1) + jg + i * kG] = a[i] * inv;
+        }
+    } else {
+        float m = -CUDART_INF_F;
+        for (int s = jg; s < ns; s += kG) {
+            const float o = p.part_ms[(u0 + s) * 128 + l0 + jr].x;
+            wgt[s * R + jr] = o;
+            m = fmaxf(m, o);
+        }
+        red[jg][jr] = m;
         __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kG; ++i) m = fmaxf(m, red[i][jr]);
+        const float m0 = m == -CUDART_INF_F ? 0.0f : m;
+        float sum = 0.0f;
+        __syncthreads();
+        for (int s = jg; s < ns; s += kG) {
+            const float k = ex2_approx(wgt[s * R + jr] - m0);
+            wgt[s * R + jr] = k;
+            sum = fmaf(p.part_ms[(u0 + s) * 128 + l0 + jr].y, k, sum);
+        }
+        red[jg][jr] = sum;
+        __syncthreads();
+        if (jg == 0) {
+            sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kG; ++i) sum += red[i][jr];
+            s_lse2[jr] = m0 + log2f(sum);
+            s_inv[jr] = 1.0f / sum;
+        }
+        __syncthreads();
+        if (p.dx) join_units<R, true>(p.part_o, u0, ns, p.feat, l0, wgt, s_inv, os);
     }
+    xv.put(p.k, p.t_len, xs);
+    __syncthreads();
     if (tid < 8 * R) {  // (R = 8: two warps have rows)
         const bool vec = p.k % kRun == 0 && (reinterpret_cast<uintptr_t>(p.w) & 15u) == 0;
         const int r = tid >> 3, s = tid & 7;
@@ -1449,29 +1493,49 @@ __global__ void __launch_bounds__(256) loss_rows_kernel(const __grid_constant__ 
             p.row_tab[(size_t)(row >> 7) * 256 + (row & 127)] = e;
         }
         float* xr = xs + r * (p.k + 1);
-        float x[16], d[16];
+        float2 x[8], d[8];
         shared_row<kRun>(xr, p.k, s, x);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) d[i] = 0.0f;
+        for (int i = 0; i < 8; ++i) d[i] = make_float2(0.f, 0.f);
         if (p.dx) shared_row<kRun>(os + r * (p.feat + 1), p.k, s, d);
         float zq = 0.0f;  // sum_i q_i (z_i - lse)
-#pragma unroll 2
-        for (int e = 0; e < p.lab.n_top; ++e) {
-            const int2 c = ent[e];
-            const bool here = valid && c.x >= 0;
-            const float q = here ? __int_as_float(c.y) : 0.0f;
-            float w[16];
-            if (here) {
-                weight_row<F32>(p.w, c.x, p.k, s, vec, w);
-            } else {
+        constexpr int kBatch = 2;
+        for (int e0 = 0; e0 < p.lab.n_top; e0 += kBatch) {
+            int c[kBatch];
+            float q[kBatch], b[kBatch], z[kBatch];
+            WeightRow<F32> w[kBatch];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) w[i] = 0.0f;
+            for (int j = 0; j < kBatch; ++j) {
+                const int2 en = valid && e0 + j < p.lab.n_top ? ent[e0 + j] : make_int2(-1, 0);
+                c[j] = en.x;
+                q[j] = __int_as_float(en.y);
+                b[j] = 0.0f;
+                if (c[j] >= 0) {
+                    w[j].fetch(p.w, c[j], p.k, s, vec);
+                    if (p.bias) b[j] = __ldg(p.bias + c[j]);
+                } else {
+                    w[j].clear();
+                }
             }
-            const float z = group_sum(dot16(x, w));
-            if (here) {
-                zq = fmaf(q, fmaf(z + (p.bias ? __ldg(p.bias + c.x) : 0.0f), p.lab.inv_temp, -lse), zq);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) d[i] = fmaf(-q, w[i], d[i]);
+            for (int j = 0; j < kBatch; ++j) {
+                float2 z2 = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) z2 = __ffma2_rn(x[i], w[j].pair(i), z2);
+                z[j] = z2.x + z2.y;
+            }
+#pragma unroll
+            for (int o = 4; o > 0; o >>= 1) {
+#pragma unroll
+                for (int j = 0; j < kBatch; ++j) z[j] += __shfl_xor_sync(0xffffffffu, z[j], o);
+            }
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) {
+                if (c[j] < 0) continue;
+                zq = fmaf(q[j], fmaf(z[j] + b[j], p.lab.inv_temp, -lse), zq);
+                const float2 nq = make_float2(-q[j], -q[j]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) d[i] = __ffma2_rn(nq, w[j].pair(i), d[i]);
             }
         }
         if (live && s == 0) {
@@ -1481,8 +1545,11 @@ __global__ void __launch_bounds__(256) loss_rows_kernel(const __grid_constant__ 
         if (p.dx) {
             __syncwarp();
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (lane_slot<kRun>(s, i) < p.k) xr[lane_slot<kRun>(s, i)] = valid ? f * d[i] : 0.0f;
+            for (int i = 0; i < 8; ++i) {
+                const int k0 = lane_slot<kRun>(s, 2 * i);
+                if (k0 < p.k) xr[k0] = valid ? f * d[i].x : 0.0f;
+                if (k0 + 1 < p.k) xr[k0 + 1] = valid ? f * d[i].y : 0.0f;
+            }
         }
     }
     if (!p.dx) return;
@@ -1530,13 +1597,16 @@ namespace {
 // A lane's 16 K slots of a packed weight's class c, in units of its class-table scale: runs of 8
 // (fp16 images), or 16 in a row (compact).
 template <int FORM>
-__device__ __forceinline__ void packed_row(const uint8_t* tiles, int c, int s, float (&v)[16]) {
+__device__ __forceinline__ void packed_row(const uint8_t* tiles, int c, int s, float2 (&v)[8]) {
     const int tile = c >> 7, r = c & 127;
     if constexpr (FORM == 1) {
         const uint4 u = __ldg(reinterpret_cast<const uint4*>(tiles + (size_t)tile * kTile8Bytes + image8_offset(r, 16 * s)));
         const uint32_t x[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = (float)(int)((x[i / 4] >> (8 * (i % 4))) & 255u) - 128.0f;
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t w = x[i / 2] >> (16 * (i % 2));
+            v[i] = make_float2((float)(int)(w & 255u) - 128.0f, (float)(int)((w >> 8) & 255u) - 128.0f);
+        }
     } else {
         const uint8_t* a = tiles + (size_t)tile * (FORM == 2 ? 2 * kTileBytes : kTileBytes);
 #pragma unroll
@@ -1549,8 +1619,7 @@ __device__ __forceinline__ void packed_row(const uint8_t* tiles, int c, int s, f
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x[i]));
-                    v[8 * j + 2 * i] = part ? v[8 * j + 2 * i] + f.x : f.x;
-                    v[8 * j + 2 * i + 1] = part ? v[8 * j + 2 * i + 1] + f.y : f.y;
+                    v[4 * j + i] = part ? __fadd2_rn(v[4 * j + i], f) : f;
                 }
             }
         }
@@ -1572,7 +1641,8 @@ __global__ void __launch_bounds__(256) loss_score_kernel(const __grid_constant__
     const int r = threadIdx.x >> 3, s = threadIdx.x & 7;
     const long long row = row0 + r;
     const bool live = row < p.rows;
-    load_rows<kLossRows>(p.x, row0, p.rows, p.k, p.t_len, xs);
+    RowLoad<kLossRows, float> xv;
+    xv.fetch(p.x, row0, p.rows, p.k, p.t_len);
     int best = 0;
     float sum = 1.0f;
     if (row >= p.split_row0 && live) {
@@ -1623,6 +1693,7 @@ __global__ void __launch_bounds__(256) loss_score_kernel(const __grid_constant__
         sum = 1.0f / p.prob[row];
     }
     best = min(max(best, 0), p.lab.n - 1);
+    xv.put(p.k, p.t_len, xs);
     __syncthreads();
     int2* ent = ents + r * p.lab.n_top;
     float entropy;
@@ -1633,13 +1704,15 @@ __global__ void __launch_bounds__(256) loss_score_kernel(const __grid_constant__
         for (int e = s; e < p.lab.n_top; e += 8) bad |= cls[e] >= p.lab.n;
         if (bad) atomicOr(p.status, kDevBadClass);
     }
-    float x[16];
+    float2 x[8];
     shared_row<kRun>(xs + r * (p.k + 1), p.k, s, x);
     auto logit = [&](int c) -> float {
-        float w[16];
+        float2 w[8], z = make_float2(0.f, 0.f);
         packed_row<FORM>(p.tiles, c, s, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z = __ffma2_rn(x[i], w[i], z);
         const float* t = p.ctab + (size_t)(c >> 7) * kCtabFloats + (c & 127);
-        return fmaf(group_sum(dot16(x, w)), __ldg(t), __ldg(t + kBlockN)) * p.lab.inv_temp;
+        return fmaf(group_sum(z.x + z.y), __ldg(t), __ldg(t + kBlockN)) * p.lab.inv_temp;
     };
     const float lse = logit(best) + logf(sum);
     float zq = 0.0f;
