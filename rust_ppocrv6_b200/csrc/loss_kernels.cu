@@ -547,8 +547,15 @@ __device__ __forceinline__ void loss_drain(uint32_t bar, uint32_t parity, const 
 struct LUnit {
     int own, c0, c1;
 };
-__device__ __forceinline__ bool lunit_exists(int u, const LossMainParams& p) {
-    return u < p.whole_units + (p.own_tiles - p.whole_units) * p.n_splits;
+// The unit that this CTA takes in wave k, or -1: CTA b takes unit b of every full wave, and unit
+// grid - 1 - b of a last one that is not full. The first units are so those of the CTAs with a unit
+// less: in the weight pass they hold class 0, the blank, whose tile has most rows' labels and takes
+// up to 1.6 times as long as the others (18,710 classes: 4 x 147 units, CTAs 0-3 have three).
+__device__ __forceinline__ int lunit_at(int k, const LossMainParams& p) {
+    const int units = p.whole_units + (p.own_tiles - p.whole_units) * p.n_splits;
+    const int base = k * (int)gridDim.x, b = (int)blockIdx.x;
+    const int u = base + (int)gridDim.x <= units ? base + b : base + (int)gridDim.x - 1 - b;
+    return u < units ? u : -1;
 }
 __device__ __forceinline__ LUnit lunit(int u, const LossMainParams& p) {
     if (u < p.whole_units) return {u, 0, p.str_tiles};
@@ -726,7 +733,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
             // ------------------------------------------------------------ producer
             uint32_t cc = 0, issued = 0, uc = 0, owns = 0;
             bool ok = true;
-            for (int u = blockIdx.x; ok && lunit_exists(u, p); u += gridDim.x, ++uc) {
+            for (int u; ok && (u = lunit_at((int)uc, p)) >= 0; ++uc) {
                 const LUnit U = lunit(u, p);
                 if (!F32) {  // the unit's own image, in the slot that the unit before the last has left
                     const uint32_t w = uc & 1u;
@@ -765,7 +772,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
             const uint64_t k_desc = smem_desc_k_sw128(base);
             uint32_t st = 0, sph = 0, b = 0, fph = 1, uc = 0;  // stage, buffer, their phases (the buffer: freed)
             bool ok = true;
-            for (int u = blockIdx.x; ok && lunit_exists(u, p); u += gridDim.x, ++uc) {
+            for (int u; ok && (u = lunit_at((int)uc, p)) >= 0; ++uc) {
                 const LUnit U = lunit(u, p);
                 const uint32_t w = F32 ? 0u : uc & 1u;
                 ok = issuer_wait(bar(kLBarAFull + w), F32 ? uc & 1u : (uc >> 1) & 1u, wt, 103);
@@ -795,7 +802,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
             const uint64_t mn_desc = smem_desc_mn_sw128(base);
             uint32_t st = 0, b = 0, pph = 0, oph = 1;  // stage, buffer and phase of its probabilities; O's release
             bool ok = true;
-            for (int u = blockIdx.x; ok && lunit_exists(u, p); u += gridDim.x) {
+            for (int k = 0, u; ok && (u = lunit_at(k, p)) >= 0; ++k) {
                 const LUnit U = lunit(u, p);
                 const int every = with_o ? add_every(U.own) : 1;
                 int held = 0;  // products in O so far
@@ -839,7 +846,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
         volatile float* tops = reinterpret_cast<volatile float*>(gbase + kMOffTop);
         uint32_t cc = 0, uc = 0, uses = 0, rc = 0;  // tiles, units, own tiles; tiles whose offsets were handed on
         bool ok = true;
-        for (int u = blockIdx.x; ok && lunit_exists(u, p); u += gridDim.x, ++uc) {
+        for (int u; ok && (u = lunit_at((int)uc, p)) >= 0; ++uc) {
             const LUnit U = lunit(u, p);
             const uint32_t n = (uint32_t)(U.c1 - U.c0);
             // This pair of warpgroups takes every tile whose number in the CTA's whole sequence has its
@@ -1095,7 +1102,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
         const int f0 = 64 * (int)g;
         uint32_t fc = 0, rc = 0, uc = 0;  // products taken, of them with an offset; units
         bool ok = true;
-        for (int u = blockIdx.x; ok && lunit_exists(u, p); u += gridDim.x, ++uc) {
+        for (int u; ok && (u = lunit_at((int)uc, p)) >= 0; ++uc) {
             const LUnit U = lunit(u, p);
             float off = -CUDART_INF_F;
             float2 acc[32];
