@@ -374,7 +374,7 @@ int rh_head_distill_device(rh_ctx *ctx, const rh_weight *w, int slot, const floa
                            float *d_loss, float *d_lse, void *d_workspace, int64_t workspace_bytes, void *stream);
 
 /* A training step: the losses and their gradients for a weight w [n][k] and bias [n] (NULL: none),
- * k <= 128, n <= 262,144. row_grad [rows] is d total / d loss[r] (NULL: 1 each; 1 / count for a
+ * k <= 128, n <= 131,072. row_grad [rows] is d total / d loss[r] (NULL: 1 each; 1 / count for a
  * mean). With f[r] = row_grad[r] (times T for distillation) and the row's distribution q over its
  * labels, dz = f (p - q), and
  *     da = dz w (laid out as a),  dw = dz^T a [n][k],  dbias[j] = sum_r dz[r][j].

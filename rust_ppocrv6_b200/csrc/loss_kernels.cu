@@ -77,7 +77,7 @@ __device__ __forceinline__ bool is_class(int c, int n) { return c >= 0 && c < n;
 // tile's maximum, which an image of fp16 alone or of bf16 parts would not hold); bf16 values are
 // copied. A row that is ignored is zero in the image, so whatever its features hold (NaN
 // included) reaches nothing.
-// The labels of a feature tile are sorted by (class tile, half of the rows), rows ascending: each
+// The labels of a feature tile are sorted by 32 classes (a softmax warp's), rows ascending: each
 // warp takes 8 rows, a group of lanes per row, and notes for every entry how many of its bin came
 // before it in the warp; a scan over warps and bins then gives every entry its place (no atomics:
 // the order is fixed).
@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(kPackThreads, 2) loss_pack_kernel(const __grid
 
     // ---- labels: which rows count, their factors, and (weight gradient) the entries with their
     // place among the warp's own of the same bin
-    const int nb = 2 * p.w_tiles;                                  // (class tile, rows below 64 or above)
+    const int nb = 4 * p.w_tiles;                                  // 32 classes a bin
     uint16_t* counts = reinterpret_cast<uint16_t*>(pack_smem);     // [16 warps][nb]
     int* start = reinterpret_cast<int*>(pack_smem + kPackWarps * 2 * (size_t)nb);  // [nb]
     int2* ents = reinterpret_cast<int2*>(start + nb);              // [128][n_top]: (class << 10 | place, factor)
@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(kPackThreads, 2) loss_pack_kernel(const __grid
             }
             for (int s = 0; s < slots; ++s) {
                 const int e = sub + 32 * s;
-                const int bin = c[s] >= 0 ? 2 * (c[s] >> 7) + (r >> 6) : -1;
+                const int bin = c[s] >= 0 ? c[s] >> 5 : -1;
                 const uint32_t same = __match_any_sync(0xffffffffu, bin);
                 const int rank = __popc(same & ((1u << lane) - 1u));
                 int at = 0;
@@ -393,21 +393,21 @@ __global__ void __launch_bounds__(kPackThreads, 2) loss_pack_kernel(const __grid
     __syncthreads();
     int base = incl - sum;
     for (int w = 0; w < warp; ++w) base += s_scan[w];
-    int32_t* off = p.sp_off + (size_t)tile * (nb + 1);
+    int2* range = p.sp_off + (size_t)tile * nb;
     for (int b = b0; b < b1; ++b) {
-        start[b] += base;
-        off[b] = start[b];
+        const int next = b + 1 < b1 ? start[b + 1] : sum;
+        range[b] = make_int2(base + start[b], base + next);
     }
-    if (tid == kPackThreads - 1) off[nb] = base + sum;
+    for (int b = b0; b < b1; ++b) start[b] += base;
     __syncthreads();
     int2* out = p.sp_ent + (size_t)tile * 128 * p.lab.n_top;
     const int live = (int)min((long long)128, p.rows - row0) * p.lab.n_top;
     for (int i = tid; i < live; i += kPackThreads) {
         const int2 e = ents[i];
         if (e.x < 0) continue;
-        const int r = i / p.lab.n_top, c = e.x >> 10, bin = 2 * (c >> 7) + (r >> 6);
+        const int r = i / p.lab.n_top, c = e.x >> 10, bin = c >> 5;
         out[start[bin] + counts[(size_t)(r >> 3) * nb + bin] + (e.x & 1023)] =
-            make_int2((r << 7) | (c & 127), __float_as_int(__int_as_float(e.y) * gs));
+            make_int2((r << 5) | (c & 31), __float_as_int(__int_as_float(e.y) * gs));
     }
 }
 
@@ -593,36 +593,29 @@ __device__ __forceinline__ void store_probs(uint32_t taddr, const float2 (&g)[8]
     }
 }
 
-// A half tile's labels (weight pass), a window of 32 at a time, rows ascending: each lane holds one
-// entry of the current window and one of the next, which is in flight meanwhile.
+// The labels of a warp's 32 classes in a tile (weight pass), a window of 32 at a time, rows
+// ascending: each lane holds one entry of the current window and, where the list goes on, one of the
+// next, in flight meanwhile.
 struct LabelWindow {
-    int2 e, n;        // (row << 7 | class, factor)
+    int2 e, n;        // (row << 5 | class, factor)
     int next, end;    // first entry after the current window
-    uint32_t groups;  // groups of 8 rows in which this warp's classes have an entry of the window
+    uint32_t groups;  // groups of 8 of this half's rows that have an entry in the window
     int last;         // group of the window's last entry where entries follow it, else beyond any group
-    bool hit;         // this lane's entry is one of this warp's classes'
+    int group;        // group of this lane's entry; outside 0..7: none, or in the other half
 };
 constexpr int kNoLabel = 0x7fffffff;
-__device__ __forceinline__ int2 window_entry(const LabelWindow& w, int at, const int2* ent) {
-    return at < w.end ? __ldg(ent + at) : make_int2(kNoLabel, 0);
+__device__ __forceinline__ int2 window_entry(const LabelWindow& w, const int2* ent, int lane) {
+    return w.next + lane < w.end ? __ldg(ent + w.next + lane) : make_int2(kNoLabel, 0);
 }
-// Both windows' loads; window_use then looks at the first, when it is needed.
-__device__ __forceinline__ void window_open(LabelWindow& w, const int2* ent, int lane) {
-    w.e = window_entry(w, w.next + lane, ent);
+__device__ __forceinline__ void window_use(LabelWindow& w, const int2* ent, int lane, int half) {
     w.next += 32;
-    w.n = window_entry(w, w.next + lane, ent);
-}
-__device__ __forceinline__ void window_use(LabelWindow& w, int quad) {
-    w.hit = w.e.x != kNoLabel && ((w.e.x & 127) >> 5) == quad;
-    const int group = (w.e.x >> 10) & 7;
-    w.groups = __reduce_or_sync(0xffffffffu, w.hit ? 1u << group : 0u);
-    w.last = w.next < w.end ? __shfl_sync(0xffffffffu, group, 31) : 8;
-}
-__device__ __forceinline__ void window_next(LabelWindow& w, const int2* ent, int lane, int quad) {
-    w.e = w.n;
-    w.next += 32;
-    w.n = window_entry(w, w.next + lane, ent);
-    window_use(w, quad);
+    w.group = (w.e.x >> 8) - 8 * half;
+    w.groups = __reduce_or_sync(0xffffffffu, (uint32_t)w.group < 8u ? 1u << w.group : 0u);
+    w.last = 8;
+    if (w.next < w.end) {
+        w.n = window_entry(w, ent, lane);
+        w.last = __shfl_sync(0xffffffffu, w.group, 31);
+    }
 }
 
 }  // namespace
@@ -855,15 +848,13 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
             const uint32_t i0 = (g ^ cc) & 1u;
             // labels of the first of them (weight pass): range, then entries
             LabelWindow lw{};
-            auto label_range = [&](int c, int& a, int& b) {
-                const int32_t* o = p.sp_off + (size_t)c * (2 * p.own_tiles + 1) + 2 * U.own + half;
-                a = __ldg(o);
-                b = __ldg(o + 1);
-            };
-            auto label_base = [&](int c) { return p.sp_ent + (size_t)c * 128 * p.n_top; };
+            const int2* ranges = p.sp_off + (size_t)(U.c0 + (int)i0) * 4 * p.own_tiles + 4 * U.own + quad;
+            const int2* ent = p.sp_ent + (size_t)(U.c0 + (int)i0) * 128 * p.n_top;
             if (WPASS && i0 < n) {
-                label_range(U.c0 + (int)i0, lw.next, lw.end);
-                window_open(lw, label_base(U.c0 + (int)i0), lane);
+                const int2 first = __ldg(ranges);
+                lw.next = first.x;
+                lw.end = first.y;
+                lw.e = window_entry(lw, ent, lane);
             }
             if (F32) {
                 // own operand -> TMEM: warpgroup wg takes K slots 64 half .. 64 half + 63 of the lane's
@@ -908,8 +899,11 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                 const float str_s = F32 ? __ldg(p.str_scale + c) : 1.0f;
                 const float gs = WPASS ? __ldg(p.g_scale + c) : 1.0f;
                 // the next tile's label range is fetched under this tile, its entries at this tile's end
-                int next_a = 0, next_b = 0;
-                if (WPASS && i + 2 < n) label_range(c + 2, next_a, next_b);
+                int2 next_range = make_int2(0, 0);
+                if (WPASS) {
+                    ranges += 8 * p.own_tiles;
+                    if (i + 2 < n) next_range = __ldg(ranges);
+                }
                 const float2 mul = make_float2(own_mul * str_s, own_mul * str_s);
                 const uint32_t buf = (cc + i) % Ring<F32>::kBufs;
                 const uint32_t t_s = t_bufs + 128u * buf;
@@ -1000,9 +994,11 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                     sum = fmaf(sum, corr, t);
                 } else {
                     const float2 le = make_float2(lane_e, lane_e);
-                    const int2* ent = label_base(c);
-                    window_use(lw, quad);
-                    const bool labelled = lw.groups != 0u || lw.last < 8;  // most tiles have none of a warp's classes
+                    bool labelled = false;  // most tiles have none of a warp's classes
+                    if (lw.next < lw.end) {
+                        window_use(lw, ent, lane, (int)half);
+                        labelled = lw.groups != 0u || lw.last < 8;
+                    }
                     float2 ts = make_float2(0.f, 0.f);
 #pragma unroll (F32 ? 1 : 4)
                     for (int q = 0; q < 4; ++q) {
@@ -1038,14 +1034,15 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                             while (true) {
                                 if ((lw.groups >> group) & 1u) {
                                     any = true;
-                                    if (lw.hit && (int)((lw.e.x >> 10) & 7) == group)
+                                    if (lw.group == group)
                                         *reinterpret_cast<volatile float*>(
                                             gbase + (patch - base) +
-                                            4u * ((uint32_t)(lw.e.x & 31) * kPatchRow + (uint32_t)((lw.e.x >> 7) & 7))) =
+                                            4u * ((uint32_t)(lw.e.x & 31) * kPatchRow + (uint32_t)((lw.e.x >> 5) & 7))) =
                                             __int_as_float(lw.e.y);
                                 }
                                 if (group < lw.last) break;  // the window reaches beyond this group, or is the last
-                                window_next(lw, ent, lane, quad);
+                                lw.e = lw.n;
+                                window_use(lw, ent, lane, (int)half);
                             }
                             if (any) {
                                 __syncwarp();
@@ -1069,9 +1066,10 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                     const float nsum = sum + t;
                     carry = t - (nsum - sum);
                     sum = nsum;
-                    lw.next = next_a;
-                    lw.end = next_b;
-                    window_open(lw, label_base(i + 2 < n ? c + 2 : c), lane);
+                    lw.next = next_range.x;
+                    lw.end = next_range.y;
+                    ent += 256 * p.n_top;
+                    lw.e = window_entry(lw, ent, lane);
                 }
                 tmem_st_wait();
                 tc_fence_before();
@@ -1740,7 +1738,7 @@ __global__ void __launch_bounds__(256) loss_score_kernel(const __grid_constant__
 namespace {
 // (counts, starts, entries; the norms' four partial sums)
 constexpr int pack_smem_bytes(int w_tiles, int n_top) {
-    return 2 * w_tiles * (2 * kPackWarps + 4) + 128 * n_top * 8;
+    return 4 * w_tiles * (2 * kPackWarps + 4) + 128 * n_top * 8;
 }
 constexpr int kPackSmemMax = pack_smem_bytes(kLossMaxClasses / 128, kLossMaxTop) + 2048;
 static_assert(kPackSmemMax <= 226 * 1024, "shared memory per block");

@@ -9,7 +9,7 @@ namespace rh {
 constexpr int kLossTile = 128;            // rows (classes) per operand tile
 constexpr int kLossImage = 128 * 128 * 2;  // one 16-bit tile image: 128 rows x 128 K slots
 constexpr int kLossMaxTop = 64;           // teacher entries per row
-constexpr int kLossMaxClasses = 1 << 18;  // class tiles are counted in shared memory (2 x 2,048 bins)
+constexpr int kLossMaxClasses = 1 << 17;  // labels are counted by 32 classes in shared memory (4,096 bins)
 constexpr int kLossRows = 32;             // rows per block of the score kernel
 constexpr int kLossMaxSplits = 148;       // ranges that an own tile's work is split into at most
 // Device status bit (status[0], beside kDevTimeout and kDevRecPlan): a target or teacher class
@@ -55,8 +55,8 @@ struct LossPackParams {
     float* x_norm;             // slots: [x_tiles][128] |x_r|
     float2* w_bound;           // slots: [w_tiles] (largest |w_j|, largest bias in log2 units)
     int norm_smem;             // set by the launcher: first float of the norms' shared memory
-    int32_t* sp_off;           // [x_tiles][2 w_tiles + 1] label ranges by class tile and half of the rows
-    int2* sp_ent;              // [x_tiles][128 n_top]: (row << 7 | class within its tile, factor bits)
+    int2* sp_off;              // [x_tiles][4 w_tiles] label ranges (first, end) by 32 classes
+    int2* sp_ent;              // [x_tiles][128 n_top]: (row << 5 | class within its 32, factor bits)
     int* status;
 };
 
@@ -71,7 +71,7 @@ struct LossMainParams {
     const float* x_norm;       // row pass, slots
     const float2* w_bound;
     const float* g_scale;      // weight pass: per streamed tile
-    const int32_t* sp_off;     // weight pass
+    const int2* sp_off;        // weight pass
     const int2* sp_ent;
     int n_top;
     int own_tiles, str_tiles;

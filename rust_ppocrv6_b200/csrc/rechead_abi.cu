@@ -889,7 +889,7 @@ LossLayout loss_layout(bool f32, int64_t rows, int64_t k, int64_t n, int64_t n_t
     L.row_tab = take((size_t)L.x_tiles * 1024);
     L.x_norm = take(L.slots ? (size_t)L.x_tiles * 512 : 0);
     L.w_bound = take(L.slots ? (size_t)L.w_tiles * 8 : 0);
-    L.sp_off = take((size_t)L.x_tiles * (size_t)(2 * L.w_tiles + 1) * 4);
+    L.sp_off = take((size_t)L.x_tiles * (size_t)L.w_tiles * 4 * sizeof(int2));
     L.sp_ent = take((size_t)L.x_tiles * 128 * (size_t)n_top * 8);
     L.part_o = take(units * (size_t)L.feat * 512);
     L.part_ms = take(units * 1024);
@@ -944,7 +944,7 @@ int check_grad_shape(int dtype, int64_t rows, int64_t k, int64_t n) {
     if (n < 1 || k < 1) return fail(RH_ERR_INVALID_ARG, "weight must be [n>=1][k>=1]");
     if (k > rh::kPadK)
         return fail(RH_ERR_UNSUPPORTED, "K = " + std::to_string(k) + " exceeds the supported maximum of 128");
-    if (n > rh::kLossMaxClasses) return fail(RH_ERR_UNSUPPORTED, "more than 262,144 classes");
+    if (n > rh::kLossMaxClasses) return fail(RH_ERR_UNSUPPORTED, "more than 131,072 classes");
     return RH_OK;
 }
 
@@ -978,7 +978,7 @@ int enqueue_grad(rh_ctx* ctx, Slot& s, int dtype, const void* d_a, int64_t rows,
     pk.slots = L.slots ? 1 : 0;
     pk.x_norm = (float*)(ws + L.x_norm);
     pk.w_bound = (float2*)(ws + L.w_bound);
-    pk.sp_off = (int32_t*)(ws + L.sp_off);
+    pk.sp_off = (int2*)(ws + L.sp_off);
     pk.sp_ent = (int2*)(ws + L.sp_ent);
     pk.status = s.d_status;
     RH_CUDA(rh::launch_loss_pack(pk, f32, st));

@@ -545,7 +545,7 @@ def test_refusals_launch_nothing(rh, ctx):
     both = [(dict(rows=-1), "inv"), (dict(rows=(1 << 30) + 1), "uns"), (dict(t_len=-1), "inv"), (dict(t_len=5), "inv"),
             (dict(slot=1), "inv"), (dict(slot=-1), "inv"), (dict(a_ptr=0), "inv"), (dict(workspace_ptr=0), "inv"),
             (dict(workspace_bytes=100), "inv")]
-    grads = [(dict(k=129), "uns"), (dict(k=0), "inv"), (dict(n=0), "inv"), (dict(n=(1 << 18) + 1), "uns"),
+    grads = [(dict(k=129), "uns"), (dict(k=0), "inv"), (dict(n=0), "inv"), (dict(n=(1 << 17) + 1), "uns"),
              (dict(w_ptr=0), "inv"), (dict(dw_ptr=0), "inv"), (dict(dtype="f16"), "inv")]
     tops = [(dict(n_top=0), "inv"), (dict(n_top=65), "inv"), (dict(temperature=0.0), "inv"),
             (dict(temperature=-1.0), "inv"), (dict(temperature=float("nan")), "inv"),
