@@ -331,15 +331,17 @@ int rh_rec_preprocess_device(rh_ctx *ctx, int slot, const uint8_t *d_rgb, int64_
  * hold anything, NaN included).
  *
  * Distillation: row r holds the teacher's entries (top_idx[r][i], top_logits[r][i]), i < n_top
- * <= 64, in any order; an entry with a negative class is absent, a class named twice counts
- * twice. With T = temperature, q = softmax(top_logits / T) over the row's entries and
+ * <= 64, in any order; an entry with a negative class or a logit of -inf is absent, a class named
+ * twice counts twice. With T = temperature, q = softmax(top_logits / T) over the row's entries and
  * p = softmax(z / T) over every class,
  *     loss[r] = T^2 sum_i q_i (log q_i - log p[top_idx[r][i]]),  lse[r] = log sum_j exp(z[r][j] / T).
  * A row with no entry is ignored, as above.
  *
  * Features are [rows][k] (t_len = 0) or the SVTR tail's [rows / t_len][k][t_len] (t_len > 0), as
  * in rh_head_decode and rh_head_decode_kt; rows are in (line, timestep) order. A bias of -inf
- * masks its class; a row with every class masked has lse -inf and loss NaN.
+ * masks its class; a row with every class masked has lse -inf and loss NaN. NaN and infinity in a
+ * row that counts are the row's result, and through it the weight's gradient's. Pointers are aligned
+ * to their element.
  *
  * A class at or above n: host calls refuse it (RH_ERR_INVALID_ARG). On the device the row
  * (cross entropy) or the entry (distillation) is taken as absent and the next rh_sync reports

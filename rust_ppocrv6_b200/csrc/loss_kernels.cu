@@ -170,8 +170,8 @@ __global__ void __launch_bounds__(kPackThreads, 2) loss_pack_kernel(const __grid
                         const int x = p.lab.target ? p.lab.target[row] : p.lab.top_idx[row * p.lab.n_top + e];
                         bad |= x >= p.lab.n;
                         if (is_class(x, p.lab.n)) {
-                            c[s] = x;
                             u[s] = p.lab.target ? 0.0f : p.lab.top_logits[row * p.lab.n_top + e] * p.lab.inv_temp;
+                            if (u[s] != -CUDART_INF_F) c[s] = x;  // (of no share: as absent)
                         }
                     }
                 }
@@ -837,7 +837,8 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
         const uint32_t t_bufs = tmem + lanes + Ring<F32>::kTS + 64u * half;
         float* ring = reinterpret_cast<float*>(gbase + kMOffRing);
         volatile float* tops = reinterpret_cast<volatile float*>(gbase + kMOffTop);
-        uint32_t cc = 0, uc = 0, uses = 0, rc = 0;  // tiles, units, own tiles; tiles whose offsets were handed on
+        // tiles, units, tiles whose offsets were handed on, tiles whose maximum was exchanged
+        uint32_t cc = 0, uc = 0, rc = 0, tc = 0;
         bool ok = true;
         for (int u; ok && (u = lunit_at((int)uc, p)) >= 0; ++uc) {
             const LUnit U = lunit(u, p);
@@ -892,7 +893,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                 bounded = __all_sync(0xffffffffu, in_bounds(reach));
             }
             float off = -CUDART_INF_F, sum = 0.0f, carry = 0.0f;  // weight pass: sum + carry = bias gradient
-            for (uint32_t i = i0; i < n; i += 2, ++uses) {
+            for (uint32_t i = i0; i < n; i += 2) {
                 const int c = U.c0 + (int)i;
                 const uint32_t s = (cc + i) % kStages;
                 const uint32_t tab = base + Ring<F32>::kTab + s * 1024u + 256u * half;
@@ -953,11 +954,11 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                         }
                     }
                     // the row's maximum over both halves of the tile
-                    volatile float* t2 = tops + (uses & 1u) * 512;  // the partner may still read the last tile's
+                    volatile float* t2 = tops + (tc & 1u) * 512;  // the partner may still read the last tile's
                     t2[wg * 128 + r] = top;
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar(kLBarTop + 4 * (int)g + quad));
-                    ok = loss_wait(bar(kLBarTop + 4 * (int)g + quad), uses & 1u, wt, 113);
+                    ok = loss_wait(bar(kLBarTop + 4 * (int)g + quad), tc++ & 1u, wt, 113);
                     if (!ok) break;
                     top = fmaxf(top, t2[(wg ^ 1u) * 128 + r]);
                     const float m = fmaxf(off, top);
@@ -1356,6 +1357,7 @@ __device__ __forceinline__ bool group_labels(const LossLabels& L, long long row,
         int c = live ? L.top_idx[at + e] : -1;
         c = is_class(c, L.n) ? c : -1;
         const float u = c >= 0 ? L.top_logits[at + e] * L.inv_temp : -CUDART_INF_F;
+        if (u == -CUDART_INF_F) c = -1;  // of no share: as absent
         ent[e] = make_int2(c, __float_as_int(u));
         any |= c >= 0;
         top = fmaxf(top, u);
@@ -1371,7 +1373,7 @@ __device__ __forceinline__ bool group_labels(const LossLabels& L, long long row,
     for (int e = s; e < L.n_top; e += 8) {
         if (ent[e].x < 0) continue;
         const float u = __int_as_float(ent[e].y) - top, q = expf(u) / sum;
-        // an entry of no share (teacher logit -inf) holds the row to nothing
+        // (a share that rounds to zero holds the row to nothing)
         if (q != 0.0f) h = fmaf(q, u - log_sum, h);
         ent[e] = make_int2(q != 0.0f ? ent[e].x : -1, __float_as_int(q));
     }

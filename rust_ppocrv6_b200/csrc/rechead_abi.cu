@@ -1985,12 +1985,16 @@ int rh_rec_preprocess_device(rh_ctx* ctx, int slot, const uint8_t* d_rgb, int64_
 // ------------------------------------------------------------------- training losses
 
 int64_t rh_head_score_workspace_bytes(rh_ctx* ctx, const rh_weight* w, int slot, int64_t rows) {
-    if (check_ctx(ctx)) return -1;
-    if (!w || slot < 0 || slot >= (int)ctx->slots.size() || check_rows(rows, 0)) {
-        fail(RH_ERR_INVALID_ARG, "null weight, slot out of range or bad row count");
-        return -1;
-    }
-    return (int64_t)score_layout(w, rows, ctx->slots[slot]->sms).total;
+    int64_t bytes = -1;
+    guarded([&]() -> int {
+        if (int rc = check_ctx(ctx)) return rc;
+        if (!w) return fail(RH_ERR_INVALID_ARG, "null weight");
+        if (slot < 0 || slot >= (int)ctx->slots.size()) return fail(RH_ERR_INVALID_ARG, "slot out of range");
+        if (int rc = check_rows(rows, 0)) return rc;
+        bytes = (int64_t)score_layout(w, rows, ctx->slots[slot]->sms).total;
+        return RH_OK;
+    });
+    return bytes;
 }
 
 int rh_head_cross_entropy(rh_ctx* ctx, const rh_weight* w, const float* a, int64_t rows, int64_t k, int64_t t_len,
@@ -2030,17 +2034,18 @@ int rh_head_distill_device(rh_ctx* ctx, const rh_weight* w, int slot, const floa
 
 int64_t rh_head_grad_workspace_bytes(rh_ctx* ctx, int slot, int dtype, int64_t rows, int64_t k, int64_t n,
                                      int64_t n_top) {
-    if (check_ctx(ctx)) return -1;
-    if (slot < 0 || slot >= (int)ctx->slots.size()) {
-        fail(RH_ERR_INVALID_ARG, "slot out of range");
-        return -1;
-    }
-    if (check_grad_shape(dtype, rows, k, n)) return -1;
-    if (n_top < 0 || n_top > rh::kLossMaxTop) {
-        fail(RH_ERR_INVALID_ARG, "n_top = " + std::to_string(n_top) + " is outside [0, 64]");
-        return -1;
-    }
-    return (int64_t)loss_layout(dtype == RH_DTYPE_F32, rows, k, n, std::max<int64_t>(n_top, 1), ctx->slots[slot]->sms).total;
+    int64_t bytes = -1;
+    guarded([&]() -> int {
+        if (int rc = check_ctx(ctx)) return rc;
+        if (slot < 0 || slot >= (int)ctx->slots.size()) return fail(RH_ERR_INVALID_ARG, "slot out of range");
+        if (int rc = check_grad_shape(dtype, rows, k, n)) return rc;
+        if (n_top < 0 || n_top > rh::kLossMaxTop)
+            return fail(RH_ERR_INVALID_ARG, "n_top = " + std::to_string(n_top) + " is outside [0, 64]");
+        bytes = (int64_t)loss_layout(dtype == RH_DTYPE_F32, rows, k, n, std::max<int64_t>(n_top, 1), ctx->slots[slot]->sms)
+                    .total;
+        return RH_OK;
+    });
+    return bytes;
 }
 
 int rh_head_cross_entropy_grad(rh_ctx* ctx, const float* a, int64_t rows, int64_t k, int64_t t_len, const float* w,

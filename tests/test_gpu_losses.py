@@ -295,6 +295,34 @@ def test_scales_of_operands_and_row_weights(rh, ctx, exp):
     check(grad(rh, ctx, d), definition(d), False)
 
 
+def test_bf16_offsets_by_bound_and_by_maximum(rh, ctx):
+    """Blocks of rows whose logits cannot reach far around the largest bias (their offset is a bound)
+    between blocks that reach hundreds (their offset follows the maximum), several units per SM."""
+    d = make(20_100, 40, 700, seed=25, scale=3.0)
+    far = (np.arange(20_100) // 128) % 3 == 1
+    d["x"] = (d["x"] * np.where(far, 6.0, 0.05)[:, None]).astype(np.float32)
+    x, w = np.linalg.norm(d["x"], axis=1), np.linalg.norm(d["w"], axis=1).max()
+    assert (x[~far] * w).max() < 25 and (x[far] * w).max() > 80
+    check(grad(rh, ctx, d, "bf16"), definition(rounded(d, "bf16")), True)
+
+
+def test_teacher_logits_of_minus_infinity_are_absent(rh, ctx):
+    d = make(150, 40, 260, seed=26, n_top=5, ignored=0.0)
+    out = np.random.default_rng(27).random((150, 5)) < 0.3
+    out[10:20] = True  # whole rows: ignored
+    a = dict(d, logits=np.where(out, -np.inf, d["logits"]).astype(np.float32))
+    b = dict(d, idx=np.where(out, -1, d["idx"]).astype(np.int32))
+    qw, _ = packed(rh, ctx, d, "int8")
+    for one, two in zip(rh.head_distill(d["x"], qw, a["idx"], a["logits"], 2.0),
+                        rh.head_distill(d["x"], qw, b["idx"], b["logits"], 2.0)):
+        assert np.array_equal(one, two) and not one[10:20].any()
+    one, two = grad(rh, ctx, a, temp=2.0), grad(rh, ctx, b, temp=2.0)
+    for i in one:
+        assert torch.equal(one[i], two[i]), i
+    assert not one["da"][10:20].any()
+    check(one, definition(b, 2.0), False)
+
+
 @pytest.mark.parametrize("want", [("loss",), ("lse",), ("loss", "lse", "da"), ("loss", "dw"), ("dw", "db"), ("da",)])
 def test_only_what_is_asked_for(rh, ctx, want):
     d = make(200, 120, 700, seed=17)
@@ -476,6 +504,19 @@ def test_score_in_the_tail_layout_on_a_stream_and_in_a_graph(rh, ctx):
     torch.cuda.synchronize()
     ctx.sync()
     assert np.array_equal(o[0].cpu().numpy(), loss.reshape(-1)) and np.array_equal(o[1].cpu().numpy(), lse.reshape(-1))
+    qw.free()
+
+
+def test_score_of_ignored_rows_is_zero_whatever_they_hold(rh, ctx):
+    d = make(300, 120, 2000, seed=33)
+    gone = d["t"] < 0
+    qw, w = packed(rh, ctx, d, "int8")
+    clean = rh.head_cross_entropy(d["x"], qw, d["t"])
+    x = d["x"].copy()
+    x[gone] = np.nan
+    dirty = rh.head_cross_entropy(x, qw, d["t"])
+    for a, b in zip(clean, dirty):
+        assert np.array_equal(a, b) and not b[gone].any()
     qw.free()
 
 
