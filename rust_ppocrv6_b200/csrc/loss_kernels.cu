@@ -865,16 +865,13 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                 tc_fence_after();
                 if ((int)(4 * half) < p.ksteps) {
                     const uint8_t* img = p.own + (size_t)U.own * kStage + g * kLossImage;
+                    uint32_t w[32];
 #pragma unroll
-                    for (int hj = 0; hj < 2; ++hj) {
-                        uint32_t w[16];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const uint4 x = *reinterpret_cast<const uint4*>(img + image_chunk(r, 8 * half + 4 * hj + j));
-                            w[4 * j] = x.x, w[4 * j + 1] = x.y, w[4 * j + 2] = x.z, w[4 * j + 3] = x.w;
-                        }
-                        tmem_st32x32b_x16(tmem + lanes + kTOwn + 64u * g + 32u * half + 16u * hj, w);
+                    for (int j = 0; j < 8; ++j) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(img + image_chunk(r, 8 * half + j));
+                        w[4 * j] = x.x, w[4 * j + 1] = x.y, w[4 * j + 2] = x.z, w[4 * j + 3] = x.w;
                     }
+                    tmem_st32x32b_x32(tmem + lanes + kTOwn + 64u * g + 32u * half, w);
                     tmem_st_wait();
                 }
                 tc_fence_before();
@@ -1290,48 +1287,49 @@ __device__ __forceinline__ float group_max(float v) {
 
 // R rows of the features into shared memory (row stride k + 1), and back: coalesced along the
 // layout's contiguous direction, every load of a thread in flight at once (k <= 128).
-template <int R, class T>
+template <int R, int NT, class T>
 struct RowLoad {
-    float v[R / 2];
+    static constexpr int kPer = R * 128 / NT, kWarps = NT / 32;  // loads a thread; warps
+    float v[kPer];
     __device__ __forceinline__ void fetch(const T* x, long long row0, long long rows, int k, long long t_len) {
         if (t_len > 0) {
             const int r = threadIdx.x % R;
             const bool live = row0 + r < rows;
             const T* at = x + (live ? x_base(row0 + r, k, t_len) : 0);
 #pragma unroll
-            for (int i = 0; i < R / 2; ++i) {
-                const int kk = threadIdx.x / R + i * (256 / R);
+            for (int i = 0; i < kPer; ++i) {
+                const int kk = threadIdx.x / R + i * (NT / R);
                 v[i] = live && kk < k ? to_f32(at[kk * t_len]) : 0.0f;
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < R / 2; ++i) {
-                const int r = (threadIdx.x >> 5) + 8 * (i / 4), kk = (threadIdx.x & 31) + 32 * (i % 4);
+            for (int i = 0; i < kPer; ++i) {  // a warp's rows, a quarter each; or (R = 8) half a row a warp
+                const int q = (threadIdx.x >> 5) * kPer + i, r = q / 4, kk = (threadIdx.x & 31) + 32 * (q % 4);
                 v[i] = row0 + r < rows && kk < k ? to_f32(x[(row0 + r) * k + kk]) : 0.0f;
             }
         }
     }
     __device__ __forceinline__ void put(int k, long long t_len, float* xs) const {
 #pragma unroll
-        for (int i = 0; i < R / 2; ++i) {
-            const int r = t_len > 0 ? threadIdx.x % R : (threadIdx.x >> 5) + 8 * (i / 4);
-            const int kk = t_len > 0 ? threadIdx.x / R + i * (256 / R) : (threadIdx.x & 31) + 32 * (i % 4);
+        for (int i = 0; i < kPer; ++i) {
+            const int q = (threadIdx.x >> 5) * kPer + i;
+            const int r = t_len > 0 ? threadIdx.x % R : q / 4;
+            const int kk = t_len > 0 ? threadIdx.x / R + i * (NT / R) : (threadIdx.x & 31) + 32 * (q % 4);
             if (kk < k) xs[r * (k + 1) + kk] = v[i];
         }
     }
 };
-template <int R, class T>
+template <int R, int NT, class T>
 __device__ __forceinline__ void store_rows(T* x, long long row0, long long rows, int k, long long t_len, const float* xs) {
     if (t_len > 0) {
         const int r = threadIdx.x % R;
         if (row0 + r >= rows) return;
         T* at = x + x_base(row0 + r, k, t_len);
 #pragma unroll 4
-        for (int kk = threadIdx.x / R; kk < k; kk += 256 / R) at[kk * t_len] = (T)xs[r * (k + 1) + kk];
+        for (int kk = threadIdx.x / R; kk < k; kk += NT / R) at[kk * t_len] = (T)xs[r * (k + 1) + kk];
     } else {
 #pragma unroll
-        for (int i = 0; i < R / 8; ++i) {
-            const int r = (threadIdx.x >> 5) + 8 * i;
+        for (int r = threadIdx.x >> 5; r < R; r += NT / 32) {
             if (row0 + r >= rows) return;
 #pragma unroll 4
             for (int kk = threadIdx.x & 31; kk < k; kk += 32) x[(row0 + r) * k + kk] = (T)xs[r * (k + 1) + kk];
@@ -1384,12 +1382,12 @@ __device__ __forceinline__ bool group_labels(const LossLabels& L, long long row,
 
 // Rows l0 .. l0 + R - 1 of the units u0 .. u0 + ns - 1's partial tiles [feat][128], weighted and
 // added in the units' order, into os [R][feat + 1] times inv[row]. A thread owns one row and every
-// (256 / R)-th feature, and keeps all of its features' loads of a unit in flight: with few rows the
+// (NT / R)-th feature, and keeps all of its features' loads of a unit in flight: with few rows the
 // work is split over many units, and their latency is what this join costs.
-template <int R, bool WEIGHTED>
+template <int R, int NT, bool WEIGHTED>
 __device__ __forceinline__ void join_units(const float* part_o, size_t u0, int ns, int feat, int l0, const float* wgt,
                                            const float* inv, float* os) {
-    constexpr int kStep = 256 / R, kPer = 128 / kStep;
+    constexpr int kStep = NT / R, kPer = 128 / kStep;
     const int r = threadIdx.x % R, f0 = threadIdx.x / R;
     float a[kPer];
 #pragma unroll
@@ -1410,18 +1408,19 @@ __device__ __forceinline__ void join_units(const float* part_o, size_t u0, int n
 
 }  // namespace
 
-// One block per R rows (32; 8 where that leaves most SMs idle). Joins the class ranges of a row
+// One block per R rows (32; 8 where that leaves most SMs idle, and then of 512 threads where there
+// are fewer blocks than SMs: each joins many units, 13.9 -> 11.6 us for 120 rows of 49 units). Joins the class ranges of a row
 // block (the largest offset, the sums and mean weight rows brought to it); then 8 lanes per row: the
 // labels' logits as f32 products, the loss, and dx = T g (sum_j p_j W_j - sum_i q_i W_ci).
-template <bool F32, int R>
-__global__ void __launch_bounds__(256, 3) loss_rows_kernel(const __grid_constant__ LossRowParams p) {
+template <bool F32, int R, int NT>
+__global__ void __launch_bounds__(NT, NT == 256 ? 3 : 1) loss_rows_kernel(const __grid_constant__ LossRowParams p) {
     using T = typename Elem<F32>::type;
     extern __shared__ __align__(16) float sm[];
     float* xs = sm;                                           // [R][k + 1]
     float* os = xs + R * (p.k + 1);                           // [R][feat + 1]
     float* wgt = os + R * (p.feat + 1);                       // [n_splits][R]
     int2* ents = reinterpret_cast<int2*>(wgt + R * p.n_splits);  // [R][n_top] (R is even: 8-byte aligned)
-    constexpr int kG = 256 / R;                // threads that share a row's ranges
+    constexpr int kG = NT / R;                 // threads that share a row's ranges
     constexpr int kRun = F32 ? 4 : 8;
     __shared__ float red[kG][R];
     __shared__ float s_lse2[R], s_inv[R];
@@ -1433,7 +1432,7 @@ __global__ void __launch_bounds__(256, 3) loss_rows_kernel(const __grid_constant
     const int ns = mb < p.whole_units ? 1 : p.n_splits;
     const size_t u0 = mb < p.whole_units ? (size_t)mb : (size_t)p.whole_units + (size_t)(mb - p.whole_units) * p.n_splits;
 
-    RowLoad<R, T> xv;
+    RowLoad<R, NT, T> xv;
     xv.fetch(static_cast<const T*>(p.x), row0, p.rows, p.k, p.t_len);
     const int jr = tid % R, jg = tid / R;
     if (ns == 1) {
@@ -1441,7 +1440,7 @@ __global__ void __launch_bounds__(256, 3) loss_rows_kernel(const __grid_constant
         const float2 ms = __ldg(p.part_ms + u0 * 128 + l0 + jr);
         if (jg == 0) s_lse2[jr] = (ms.x == -CUDART_INF_F ? 0.0f : ms.x) + log2f(ms.y);
         if (p.dx) {
-            constexpr int kPer = R / 2;
+            constexpr int kPer = 128 / kG;
             const float* po = p.part_o + u0 * p.feat * 128 + l0 + jr;
             const float inv = 1.0f / ms.y;
             float a[kPer];
@@ -1480,7 +1479,7 @@ __global__ void __launch_bounds__(256, 3) loss_rows_kernel(const __grid_constant
             s_inv[jr] = 1.0f / sum;
         }
         __syncthreads();
-        if (p.dx) join_units<R, true>(p.part_o, u0, ns, p.feat, l0, wgt, s_inv, os);
+        if (p.dx) join_units<R, NT, true>(p.part_o, u0, ns, p.feat, l0, wgt, s_inv, os);
     }
     xv.put(p.k, p.t_len, xs);
     __syncthreads();
@@ -1561,7 +1560,7 @@ __global__ void __launch_bounds__(256, 3) loss_rows_kernel(const __grid_constant
     }
     if (!p.dx) return;
     __syncthreads();
-    store_rows<R>(static_cast<T*>(p.dx), row0, p.rows, p.k, p.t_len, xs);
+    store_rows<R, NT>(static_cast<T*>(p.dx), row0, p.rows, p.k, p.t_len, xs);
 }
 
 // One block per R classes (32, or 8 as above): the row ranges' partial sums added in their order,
@@ -1574,7 +1573,7 @@ __global__ void __launch_bounds__(256) loss_reduce_kernel(const __grid_constant_
     const int j0 = (int)blockIdx.x * R, tile = j0 >> 7, l0 = j0 & 127;
     const int ns = tile < p.whole_units ? 1 : p.n_splits;
     const size_t u0 = tile < p.whole_units ? (size_t)tile : (size_t)p.whole_units + (size_t)(tile - p.whole_units) * p.n_splits;
-    join_units<R, false>(p.part_o, u0, ns, p.feat, l0, nullptr, nullptr, sm);
+    join_units<R, 256, false>(p.part_o, u0, ns, p.feat, l0, nullptr, nullptr, sm);
     if (p.db && threadIdx.x < R && j0 + (int)threadIdx.x < p.n) {
         float a = 0.0f;
         for (int s = 0; s < ns; ++s) a += p.part_ms[(u0 + s) * 128 + l0 + threadIdx.x].x;
@@ -1583,8 +1582,7 @@ __global__ void __launch_bounds__(256) loss_reduce_kernel(const __grid_constant_
     __syncthreads();
     T* dw = static_cast<T*>(p.dw);
 #pragma unroll
-    for (int i = 0; i < R / 8; ++i) {
-        const int r = (threadIdx.x >> 5) + 8 * i;
+    for (int r = threadIdx.x >> 5; r < R; r += 8) {
         if (j0 + r < p.n) {
             for (int kk = threadIdx.x & 31; kk < p.k; kk += 32) dw[(long long)(j0 + r) * p.k + kk] = (T)sm[r * (p.feat + 1) + kk];
         }
@@ -1648,7 +1646,7 @@ __global__ void __launch_bounds__(256) loss_score_kernel(const __grid_constant__
     const int r = threadIdx.x >> 3, s = threadIdx.x & 7;
     const long long row = row0 + r;
     const bool live = row < p.rows;
-    RowLoad<kLossRows, float> xv;
+    RowLoad<kLossRows, 256, float> xv;
     xv.fetch(p.x, row0, p.rows, p.k, p.t_len);
     int best = 0;
     float sum = 1.0f;
@@ -1767,8 +1765,8 @@ cudaError_t loss_kernel_setup() {
     if ((e = smem_attr(loss_main_kernel<false, true, true>, kMSmemBytes)) != cudaSuccess) return e;
     if ((e = smem_attr(loss_pack_kernel<true>, kPackSmemMax)) != cudaSuccess) return e;
     if ((e = smem_attr(loss_pack_kernel<false>, kPackSmemMax)) != cudaSuccess) return e;
-    if ((e = smem_attr(loss_rows_kernel<true, 32>, kRowsSmemMax)) != cudaSuccess) return e;
-    return smem_attr(loss_rows_kernel<false, 32>, kRowsSmemMax);
+    if ((e = smem_attr(loss_rows_kernel<true, 32, 256>, kRowsSmemMax)) != cudaSuccess) return e;
+    return smem_attr(loss_rows_kernel<false, 32, 256>, kRowsSmemMax);
 }
 
 namespace {
@@ -1819,11 +1817,14 @@ cudaError_t launch_loss_rows(const LossRowParams& p, bool f32, int sms, cudaStre
     const int tiles = (int)((p.rows + kLossTile - 1) / kLossTile);  // the last tile's padding rows too
     const int r = few_blocks(tiles, sms) ? 8 : 32;
     void (*k)(LossRowParams);
-    if (f32)
-        k = r == 32 ? loss_rows_kernel<true, 32> : loss_rows_kernel<true, 8>;
+    const int grid = tiles * (kLossTile / r), threads = r == 8 && grid <= sms ? 512 : 256;
+    if (r == 32)
+        k = f32 ? loss_rows_kernel<true, 32, 256> : loss_rows_kernel<false, 32, 256>;
+    else if (threads == 256)
+        k = f32 ? loss_rows_kernel<true, 8, 256> : loss_rows_kernel<false, 8, 256>;
     else
-        k = r == 32 ? loss_rows_kernel<false, 32> : loss_rows_kernel<false, 8>;
-    return launch_chained(k, tiles * (kLossTile / r), 256, rows_smem_bytes(r, p.k, p.feat, p.n_splits, p.lab.n_top), stream, p);
+        k = f32 ? loss_rows_kernel<true, 8, 512> : loss_rows_kernel<false, 8, 512>;
+    return launch_chained(k, grid, threads, rows_smem_bytes(r, p.k, p.feat, p.n_splits, p.lab.n_top), stream, p);
 }
 
 cudaError_t launch_loss_reduce(const LossReduceParams& p, bool f32, int sms, cudaStream_t stream) {
