@@ -1289,7 +1289,7 @@ __device__ __forceinline__ float group_max(float v) {
 // layout's contiguous direction, every load of a thread in flight at once (k <= 128).
 template <int R, int NT, class T>
 struct RowLoad {
-    static constexpr int kPer = R * 128 / NT, kWarps = NT / 32;  // loads a thread; warps
+    static constexpr int kPer = R * 128 / NT;  // loads a thread
     float v[kPer];
     __device__ __forceinline__ void fetch(const T* x, long long row0, long long rows, int k, long long t_len) {
         if (t_len > 0) {
