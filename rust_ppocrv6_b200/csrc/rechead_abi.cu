@@ -824,7 +824,7 @@ int guarded(F&& f) {
 // tiles plus `overhead` for the unit's own operand, pipeline fill and hand-over), the reader's
 // join (about 1/20 tile a range) and the partial tiles' traffic (64 KB each, written and read:
 // about 1/100 tile each). `uneven`: how much longer than the others a unit may run; in the weight
-// pass the class tile that holds most rows' label (the blank's) takes up to 1.3 times as long, so
+// pass the class tile that holds most rows' label (the blank's) takes up to 1.6 times as long, so
 // its rows are better spread over several units than left to one SM.
 struct LossPlan {
     int own = 0, str = 0, whole = 0, splits = 1, per = 0, grid = 0;
