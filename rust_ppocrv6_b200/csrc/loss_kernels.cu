@@ -1648,6 +1648,12 @@ __global__ void __launch_bounds__(256) loss_score_kernel(const __grid_constant__
     const bool live = row < p.rows;
     RowLoad<kLossRows, 256, float> xv;
     xv.fetch(p.x, row0, p.rows, p.k, p.t_len);
+    // the caller's features and labels are there already; only what the decode kernel writes is waited for
+    int2* ent = ents + r * p.lab.n_top;
+    float entropy;
+    const bool valid = group_labels(p.lab, row, live, s, ent, entropy);
+    xv.put(p.k, p.t_len, xs);
+    wait_previous();
     int best = 0;
     float sum = 1.0f;
     if (row >= p.split_row0 && live) {
@@ -1698,11 +1704,7 @@ __global__ void __launch_bounds__(256) loss_score_kernel(const __grid_constant__
         sum = 1.0f / p.prob[row];
     }
     best = min(max(best, 0), p.lab.n - 1);
-    xv.put(p.k, p.t_len, xs);
     __syncthreads();
-    int2* ent = ents + r * p.lab.n_top;
-    float entropy;
-    const bool valid = group_labels(p.lab, row, live, s, ent, entropy);
     if (live) {
         const int* cls = p.lab.target ? p.lab.target + row : p.lab.top_idx + row * p.lab.n_top;
         bool bad = false;
@@ -1843,14 +1845,9 @@ cudaError_t launch_loss_table(const float* ctab, long long n_floats, float inv_t
 }
 
 cudaError_t launch_loss_score(const LossScoreParams& p, cudaStream_t stream) {
-    const int grid = (int)((p.rows + kLossRows - 1) / kLossRows), smem = score_smem_bytes(p.k, p.lab.n_top);
-    if (p.form == 0)
-        loss_score_kernel<0><<<grid, 256, smem, stream>>>(p);
-    else if (p.form == 1)
-        loss_score_kernel<1><<<grid, 256, smem, stream>>>(p);
-    else
-        loss_score_kernel<2><<<grid, 256, smem, stream>>>(p);
-    return cudaGetLastError();
+    const int grid = (int)((p.rows + kLossRows - 1) / kLossRows);
+    void (*k)(LossScoreParams) = p.form == 0 ? loss_score_kernel<0> : p.form == 1 ? loss_score_kernel<1> : loss_score_kernel<2>;
+    return launch_chained(k, grid, 256, score_smem_bytes(p.k, p.lab.n_top), stream, p);
 }
 
 }  // namespace rh
