@@ -567,8 +567,8 @@ __device__ __forceinline__ LUnit lunit(int u, const LossMainParams& p) {
 // 16 columns' values (8 pairs) as 16-bit tensor-core operands, over the 16 score columns they come
 // from: f32 as fp16 hi (8 columns) and lo (8 columns), whose sum holds ~22 bits and whose products
 // are exact in the f32 accumulator; bf16 by one rounding (half a step of the operand type, as the
-// features' own).
-template <bool F32>
+// features' own), or with TWO as hi and lo in the same places, whose sum is 2^-16 off at most.
+template <bool F32, bool TWO = false>
 __device__ __forceinline__ void store_probs(uint32_t taddr, const float2 (&g)[8]) {
     if constexpr (F32) {
         uint32_t w[16];
@@ -590,6 +590,17 @@ __device__ __forceinline__ void store_probs(uint32_t taddr, const float2 (&g)[8]
             w[i] = *reinterpret_cast<const uint32_t*>(&h);
         }
         tmem_st32x32b_x8(taddr, w);
+        if constexpr (TWO) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                // a bf16 is the upper half of the f32 of the same value
+                const float2 d = __fadd2_rn(g[i], make_float2(-__uint_as_float(w[i] << 16),
+                                                              -__uint_as_float(w[i] & 0xffff0000u)));
+                const __nv_bfloat162 l = __floats2bfloat162_rn(d.x, d.y);
+                w[i] = *reinterpret_cast<const uint32_t*>(&l);
+            }
+            tmem_st32x32b_x8(taddr + 8u, w);
+        }
     }
 }
 
@@ -627,6 +638,13 @@ __device__ __forceinline__ void window_use(LabelWindow& w, const int2* ent, int 
 // takes the adding off every tile's path, where the offset does not move (the weight pass; the row
 // pass where every row of the own tile is bounded, see below).
 constexpr int kAddEvery = 32;
+// bf16 weight pass over at most this many tiles of rows: the probabilities less labels in two parts,
+// for a second run of 8 instructions a tile. A class that few rows name has a gradient of few terms,
+// whose rounding is not averaged away: with one part dw of 3 to 8 rows was off by 1.5 times its own
+// type's rounding, of 128 or more by 1.3 times, with two parts by that rounding alone. Above it one
+// rounding does. A variant of its own (TWO): a test inside the kernel alone cost steps of 61,440 and
+// 122,880 rows 4-8 % (122,880 rows: 2,324 against 2,242 us).
+constexpr int kTwoPartTiles = 8;
 
 // Units (own tile, range of streamed tiles), persistent over the grid. Per streamed tile: scores
 // S = own . tile^T (tensor core), a softmax warpgroup turns them into
@@ -640,7 +658,7 @@ constexpr int kAddEvery = 32;
 // spread of at most 80 binary orders the upper bound itself is the offset, every probability is at
 // most 1, and what underflows (below 2^-126) is 2^-46 of the largest. Rows beyond it (a warp at a
 // time) follow the running maximum as the others do.
-template <bool F32, bool WPASS, bool SLOTS>
+template <bool F32, bool WPASS, bool SLOTS, bool TWO = false>
 __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid_constant__ LossMainParams p) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
@@ -812,6 +830,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                             mma_rows_f32_warp(tmem + kTO, a, b_desc, id_o);
                         else
                             mma_rows_bf16_warp(tmem + kTO, a, b_desc, id_o, held > 0 ? 1u : 0u);
+                        if (TWO) mma_rows_bf16_warp(tmem + kTO, a + 8u, b_desc, id_o, 1u);
                         if (++held == every || c + 1 == U.c1) {
                             mma_commit_warp(bar(kLBarOFull));
                             oph ^= 1u;
@@ -1057,7 +1076,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                         }
 #pragma unroll
                         for (int j = 0; j < 8; j += 2) ts = __fadd2_rn(ts, __fadd2_rn(pr[j], pr[j + 1]));
-                        store_probs<F32>(t_s + 16u * q, pr);
+                        store_probs<F32, TWO>(t_s + 16u * q, pr);
                     }
                     // bias gradient with the rounding error carried (up to thousands of tiles)
                     const float t = fmaf(ts.x + ts.y, F32 ? gs : 1.0f, carry);
@@ -1765,6 +1784,8 @@ cudaError_t loss_kernel_setup() {
     if ((e = smem_attr(loss_main_kernel<false, true, false>, kMSmemBytes)) != cudaSuccess) return e;
     if ((e = smem_attr(loss_main_kernel<false, false, true>, kMSmemBytes)) != cudaSuccess) return e;
     if ((e = smem_attr(loss_main_kernel<false, true, true>, kMSmemBytes)) != cudaSuccess) return e;
+    if ((e = smem_attr(loss_main_kernel<false, true, false, true>, kMSmemBytes)) != cudaSuccess) return e;
+    if ((e = smem_attr(loss_main_kernel<false, true, true, true>, kMSmemBytes)) != cudaSuccess) return e;
     if ((e = smem_attr(loss_pack_kernel<true>, kPackSmemMax)) != cudaSuccess) return e;
     if ((e = smem_attr(loss_pack_kernel<false>, kPackSmemMax)) != cudaSuccess) return e;
     if ((e = smem_attr(loss_rows_kernel<true, 32, 256>, kRowsSmemMax)) != cudaSuccess) return e;
@@ -1808,6 +1829,8 @@ cudaError_t launch_loss_main(const LossMainParams& p, bool f32, bool slots, bool
     void (*k)(LossMainParams);
     if (f32)
         k = weight_pass ? loss_main_kernel<true, true, false> : loss_main_kernel<true, false, false>;
+    else if (weight_pass && p.str_tiles <= kTwoPartTiles)
+        k = slots ? loss_main_kernel<false, true, true, true> : loss_main_kernel<false, true, false, true>;
     else if (slots)
         k = weight_pass ? loss_main_kernel<false, true, true> : loss_main_kernel<false, false, true>;
     else

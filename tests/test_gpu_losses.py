@@ -610,3 +610,22 @@ def test_refusals_launch_nothing(rh, ctx):
     ctx.sync()
     assert ctx.launch_count(0) == before and not buf.any()
     qw.free()
+
+
+@pytest.mark.parametrize("rows,k,n,n_top,t_len", [(1, 120, 18_710, 0, 0), (3, 80, 6906, 0, 3), (5, 61, 724, 13, 0),
+                                                  (8, 120, 18_710, 17, 0), (126, 128, 300, 3, 42), (129, 122, 620, 0, 0),
+                                                  (1000, 33, 129, 5, 8), (1024, 120, 2500, 0, 0)])
+def test_bf16_weight_gradient_of_few_rows(rh, ctx, rows, k, n, n_top, t_len):
+    """Up to 1,024 rows p - q is in two bf16 parts: hi leaves 2^-8 of a value, lo 2^-8 of that, so an
+    operand is 2^-16 off and dw has its own rounding (2^-8) and little beside it."""
+    d = make(rows, k, n, seed=rows + k, n_top=n_top)
+    d = rounded(d, "bf16")
+    temp = 2.0 if n_top else 1.0
+    ref = definition(d, temp)
+    got = grad(rh, ctx, d, "bf16", temp, t_len=t_len)
+    check(got, ref, True)
+    fpq = ref["fp"] + ref["fq"]
+    e = ((128 * U * ref["A"])[:, None] * ref["fp"] + (80 + (rows + 127) // 128) * U * fpq + 2.0 ** -16 * fpq).T @ ref["x"].abs()
+    e = e + 2.0 ** -38 * ref["f"].abs().amax() * ref["x"].abs().sum(0)
+    err = (got["dw"].double() - ref["dw"]).abs()
+    assert not (err > e + BF * (ref["dw"].abs() + e)).any()
