@@ -638,12 +638,13 @@ __device__ __forceinline__ void window_use(LabelWindow& w, const int2* ent, int 
 // takes the adding off every tile's path, where the offset does not move (the weight pass; the row
 // pass where every row of the own tile is bounded, see below).
 constexpr int kAddEvery = 32;
-// bf16 weight pass over at most this many tiles of rows: the probabilities less labels in two parts,
-// for a second run of 8 instructions a tile. A class that few rows name has a gradient of few terms,
-// whose rounding is not averaged away: with one part dw of 3 to 8 rows was off by 1.5 times its own
-// type's rounding, of 128 or more by 1.3 times, with two parts by that rounding alone. Above it one
-// rounding does. A variant of its own (TWO): a test inside the kernel alone cost steps of 61,440 and
-// 122,880 rows 4-8 % (122,880 rows: 2,324 against 2,242 us).
+// bf16 passes over at most this many streamed tiles: the probabilities in two parts, for a second run
+// of 8 instructions a tile. A class that few rows name has a gradient of few terms, and a row's mean
+// weight over few classes cancels against its label's: their rounding is not averaged away. With one
+// part dw of 3 to 8 rows and da over 87 classes were off by 1.5 to 1.9 times their own type's
+// rounding, of 128 or more rows or classes mostly by 1.3 times, with two parts by that rounding alone.
+// Above it one rounding does. A variant of its own (TWO): a test inside the kernel alone cost steps of
+// 61,440 and 122,880 rows 4-8 % (122,880 rows: 2,324 against 2,242 us).
 constexpr int kTwoPartTiles = 8;
 
 // Units (own tile, range of streamed tiles), persistent over the grid. Per streamed tile: scores
@@ -948,7 +949,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                             pr[j] = make_float2(ex2_approx(a.x), ex2_approx(a.y));
                             ts = __fadd2_rn(ts, pr[j]);
                         }
-                        if (with_o) store_probs<F32>(t_s + 16u * q, pr);
+                        if (with_o) store_probs<F32, TWO>(t_s + 16u * q, pr);
                     }
                     sum += ts.x + ts.y;
                 } else if constexpr (!WPASS) {
@@ -1005,7 +1006,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                             pr[j / 2 + 1] = make_float2(ex2_approx(b.x), ex2_approx(b.y));
                             ts = __fadd2_rn(ts, __fadd2_rn(pr[j / 2], pr[j / 2 + 1]));
                         }
-                        if (with_o) store_probs<F32>(t_s + 16u * q, pr);
+                        if (with_o) store_probs<F32, TWO>(t_s + 16u * q, pr);
                     }
                     const float t = F32 ? (ts.x + ts.y) * (1.0f / 16384.0f) : ts.x + ts.y;
                     sum = fmaf(sum, corr, t);
@@ -1784,6 +1785,8 @@ cudaError_t loss_kernel_setup() {
     if ((e = smem_attr(loss_main_kernel<false, true, false>, kMSmemBytes)) != cudaSuccess) return e;
     if ((e = smem_attr(loss_main_kernel<false, false, true>, kMSmemBytes)) != cudaSuccess) return e;
     if ((e = smem_attr(loss_main_kernel<false, true, true>, kMSmemBytes)) != cudaSuccess) return e;
+    if ((e = smem_attr(loss_main_kernel<false, false, false, true>, kMSmemBytes)) != cudaSuccess) return e;
+    if ((e = smem_attr(loss_main_kernel<false, false, true, true>, kMSmemBytes)) != cudaSuccess) return e;
     if ((e = smem_attr(loss_main_kernel<false, true, false, true>, kMSmemBytes)) != cudaSuccess) return e;
     if ((e = smem_attr(loss_main_kernel<false, true, true, true>, kMSmemBytes)) != cudaSuccess) return e;
     if ((e = smem_attr(loss_pack_kernel<true>, kPackSmemMax)) != cudaSuccess) return e;
@@ -1829,8 +1832,10 @@ cudaError_t launch_loss_main(const LossMainParams& p, bool f32, bool slots, bool
     void (*k)(LossMainParams);
     if (f32)
         k = weight_pass ? loss_main_kernel<true, true, false> : loss_main_kernel<true, false, false>;
-    else if (weight_pass && p.str_tiles <= kTwoPartTiles)
+    else if (p.str_tiles <= kTwoPartTiles && weight_pass)
         k = slots ? loss_main_kernel<false, true, true, true> : loss_main_kernel<false, true, false, true>;
+    else if (p.str_tiles <= kTwoPartTiles)
+        k = slots ? loss_main_kernel<false, false, true, true> : loss_main_kernel<false, false, false, true>;
     else if (slots)
         k = weight_pass ? loss_main_kernel<false, true, true> : loss_main_kernel<false, false, true>;
     else

@@ -629,3 +629,20 @@ def test_bf16_weight_gradient_of_few_rows(rh, ctx, rows, k, n, n_top, t_len):
     e = e + 2.0 ** -38 * ref["f"].abs().amax() * ref["x"].abs().sum(0)
     err = (got["dw"].double() - ref["dw"]).abs()
     assert not (err > e + BF * (ref["dw"].abs() + e)).any()
+
+
+@pytest.mark.parametrize("rows,k,n,n_top", [(2, 30, 268, 0), (14_174, 121, 87, 0), (300, 128, 1024, 0), (77, 127, 129, 9),
+                                            (5000, 16, 1000, 3)])
+def test_bf16_feature_gradient_over_few_classes(rh, ctx, rows, k, n, n_top):
+    """Up to 1,024 classes p is in two bf16 parts, 2^-16 off, so da keeps what the mean weight leaves
+    over the label's, besides its own rounding."""
+    d = rounded(make(rows, k, n, seed=rows + n, n_top=n_top), "bf16")
+    temp = 2.0 if n_top else 1.0
+    ref = definition(d, temp)
+    got = grad(rh, ctx, d, "bf16", temp)
+    check(got, ref, True)
+    fpq = ref["fp"] + ref["fq"]
+    e = ((128 * U * ref["A"])[:, None] * ref["fp"] + (80 + (n + 127) // 128) * U * fpq + 2.0 ** -16 * fpq) @ ref["w"].abs()
+    e = e + 2.0 ** -38 * ref["f"].abs().amax() * ref["w"].abs().sum(0)
+    err = (got["da"].double() - ref["da"]).abs()
+    assert not (err > e + BF * (ref["da"].abs() + e)).any()
