@@ -66,6 +66,14 @@ __device__ __forceinline__ float warp_max(float v) {
     for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
+// What an earlier kernel of the same chain wrote. The kernel that reads it may have been resident since
+// before the write (launch_next), so it is no read-only data: the non-coherent path of __ldg could return
+// a line that this SM's L1 kept of the same address, as one workspace part serves one kernel after the
+// other. Read from L2. (__ldg is for what the caller brings: weight, bias, packed tiles.)
+template <class T>
+__device__ __forceinline__ T chain_load(const T* p) {
+    return __ldcg(p);
+}
 // Whether class c is one of a row's labels at all.
 __device__ __forceinline__ bool is_class(int c, int n) { return c >= 0 && c < n; }
 
@@ -616,7 +624,7 @@ struct LabelWindow {
 };
 constexpr int kNoLabel = 0x7fffffff;
 __device__ __forceinline__ int2 window_entry(const LabelWindow& w, const int2* ent, int lane) {
-    return w.next + lane < w.end ? __ldg(ent + w.next + lane) : make_int2(kNoLabel, 0);
+    return w.next + lane < w.end ? chain_load(ent + w.next + lane) : make_int2(kNoLabel, 0);
 }
 __device__ __forceinline__ void window_use(LabelWindow& w, const int2* ent, int lane, int half) {
     w.next += 32;
@@ -717,7 +725,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
     if (SLOTS && !WPASS && warp >= 2) {
         bool nan = false;
         for (int t = lane; t < p.str_tiles; t += 32) {
-            const float2 b = __ldg(p.w_bound + t);
+            const float2 b = chain_load(p.w_bound + t);
             nan |= isnan(b.x);
             w_max = fmaxf(w_max, b.x);
             e_max = fmaxf(e_max, b.y);
@@ -726,7 +734,9 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
         e_max = warp_max(e_max);
         if (__any_sync(0xffffffffu, nan)) w_max = CUDART_INF_F;
     }
-    auto reach_of = [&](int own, int row) { return p.logit_scale * __ldg(p.x_norm + (size_t)own * 128 + row) * w_max * 1.001f; };
+    auto reach_of = [&](int own, int row) {
+        return p.logit_scale * chain_load(p.x_norm + (size_t)own * 128 + row) * w_max * 1.001f;
+    };
     auto in_bounds = [&](float reach) { return reach <= 40.0f && fabsf(reach + e_max) < 1e6f; };
     // tiles added up in TMEM at a time, for this own tile (every role that asks finds the same)
     auto add_every = [&](int own) -> int {
@@ -872,7 +882,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
             const int2* ranges = p.sp_off + (size_t)(U.c0 + (int)i0) * 4 * p.own_tiles + 4 * U.own + quad;
             const int2* ent = p.sp_ent + (size_t)(U.c0 + (int)i0) * 128 * p.n_top;
             if (WPASS && i0 < n) {
-                const int2 first = __ldg(ranges);
+                const int2 first = chain_load(ranges);
                 lw.next = first.x;
                 lw.end = first.y;
                 lw.e = window_entry(lw, ent, lane);
@@ -888,7 +898,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                     uint32_t w[32];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(img + image_chunk(r, 8 * half + j));
+                        const uint4 x = chain_load(reinterpret_cast<const uint4*>(img + image_chunk(r, 8 * half + j)));
                         w[4 * j] = x.x, w[4 * j + 1] = x.y, w[4 * j + 2] = x.z, w[4 * j + 3] = x.w;
                     }
                     tmem_st32x32b_x32(tmem + lanes + kTOwn + 64u * g + 32u * half, w);
@@ -898,8 +908,8 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                 mbar_arrive(bar(kLBarAFull));
             }
 
-            const float own_mul = F32 ? p.logit_scale * __ldg(p.own_scale + U.own) : p.logit_scale;
-            const float lane_e = WPASS && !SLOTS ? __ldg(p.lane_e + (size_t)U.own * 128 + r) : 0.0f;
+            const float own_mul = F32 ? p.logit_scale * chain_load(p.own_scale + U.own) : p.logit_scale;
+            const float lane_e = WPASS && !SLOTS ? chain_load(p.lane_e + (size_t)U.own * 128 + r) : 0.0f;
             // the tiles' offsets go to the adding warps only where they move
             const bool ringed = !WPASS && with_o && add_every(U.own) == 1;
             bool bounded = false;
@@ -914,13 +924,13 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                 const int c = U.c0 + (int)i;
                 const uint32_t s = (cc + i) % kStages;
                 const uint32_t tab = base + Ring<F32>::kTab + s * 1024u + 256u * half;
-                const float str_s = F32 ? __ldg(p.str_scale + c) : 1.0f;
-                const float gs = WPASS ? __ldg(p.g_scale + c) : 1.0f;
+                const float str_s = F32 ? chain_load(p.str_scale + c) : 1.0f;
+                const float gs = WPASS ? chain_load(p.g_scale + c) : 1.0f;
                 // the next tile's label range is fetched under this tile, its entries at this tile's end
                 int2 next_range = make_int2(0, 0);
                 if (WPASS) {
                     ranges += 8 * p.own_tiles;
-                    if (i + 2 < n) next_range = __ldg(ranges);
+                    if (i + 2 < n) next_range = chain_load(ranges);
                 }
                 const float2 mul = make_float2(own_mul * str_s, own_mul * str_s);
                 const uint32_t buf = (cc + i) % Ring<F32>::kBufs;
@@ -1127,8 +1137,8 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
             if (with_o) {
                 const int every = add_every(U.own);
                 for (int c = U.c0; c < U.c1; c += every, ++fc) {
-                    float om = F32 ? __ldg(p.str_scale + c) : 1.0f;  // value of one unit of the product
-                    if (F32) om *= WPASS ? __ldg(p.g_scale + c) : 1.0f / 16384.0f;
+                    float om = F32 ? chain_load(p.str_scale + c) : 1.0f;  // value of one unit of the product
+                    if (F32) om *= WPASS ? chain_load(p.g_scale + c) : 1.0f / 16384.0f;
                     float corr = 1.0f;
                     if (!WPASS && every == 1) {
                         ok = loss_wait(bar(kLBarRing + (int)(rc & 3u)), (rc >> 2) & 1u, wt, 112);
@@ -1418,7 +1428,7 @@ __device__ __forceinline__ void join_units(const float* part_o, size_t u0, int n
         const float w = WEIGHTED ? wgt[s * R + r] : 1.0f;
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
-            if (f0 + i * kStep < feat) a[i] = fmaf(__ldg(po + (size_t)i * kStep * 128), w, a[i]);
+            if (f0 + i * kStep < feat) a[i] = fmaf(chain_load(po + (size_t)i * kStep * 128), w, a[i]);
     }
     const float k = WEIGHTED ? inv[r] : 1.0f;
 #pragma unroll
@@ -1457,7 +1467,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 3 : 1) loss_rows_kernel(const 
     const int jr = tid % R, jg = tid / R;
     if (ns == 1) {
         // one unit has the whole class range: nothing to join
-        const float2 ms = __ldg(p.part_ms + u0 * 128 + l0 + jr);
+        const float2 ms = chain_load(p.part_ms + u0 * 128 + l0 + jr);
         if (jg == 0) s_lse2[jr] = (ms.x == -CUDART_INF_F ? 0.0f : ms.x) + log2f(ms.y);
         if (p.dx) {
             constexpr int kPer = 128 / kG;
@@ -1465,7 +1475,8 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 3 : 1) loss_rows_kernel(const 
             const float inv = 1.0f / ms.y;
             float a[kPer];
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) a[i] = jg + i * kG < p.feat ? __ldg(po + (size_t)(jg + i * kG) * 128) : 0.0f;
+            for (int i = 0; i < kPer; ++i)
+                a[i] = jg + i * kG < p.feat ? chain_load(po + (size_t)(jg + i * kG) * 128) : 0.0f;
 #pragma unroll
             for (int i = 0; i < kPer; ++i)
                 if (jg + i * kG < p.feat) os[jr * (p.feat + 1) + jg + i * kG] = a[i] * inv;
@@ -1473,7 +1484,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 3 : 1) loss_rows_kernel(const 
     } else {
         float m = -CUDART_INF_F;
         for (int s = jg; s < ns; s += kG) {
-            const float o = p.part_ms[(u0 + s) * 128 + l0 + jr].x;
+            const float o = chain_load(p.part_ms + (u0 + s) * 128 + l0 + jr).x;
             wgt[s * R + jr] = o;
             m = fmaxf(m, o);
         }
@@ -1487,7 +1498,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 3 : 1) loss_rows_kernel(const 
         for (int s = jg; s < ns; s += kG) {
             const float k = ex2_approx(wgt[s * R + jr] - m0);
             wgt[s * R + jr] = k;
-            sum = fmaf(p.part_ms[(u0 + s) * 128 + l0 + jr].y, k, sum);
+            sum = fmaf(chain_load(p.part_ms + (u0 + s) * 128 + l0 + jr).y, k, sum);
         }
         red[jg][jr] = sum;
         __syncthreads();
@@ -1596,7 +1607,7 @@ __global__ void __launch_bounds__(256) loss_reduce_kernel(const __grid_constant_
     join_units<R, 256, false>(p.part_o, u0, ns, p.feat, l0, nullptr, nullptr, sm);
     if (p.db && threadIdx.x < R && j0 + (int)threadIdx.x < p.n) {
         float a = 0.0f;
-        for (int s = 0; s < ns; ++s) a += p.part_ms[(u0 + s) * 128 + l0 + threadIdx.x].x;
+        for (int s = 0; s < ns; ++s) a += chain_load(p.part_ms + (u0 + s) * 128 + l0 + threadIdx.x).x;
         p.db[j0 + threadIdx.x] = a;
     }
     __syncthreads();
@@ -1687,7 +1698,7 @@ __global__ void __launch_bounds__(256) loss_score_kernel(const __grid_constant__
             float4 v[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                v[j] = i0 + 8 * j < p.n_splits ? __ldg(part + (size_t)(i0 + 8 * j) * step)
+                v[j] = i0 + 8 * j < p.n_splits ? chain_load(part + (size_t)(i0 + 8 * j) * step)
                                                : make_float4(-CUDART_INF_F, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -1720,8 +1731,8 @@ __global__ void __launch_bounds__(256) loss_score_kernel(const __grid_constant__
             m = M;
         }
     } else if (live) {
-        best = p.idx[row];
-        sum = 1.0f / p.prob[row];
+        best = chain_load(p.idx + row);
+        sum = 1.0f / chain_load(p.prob + row);
     }
     best = min(max(best, 0), p.lab.n - 1);
     __syncthreads();
