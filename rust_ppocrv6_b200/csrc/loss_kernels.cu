@@ -9,12 +9,19 @@
 //  loss_pack_kernel    operand tiles of 128 rows as tensor-core images, labels sorted by class tile
 //  loss_main_kernel    the dense work, in one of two directions that mirror each other:
 //                        row pass    own = 128 rows of x, streamed = W tiles: running (max, sum) of
-//                                    the softmax and the mean weight row sum_j p_j W_j
+//                                    the softmax and sum_j p_j W_j, over the classes that the row
+//                                    does not name
 //                        weight pass own = 128 classes, streamed = x tiles: dz^T x with p from the
-//                                    rows' lse
-//  loss_rows_kernel    joins a row's class ranges: loss, lse, dx = T g (sum_j p_j W_j - sum_i q_i W_ci)
+//                                    rows' lse, and dz of the named classes as the row kernel left it
+//  loss_rows_kernel    joins a row's class ranges and adds the named classes: loss, lse, their dz, dx
 //  loss_reduce_kernel  joins a class's row ranges: dW, db
 //  loss_score_kernel   loss and lse of a packed head from the decode kernel's (argmax, probability)
+//
+// The classes that a row names are kept out of the dense products, because there p - q cancels: a row
+// whose target has p = 0.9999 has a gradient of 1e-4 of p, and p rounded to bf16 (2^-9), or added up by
+// a tensor core that rounds toward zero (2^-23 a step), would be off by more than that. The row kernel
+// forms their logits in f32 and takes 1 - p as what it is, the other classes' share. (With the named
+// classes in the products, da of rows with p of 0.9 to 0.99999 was 10 to 50,000 times further off.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math_constants.h>
@@ -88,7 +95,7 @@ __device__ __forceinline__ bool is_class(int c, int n) { return c >= 0 && c < n;
 // The labels of a feature tile are sorted by 32 classes (a softmax warp's), rows ascending: each
 // warp takes 8 rows, a group of lanes per row, and notes for every entry how many of its bin came
 // before it in the warp; a scan over warps and bins then gives every entry its place (no atomics:
-// the order is fixed).
+// the order is fixed). A class that a row names twice has one place, its first entry's.
 constexpr int kPackThreads = 512, kPackWarps = kPackThreads / 32, kPackItems = 2048 / kPackThreads;
 
 template <bool F32>
@@ -151,9 +158,8 @@ __global__ void __launch_bounds__(kPackThreads, 2) loss_pack_kernel(const __grid
     const int nb = 4 * p.w_tiles;                                  // 32 classes a bin
     uint16_t* counts = reinterpret_cast<uint16_t*>(pack_smem);     // [16 warps][nb]
     int* start = reinterpret_cast<int*>(pack_smem + kPackWarps * 2 * (size_t)nb);  // [nb]
-    int2* ents = reinterpret_cast<int2*>(start + nb);              // [128][n_top]: (class << 10 | place, factor)
-    const bool sort = !is_w && p.sort_labels;
-    if (sort) {
+    int* ents = start + nb;                                        // [128][n_top]: class << 10 | place, or -1
+    if (!is_w) {
         for (int i = tid; i < kPackWarps * nb / 2; i += kPackThreads) reinterpret_cast<uint32_t*>(counts)[i] = 0u;
         __syncthreads();
     }
@@ -168,7 +174,6 @@ __global__ void __launch_bounds__(kPackThreads, 2) loss_pack_kernel(const __grid
             const long long row = row0 + r;
             const bool live = grp < per && row < p.rows;
             int c[2] = {-1, -1};
-            float u[2] = {-CUDART_INF_F, -CUDART_INF_F}, q[2] = {0.0f, 0.0f};
             bool bad = false;
             float g = 0.0f;
             if (live) {
@@ -178,8 +183,9 @@ __global__ void __launch_bounds__(kPackThreads, 2) loss_pack_kernel(const __grid
                         const int x = p.lab.target ? p.lab.target[row] : p.lab.top_idx[row * p.lab.n_top + e];
                         bad |= x >= p.lab.n;
                         if (is_class(x, p.lab.n)) {
-                            u[s] = p.lab.target ? 0.0f : p.lab.top_logits[row * p.lab.n_top + e] * p.lab.inv_temp;
-                            if (u[s] != -CUDART_INF_F) c[s] = x;  // (of no share: as absent)
+                            const float u = p.lab.target ? 0.0f
+                                                         : p.lab.top_logits[row * p.lab.n_top + e] * p.lab.inv_temp;
+                            if (u != -CUDART_INF_F) c[s] = x;  // (of no share: as absent)
                         }
                     }
                 }
@@ -194,42 +200,20 @@ __global__ void __launch_bounds__(kPackThreads, 2) loss_pack_kernel(const __grid
                 s_valid[r] = valid ? 1 : 0;
                 s_norm[r] = f;  // the factors, until the norms need the place
             }
-            if (!sort) continue;
-            float top = fmaxf(u[0], u[1]);
-            for (int o = width >> 1; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            float sum = 0.0f;
-            for (int s = 0; s < slots; ++s) {
-                q[s] = c[s] >= 0 ? expf(u[s] - top) : 0.0f;
-                sum += q[s];
-            }
-            for (int o = width >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            float share[2] = {c[0] >= 0 ? q[0] / sum : 0.0f, c[1] >= 0 ? q[1] / sum : 0.0f};
-            // a class named twice: one entry with both shares (rare; beyond 32 entries a lane holds two,
-            // which one match does not compare)
+            // a class named twice (rare; beyond 32 entries a lane holds two, which one match does not
+            // compare)
             const uint32_t twice = __match_any_sync(0xffffffffu, c[0] >= 0 ? c[0] : ~lane) & gm;
             if (slots == 2 || __any_sync(0xffffffffu, __popc(twice) > 1)) {
                 bool dup[2] = {false, false};
-                float all[2] = {share[0], share[1]};
                 for (int j = 0; j < p.lab.n_top; ++j) {
                     const int from = grp * width + (j & (width - 1));
                     const int cj = __shfl_sync(0xffffffffu, j < 32 ? c[0] : c[1], from);
-                    const float qj = __shfl_sync(0xffffffffu, j < 32 ? share[0] : share[1], from);
 #pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        const int e = sub + 32 * s;
-                        if (cj >= 0 && cj == c[s] && j != e) {
-                            if (j < e)
-                                dup[s] = true;
-                            else
-                                all[s] += qj;
-                        }
-                    }
+                    for (int s = 0; s < 2; ++s) dup[s] |= cj >= 0 && cj == c[s] && j < sub + 32 * s;
                 }
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    share[s] = all[s];
+                for (int s = 0; s < 2; ++s)
                     if (dup[s]) c[s] = -1;
-                }
             }
             for (int s = 0; s < slots; ++s) {
                 const int e = sub + 32 * s;
@@ -243,15 +227,13 @@ __global__ void __launch_bounds__(kPackThreads, 2) loss_pack_kernel(const __grid
                     if (rank == 0) mine[bin] = (uint16_t)(at + __popc(same));
                 }
                 __syncwarp();
-                if (live && e < p.lab.n_top)
-                    ents[r * p.lab.n_top + e] =
-                        make_int2(c[s] >= 0 ? (c[s] << 10) | (at + rank) : -1, __float_as_int(-share[s] * f));
+                if (live && e < p.lab.n_top) ents[r * p.lab.n_top + e] = c[s] >= 0 ? (c[s] << 10) | (at + rank) : -1;
             }
         }
         __syncthreads();
     }
-    float gs = 1.0f;  // scale of this tile's gradient factors
     if (!is_w) {
+        float gs = 1.0f;  // scale of this tile's gradient factors
         const float f = tid < 128 ? s_norm[tid] : 0.0f;
         if (F32) {
             const float m = warp_max(fabsf(f));
@@ -376,7 +358,7 @@ __global__ void __launch_bounds__(kPackThreads, 2) loss_pack_kernel(const __grid
             }
         }
     }
-    if (!sort) return;
+    if (is_w) return;
 
     // ---- the entries' places: counts -> each warp's first position within its bin, bins' starts
     const int per = (nb + kPackThreads - 1) / kPackThreads, b0 = tid * per, b1 = min(nb, b0 + per);
@@ -411,11 +393,14 @@ __global__ void __launch_bounds__(kPackThreads, 2) loss_pack_kernel(const __grid
     int2* out = p.sp_ent + (size_t)tile * 128 * p.lab.n_top;
     const int live = (int)min((long long)128, p.rows - row0) * p.lab.n_top;
     for (int i = tid; i < live; i += kPackThreads) {
-        const int2 e = ents[i];
-        if (e.x < 0) continue;
-        const int r = i / p.lab.n_top, c = e.x >> 10, bin = c >> 5;
-        out[start[bin] + counts[(size_t)(r >> 3) * nb + bin] + (e.x & 1023)] =
-            make_int2((r << 5) | (c & 31), __float_as_int(__int_as_float(e.y) * gs));
+        const int e = ents[i];
+        int at = -1;
+        if (e >= 0) {
+            const int r = i / p.lab.n_top, c = e >> 10, bin = c >> 5;
+            at = start[bin] + counts[(size_t)(r >> 3) * nb + bin] + (e & 1023);
+            out[at].x = (r << 5) | (c & 31);
+        }
+        p.sp_pos[(size_t)tile * 128 * p.lab.n_top + i] = at;
     }
 }
 
@@ -456,6 +441,7 @@ constexpr uint32_t kMOffMs = kMOffMisc + 64;      // [4][128] float2: the softma
 constexpr uint32_t kMOffUnion = kMOffMs + 4096;
 constexpr uint32_t kMOffRing = kMOffUnion;         // row pass: [4 tiles][128] f32, offset of a tile's probabilities
 constexpr uint32_t kMOffTop = kMOffUnion + 2048;   // row pass: [2][4][128] f32, maxima of a tile's two halves
+constexpr uint32_t kMOffNamed = kMOffTop + 4096;   // row pass: [16 warps][32 rows][2] bits of the named columns
 constexpr uint32_t kPatchRow = 12;                 // floats per class row of a label patch (8 used:
                                                    // the 16-byte rows then fall on distinct banks)
 constexpr uint32_t kMOffPatch = kMOffUnion;        // weight pass: [16 warps][32][kPatchRow] f32
@@ -463,6 +449,7 @@ constexpr uint32_t kMSmemUsed = kMOffPatch + 16 * 32 * kPatchRow * 4;
 constexpr uint32_t kMSmemBytes = kMSmemUsed + 1024;
 static_assert(Ring<true>::kEnd <= kMOffBars && Ring<false>::kEnd <= kMOffBars && Ring<false>::kOwn % 1024 == 0, "shared memory map");
 static_assert(kMSmemBytes <= 227 * 1024, "shared memory per CTA");
+static_assert(kMOffNamed + 16 * 64 * 4 <= kMSmemUsed, "row pass within the union");
 
 constexpr int kLBarFull = 0;               // [4] tile and column table landed
 constexpr int kLBarEmpty = 4;              // [4] the tile's products done, its softmax warps done with the table
@@ -616,13 +603,23 @@ __device__ __forceinline__ void store_probs(uint32_t taddr, const float2 (&g)[8]
 // ascending: each lane holds one entry of the current window and, where the list goes on, one of the
 // next, in flight meanwhile.
 struct LabelWindow {
-    int2 e, n;        // (row << 5 | class, factor)
+    int2 e, n;        // (row << 5 | class, gradient)
     int next, end;    // first entry after the current window
     uint32_t groups;  // groups of 8 of this half's rows that have an entry in the window
     int last;         // group of the window's last entry where entries follow it, else beyond any group
     int group;        // group of this lane's entry; outside 0..7: none, or in the other half
 };
 constexpr int kNoLabel = 0x7fffffff;
+constexpr int kNoPatch = -1;  // a patch cell without an entry: bits that no computed value has
+// The labels of a warp's 64 columns in a tile (row pass): entries of two runs of 32 classes, one after
+// the other.
+struct NamedRange {
+    int next, mid, end;  // first entry, first of the second 32 classes, end
+    int e;               // this lane's of the first 32 entries: row << 5 | class within its 32
+};
+__device__ __forceinline__ int named_entry(const int2* ent, int i, int end) {
+    return i < end ? chain_load(&ent[i].x) : kNoLabel;
+}
 __device__ __forceinline__ int2 window_entry(const LabelWindow& w, const int2* ent, int lane) {
     return w.next + lane < w.end ? chain_load(ent + w.next + lane) : make_int2(kNoLabel, 0);
 }
@@ -647,19 +644,21 @@ __device__ __forceinline__ void window_use(LabelWindow& w, const int2* ent, int 
 // pass where every row of the own tile is bounded, see below).
 constexpr int kAddEvery = 32;
 // bf16 passes over at most this many streamed tiles: the probabilities in two parts, for a second run
-// of 8 instructions a tile. A class that few rows name has a gradient of few terms, and a row's mean
-// weight over few classes cancels against its label's: their rounding is not averaged away. With one
-// part dw of 3 to 8 rows and da over 87 classes were off by 1.5 to 1.9 times their own type's
-// rounding, of 128 or more rows or classes mostly by 1.3 times, with two parts by that rounding alone.
+// of 8 instructions a tile. Sums of few terms do not average their rounding away: with one part dw of 3
+// to 8 rows and da over 87 classes were off by 1.5 to 1.9 times their own type's rounding, of 128 or
+// more rows or classes mostly by 1.3 times, with two parts by that rounding alone. (A class that few
+// rows name has few large terms in a long step too, and keeps the one rounding there: 2^-9 of each
+// term, as of any gradient that enters a bf16 product.)
 // Above it one rounding does. A variant of its own (TWO): a test inside the kernel alone cost steps of
 // 61,440 and 122,880 rows 4-8 % (122,880 rows: 2,324 against 2,242 us).
 constexpr int kTwoPartTiles = 8;
 
 // Units (own tile, range of streamed tiles), persistent over the grid. Per streamed tile: scores
 // S = own . tile^T (tensor core), a softmax warpgroup turns them into
-// probabilities (row pass: against the running maximum; weight pass: 2^(s - lse) times the rows'
-// gradient factors, less the labels' shares) in the same TMEM columns, and a second product
-// O = P . tile reads the same tile the other way round; the adding warps sum it in registers.
+// probabilities (row pass: against the running maximum, the classes that the row names left out;
+// weight pass: 2^(s - lse) times the rows' gradient factors, the labels' gradients in their place) in
+// the same TMEM columns, and a second product O = P . tile reads the same tile the other way round;
+// the adding warps sum it in registers.
 // f32: three products each (hi.lo, lo.hi, hi.hi).
 // bf16 with slots: the scores come with their bias, so they need no column table in the row pass;
 // and as bf16 probabilities have f32's range, a row's offset need not follow its maximum: by
@@ -708,7 +707,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
         fence_mbar_init();
     }
     for (uint32_t i = threadIdx.x; i < 16 * 32 * kPatchRow; i += kMainThreads)
-        reinterpret_cast<float*>(gbase + kMOffPatch)[i] = 0.0f;
+        reinterpret_cast<int*>(gbase + kMOffPatch)[i] = WPASS ? kNoPatch : 0;
     if (warp == 1) {
         tmem_alloc(base + kMOffMisc, 512);
         tmem_relinquish();
@@ -887,6 +886,16 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                 lw.end = first.y;
                 lw.e = window_entry(lw, ent, lane);
             }
+            // the same for the row pass: which of its columns the warp's rows name
+            NamedRange nr{};
+            const int4* named = reinterpret_cast<const int4*>(p.sp_off + (size_t)U.own * 4 * p.str_tiles +
+                                                              4 * (U.c0 + (int)i0) + 2 * (int)half);
+            const int2* named_ent = p.sp_ent + (size_t)U.own * 128 * p.n_top;
+            uint32_t* bits = reinterpret_cast<uint32_t*>(gbase + kMOffNamed) + (warp - 4) * 64;
+            if (!WPASS && i0 < n) {
+                const int4 first = chain_load(named);
+                nr = {first.x, first.y, first.w, named_entry(named_ent, first.x + lane, first.w)};
+            }
             if (F32) {
                 // own operand -> TMEM: warpgroup wg takes K slots 64 half .. 64 half + 63 of the lane's
                 // row, of the high part (even tiles' warpgroups) or the low part (odd)
@@ -932,7 +941,14 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                     ranges += 8 * p.own_tiles;
                     if (i + 2 < n) next_range = chain_load(ranges);
                 }
-                const float2 mul = make_float2(own_mul * str_s, own_mul * str_s);
+                int4 next_named = make_int4(0, 0, 0, 0);
+                if (!WPASS) {
+                    named += 4;
+                    if (i + 2 < n) next_named = chain_load(named);
+                }
+                // (not below the least normal: a named column's -inf must stay one)
+                const float mul1 = fmaxf(own_mul * str_s, 1.17549435e-38f);
+                const float2 mul = make_float2(mul1, mul1);
                 const uint32_t buf = (cc + i) % Ring<F32>::kBufs;
                 const uint32_t t_s = t_bufs + 128u * buf;
                 ok = loss_wait(bar(kLBarSFull + (int)buf), ((cc + i) / Ring<F32>::kBufs) & 1u, wt, 107);
@@ -941,6 +957,37 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                 ok = ok && loss_wait(bar(kLBarFull + s), ((cc + i) / kStages) & 1u, wt, 108);
                 if (!ok) break;
                 tc_fence_after();
+                // the named columns of the warp's rows, a row a lane: their scores become -inf
+                uint32_t bits0 = 0, bits1 = 0, chunks = 0;
+                if (!WPASS && nr.next < nr.end) {
+                    bool hit = false;
+                    for (int at = nr.next; at < nr.end; at += 32) {
+                        if (at != nr.next) nr.e = named_entry(named_ent, at + lane, nr.end);
+                        if (nr.e >> 10 == quad) {
+                            atomicOr(bits + ((nr.e >> 5) & 31) * 2 + (at + lane >= nr.mid ? 1 : 0), 1u << (nr.e & 31));
+                            hit = true;
+                        }
+                    }
+                    if (__any_sync(0xffffffffu, hit)) {
+                        __syncwarp();
+                        bits0 = bits[2 * lane];
+                        bits1 = bits[2 * lane + 1];
+                        bits[2 * lane] = bits[2 * lane + 1] = 0u;
+                        const uint32_t all0 = __reduce_or_sync(0xffffffffu, bits0);
+                        const uint32_t all1 = __reduce_or_sync(0xffffffffu, bits1);
+                        chunks = ((all0 & 0xffffu) ? 1u : 0u) | ((all0 >> 16) ? 2u : 0u) | ((all1 & 0xffffu) ? 4u : 0u) |
+                                 ((all1 >> 16) ? 8u : 0u);
+                    }
+                }
+                // (a chunk of 16 columns in which no row of the warp names one passes by)
+                auto drop_named = [&](uint32_t (&x)[16], int q) {
+                    if ((chunks >> q) & 1u) {
+                        const uint32_t here = (q < 2 ? bits0 : bits1) >> (16 * (q & 1));
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if ((here >> j) & 1u) x[j] = 0xff800000u;
+                    }
+                };
                 if (SLOTS && !WPASS && bounded) {
                     off = upper;
                     if (with_o && half == 0 && ringed) ring[((rc + i) & 3u) * 128 + r] = off;
@@ -951,6 +998,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                         uint32_t x[16];
                         tmem_ld32x32b_x16(t_s + 16u * q, x);
                         tmem_ld_wait16(x);
+                        drop_named(x, q);
                         float2 pr[8];
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
@@ -969,6 +1017,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                         uint32_t x[16];
                         tmem_ld32x32b_x16(t_s + 16u * q, x);
                         tmem_ld_wait16(x);
+                        drop_named(x, q);
 #pragma unroll
                         for (int j = 0; j < 16; j += 4) {
                             const float4 e = SLOTS ? make_float4(0.f, 0.f, 0.f, 0.f) : lds128(tab + 4u * (16 * q + j));
@@ -1002,6 +1051,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                         uint32_t x[16];
                         tmem_ld32x32b_x16(t_s + 16u * q, x);
                         tmem_ld_wait16(x);
+                        drop_named(x, q);
                         float2 pr[8];
 #pragma unroll
                         for (int j = 0; j < 16; j += 4) {
@@ -1053,8 +1103,8 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                                 pr[j / 2 + 1] = __fmul2_rn(pr[j / 2 + 1], make_float2(f.z, f.w));
                             }
                         }
-                        // the labels' shares, 8 columns (rows of x) at a time through a patch of
-                        // shared memory: entries scatter into it, each lane then adds its class's row
+                        // the labels' gradients, 8 columns (rows of x) at a time through a patch of
+                        // shared memory: entries scatter into it, each lane then takes its class's row
 #pragma unroll
                         for (int h = 0; h < 2 && labelled; ++h) {
                             const int group = 2 * q + h;
@@ -1077,10 +1127,14 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                                 const uint32_t row = patch + 4u * (uint32_t)lane * kPatchRow;
 #pragma unroll
                                 for (int j = 0; j < 2; ++j) {
-                                    const float4 d = lds128(row + 16u * j);
-                                    pr[4 * h + 2 * j] = __fadd2_rn(pr[4 * h + 2 * j], make_float2(d.x, d.y));
-                                    pr[4 * h + 2 * j + 1] = __fadd2_rn(pr[4 * h + 2 * j + 1], make_float2(d.z, d.w));
-                                    sts128(row + 16u * j, make_float4(0.f, 0.f, 0.f, 0.f));
+                                    const uint4 d = lds128u(row + 16u * j);
+                                    float2 &lo = pr[4 * h + 2 * j], &hi = pr[4 * h + 2 * j + 1];
+                                    if (d.x != (uint32_t)kNoPatch) lo.x = __uint_as_float(d.x);
+                                    if (d.y != (uint32_t)kNoPatch) lo.y = __uint_as_float(d.y);
+                                    if (d.z != (uint32_t)kNoPatch) hi.x = __uint_as_float(d.z);
+                                    if (d.w != (uint32_t)kNoPatch) hi.y = __uint_as_float(d.w);
+                                    sts128u(row + 16u * j, make_uint4((uint32_t)kNoPatch, (uint32_t)kNoPatch,
+                                                                      (uint32_t)kNoPatch, (uint32_t)kNoPatch));
                                 }
                                 __syncwarp();
                             }
@@ -1099,6 +1153,8 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                     ent += 256 * p.n_top;
                     lw.e = window_entry(lw, ent, lane);
                 }
+                if (!WPASS) nr = {next_named.x, next_named.y, next_named.w,
+                                  named_entry(named_ent, next_named.x + lane, next_named.w)};
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
@@ -1368,7 +1424,8 @@ __device__ __forceinline__ void store_rows(T* x, long long row0, long long rows,
 }
 
 // A row's labels in a group of 8 lanes: their shares q into shared memory as (class or -1, q), and
-// sum_i q_i log q_i. False when the row has none (it is then ignored), or none is asked for.
+// sum_i q_i log q_i; a share may round to zero. False when the row has none (it is then ignored), or
+// none is asked for.
 __device__ __forceinline__ bool group_labels(const LossLabels& L, long long row, bool live, int s, int2* ent, float& entropy) {
     entropy = 0.0f;
     if (L.target) {
@@ -1403,7 +1460,7 @@ __device__ __forceinline__ bool group_labels(const LossLabels& L, long long row,
         const float u = __int_as_float(ent[e].y) - top, q = expf(u) / sum;
         // (a share that rounds to zero holds the row to nothing)
         if (q != 0.0f) h = fmaf(q, u - log_sum, h);
-        ent[e] = make_int2(q != 0.0f ? ent[e].x : -1, __float_as_int(q));
+        ent[e] = make_int2(ent[e].x, __float_as_int(q));
     }
     entropy = group_sum(h);
     __syncwarp();
@@ -1411,12 +1468,12 @@ __device__ __forceinline__ bool group_labels(const LossLabels& L, long long row,
 }
 
 // Rows l0 .. l0 + R - 1 of the units u0 .. u0 + ns - 1's partial tiles [feat][128], weighted and
-// added in the units' order, into os [R][feat + 1] times inv[row]. A thread owns one row and every
+// added in the units' order, into os [R][feat + 1]. A thread owns one row and every
 // (NT / R)-th feature, and keeps all of its features' loads of a unit in flight: with few rows the
 // work is split over many units, and their latency is what this join costs.
 template <int R, int NT, bool WEIGHTED>
 __device__ __forceinline__ void join_units(const float* part_o, size_t u0, int ns, int feat, int l0, const float* wgt,
-                                           const float* inv, float* os) {
+                                           float* os) {
     constexpr int kStep = NT / R, kPer = 128 / kStep;
     const int r = threadIdx.x % R, f0 = threadIdx.x / R;
     float a[kPer];
@@ -1430,18 +1487,23 @@ __device__ __forceinline__ void join_units(const float* part_o, size_t u0, int n
         for (int i = 0; i < kPer; ++i)
             if (f0 + i * kStep < feat) a[i] = fmaf(chain_load(po + (size_t)i * kStep * 128), w, a[i]);
     }
-    const float k = WEIGHTED ? inv[r] : 1.0f;
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
-        if (f0 + i * kStep < feat) os[r * (feat + 1) + f0 + i * kStep] = a[i] * k;
+        if (f0 + i * kStep < feat) os[r * (feat + 1) + f0 + i * kStep] = a[i];
 }
 
 }  // namespace
 
-// One block per R rows (32; 8 where that leaves most SMs idle, and then of 512 threads where there
-// are fewer blocks than SMs: each joins many units, 13.9 -> 11.6 us for 120 rows of 49 units). Joins the class ranges of a row
-// block (the largest offset, the sums and mean weight rows brought to it); then 8 lanes per row: the
-// labels' logits as f32 products, the loss, and dx = T g (sum_j p_j W_j - sum_i q_i W_ci).
+// One block per R rows (32; 8 where that leaves most SMs idle, and then of 512 threads where there are
+// fewer blocks than SMs: each joins many units). Joins the class ranges of a row block (the largest
+// offset, the sums and weighted rows brought to it: U and O over the classes that the row does not
+// name); then 8 lanes per row: the labels' logits z_i as f32 products, e_i = 2^(z_i - M), S = U + sum_i
+// e_i, lse = M + log S, the labels' gradients f (e_i / S - q_i), the loss, and
+// dx = f (O / S + sum_i (e_i / S - q_i) W_ci).
+// Where one label holds the row, e / S - q is the difference of two numbers near 1. It is taken, for
+// the entry with the largest share, as (e_t (1 - q_t) - q_t (S - e_t)) / S with both differences summed
+// from the other entries; a single entry (q = 1) so has -U / S, and its loss log(1 + U / e), to f32's
+// precision of themselves.
 template <bool F32, int R, int NT>
 __global__ void __launch_bounds__(NT, NT == 256 ? 3 : 1) loss_rows_kernel(const __grid_constant__ LossRowParams p) {
     using T = typename Elem<F32>::type;
@@ -1450,10 +1512,12 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 3 : 1) loss_rows_kernel(const 
     float* os = xs + R * (p.k + 1);                           // [R][feat + 1]
     float* wgt = os + R * (p.feat + 1);                       // [n_splits][R]
     int2* ents = reinterpret_cast<int2*>(wgt + R * p.n_splits);  // [R][n_top] (R is even: 8-byte aligned)
+    float* zs = reinterpret_cast<float*>(ents + R * p.lab.n_top);  // [R][n_top]: z_i, then e_i / S - q_i
+    int* places = reinterpret_cast<int*>(zs + R * p.lab.n_top);    // [R][n_top]: sp_pos
     constexpr int kG = NT / R;                 // threads that share a row's ranges
     constexpr int kRun = F32 ? 4 : 8;
     __shared__ float red[kG][R];
-    __shared__ float s_lse2[R], s_inv[R];
+    __shared__ float s_off[R], s_sum[R];
     const int tid = threadIdx.x;
     launch_next();
     wait_previous();
@@ -1468,18 +1532,20 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 3 : 1) loss_rows_kernel(const 
     if (ns == 1) {
         // one unit has the whole class range: nothing to join
         const float2 ms = chain_load(p.part_ms + u0 * 128 + l0 + jr);
-        if (jg == 0) s_lse2[jr] = (ms.x == -CUDART_INF_F ? 0.0f : ms.x) + log2f(ms.y);
+        if (jg == 0) {
+            s_off[jr] = ms.x;
+            s_sum[jr] = ms.y;
+        }
         if (p.dx) {
             constexpr int kPer = 128 / kG;
             const float* po = p.part_o + u0 * p.feat * 128 + l0 + jr;
-            const float inv = 1.0f / ms.y;
             float a[kPer];
 #pragma unroll
             for (int i = 0; i < kPer; ++i)
                 a[i] = jg + i * kG < p.feat ? chain_load(po + (size_t)(jg + i * kG) * 128) : 0.0f;
 #pragma unroll
             for (int i = 0; i < kPer; ++i)
-                if (jg + i * kG < p.feat) os[jr * (p.feat + 1) + jg + i * kG] = a[i] * inv;
+                if (jg + i * kG < p.feat) os[jr * (p.feat + 1) + jg + i * kG] = a[i];
         }
     } else {
         float m = -CUDART_INF_F;
@@ -1506,11 +1572,11 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 3 : 1) loss_rows_kernel(const 
             sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < kG; ++i) sum += red[i][jr];
-            s_lse2[jr] = m0 + log2f(sum);
-            s_inv[jr] = 1.0f / sum;
+            s_off[jr] = m;
+            s_sum[jr] = sum;
         }
         __syncthreads();
-        if (p.dx) join_units<R, NT, true>(p.part_o, u0, ns, p.feat, l0, wgt, s_inv, os);
+        if (p.dx) join_units<R, NT, true>(p.part_o, u0, ns, p.feat, l0, wgt, os);
     }
     xv.put(p.k, p.t_len, xs);
     __syncthreads();
@@ -1520,32 +1586,26 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 3 : 1) loss_rows_kernel(const 
         const long long row = row0 + r;
         const bool live = row < p.rows;
         int2* ent = ents + r * p.lab.n_top;
+        float* zr = zs + r * p.lab.n_top;
+        int* place = places + r * p.lab.n_top;
+        for (int e = s; live && e < p.lab.n_top; e += 8) place[e] = chain_load(p.sp_pos + row * p.lab.n_top + e);
+        const float f_scaled = F32 ? chain_load(p.row_tab + (size_t)(row >> 7) * 256 + 128 + (row & 127)) : 0.0f;
         float entropy;
         const bool valid = group_labels(p.lab, row, live, s, ent, entropy);
         const float f = live ? p.lab.temp * (p.row_grad ? p.row_grad[row] : 1.0f) : 0.0f;
-        const float lse2 = s_lse2[r], lse = lse2 * kLn2;
-        if (s == 0) {
-            float e = -CUDART_INF_F;  // no share of anything
-            if (valid) e = F32 ? -lse2 : log2f(fabsf(f)) - lse2;
-            p.row_tab[(size_t)(row >> 7) * 256 + (row & 127)] = e;
-        }
         float* xr = xs + r * (p.k + 1);
-        float2 x[8], d[8];
+        float2 x[8];
         shared_row<kRun>(xr, p.k, s, x);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] = make_float2(0.f, 0.f);
-        if (p.dx) shared_row<kRun>(os + r * (p.feat + 1), p.k, s, d);
-        float zq = 0.0f;  // sum_i q_i (z_i - lse)
+
+        // the labels' logits in log2 units over T, rounded as the scores are
         constexpr int kBatch = 2;
         for (int e0 = 0; e0 < p.lab.n_top; e0 += kBatch) {
             int c[kBatch];
-            float q[kBatch], b[kBatch], z[kBatch];
+            float b[kBatch], z[kBatch];
             WeightRow<F32> w[kBatch];
 #pragma unroll
             for (int j = 0; j < kBatch; ++j) {
-                const int2 en = valid && e0 + j < p.lab.n_top ? ent[e0 + j] : make_int2(-1, 0);
-                c[j] = en.x;
-                q[j] = __int_as_float(en.y);
+                c[j] = valid && e0 + j < p.lab.n_top ? ent[e0 + j].x : -1;
                 b[j] = 0.0f;
                 if (c[j] >= 0) {
                     w[j].fetch(p.w, c[j], p.k, s, vec);
@@ -1567,20 +1627,128 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 3 : 1) loss_rows_kernel(const 
                 for (int j = 0; j < kBatch; ++j) z[j] += __shfl_xor_sync(0xffffffffu, z[j], o);
             }
 #pragma unroll
-            for (int j = 0; j < kBatch; ++j) {
-                if (c[j] < 0) continue;
-                zq = fmaf(q[j], fmaf(z[j] + b[j], p.lab.inv_temp, -lse), zq);
-                const float2 nq = make_float2(-q[j], -q[j]);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) d[i] = __ffma2_rn(nq, w[j].pair(i), d[i]);
+            for (int j = 0; j < kBatch; ++j)
+                if (s == 0 && e0 + j < p.lab.n_top)
+                    zr[e0 + j] = p.slots ? (z[j] + b[j]) * p.logit_scale
+                                         : fmaf(z[j], p.logit_scale, b[j] * p.logit_scale);
+        }
+        __syncwarp();
+
+        // the row's sum, from the classes that it does not name (U, relative to off) and its labels.
+        // A class named again keeps its first entry, with both shares.
+        float kl2 = 0.0f, q_top = -1.0f, z_max = -CUDART_INF_F;
+        int top = p.lab.n_top, count = 0;
+        for (int e = s; e < p.lab.n_top; e += 8) {
+            if (!valid || ent[e].x < 0) continue;
+            ++count;
+            z_max = fmaxf(z_max, zr[e]);
+        }
+        count = __reduce_add_sync(0xffu << (tid & 24), count);
+        z_max = group_max(z_max);
+        const float off = s_off[r];
+        const float m = fmaxf(off, z_max), m0 = m == -CUDART_INF_F ? 0.0f : m;
+        const float scale_u = off == -CUDART_INF_F ? 0.0f : ex2_approx(off - m0);
+        const float u_sum = s_sum[r] * scale_u;
+        bool again = false;
+        for (int e = s; e < p.lab.n_top; e += 8) {
+            if (!valid || ent[e].x < 0) continue;
+            if (place[e] < 0) again = true;
+        }
+        if (__any_sync(0xffffffffu, again)) {
+            for (int e = s; e < p.lab.n_top; e += 8) {
+                const int2 en = ent[e];
+                if (!valid || en.x < 0 || place[e] < 0) continue;
+                float q = __int_as_float(en.y);
+                for (int j = 0; j < p.lab.n_top; ++j)  // (only entries that stay are written, only others read)
+                    if (j != e && ent[j].x == en.x) q += __int_as_float(ent[j].y);
+                ent[e].y = __float_as_int(q);
+            }
+            __syncwarp();
+            for (int e = s; e < p.lab.n_top; e += 8)
+                if (valid && ent[e].x >= 0 && place[e] < 0) ent[e].x = -1;
+            __syncwarp();
+        }
+        for (int e = s; e < p.lab.n_top; e += 8) {
+            if (!valid || ent[e].x < 0) continue;
+            const float q = __int_as_float(ent[e].y);
+            if (q > q_top) {
+                q_top = q;
+                top = e;
             }
         }
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) {
+            const float oq = __shfl_xor_sync(0xffffffffu, q_top, o);
+            const int ot = __shfl_xor_sync(0xffffffffu, top, o);
+            if (oq > q_top || (oq == q_top && ot < top)) {
+                q_top = oq;
+                top = ot;
+            }
+        }
+        float e_rest = 0.0f, q_rest = 0.0f;
+        for (int e = s; e < p.lab.n_top; e += 8) {
+            if (!valid || ent[e].x < 0 || e == top) continue;
+            e_rest += ex2_approx(zr[e] - m0);
+            q_rest += __int_as_float(ent[e].y);
+        }
+        e_rest = group_sum(e_rest);
+        q_rest = group_sum(q_rest);
+        const float z_top = top < p.lab.n_top ? zr[top] : -CUDART_INF_F;
+        const float e_top = ex2_approx(z_top - m0), others = u_sum + e_rest, total = others + e_top;
+        const float inv = 1.0f / total, lse2 = m + log2f(total);
+        __syncwarp();
+        // the labels' gradients over f, and their part of the loss
+        const float fs = F32 ? f_scaled : f;
+        int2* tile_ent = p.sp_ent + (row >> 7) * 128 * p.lab.n_top;
+        for (int e = s; e < p.lab.n_top; e += 8) {
+            if (!valid || ent[e].x < 0) continue;
+            const float q = __int_as_float(ent[e].y), z = zr[e];
+            if (q != 0.0f) kl2 = fmaf(q, z - lse2, kl2);
+            const float d = e == top ? (e_top * q_rest - q * others) * inv : fmaf(ex2_approx(z - m0), inv, -q);
+            zr[e] = d;
+            tile_ent[place[e]].y = __float_as_int(fs * d);
+        }
+        kl2 = group_sum(kl2);
+        __syncwarp();
+        if (s == 0) {
+            float e = -CUDART_INF_F;  // no share of anything
+            if (valid) e = F32 ? -lse2 : log2f(fabsf(f)) - lse2;
+            p.row_tab[(size_t)(row >> 7) * 256 + (row & 127)] = e;
+        }
         if (live && s == 0) {
-            if (p.loss) p.loss[row] = valid ? (entropy - zq) * p.lab.temp * p.lab.temp : 0.0f;
-            if (p.lse) p.lse[row] = valid ? lse : 0.0f;
+            float loss = entropy - kl2 * kLn2;
+            if (count == 1 && q_top == 1.0f && z_top < CUDART_INF_F)  // one label: what the other classes leave
+                loss = z_top >= off ? log1pf(s_sum[r] * ex2_approx(off - z_top))
+                                    : (off - z_top) * kLn2 + logf(s_sum[r] + ex2_approx(z_top - off));
+            if (p.loss) p.loss[row] = valid ? loss * p.lab.temp * p.lab.temp : 0.0f;
+            if (p.lse) p.lse[row] = valid ? lse2 * kLn2 : 0.0f;
         }
         if (p.dx) {
-            __syncwarp();
+            float2 d[8];
+            shared_row<kRun>(os + r * (p.feat + 1), p.k, s, d);
+            const float2 ku = make_float2(scale_u * inv, scale_u * inv);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) d[i] = __fmul2_rn(d[i], ku);
+            for (int e0 = 0; e0 < p.lab.n_top; e0 += kBatch) {
+                WeightRow<F32> w[kBatch];
+                float2 g[kBatch];
+#pragma unroll
+                for (int j = 0; j < kBatch; ++j) {
+                    const int c = valid && e0 + j < p.lab.n_top ? ent[e0 + j].x : -1;
+                    g[j] = make_float2(0.f, 0.f);
+                    if (c >= 0) {
+                        w[j].fetch(p.w, c, p.k, s, vec);
+                        g[j].x = g[j].y = zr[e0 + j];
+                    } else {
+                        w[j].clear();
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < kBatch; ++j) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) d[i] = __ffma2_rn(g[j], w[j].pair(i), d[i]);
+                }
+            }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int k0 = lane_slot<kRun>(s, 2 * i);
@@ -1604,7 +1772,7 @@ __global__ void __launch_bounds__(256) loss_reduce_kernel(const __grid_constant_
     const int j0 = (int)blockIdx.x * R, tile = j0 >> 7, l0 = j0 & 127;
     const int ns = tile < p.whole_units ? 1 : p.n_splits;
     const size_t u0 = tile < p.whole_units ? (size_t)tile : (size_t)p.whole_units + (size_t)(tile - p.whole_units) * p.n_splits;
-    join_units<R, 256, false>(p.part_o, u0, ns, p.feat, l0, nullptr, nullptr, sm);
+    join_units<R, 256, false>(p.part_o, u0, ns, p.feat, l0, nullptr, sm);
     if (p.db && threadIdx.x < R && j0 + (int)threadIdx.x < p.n) {
         float a = 0.0f;
         for (int s = 0; s < ns; ++s) a += chain_load(p.part_ms + (u0 + s) * 128 + l0 + threadIdx.x).x;
@@ -1757,7 +1925,7 @@ __global__ void __launch_bounds__(256) loss_score_kernel(const __grid_constant__
 #pragma unroll 2
     for (int e = 0; e < p.lab.n_top; ++e) {
         const int2 c = ent[e];
-        const bool here = valid && c.x >= 0;
+        const bool here = valid && c.x >= 0 && __int_as_float(c.y) != 0.0f;
         const float z = logit(here ? c.x : 0);
         if (here) zq = fmaf(__int_as_float(c.y), z - lse, zq);
     }
@@ -1771,14 +1939,14 @@ __global__ void __launch_bounds__(256) loss_score_kernel(const __grid_constant__
 namespace {
 // (counts, starts, entries; the norms' four partial sums)
 constexpr int pack_smem_bytes(int w_tiles, int n_top) {
-    return 4 * w_tiles * (2 * kPackWarps + 4) + 128 * n_top * 8;
+    return 4 * w_tiles * (2 * kPackWarps + 4) + 128 * n_top * 4;
 }
 constexpr int kPackSmemMax = pack_smem_bytes(kLossMaxClasses / 128, kLossMaxTop) + 2048;
 static_assert(kPackSmemMax <= 226 * 1024, "shared memory per block");
 int rows_smem_bytes(int r, int k, int feat, int n_splits, int n_top) {
-    return r * ((k + 1 + feat + 1 + n_splits) * 4 + n_top * 8);
+    return r * ((k + 1 + feat + 1 + n_splits) * 4 + n_top * 16);
 }
-constexpr int kRowsSmemMax = 32 * ((2 * 129 + kLossMaxSplits) * 4 + kLossMaxTop * 8);
+constexpr int kRowsSmemMax = 32 * ((2 * 129 + kLossMaxSplits) * 4 + kLossMaxTop * 16);
 int score_smem_bytes(int k, int n_top) { return kLossRows * ((k + 1) * 4 + n_top * 8); }
 // Blocks of 32 rows would leave SMs idle: four times as many of 8.
 bool few_blocks(int tiles, int sms) { return tiles * (kLossTile / 32) < 2 * sms; }
@@ -1827,7 +1995,7 @@ cudaError_t launch_chained(void (*kernel)(P), int grid, int threads, int smem, c
 
 cudaError_t launch_loss_pack(const LossPackParams& p, bool f32, cudaStream_t stream) {
     const int grid = p.w_tiles + p.x_tiles;
-    const int labels = p.sort_labels ? pack_smem_bytes(p.w_tiles, p.lab.n_top) : 0;
+    const int labels = pack_smem_bytes(p.w_tiles, p.lab.n_top);
     LossPackParams q = p;
     q.norm_smem = (labels + 3) / 4;
     const int smem = 4 * q.norm_smem + (p.slots && p.t_len > 0 ? 2048 : 0);

@@ -29,7 +29,7 @@ struct LossLabels {
 };
 
 // Operand tiles of a training step: features and weight as tensor-core images, the class table,
-// the rows' gradient factors and, for the weight's gradient, the labels sorted by class tile.
+// the rows' gradient factors and the labels sorted by class tile.
 struct LossPackParams {
     const void* x;             // [rows][k], or [rows / t_len][k][t_len] (t_len > 0)
     const void* w;             // [n][k]
@@ -39,7 +39,6 @@ struct LossPackParams {
     long long rows, t_len;
     int k, x_tiles, w_tiles;
     float logit_scale;         // log2(e) / T
-    int sort_labels;           // fill sp_off / sp_ent (the weight's gradient is wanted)
     uint8_t* x_img;            // x_tiles images (f32: high image, then low image)
     uint8_t* w_img;
     float* x_scale;            // [x_tiles] value of one unit of the image (f32; a power of two)
@@ -56,7 +55,10 @@ struct LossPackParams {
     float2* w_bound;           // slots: [w_tiles] (largest |w_j|, largest bias in log2 units)
     int norm_smem;             // set by the launcher: first float of the norms' shared memory
     int2* sp_off;              // [x_tiles][4 w_tiles] label ranges (first, end) by 32 classes
-    int2* sp_ent;              // [x_tiles][128 n_top]: (row << 5 | class within its 32, factor bits)
+    int2* sp_ent;              // [x_tiles][128 n_top]: (row << 5 | class within its 32, bits of the gradient
+                               // dz, scaled as the factors; by the row kernel)
+    int* sp_pos;               // [x_tiles][128 n_top]: an entry's place in its tile's sp_ent; -1: absent, or
+                               // of a class that an earlier entry of the row names
     int* status;
 };
 
@@ -71,7 +73,7 @@ struct LossMainParams {
     const float* x_norm;       // row pass, slots
     const float2* w_bound;
     const float* g_scale;      // weight pass: per streamed tile
-    const int2* sp_off;        // weight pass
+    const int2* sp_off;
     const int2* sp_ent;
     int n_top;
     int own_tiles, str_tiles;
@@ -89,7 +91,8 @@ struct LossMainParams {
     unsigned long long timeout_ns;
 };
 
-// Rows of a training step after the row pass: loss, lse, the feature gradient and the row table.
+// Rows of a training step after the row pass: loss, lse, the feature gradient, the row table and the
+// labels' own gradients.
 struct LossRowParams {
     const void* x;
     const void* w;
@@ -99,8 +102,12 @@ struct LossRowParams {
     long long rows, t_len;
     int k, feat;
     int whole_units, n_splits;
+    float logit_scale;
+    int slots;                 // bias within the scores (bf16), or added to them in log2 units
     const float* part_o;
     const float2* part_ms;
+    const int* sp_pos;
+    int2* sp_ent;
     float* row_tab;
     float* loss;               // [rows] or null
     float* lse;                // [rows] or null

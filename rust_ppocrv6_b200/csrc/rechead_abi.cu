@@ -860,8 +860,8 @@ struct LossLayout {
     LossPlan row, cls;
     int x_tiles = 0, w_tiles = 0, feat = 0;
     bool slots = false;  // the bias rides in three spare K slots
-    size_t x_img, w_img, x_scale, w_scale, g_scale, class_e, row_tab, x_norm, w_bound, sp_off, sp_ent, part_o, part_ms,
-        total;
+    size_t x_img, w_img, x_scale, w_scale, g_scale, class_e, row_tab, x_norm, w_bound, sp_off, sp_ent, sp_pos, part_o,
+        part_ms, total;
 };
 LossLayout loss_layout(bool f32, int64_t rows, int64_t k, int64_t n, int64_t n_top, int sms) {
     LossLayout L;
@@ -891,6 +891,7 @@ LossLayout loss_layout(bool f32, int64_t rows, int64_t k, int64_t n, int64_t n_t
     L.w_bound = take(L.slots ? (size_t)L.w_tiles * 8 : 0);
     L.sp_off = take((size_t)L.x_tiles * (size_t)L.w_tiles * 4 * sizeof(int2));
     L.sp_ent = take((size_t)L.x_tiles * 128 * (size_t)n_top * 8);
+    L.sp_pos = take((size_t)L.x_tiles * 128 * (size_t)n_top * 4);
     L.part_o = take(units * (size_t)L.feat * 512);
     L.part_ms = take(units * 1024);
     L.total = at + 256;  // the caller's pointer is brought to a 256-byte boundary
@@ -967,7 +968,6 @@ int enqueue_grad(rh_ctx* ctx, Slot& s, int dtype, const void* d_a, int64_t rows,
     pk.x_tiles = L.x_tiles;
     pk.w_tiles = L.w_tiles;
     pk.logit_scale = logit_scale;
-    pk.sort_labels = d_dw ? 1 : 0;
     pk.x_img = ws + L.x_img;
     pk.w_img = ws + L.w_img;
     pk.x_scale = (float*)(ws + L.x_scale);
@@ -980,6 +980,7 @@ int enqueue_grad(rh_ctx* ctx, Slot& s, int dtype, const void* d_a, int64_t rows,
     pk.w_bound = (float2*)(ws + L.w_bound);
     pk.sp_off = (int2*)(ws + L.sp_off);
     pk.sp_ent = (int2*)(ws + L.sp_ent);
+    pk.sp_pos = (int*)(ws + L.sp_pos);
     pk.status = s.d_status;
     RH_CUDA(rh::launch_loss_pack(pk, f32, st));
     s.launches++;
@@ -992,6 +993,8 @@ int enqueue_grad(rh_ctx* ctx, Slot& s, int dtype, const void* d_a, int64_t rows,
     m.col_tab = pk.class_e;
     m.x_norm = pk.x_norm;
     m.w_bound = pk.w_bound;
+    m.sp_off = pk.sp_off;
+    m.sp_ent = pk.sp_ent;
     m.own_tiles = L.x_tiles;
     m.str_tiles = L.w_tiles;
     m.n_top = lab.n_top;
@@ -1026,6 +1029,10 @@ int enqueue_grad(rh_ctx* ctx, Slot& s, int dtype, const void* d_a, int64_t rows,
     r.n_splits = L.row.splits;
     r.part_o = m.part_o;
     r.part_ms = m.part_ms;
+    r.logit_scale = logit_scale;
+    r.slots = pk.slots;
+    r.sp_pos = pk.sp_pos;
+    r.sp_ent = pk.sp_ent;
     r.row_tab = pk.row_tab;
     r.loss = d_loss;
     r.lse = d_lse;
@@ -1041,8 +1048,6 @@ int enqueue_grad(rh_ctx* ctx, Slot& s, int dtype, const void* d_a, int64_t rows,
     m.col_tab = pk.row_tab;
     m.lane_e = pk.class_e;
     m.g_scale = pk.g_scale;
-    m.sp_off = pk.sp_off;
-    m.sp_ent = pk.sp_ent;
     m.own_tiles = L.w_tiles;
     m.str_tiles = L.x_tiles;
     m.whole_units = L.cls.whole;

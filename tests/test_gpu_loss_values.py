@@ -15,7 +15,7 @@ below 2^-38 of the largest of the 128 values they stand beside.
 import numpy as np
 import pytest
 
-from test_gpu_losses import check, cuda, definition, grad, make, packed, rounded
+from test_gpu_losses import BF, U, check, cuda, definition, grad, make, packed, rounded
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -34,6 +34,104 @@ def ctx(rh):
     c = rh.Context()
     yield c
     c.close()
+
+
+def confident(rows, k, n, seed, low=-5.0, high=-1.0):
+    """Targets with 1 - p spread over 10^low .. 10^high: noise on every class, and the target's own
+    weight row in the share that lifts its logit to there."""
+    g = np.random.default_rng(seed)
+    w = (0.5 / np.sqrt(k) * g.standard_normal((n, k))).astype(np.float32)
+    t = g.integers(0, n, rows)
+    t[g.random(rows) < 0.5] = 0
+    x = g.standard_normal((rows, k))
+    b = (0.01 * g.standard_normal(n)).astype(np.float32)
+    miss = 10.0 ** g.uniform(low, high, rows)
+    wt = w[t].astype(np.float64)
+    for _ in range(3):  # (the share moves the other logits too)
+        z = x @ w.T.astype(np.float64) + b
+        zt = z[np.arange(rows), t].copy()
+        z[np.arange(rows), t] = -np.inf
+        rest = np.log(np.exp(z - z.max(1, keepdims=True)).sum(1)) + z.max(1)
+        x += ((rest + np.log((1 - miss) / miss) - zt) / (wt ** 2).sum(1))[:, None] * wt
+    return {"x": x.astype(np.float32), "w": w, "b": b, "t": t.astype(np.int32),
+            "g": (g.choice([-1.0, 1.0], rows) * g.uniform(0.5, 1.5, rows) / rows).astype(np.float32)}
+
+
+def near_teacher(rows, k, n, n_top, seed, temp, spread=0.03):
+    """A student whose best classes' logits are the teacher's but for a few percent of a unit."""
+    d = confident(rows, k, n, seed, -4.0, 0.0)
+    d["x"] = torch.as_tensor(d["x"]).bfloat16().float().numpy()
+    d["w"] = torch.as_tensor(d["w"]).bfloat16().float().numpy()
+    z = d["x"].astype(np.float64) @ d["w"].T.astype(np.float64) + d["b"]
+    idx = np.argsort(-z, axis=1)[:, :n_top]
+    g = np.random.default_rng(seed + 1)
+    logits = np.take_along_axis(z, idx, 1) + temp * spread * g.standard_normal(idx.shape)
+    del d["t"]
+    return dict(d, idx=idx.astype(np.int32), logits=logits.astype(np.float32))
+
+
+def value_bounds(ref, bf16, several):
+    """Elementwise bounds of da, dw and db against |dz| (several: rows may have several labels)."""
+    rows, n = ref["x"].shape[0], ref["w"].shape[0]
+    tr, tc = (rows + 127) // 128, (n + 127) // 128
+    fp, fq, A, w, x = ref["fp"], ref["fq"], ref["A"][:, None], ref["w"].abs(), ref["x"].abs()
+    dz = (fp - fq).abs()
+    lab = fq > 0
+    own = 128 * U * A * dz
+    if several:
+        own = own + torch.where(lab, 128 * U * A * fp + 16 * U * (fp + fq) + 8 * U * A * fq, 0.0)
+    rnd = BF if bf16 else 0.0
+    e_da = (own + (80 + tc) * U * dz + rnd * torch.where(lab, 0.0, dz)) @ w
+    e_dw = (own + (80 + tr) * U * dz + rnd * dz).T @ x
+    e_db = (own + (32 + tr) * U * dz).sum(0)
+    if not bf16:
+        e_da = e_da + 2.0 ** -38 * torch.where(lab, 0.0, fp).amax(1, keepdim=True) * w.sum(0)
+        top = torch.cat([t.amax().expand(t.shape[0], 1) for t in dz.split(128)])
+        e_dw = e_dw + 2.0 ** -38 * (top * x).sum(0)
+    return {"da": e_da + rnd * (ref["da"].abs() + e_da), "dw": e_dw + rnd * (ref["dw"].abs() + e_dw), "db": e_db}
+
+
+def check_values(got, ref, bf16, several):
+    for name, bound in value_bounds(ref, bf16, several).items():
+        err = (got[name].double() - ref[name]).abs()
+        over = (err > bound) | torch.isnan(got[name].double())
+        assert not over.any(), (f"{name}: {int(over.sum())} of {over.numel()} beyond the bound, error / bound "
+                                f"{(err / bound.clamp(min=1e-300)).max():.3g}")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,k,n,t_len", [(384, 120, 18710, 0), (130, 80, 6906, 65),
+                                            (1300, 120, 1500, 0), (200, 128, 300, 0), (60, 17, 129, 20)])
+def test_gradients_of_confident_rows(rh, ctx, rows, k, n, t_len, dtype):
+    """p of the target from 0.9 to 0.99999: a trained head's rows."""
+    d = rounded(confident(rows, k, n, seed=rows + k), dtype)
+    ref = definition(d)
+    got = grad(rh, ctx, d, dtype, t_len=t_len)
+    check_values(got, ref, dtype == "bf16", False)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,k,n,n_top,temp", [(256, 120, 18710, 8, 2.0), (256, 80, 6906, 32, 1.0),
+                                                 (1200, 120, 2000, 3, 2.0), (40, 64, 129, 64, 4.0)])
+def test_gradients_of_a_student_near_its_teacher(rh, ctx, rows, k, n, n_top, temp, dtype):
+    d = near_teacher(rows, k, n, n_top, seed=rows + n, temp=temp)
+    ref = definition(d, temp)
+    check_values(grad(rh, ctx, d, dtype, temp), ref, dtype == "bf16", True)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [300, 18710])
+def test_losses_near_zero_keep_their_digits(rh, ctx, n, dtype):
+    """The loss of a confident row is what the other classes leave, down to 1 - p = 1e-9: within 128 u A
+    and (112 + tiles) u of itself (the sum over the tiles, the logarithm), and never negative."""
+    d = rounded(confident(200, 120, n, seed=5, low=-9.0, high=-1.0), dtype)
+    ref = definition(d)
+    p = ref["fq"] > 0
+    miss = torch.where(p, 0.0, ref["fp"] / ref["f"].abs()[:, None]).sum(1)
+    want = torch.log1p(miss / (1 - miss))
+    loss = grad(rh, ctx, d, dtype, want=("loss", "lse"))["loss"].double()
+    err = (loss - want).abs()
+    assert (loss >= 0).all() and not (err > want * (128 * U * ref["A"] + (112 + (n + 127) // 128) * U)).any(), float((err / want).max())
 
 
 @pytest.mark.parametrize("form", ["int8", "compact", "f32"])
