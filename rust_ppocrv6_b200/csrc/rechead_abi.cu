@@ -955,7 +955,7 @@ int enqueue_grad(rh_ctx* ctx, Slot& s, int dtype, const void* d_a, int64_t rows,
                  float* d_loss, float* d_lse, void* d_da, void* d_dw, float* d_dbias, uint8_t* ws, const LossLayout& L,
                  cudaStream_t st) {
     const bool f32 = dtype == RH_DTYPE_F32;
-    const float logit_scale = 1.4426950408889634f / lab.temp;
+    const float logit_scale = (float)(1.4426950408889634 / (double)lab.temp);
     rh::LossPackParams pk{};
     pk.x = d_a;
     pk.w = d_w;
@@ -1002,12 +1002,7 @@ int enqueue_grad(rh_ctx* ctx, Slot& s, int dtype, const void* d_a, int64_t rows,
     m.whole_units = L.row.whole;
     m.n_splits = L.row.splits;
     m.tiles_per_split = L.row.per;
-    // The tensor core's f32 accumulator rounds toward zero (measured: a logit of n full-size steps is
-    // short by 0.36 n 2^-23 of itself on average, which is half a last place averaged over a binade).
-    // The mean loss of the high parts' steps is given back with the scale; the low parts' are 2^-11 of
-    // it. Without it the errors of small f32 batches were 1.4 times as large, and one in four of them
-    // further from the exact gradients than f32 arithmetic.
-    m.logit_scale = (float)(1.4426950408889634 / (double)lab.temp * (1.0 + 0.36 * m.ksteps * 0x1p-23));
+    m.logit_scale = logit_scale;
     m.part_o = d_da ? (float*)(ws + L.part_o) : nullptr;
     m.part_ms = (float2*)(ws + L.part_ms);
     m.status = s.d_status;

@@ -134,6 +134,34 @@ def test_losses_near_zero_keep_their_digits(rh, ctx, n, dtype):
     assert (loss >= 0).all() and not (err > want * (128 * U * ref["A"] + (112 + (n + 127) // 128) * U)).any(), float((err / want).max())
 
 
+def exact_logits(rh, ctx, dtype):
+    """Rows of one feature: every product is exact and each of n classes has the row's z as its logit.
+    Returns z, n and the step's lse and loss."""
+    k, n = 120, 700
+    z = np.array([1, 3, 40, 96, 376, 1000, 1504, 3008, -3008, 12032], np.float64)
+    x, w = np.zeros((z.size, k), np.float32), np.zeros((n, k), np.float32)
+    x[:, 3], w[:, 3] = z / 8, 8.0
+    d = {"x": x, "w": w, "b": np.zeros(n, np.float32), "t": np.full(z.size, 5, np.int32), "g": np.ones(z.size, np.float32)}
+    got = grad(rh, ctx, d, dtype)
+    return z, n, got["lse"].double().cpu().numpy(), got["loss"].double().cpu().numpy()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_exact_logits_give_an_exact_sum(rh, ctx, dtype):
+    """lse = z + log n. Roundings on the way: z in log2 units (the factor and the product: 1.2 u |z|), the
+    offset (u |z|), the sum and its logarithm (16 u of a value below 16), the way back (2.2 u |lse|)."""
+    z, n, lse, _ = exact_logits(rh, ctx, dtype)
+    err = np.abs(lse - (z + np.log(n)))
+    assert (err <= 4.4 * U * np.abs(z) + 64 * U * np.log(n)).all(), err / (U * np.abs(z))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_exact_logits_give_an_exact_loss(rh, ctx, dtype):
+    """The loss is log n whatever z is: it is formed from differences of logits, which are zero."""
+    z, n, _, loss = exact_logits(rh, ctx, dtype)
+    assert (np.abs(loss - np.log(n)) <= 64 * U * np.log(n)).all(), loss - np.log(n)
+
+
 @pytest.mark.parametrize("form", ["int8", "compact", "f32"])
 @pytest.mark.parametrize("rows", [1, 200])
 def test_score_with_every_class_masked(rh, ctx, form, rows):
