@@ -396,10 +396,11 @@ int rh_head_distill_grad(rh_ctx *ctx, const float *a, int64_t rows, int64_t k, i
  * The classes that a row names have their logits and p - q in f32, whatever the type: a confident
  * row's gradient, and its loss, keep their digits however near 1 its probability is. bf16: products of
  * bf16 operands in f32, with the gradients dz rounded to bf16 for the second product (dw of up to
- * 1,024 rows, da over up to 1,024 classes: in two bf16 parts). f32: operands
- * split into two fp16 parts, 22 bits of each value and never finer than 2^-38
- * of the largest of its 128 rows: a value below 2^-16 of that largest one keeps fewer bits, else
- * results are as those of f32 arithmetic. n_top: entries per row (0 or 1 for cross entropy);
+ * 1,024 rows, da over up to 1,024 classes: in two bf16 parts). f32: operands (a, w, the
+ * probabilities and dz) split into two fp16 parts, 22 bits of each value and never finer than 2^-38 of
+ * the largest of its 128 rows (of dz: of the 128 rows' largest gradient of a logit; of the
+ * probabilities: of the row's largest that it does not name): a value below 2^-16 of that largest one
+ * keeps fewer bits, else results are as those of f32 arithmetic. n_top: entries per row (0 or 1 for cross entropy);
  * workspace bytes: -1 on bad arguments. */
 int64_t rh_head_grad_workspace_bytes(rh_ctx *ctx, int slot, int dtype, int64_t rows, int64_t k, int64_t n,
                                      int64_t n_top);

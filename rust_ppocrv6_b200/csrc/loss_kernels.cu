@@ -233,20 +233,14 @@ __global__ void __launch_bounds__(kPackThreads, 2) loss_pack_kernel(const __grid
         __syncthreads();
     }
     if (!is_w) {
-        float gs = 1.0f;  // scale of this tile's gradient factors
         const float f = tid < 128 ? s_norm[tid] : 0.0f;
         if (F32) {
-            const float m = warp_max(fabsf(f));
-            if (lane == 0) red[warp] = m;
-            __syncthreads();
-            const int sh = shift_to(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), 13);
-            gs = pow2i(sh);
-            if (tid == 0) p.g_scale[tile] = pow2i(-sh);
+            if (tid == 0) p.tile_done[tile] = 0;
         } else {
             const int neg = __syncthreads_or(f < 0.0f);
             if (tid == 0) p.g_scale[tile] = neg ? 1.0f : 0.0f;
         }
-        if (tid < 128) p.row_tab[(size_t)tile * 256 + 128 + tid] = F32 ? f * gs : copysignf(1.0f, f);
+        if (tid < 128) p.row_tab[(size_t)tile * 256 + 128 + tid] = F32 ? f : copysignf(1.0f, f);
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < kPackItems; ++i) {
@@ -1072,6 +1066,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                     sum = fmaf(sum, corr, t);
                 } else {
                     const float2 le = make_float2(lane_e, lane_e);
+                    const float gs_up = __uint_as_float(0x7f000000u - __float_as_uint(gs));  // f32: 1 / gs, a power of two
                     bool labelled = false;  // most tiles have none of a warp's classes
                     if (lw.next < lw.end) {
                         window_use(lw, ent, lane, (int)half);
@@ -1116,7 +1111,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                                         *reinterpret_cast<volatile float*>(
                                             gbase + (patch - base) +
                                             4u * ((uint32_t)(lw.e.x & 31) * kPatchRow + (uint32_t)((lw.e.x >> 5) & 7))) =
-                                            __int_as_float(lw.e.y);
+                                            F32 ? __int_as_float(lw.e.y) * gs_up : __int_as_float(lw.e.y);
                                 }
                                 if (group < lw.last) break;  // the window reaches beyond this group, or is the last
                                 lw.e = lw.n;
@@ -1518,6 +1513,8 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 3 : 1) loss_rows_kernel(const 
     constexpr int kRun = F32 ? 4 : 8;
     __shared__ float red[kG][R];
     __shared__ float s_off[R], s_sum[R];
+    __shared__ float s_top[R], s_factor[R];
+    __shared__ bool s_last;
     const int tid = threadIdx.x;
     launch_next();
     wait_previous();
@@ -1589,7 +1586,6 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 3 : 1) loss_rows_kernel(const 
         float* zr = zs + r * p.lab.n_top;
         int* place = places + r * p.lab.n_top;
         for (int e = s; live && e < p.lab.n_top; e += 8) place[e] = chain_load(p.sp_pos + row * p.lab.n_top + e);
-        const float f_scaled = F32 ? chain_load(p.row_tab + (size_t)(row >> 7) * 256 + 128 + (row & 127)) : 0.0f;
         float entropy;
         const bool valid = group_labels(p.lab, row, live, s, ent, entropy);
         const float f = live ? p.lab.temp * (p.row_grad ? p.row_grad[row] : 1.0f) : 0.0f;
@@ -1698,7 +1694,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 3 : 1) loss_rows_kernel(const 
         const float inv = 1.0f / total, lse2 = m + log2f(total);
         __syncwarp();
         // the labels' gradients over f, and their part of the loss
-        const float fs = F32 ? f_scaled : f;
+        float largest = u_sum * inv;
         int2* tile_ent = p.sp_ent + (row >> 7) * 128 * p.lab.n_top;
         for (int e = s; e < p.lab.n_top; e += 8) {
             if (!valid || ent[e].x < 0) continue;
@@ -1706,10 +1702,16 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 3 : 1) loss_rows_kernel(const 
             if (q != 0.0f) kl2 = fmaf(q, z - lse2, kl2);
             const float d = e == top ? (e_top * q_rest - q * others) * inv : fmaf(ex2_approx(z - m0), inv, -q);
             zr[e] = d;
-            tile_ent[place[e]].y = __float_as_int(fs * d);
+            largest = fmaxf(largest, fabsf(d));
+            tile_ent[place[e]].y = __float_as_int(f * d);
         }
         kl2 = group_sum(kl2);
+        largest = group_max(largest);
         __syncwarp();
+        if (F32 && s == 0) {
+            s_top[r] = valid ? fabsf(f) * largest : 0.0f;
+            s_factor[r] = valid ? fabsf(f) : 0.0f;
+        }
         if (s == 0) {
             float e = -CUDART_INF_F;  // no share of anything
             if (valid) e = F32 ? -lse2 : log2f(fabsf(f)) - lse2;
@@ -1757,9 +1759,37 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 3 : 1) loss_rows_kernel(const 
             }
         }
     }
-    if (!p.dx) return;
-    __syncthreads();
-    store_rows<R, NT>(static_cast<T*>(p.dx), row0, p.rows, p.k, p.t_len, xs);
+    if (F32 || p.dx) __syncthreads();
+    if (p.dx) store_rows<R, NT>(static_cast<T*>(p.dx), row0, p.rows, p.k, p.t_len, xs);
+    if constexpr (F32) {
+        // The scale of a tile's gradients: its largest comes to 2^13, so that the weight pass's fp16 pairs
+        // hold down to 2^-38 of it (of the largest factor f alone, the gradients that confident rows leave
+        // would be below the pairs' last step). The last of a tile's blocks knows it.
+        if (tid < 32) {
+            const float t = warp_max(tid < R ? s_top[tid] : 0.0f), g = warp_max(tid < R ? s_factor[tid] : 0.0f);
+            if (tid == 0) {
+                p.tile_top[(size_t)mb * kLossTopSlots + l0 / R] = make_float2(t, g);
+                __threadfence();
+                s_last = atomicAdd(p.tile_done + mb, 1) == kLossTile / R - 1;
+            }
+        }
+        __syncthreads();
+        if (!s_last) return;
+        __threadfence();
+        if (tid >= kLossTile) return;
+        float t = 0.0f, g = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kLossTile / R; ++i) {
+            const float2 v = chain_load(p.tile_top + (size_t)mb * kLossTopSlots + i);
+            t = fmaxf(t, v.x);
+            g = fmaxf(g, v.y);
+        }
+        // (times the features' scale it must stay a normal number, and the factors themselves finite)
+        const int sh = min(min(shift_to(t, 13), 96), shift_to(g, 100));
+        float* factor = p.row_tab + (size_t)mb * 256 + 128 + tid;
+        *factor = chain_load(factor) * pow2i(sh);
+        if (tid == 0) p.g_scale[mb] = pow2i(-sh);
+    }
 }
 
 // One block per R classes (32, or 8 as above): the row ranges' partial sums added in their order,

@@ -11,6 +11,7 @@ constexpr int kLossImage = 128 * 128 * 2;  // one 16-bit tile image: 128 rows x 
 constexpr int kLossMaxTop = 64;           // teacher entries per row
 constexpr int kLossMaxClasses = 1 << 17;  // labels are counted by 32 classes in shared memory (4,096 bins)
 constexpr int kLossRows = 32;             // rows per block of the score kernel
+constexpr int kLossTopSlots = 16;         // blocks of the row kernel per tile at most
 constexpr int kLossMaxSplits = 148;       // ranges that an own tile's work is split into at most
 // Device status bit (status[0], beside kDevTimeout and kDevRecPlan): a target or teacher class
 // at or above the class count; the row or entry was taken as absent.
@@ -45,10 +46,11 @@ struct LossPackParams {
     float* w_scale;            // [w_tiles]
     float* class_e;            // [w_tiles][128] bias * log2(e) / T; padding classes -inf
     float* row_tab;            // [x_tiles][256]. f32: 128 x (-lse, log2 units; written by the row kernel),
-                               // 128 x gradient factor scaled by the tile's power of two. bf16: 128 x
+                               // 128 x gradient factor, scaled by the row kernel to g_scale's unit. bf16: 128 x
                                // (log2 |factor| - lse; by the row kernel), 128 x the factor's sign
-    float* g_scale;            // [x_tiles] f32: value of one unit of the tile's gradient factors; bf16: 1
-                               // where a factor is negative, else 0
+    float* g_scale;            // [x_tiles] f32: value of one unit of the tile's gradients (a power of two; by
+                               // the row kernel); bf16: 1 where a factor is negative, else 0
+    int* tile_done;            // [x_tiles] f32: blocks of the row kernel that are done, set to 0
     int slots;                 // bf16, k <= 125: K slots k..k+2 hold the bias in three parts (weight) and 1
                                // (features), so that the scores come with their bias
     float* x_norm;             // slots: [x_tiles][128] |x_r|
@@ -56,7 +58,7 @@ struct LossPackParams {
     int norm_smem;             // set by the launcher: first float of the norms' shared memory
     int2* sp_off;              // [x_tiles][4 w_tiles] label ranges (first, end) by 32 classes
     int2* sp_ent;              // [x_tiles][128 n_top]: (row << 5 | class within its 32, bits of the gradient
-                               // dz, scaled as the factors; by the row kernel)
+                               // dz; by the row kernel)
     int* sp_pos;               // [x_tiles][128 n_top]: an entry's place in its tile's sp_ent; -1: absent, or
                                // of a class that an earlier entry of the row names
     int* status;
@@ -108,6 +110,9 @@ struct LossRowParams {
     const float2* part_ms;
     const int* sp_pos;
     int2* sp_ent;
+    float2* tile_top;          // [x_tiles][kLossTopSlots] f32: a block's largest |dz| and |factor|
+    int* tile_done;
+    float* g_scale;
     float* row_tab;
     float* loss;               // [rows] or null
     float* lse;                // [rows] or null

@@ -860,8 +860,8 @@ struct LossLayout {
     LossPlan row, cls;
     int x_tiles = 0, w_tiles = 0, feat = 0;
     bool slots = false;  // the bias rides in three spare K slots
-    size_t x_img, w_img, x_scale, w_scale, g_scale, class_e, row_tab, x_norm, w_bound, sp_off, sp_ent, sp_pos, part_o,
-        part_ms, total;
+    size_t x_img, w_img, x_scale, w_scale, g_scale, class_e, row_tab, x_norm, w_bound, tile_top, tile_done, sp_off, sp_ent,
+        sp_pos, part_o, part_ms, total;
 };
 LossLayout loss_layout(bool f32, int64_t rows, int64_t k, int64_t n, int64_t n_top, int sms) {
     LossLayout L;
@@ -889,6 +889,8 @@ LossLayout loss_layout(bool f32, int64_t rows, int64_t k, int64_t n, int64_t n_t
     L.row_tab = take((size_t)L.x_tiles * 1024);
     L.x_norm = take(L.slots ? (size_t)L.x_tiles * 512 : 0);
     L.w_bound = take(L.slots ? (size_t)L.w_tiles * 8 : 0);
+    L.tile_top = take(f32 ? (size_t)L.x_tiles * rh::kLossTopSlots * sizeof(float2) : 0);
+    L.tile_done = take(f32 ? (size_t)L.x_tiles * 4 : 0);
     L.sp_off = take((size_t)L.x_tiles * (size_t)L.w_tiles * 4 * sizeof(int2));
     L.sp_ent = take((size_t)L.x_tiles * 128 * (size_t)n_top * 8);
     L.sp_pos = take((size_t)L.x_tiles * 128 * (size_t)n_top * 4);
@@ -975,6 +977,7 @@ int enqueue_grad(rh_ctx* ctx, Slot& s, int dtype, const void* d_a, int64_t rows,
     pk.class_e = (float*)(ws + L.class_e);
     pk.row_tab = (float*)(ws + L.row_tab);
     pk.g_scale = (float*)(ws + L.g_scale);
+    pk.tile_done = (int*)(ws + L.tile_done);
     pk.slots = L.slots ? 1 : 0;
     pk.x_norm = (float*)(ws + L.x_norm);
     pk.w_bound = (float2*)(ws + L.w_bound);
@@ -1028,6 +1031,9 @@ int enqueue_grad(rh_ctx* ctx, Slot& s, int dtype, const void* d_a, int64_t rows,
     r.slots = pk.slots;
     r.sp_pos = pk.sp_pos;
     r.sp_ent = pk.sp_ent;
+    r.tile_top = (float2*)(ws + L.tile_top);
+    r.tile_done = pk.tile_done;
+    r.g_scale = pk.g_scale;
     r.row_tab = pk.row_tab;
     r.loss = d_loss;
     r.lse = d_lse;

@@ -100,7 +100,7 @@ def check_values(got, ref, bf16, several):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("rows,k,n,t_len", [(384, 120, 18710, 0), (130, 80, 6906, 65),
+@pytest.mark.parametrize("rows,k,n,t_len", [(384, 120, 18710, 0), (130, 80, 6906, 65), (1, 120, 18710, 0),
                                             (1300, 120, 1500, 0), (200, 128, 300, 0), (60, 17, 129, 20)])
 def test_gradients_of_confident_rows(rh, ctx, rows, k, n, t_len, dtype):
     """p of the target from 0.9 to 0.99999: a trained head's rows."""
@@ -111,7 +111,7 @@ def test_gradients_of_confident_rows(rh, ctx, rows, k, n, t_len, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("rows,k,n,n_top,temp", [(256, 120, 18710, 8, 2.0), (256, 80, 6906, 32, 1.0),
+@pytest.mark.parametrize("rows,k,n,n_top,temp", [(256, 120, 18710, 8, 2.0), (256, 80, 6906, 32, 1.0), (1, 120, 700, 4, 1.0),
                                                  (1200, 120, 2000, 3, 2.0), (40, 64, 129, 64, 4.0)])
 def test_gradients_of_a_student_near_its_teacher(rh, ctx, rows, k, n, n_top, temp, dtype):
     d = near_teacher(rows, k, n, n_top, seed=rows + n, temp=temp)
@@ -160,6 +160,23 @@ def test_exact_logits_give_an_exact_loss(rh, ctx, dtype):
     """The loss is log n whatever z is: it is formed from differences of logits, which are zero."""
     z, n, _, loss = exact_logits(rh, ctx, dtype)
     assert (np.abs(loss - np.log(n)) <= 64 * U * np.log(n)).all(), loss - np.log(n)
+
+
+def test_weight_gradient_of_unnamed_classes_in_confident_tiles(rh, ctx):
+    """f32, every row with 1 - p near 1e-9: the classes that no row names have gradients of 1e-13 of a row's
+    weight, and keep their digits (each class row by itself, against its own size)."""
+    d = confident(256, 120, 18710, seed=8, low=-9.2, high=-8.8)
+    ref = definition(d)
+    got = grad(rh, ctx, d)
+    named = ref["fq"].sum(0) > 0
+    dz = (ref["fp"] - ref["fq"]).abs()
+    bound = ((128 * U * ref["A"][:, None] + 82 * U) * dz).T @ ref["x"].abs()
+    top = torch.cat([t.amax().expand(t.shape[0], 1) for t in dz.split(128)])
+    bound = bound + 2.0 ** -38 * (top * ref["x"].abs()).sum(0)
+    err = (got["dw"].double() - ref["dw"]).abs()[~named]
+    assert not (err > bound[~named]).any(), float((err / bound[~named]).max())
+    size = ref["dw"][~named].norm(dim=1)
+    assert ((got["dw"].double() - ref["dw"])[~named].norm(dim=1) <= 1e-3 * size).all()
 
 
 @pytest.mark.parametrize("form", ["int8", "compact", "f32"])
