@@ -258,11 +258,11 @@ __global__ void __launch_bounds__(kPackThreads, 2) loss_pack_kernel(const __grid
     // ---- scale and images
     float up = 1.0f;
     if (F32) {
-        float top = 0.0f;
+        float top = 0.0f;  // of the finite values: an infinity is its own row's alone
 #pragma unroll
         for (int i = 0; i < kPackItems; ++i) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[i][j]));
+            for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[i][j]) <= CUDART_MAX_NORMAL_F ? fabsf(v[i][j]) : 0.0f);
         }
         top = warp_max(top);
         if (lane == 0) red[warp] = top;

@@ -179,6 +179,25 @@ def test_weight_gradient_of_unnamed_classes_in_confident_tiles(rh, ctx):
     assert ((got["dw"].double() - ref["dw"])[~named].norm(dim=1) <= 1e-3 * size).all()
 
 
+@pytest.mark.parametrize("exp", [-14, 0, 17])
+@pytest.mark.parametrize("what", [np.inf, -np.inf, np.nan])
+def test_a_row_that_is_not_finite_keeps_to_itself(rh, ctx, what, exp):
+    """f32: one infinity or NaN in a counted row; the rows beside it are as their definition."""
+    d = make(200, 60, 300, seed=61, ignored=0.0)
+    d["x"], d["w"] = d["x"] * np.float32(2.0 ** exp), d["w"] * np.float32(2.0 ** -exp)
+    ref = definition(d)
+    x = d["x"].copy()
+    x[17, 5] = what
+    got = grad(rh, ctx, dict(d, x=x))
+    others = torch.arange(200, device="cuda") != 17
+    got = {i: got[i][others] for i in ("loss", "lse", "da")}
+    whole = {i: torch.zeros_like(ref[i]) for i in got}
+    for i in got:
+        whole[i][others] = got[i].double()
+        whole[i][17] = ref[i][17]
+    check(whole, ref, False, ("loss", "lse", "da"))
+
+
 @pytest.mark.parametrize("form", ["int8", "compact", "f32"])
 @pytest.mark.parametrize("rows", [1, 200])
 def test_score_with_every_class_masked(rh, ctx, form, rows):
