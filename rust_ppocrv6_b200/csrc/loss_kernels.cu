@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kPackThreads, 2) loss_pack_kernel(const __grid
                 }
                 g = p.row_grad ? p.row_grad[row] : 1.0f;
             }
-            if (bad) atomicOr(p.status, kDevBadClass);
+            if (bad) atomicOr(p.status + kStatusBadClass, 1);
             const uint32_t have = __ballot_sync(0xffffffffu, c[0] >= 0 || c[1] >= 0);
             const uint32_t gm = (width == 32 ? 0xffffffffu : ((1u << width) - 1u) << (grp * width));
             const bool valid = (have & gm) != 0u;
@@ -1938,7 +1938,7 @@ __global__ void __launch_bounds__(256) loss_score_kernel(const __grid_constant__
         const int* cls = p.lab.target ? p.lab.target + row : p.lab.top_idx + row * p.lab.n_top;
         bool bad = false;
         for (int e = s; e < p.lab.n_top; e += 8) bad |= cls[e] >= p.lab.n;
-        if (bad) atomicOr(p.status, kDevBadClass);
+        if (bad) atomicOr(p.status + kStatusBadClass, 1);
     }
     float2 x[8];
     shared_row<kRun>(xs + r * (p.k + 1), p.k, s, x);

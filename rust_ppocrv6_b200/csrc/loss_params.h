@@ -13,9 +13,11 @@ constexpr int kLossMaxClasses = 1 << 17;  // labels are counted by 32 classes in
 constexpr int kLossRows = 32;             // rows per block of the score kernel
 constexpr int kLossTopSlots = 16;         // blocks of the row kernel per tile at most
 constexpr int kLossMaxSplits = 148;       // ranges that an own tile's work is split into at most
-// Device status bit (status[0], beside kDevTimeout and kDevRecPlan): a target or teacher class
-// at or above the class count; the row or entry was taken as absent.
-constexpr int kDevBadClass = 4;
+// Device status word (status[2], non-zero: set): a target or teacher class at or above the class count;
+// the row or entry was taken as absent. Apart from status[0] and [1], which every host call on the slot
+// reads: a bad label is its own call's, told by the next rh_sync.
+constexpr int kStatusBadClass = 2;
+constexpr int kStatusWords = 3;
 
 // What a row is held to: a target class, or a teacher's top logits. Exactly one of target and
 // top_idx is set.

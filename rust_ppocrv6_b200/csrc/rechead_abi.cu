@@ -290,19 +290,25 @@ int status_error(Slot& s, const int* st) {
         if (st[0] & rh::kDevTimeout)
             return fail(RH_ERR_TIMEOUT, "device wait timed out (site " + std::to_string(st[1]) +
                                             "); the kernel gave up and the context is still usable");
-        if (st[0] & rh::kDevBadClass)
-            return fail(RH_ERR_INVALID_ARG,
-                        "a target or teacher class is not below the class count; its row or entry was taken as absent");
         return fail(RH_ERR_CUDA, "device status " + std::to_string(st[0]));
     }
     return RH_OK;
 }
 
+// rh_sync's look at the status: what status_error reports, and the device forms' bad labels.
 int read_status(Slot& s) {
-    int st[2] = {0, 0};
+    int st[rh::kStatusWords] = {};
     RH_CUDA(cudaMemcpyAsync(st, s.d_status, sizeof(st), cudaMemcpyDeviceToHost, s.stream));
     RH_CUDA(cudaStreamSynchronize(s.stream));
-    return status_error(s, st);
+    if (st[rh::kStatusBadClass] != 0) {
+        RH_CUDA(cudaMemsetAsync(s.d_status + rh::kStatusBadClass, 0, sizeof(int), s.stream));
+        RH_CUDA(cudaStreamSynchronize(s.stream));
+    }
+    if (int rc = status_error(s, st)) return rc;
+    if (st[rh::kStatusBadClass] != 0)
+        return fail(RH_ERR_INVALID_ARG,
+                    "a target or teacher class is not below the class count; its row or entry was taken as absent");
+    return RH_OK;
 }
 
 // Waits for the work queued on the slot's stream and checks the device status, whose copy back
@@ -1364,9 +1370,9 @@ int rh_ctx_create(const int* devices, int n_devices, rh_ctx** out) {
         RH_CUDA(cudaStreamCreateWithFlags(&s->stream, cudaStreamNonBlocking));
         RH_CUDA(cudaStreamCreateWithFlags(&s->copy_stream, cudaStreamNonBlocking));
         RH_CUDA(cudaEventCreateWithFlags(&s->copied, cudaEventDisableTiming));
-        RH_CUDA(cudaMalloc(&s->d_status, 2 * sizeof(int)));
+        RH_CUDA(cudaMalloc(&s->d_status, rh::kStatusWords * sizeof(int)));
         RH_CUDA(cudaHostAlloc(reinterpret_cast<void**>(&s->h_status), 2 * sizeof(int), cudaHostAllocDefault));
-        RH_CUDA(cudaMemsetAsync(s->d_status, 0, 2 * sizeof(int), s->stream));
+        RH_CUDA(cudaMemsetAsync(s->d_status, 0, rh::kStatusWords * sizeof(int), s->stream));
         RH_CUDA(cudaStreamSynchronize(s->stream));
         ctx->slots.push_back(std::move(s));
     }

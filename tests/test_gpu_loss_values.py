@@ -198,6 +198,29 @@ def test_a_row_that_is_not_finite_keeps_to_itself(rh, ctx, what, exp):
     check(whole, ref, False, ("loss", "lse", "da"))
 
 
+def test_a_bad_class_on_the_device_fails_no_other_call(rh, ctx):
+    """It is the next sync's to report; calls on the same device go on."""
+    d = make(50, 24, 90, seed=24, ignored=0.0)
+    qw, _ = packed(rh, ctx, d, "int8")
+    want = rh.head_decode(d["x"], qw)
+    step = rh.head_cross_entropy_grad(d["x"], d["w"], d["t"], d["b"], ctx=ctx)
+    keep = {}
+    grad(rh, ctx, d, keep=keep)
+    keep["s"]["t"][7] = 90
+    for _ in range(2):
+        keep["call"](0)
+        torch.cuda.synchronize()
+        got = rh.head_decode(d["x"], qw)
+        assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+        again = rh.head_cross_entropy_grad(d["x"], d["w"], d["t"], d["b"], ctx=ctx)
+        assert all(np.array_equal(i, j) for i, j in zip(again, step))
+        with pytest.raises(rh.RecHeadError) as e:
+            ctx.sync()
+        assert e.value.code == rh.RH_ERR_INVALID_ARG and "class" in str(e.value)
+        ctx.sync()  # reported once
+    qw.free()
+
+
 @pytest.mark.parametrize("form", ["int8", "compact", "f32"])
 @pytest.mark.parametrize("rows", [1, 200])
 def test_score_with_every_class_masked(rh, ctx, form, rows):
