@@ -417,7 +417,12 @@ namespace {
 constexpr int kMainThreads = 896;
 constexpr int kLaunchRegs = 72;  // 65,536 registers / 896 threads
 constexpr int kCtrlRegs = 40, kSoftRegs = 72, kAddRegs = 88;
-static_assert(128 * kCtrlRegs + 512 * kSoftRegs + 256 * kAddRegs <= kMainThreads * kLaunchRegs, "register split");
+// What the producer and issuers give back has to cover what the adding warps take: their setmaxnreg
+// waits for it, without a limit. `launch`: registers a thread that a variant was built with, which the
+// softmax warps keep; loss_kernel_setup checks it for each.
+constexpr bool split_fits(int launch) { return 128 * (launch - kCtrlRegs) >= 256 * (kAddRegs - launch); }
+static_assert(kSoftRegs == kLaunchRegs && split_fits(kLaunchRegs) && !split_fits(kLaunchRegs - 8), "register split");
+static_assert(kMainThreads * kLaunchRegs <= 65536, "registers of an SM");
 
 template <bool F32>
 struct Ring {
@@ -1986,18 +1991,21 @@ cudaError_t smem_attr(K* k, int bytes) {
 }
 }  // namespace
 
-cudaError_t loss_kernel_setup() {
+cudaError_t loss_kernel_setup(int* wrong_registers) {
     cudaError_t e;
-    if ((e = smem_attr(loss_main_kernel<true, false, false>, kMSmemBytes)) != cudaSuccess) return e;
-    if ((e = smem_attr(loss_main_kernel<true, true, false>, kMSmemBytes)) != cudaSuccess) return e;
-    if ((e = smem_attr(loss_main_kernel<false, false, false>, kMSmemBytes)) != cudaSuccess) return e;
-    if ((e = smem_attr(loss_main_kernel<false, true, false>, kMSmemBytes)) != cudaSuccess) return e;
-    if ((e = smem_attr(loss_main_kernel<false, false, true>, kMSmemBytes)) != cudaSuccess) return e;
-    if ((e = smem_attr(loss_main_kernel<false, true, true>, kMSmemBytes)) != cudaSuccess) return e;
-    if ((e = smem_attr(loss_main_kernel<false, false, false, true>, kMSmemBytes)) != cudaSuccess) return e;
-    if ((e = smem_attr(loss_main_kernel<false, false, true, true>, kMSmemBytes)) != cudaSuccess) return e;
-    if ((e = smem_attr(loss_main_kernel<false, true, false, true>, kMSmemBytes)) != cudaSuccess) return e;
-    if ((e = smem_attr(loss_main_kernel<false, true, true, true>, kMSmemBytes)) != cudaSuccess) return e;
+    void (*const main_kernels[])(LossMainParams) = {
+        loss_main_kernel<true, false, false>,        loss_main_kernel<true, true, false>,
+        loss_main_kernel<false, false, false>,       loss_main_kernel<false, true, false>,
+        loss_main_kernel<false, false, true>,        loss_main_kernel<false, true, true>,
+        loss_main_kernel<false, false, false, true>, loss_main_kernel<false, true, false, true>,
+        loss_main_kernel<false, false, true, true>,  loss_main_kernel<false, true, true, true>};
+    *wrong_registers = 0;
+    for (auto k : main_kernels) {
+        cudaFuncAttributes a{};
+        if ((e = cudaFuncGetAttributes(&a, k)) != cudaSuccess) return e;
+        if (!split_fits(a.numRegs)) *wrong_registers = a.numRegs;
+        if ((e = smem_attr(k, kMSmemBytes)) != cudaSuccess) return e;
+    }
     if ((e = smem_attr(loss_pack_kernel<true>, kPackSmemMax)) != cudaSuccess) return e;
     if ((e = smem_attr(loss_pack_kernel<false>, kPackSmemMax)) != cudaSuccess) return e;
     if ((e = smem_attr(loss_rows_kernel<true, 32, 256>, kRowsSmemMax)) != cudaSuccess) return e;

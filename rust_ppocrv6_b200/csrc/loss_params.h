@@ -149,7 +149,9 @@ struct LossScoreParams {
     int* status;
 };
 
-cudaError_t loss_kernel_setup();
+// wrong_registers: 0, or the registers a thread of a main kernel whose register split would not be met
+// (it is then not to be launched).
+cudaError_t loss_kernel_setup(int* wrong_registers);
 cudaError_t launch_loss_pack(const LossPackParams& p, bool f32, cudaStream_t stream);
 cudaError_t launch_loss_main(const LossMainParams& p, bool f32, bool slots, bool weight_pass, int grid,
                              cudaStream_t stream);

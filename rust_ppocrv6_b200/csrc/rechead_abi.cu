@@ -74,6 +74,7 @@ struct Slot {
     cudaEvent_t part_done = nullptr;  // recorded after the last merge that reads `partial`
     std::mutex mu;
     int64_t launches = 0;
+    int loss_wrong_registers = 0;  // of loss_kernel_setup
     // Frees everything, also on a context whose creation failed part-way.
     ~Slot() {
         cudaSetDevice(device);
@@ -962,6 +963,10 @@ int enqueue_grad(rh_ctx* ctx, Slot& s, int dtype, const void* d_a, int64_t rows,
                  const void* d_w, int64_t n, const float* d_bias, const rh::LossLabels& lab, const float* d_row_grad,
                  float* d_loss, float* d_lse, void* d_da, void* d_dw, float* d_dbias, uint8_t* ws, const LossLayout& L,
                  cudaStream_t st) {
+    if (s.loss_wrong_registers)
+        return fail(RH_ERR_UNSUPPORTED, "a training step's kernel was built with " +
+                                            std::to_string(s.loss_wrong_registers) +
+                                            " registers a thread, too few for its register split");
     const bool f32 = dtype == RH_DTYPE_F32;
     const float logit_scale = (float)(1.4426950408889634 / (double)lab.temp);
     rh::LossPackParams pk{};
@@ -1366,7 +1371,7 @@ int rh_ctx_create(const int* devices, int n_devices, rh_ctx** out) {
         s->sms = prop.multiProcessorCount;
         RH_CUDA(cudaSetDevice(d));
         RH_CUDA(rh::head_kernel_setup());
-        RH_CUDA(rh::loss_kernel_setup());
+        RH_CUDA(rh::loss_kernel_setup(&s->loss_wrong_registers));
         RH_CUDA(cudaStreamCreateWithFlags(&s->stream, cudaStreamNonBlocking));
         RH_CUDA(cudaStreamCreateWithFlags(&s->copy_stream, cudaStreamNonBlocking));
         RH_CUDA(cudaEventCreateWithFlags(&s->copied, cudaEventDisableTiming));
