@@ -348,7 +348,8 @@ int rh_rec_preprocess_device(rh_ctx *ctx, int slot, const uint8_t *d_rgb, int64_
  * RH_ERR_INVALID_ARG.
  *
  * Device forms take a workspace of device memory (any alignment) of at least the bytes that
- * rh_head_score_workspace_bytes / rh_head_grad_workspace_bytes name; it holds nothing between
+ * rh_head_score_workspace_bytes / rh_head_grad_workspace_bytes name for its rows or any larger number
+ * (a workspace for the largest batch serves every smaller one); it holds nothing between
  * calls, and calls whose work may overlap need one each. They allocate nothing and can be captured
  * into a CUDA graph. They leave the caller's current device as it was. Results do not depend on
  * what else runs: sums are taken in a fixed order, without atomics.

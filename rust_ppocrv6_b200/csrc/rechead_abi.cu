@@ -870,7 +870,9 @@ struct LossLayout {
     size_t x_img, w_img, x_scale, w_scale, g_scale, class_e, row_tab, x_norm, w_bound, tile_top, tile_done, sp_off, sp_ent,
         sp_pos, part_o, part_ms, total;
 };
-LossLayout loss_layout(bool f32, int64_t rows, int64_t k, int64_t n, int64_t n_top, int sms) {
+// up_to: with room for every smaller number of rows as well. The plans of fewer rows may have more units
+// (a split has up to 4 sms of them), at most as many as `most` says, which grows with the rows.
+LossLayout loss_layout(bool f32, int64_t rows, int64_t k, int64_t n, int64_t n_top, int sms, bool up_to = false) {
     LossLayout L;
     L.x_tiles = (int)((rows + 127) / 128);
     L.w_tiles = (int)((n + 127) / 128);
@@ -886,7 +888,11 @@ LossLayout loss_layout(bool f32, int64_t rows, int64_t k, int64_t n, int64_t n_t
         return here;
     };
     const size_t img = (size_t)rh::kLossImage * (f32 ? 2 : 1);
-    const size_t units = (size_t)std::max(L.row.units, L.cls.units);
+    auto most = [&](int64_t own, int64_t str) {
+        return std::min(own * std::min<int64_t>(str, rh::kLossMaxSplits), own + 4 * (int64_t)sms);
+    };
+    const size_t units = up_to ? (size_t)std::max(most(L.x_tiles, L.w_tiles), most(L.w_tiles, L.x_tiles))
+                               : (size_t)std::max(L.row.units, L.cls.units);
     L.x_img = take((size_t)L.x_tiles * img);
     L.w_img = take((size_t)L.w_tiles * img);
     L.x_scale = take((size_t)L.x_tiles * 4);
@@ -1200,7 +1206,7 @@ int grad_host(rh_ctx* ctx, const float* a, int64_t rows, int64_t k, int64_t t_le
 // Scores of a packed head: the decode kernel's (argmax, probability) at temperature T, then the
 // labels' logits. Workspace: idx, prob, the split's partial rows and, for T != 1, a class table.
 struct ScoreLayout {
-    size_t idx, prob, table, partial, total;
+    size_t idx, prob, table, partial, partial_bytes, total;
 };
 ScoreLayout score_layout(const rh_weight* w, int64_t rows, int sms) {
     ScoreLayout L;
@@ -1216,7 +1222,9 @@ ScoreLayout score_layout(const rh_weight* w, int64_t rows, int sms) {
     L.idx = take((size_t)rows * 4);
     L.prob = take((size_t)rows * 4);
     L.table = take((size_t)w->g.n_chunks * rh::kCtabFloats * 4);
-    L.partial = take((size_t)splits * (size_t)split * sizeof(float4));
+    L.partial = at;
+    take((size_t)splits * (size_t)split * sizeof(float4));
+    L.partial_bytes = at - L.partial;
     L.total = at + 256;
     return L;
 }
@@ -2013,7 +2021,14 @@ int64_t rh_head_score_workspace_bytes(rh_ctx* ctx, const rh_weight* w, int slot,
         if (!w) return fail(RH_ERR_INVALID_ARG, "null weight");
         if (slot < 0 || slot >= (int)ctx->slots.size()) return fail(RH_ERR_INVALID_ARG, "slot out of range");
         if (int rc = check_rows(rows, 0)) return rc;
-        bytes = (int64_t)score_layout(w, rows, ctx->slots[slot]->sms).total;
+        // room for every smaller number of rows too: the split rows' partials of any rest of the row blocks
+        const int sms = ctx->slots[slot]->sms;
+        const ScoreLayout L = score_layout(w, rows, sms);
+        size_t partial = 0;
+        for (int64_t m = std::min(rows, (int64_t)(sms - 1) * rh::kBlockM); m > 0;
+             m = (m - 1) / rh::kBlockM * rh::kBlockM)
+            partial = std::max(partial, score_layout(w, m, sms).partial_bytes);
+        bytes = (int64_t)(L.total - L.partial_bytes + partial);
         return RH_OK;
     });
     return bytes;
@@ -2063,7 +2078,8 @@ int64_t rh_head_grad_workspace_bytes(rh_ctx* ctx, int slot, int dtype, int64_t r
         if (int rc = check_grad_shape(dtype, rows, k, n)) return rc;
         if (n_top < 0 || n_top > rh::kLossMaxTop)
             return fail(RH_ERR_INVALID_ARG, "n_top = " + std::to_string(n_top) + " is outside [0, 64]");
-        bytes = (int64_t)loss_layout(dtype == RH_DTYPE_F32, rows, k, n, std::max<int64_t>(n_top, 1), ctx->slots[slot]->sms)
+        bytes = (int64_t)loss_layout(dtype == RH_DTYPE_F32, rows, k, n, std::max<int64_t>(n_top, 1), ctx->slots[slot]->sms,
+                                     true)
                     .total;
         return RH_OK;
     });

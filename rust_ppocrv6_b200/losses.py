@@ -142,13 +142,13 @@ def _dtype(dtype: str) -> int:
 
 
 def head_loss_workspace_bytes(qw: QuantizedWeight, rows: int, slot: int = 0) -> int:
-    """Workspace of the score device forms."""
+    """Workspace of the score device forms for up to `rows` rows."""
     return _bytes(load().rh_head_score_workspace_bytes(qw._ctx.handle, qw.handle, slot, rows))
 
 
 def head_grad_workspace_bytes(ctx: Context, dtype: str, rows: int, k: int, n: int, n_top: int = 0,
                               slot: int = 0) -> int:
-    """Workspace of the grad device forms (n_top 0: cross entropy)."""
+    """Workspace of the grad device forms for up to `rows` rows (n_top 0: cross entropy)."""
     dt = _dtype(dtype)
     return _bytes(load().rh_head_grad_workspace_bytes(ctx.handle, slot, dt, rows, k, n, n_top))
 

@@ -250,6 +250,48 @@ def test_bf16_with_few_spare_slots(rh, ctx, k, t_len):
     check(grad(rh, ctx, d, "bf16", t_len=t_len), definition(d), True)
 
 
+def needs(call):
+    """The workspace bytes that a call asks for when it is refused for want of them."""
+    with pytest.raises(Exception) as e:
+        call()
+    return int(str(e.value).rsplit(" ", 1)[1])
+
+
+def grad_needs(rh, ctx, dtype, rows, k, n, n_top):
+    p = 256  # never read: refused before
+    head, out = (ctx, dtype, p, rows, k, p, n, p), (p, p, p, p, p, p, p, 0)
+    if n_top == 0:
+        return needs(lambda: rh.head_cross_entropy_grad_device(*head, p, *out))
+    return needs(lambda: rh.head_distill_grad_device(*head, p, p, n_top, 1.0, *out))
+
+
+def score_needs(rh, qw, rows, n_top):
+    p = 256
+    if n_top == 0:
+        return needs(lambda: rh.head_cross_entropy_device(qw, p, rows, p, p, p, p, 0))
+    return needs(lambda: rh.head_distill_device(qw, p, rows, p, p, n_top, 1.0, p, p, p, 0))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("k,n,n_top", [(120, 18710, 0), (80, 6906, 16), (128, 300, 3), (40, 131_072, 64)])
+def test_a_workspace_serves_every_smaller_batch(rh, ctx, k, n, n_top, dtype):
+    rows = [1, 100, 128, 129, 500, 2000, 4018, 9000, 18_943, 18_945, 25_000, 61_440, 100_000, 122_880, 128_896]
+    named = [rh.head_grad_workspace_bytes(ctx, dtype, r, k, n, n_top) for r in rows]
+    asked = [grad_needs(rh, ctx, dtype, r, k, n, n_top) for r in rows]
+    assert named == sorted(named) and all(a <= b for a, b in zip(asked, named))
+    assert all(max(asked[:i + 1]) <= named[i] for i in range(len(rows)))
+
+
+@pytest.mark.parametrize("form", ["int8", "f32"])
+def test_a_score_workspace_serves_every_smaller_batch(rh, ctx, form):
+    qw, _ = packed(rh, ctx, make(1, 40, 18710, seed=1), form)
+    rows = [1, 127, 128, 129, 500, 2000, 4018, 9000, 18_943, 18_945, 25_000, 61_440, 122_880, 128_896]
+    named = [rh.head_loss_workspace_bytes(qw, r) for r in rows]
+    asked = [score_needs(rh, qw, r, 0) for r in rows]
+    assert named == sorted(named) and all(max(asked[:i + 1]) <= named[i] for i in range(len(rows)))
+    qw.free()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("rows,k,n,n_top,t_len", [(1, 1, 1, 0, 0), (129, 121, 131, 0, 0), (3, 120, 18710, 5, 3),
                                                   (700, 120, 300, 0, 7), (127, 33, 257, 64, 0)])
@@ -270,7 +312,7 @@ def test_nothing_is_written_outside_the_buffers(rh, ctx, rows, k, n, n_top, t_le
         return buf[guard:guard + nbytes]
 
     out = {i: fenced(t.numel() * t.element_size()) for i, t in ref.items()}
-    ws = fenced(rh.head_grad_workspace_bytes(ctx, dtype, rows, k, n, n_top))
+    ws = fenced(grad_needs(rh, ctx, dtype, rows, k, n, n_top))
     head = (ctx, dtype, x.data_ptr(), rows, k, w.data_ptr(), n, b.data_ptr())
     tail = (g.data_ptr(), *[out[i].data_ptr() for i in ("loss", "lse", "da", "dw", "db")], ws.data_ptr(), ws.numel())
     torch.cuda.synchronize()
@@ -297,7 +339,7 @@ def test_score_writes_nothing_outside_its_buffers(rh, ctx, form, rows, n, n_top)
     d = make(rows, 120, n, seed=rows, n_top=n_top)
     qw, _ = packed(rh, ctx, d, form)
     x = cuda(d["x"])
-    need = rh.head_loss_workspace_bytes(qw, rows)
+    need = score_needs(rh, qw, rows, n_top)
     sizes, guard = (4 * rows, 4 * rows, need), 4096
     bufs = [torch.full((s + 2 * guard,), 0xA5, dtype=torch.uint8, device="cuda") for s in sizes]
     o = [b[guard:guard + s].data_ptr() for b, s in zip(bufs, sizes)]
