@@ -1868,7 +1868,8 @@ __device__ __forceinline__ void packed_row(const uint8_t* tiles, int c, int s, f
 }  // namespace
 
 // One block per 32 rows, 8 lanes per row: the logits of the row's labels and of its argmax as f32
-// products with the packed weight. lse = z[argmax] / T + log(sum of exponentials relative to it).
+// products with the packed weight. lse = z[argmax] / T + log(sum of exponentials relative to it); a loss
+// is formed from differences of logits.
 // Rows whose class range was split are joined here, from the decode kernel's partial (maximum, sum,
 // argmax) rows.
 template <int FORM>
@@ -1889,9 +1890,9 @@ __global__ void __launch_bounds__(256) loss_score_kernel(const __grid_constant__
     xv.put(p.k, p.t_len, xs);
     wait_previous();
     int best = 0;
-    float sum = 1.0f;
+    float sum = 1.0f, m = CUDART_NAN_F;  // m: the decode kernel's maximum, where it is known
     if (row >= p.split_row0 && live) {
-        float m = -CUDART_INF_F;
+        m = -CUDART_INF_F;
         sum = 0.0f;
         best = 0x7fffffff;
         // eight ranges' entries in flight at a time: their latency is what this join costs
@@ -1955,14 +1956,23 @@ __global__ void __launch_bounds__(256) loss_score_kernel(const __grid_constant__
         const float* t = p.ctab + (size_t)(c >> 7) * kCtabFloats + (c & 127);
         return fmaf(group_sum(z.x + z.y), __ldg(t), __ldg(t + kBlockN)) * p.lab.inv_temp;
     };
-    const float lse = logit(best) + logf(sum);
+    // lse - z[best] from the other classes' sum. That is relative to the tensor core's z[best], a sum that
+    // rounds toward zero and is some 2^-22 of itself short; where the row's maximum is at hand the sum is
+    // brought to the f32 logit (z in log2 units in two parts, so that the difference keeps its digits).
+    const float z_best = logit(best);
+    float rest = sum < 1.0f ? 0.0f : sum - 1.0f;
+    const float z_hi = z_best * 1.4426950408889634f;
+    const float z_lo = fmaf(z_best, 1.4426950408889634f, -z_hi);
+    const float off = (m - z_hi) - z_lo;
+    if (fabsf(off) < 1.0f) rest *= ex2_approx(off);
+    const float gap = log1pf(rest), lse = z_best + gap;
     float zq = 0.0f;
 #pragma unroll 2
     for (int e = 0; e < p.lab.n_top; ++e) {
         const int2 c = ent[e];
         const bool here = valid && c.x >= 0 && __int_as_float(c.y) != 0.0f;
         const float z = logit(here ? c.x : 0);
-        if (here) zq = fmaf(__int_as_float(c.y), z - lse, zq);
+        if (here) zq = fmaf(__int_as_float(c.y), (z - z_best) - gap, zq);
     }
     if (live && s == 0) {
         if (p.loss) p.loss[row] = valid ? (entropy - zq) * p.lab.temp * p.lab.temp : 0.0f;
