@@ -81,6 +81,9 @@ template <class T>
 __device__ __forceinline__ T chain_load(const T* p) {
     return __ldcg(p);
 }
+__device__ __forceinline__ float2 as_pair(uint32_t a, uint32_t b) {
+    return make_float2(__uint_as_float(a), __uint_as_float(b));
+}
 // Whether class c is one of a row's labels at all.
 __device__ __forceinline__ bool is_class(int c, int n) { return c >= 0 && c < n; }
 
@@ -407,8 +410,7 @@ namespace {
 // Softmax and adding are apart so that a softmax warpgroup goes on to its next tile without waiting
 // for the tensor core to use its last. Two issuers, because the tensor core queues only a few
 // instructions: while one waits on its barriers the other's products run (with one issuer, its waits
-// and the products added up: f32 took 3,870 cycles a tile without any softmax work, of which 48
-// instructions of 64 cycles were products).
+// and the products add up).
 // Scores live in buffers of 128 TMEM columns: two in f32, whose own operand (hi | lo) takes 128
 // columns; three in bf16, whose own operand stays in shared memory, so that the next scores are there
 // when a softmax warpgroup comes for them. (An operand in TMEM costs the tensor core less
@@ -446,7 +448,8 @@ constexpr uint32_t kPatchRow = 12;                 // floats per class row of a 
 constexpr uint32_t kMOffPatch = kMOffUnion;        // weight pass: [16 warps][32][kPatchRow] f32
 constexpr uint32_t kMSmemUsed = kMOffPatch + 16 * 32 * kPatchRow * 4;
 constexpr uint32_t kMSmemBytes = kMSmemUsed + 1024;
-static_assert(Ring<true>::kEnd <= kMOffBars && Ring<false>::kEnd <= kMOffBars && Ring<false>::kOwn % 1024 == 0, "shared memory map");
+static_assert(Ring<true>::kEnd <= kMOffBars && Ring<false>::kEnd <= kMOffBars && Ring<false>::kOwn % 1024 == 0,
+              "shared memory map");
 static_assert(kMSmemBytes <= 227 * 1024, "shared memory per CTA");
 static_assert(kMOffNamed + 16 * 64 * 4 <= kMSmemUsed, "row pass within the union");
 
@@ -480,8 +483,8 @@ struct Waiter {
 
 // Bounded wait: gives up when another role has, or after the time limit (device status set);
 // every role then leaves its loop and the kernel ends normally.
-__device__ __forceinline__ bool loss_wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, int* status,
-                                            unsigned long long timeout_ns, int where) {
+__device__ __forceinline__ bool loss_wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag,
+                                               int* status, unsigned long long timeout_ns, int where) {
     const uint64_t t0 = globaltimer_ns();
     while (true) {
         if (mbar_try_wait_sleep(bar, parity, kLSleepNs)) return true;
@@ -648,8 +651,8 @@ constexpr int kAddEvery = 32;
 // more rows or classes mostly by 1.3 times, with two parts by that rounding alone. (A class that few
 // rows name has few large terms in a long step too, and keeps the one rounding there: 2^-9 of each
 // term, as of any gradient that enters a bf16 product.)
-// Above it one rounding does. A variant of its own (TWO): a test inside the kernel alone cost steps of
-// 61,440 and 122,880 rows 4-8 % (122,880 rows: 2,324 against 2,242 us).
+// Above it one rounding does: of 122,880 rows, gradients lie as near float64 as f32 arithmetic's rounded
+// once (1.8e-3 both). A variant of its own (TWO): a test inside the kernel alone slowed long steps down.
 constexpr int kTwoPartTiles = 8;
 
 // Units (own tile, range of streamed tiles), persistent over the grid. Per streamed tile: scores
@@ -761,8 +764,8 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                     if (!ok) break;
                     if (elect_one()) {
                         mbar_arrive_expect_tx(bar(kLBarAFull + w), kLossImage);
-                        bulk_copy_g2s(base + Ring<F32>::kOwn + w * kLossImage, p.own + (size_t)U.own * kLossImage, kLossImage,
-                                      bar(kLBarAFull + w));
+                        bulk_copy_g2s(base + Ring<F32>::kOwn + w * kLossImage, p.own + (size_t)U.own * kLossImage,
+                                      kLossImage, bar(kLBarAFull + w));
                     }
                     __syncwarp();
                     owns = uc + 1;
@@ -774,8 +777,8 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                     if (elect_one()) {
                         mbar_arrive_expect_tx(bar(kLBarFull + s), kStage + kTabBytes);
                         bulk_copy_g2s(base + s * kStage, p.str + (size_t)c * kStage, kStage, bar(kLBarFull + s));
-                        bulk_copy_g2s(base + Ring<F32>::kTab + s * 1024u, p.col_tab + (size_t)c * (kTabBytes / 4), kTabBytes,
-                                      bar(kLBarFull + s));
+                        bulk_copy_g2s(base + Ring<F32>::kTab + s * 1024u, p.col_tab + (size_t)c * (kTabBytes / 4),
+                                      kTabBytes, bar(kLBarFull + s));
                     }
                     __syncwarp();
                     issued = cc + 1;
@@ -974,8 +977,8 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                         bits[2 * lane] = bits[2 * lane + 1] = 0u;
                         const uint32_t all0 = __reduce_or_sync(0xffffffffu, bits0);
                         const uint32_t all1 = __reduce_or_sync(0xffffffffu, bits1);
-                        chunks = ((all0 & 0xffffu) ? 1u : 0u) | ((all0 >> 16) ? 2u : 0u) | ((all1 & 0xffffu) ? 4u : 0u) |
-                                 ((all1 >> 16) ? 8u : 0u);
+                        chunks = ((all0 & 0xffffu) ? 1u : 0u) | ((all0 >> 16) ? 2u : 0u) |
+                                 ((all1 & 0xffffu) ? 4u : 0u) | ((all1 >> 16) ? 8u : 0u);
                     }
                 }
                 // (a chunk of 16 columns in which no row of the warp names one passes by)
@@ -1001,8 +1004,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                         float2 pr[8];
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
-                            const float2 a = __ffma2_rn(make_float2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])),
-                                                        mul, sub2);
+                            const float2 a = __ffma2_rn(as_pair(x[2 * j], x[2 * j + 1]), mul, sub2);
                             pr[j] = make_float2(ex2_approx(a.x), ex2_approx(a.y));
                             ts = __fadd2_rn(ts, pr[j]);
                         }
@@ -1020,10 +1022,8 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
 #pragma unroll
                         for (int j = 0; j < 16; j += 4) {
                             const float4 e = SLOTS ? make_float4(0.f, 0.f, 0.f, 0.f) : lds128(tab + 4u * (16 * q + j));
-                            const float2 a = __ffma2_rn(make_float2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), mul,
-                                                        make_float2(e.x, e.y));
-                            const float2 b = __ffma2_rn(make_float2(__uint_as_float(x[j + 2]), __uint_as_float(x[j + 3])),
-                                                        mul, make_float2(e.z, e.w));
+                            const float2 a = __ffma2_rn(as_pair(x[j], x[j + 1]), mul, make_float2(e.x, e.y));
+                            const float2 b = __ffma2_rn(as_pair(x[j + 2], x[j + 3]), mul, make_float2(e.z, e.w));
                             top = max3f(top, a.x, a.y);
                             top = max3f(top, b.x, b.y);
                         }
@@ -1055,10 +1055,8 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
 #pragma unroll
                         for (int j = 0; j < 16; j += 4) {
                             const float4 e = SLOTS ? make_float4(0.f, 0.f, 0.f, 0.f) : lds128(tab + 4u * (16 * q + j));
-                            float2 a = __ffma2_rn(make_float2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), mul,
-                                                  make_float2(e.x, e.y));
-                            float2 b = __ffma2_rn(make_float2(__uint_as_float(x[j + 2]), __uint_as_float(x[j + 3])), mul,
-                                                  make_float2(e.z, e.w));
+                            float2 a = __ffma2_rn(as_pair(x[j], x[j + 1]), mul, make_float2(e.x, e.y));
+                            float2 b = __ffma2_rn(as_pair(x[j + 2], x[j + 3]), mul, make_float2(e.z, e.w));
                             a = __fadd2_rn(a, sub2);
                             b = __fadd2_rn(b, sub2);
                             pr[j / 2] = make_float2(ex2_approx(a.x), ex2_approx(a.y));
@@ -1071,7 +1069,8 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                     sum = fmaf(sum, corr, t);
                 } else {
                     const float2 le = make_float2(lane_e, lane_e);
-                    const float gs_up = __uint_as_float(0x7f000000u - __float_as_uint(gs));  // f32: 1 / gs, a power of two
+                    // f32: 1 / gs, as gs is a power of two
+                    const float gs_up = __uint_as_float(0x7f000000u - __float_as_uint(gs));
                     bool labelled = false;  // most tiles have none of a warp's classes
                     if (lw.next < lw.end) {
                         window_use(lw, ent, lane, (int)half);
@@ -1087,10 +1086,8 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
 #pragma unroll
                         for (int j = 0; j < 16; j += 4) {
                             const float4 e = lds128(tab + 4u * (16 * q + j));
-                            float2 a = __ffma2_rn(make_float2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), mul,
-                                                  make_float2(e.x, e.y));
-                            float2 b = __ffma2_rn(make_float2(__uint_as_float(x[j + 2]), __uint_as_float(x[j + 3])), mul,
-                                                  make_float2(e.z, e.w));
+                            float2 a = __ffma2_rn(as_pair(x[j], x[j + 1]), mul, make_float2(e.x, e.y));
+                            float2 b = __ffma2_rn(as_pair(x[j + 2], x[j + 3]), mul, make_float2(e.z, e.w));
                             if (!SLOTS) {
                                 a = __fadd2_rn(a, le);
                                 b = __fadd2_rn(b, le);
@@ -1114,8 +1111,8 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                                     any = true;
                                     if (lw.group == group)
                                         *reinterpret_cast<volatile float*>(
-                                            gbase + (patch - base) +
-                                            4u * ((uint32_t)(lw.e.x & 31) * kPatchRow + (uint32_t)((lw.e.x >> 5) & 7))) =
+                                            gbase + (patch - base) + 4u * (uint32_t)(lw.e.x & 31) * kPatchRow +
+                                            4u * (uint32_t)((lw.e.x >> 5) & 7)) =
                                             F32 ? __int_as_float(lw.e.y) * gs_up : __int_as_float(lw.e.y);
                                 }
                                 if (group < lw.last) break;  // the window reaches beyond this group, or is the last
@@ -1169,7 +1166,8 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
             if (ringed) rc += n;
             ok = loss_wait(bar(kLBarMsEmpty), (uc & 1u) ^ 1u, wt, 110);
             if (!ok) break;
-            reinterpret_cast<float2*>(gbase + kMOffMs)[wg * 128 + r] = WPASS ? make_float2(sum, carry) : make_float2(off, sum);
+            reinterpret_cast<float2*>(gbase + kMOffMs)[wg * 128 + r] =
+                WPASS ? make_float2(sum, carry) : make_float2(off, sum);
             mbar_arrive(bar(kLBarMsFull));
         }
     } else {
@@ -1223,8 +1221,7 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                             }
 #pragma unroll
                             for (int j = 0; j < 8; ++j)
-                                acc[8 * q + j] = __ffma2_rn(make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])),
-                                                            om2, acc[8 * q + j]);
+                                acc[8 * q + j] = __ffma2_rn(as_pair(v[2 * j], v[2 * j + 1]), om2, acc[8 * q + j]);
                         }
                     }
                     tc_fence_before();
@@ -1406,7 +1403,8 @@ struct RowLoad {
     }
 };
 template <int R, int NT, class T>
-__device__ __forceinline__ void store_rows(T* x, long long row0, long long rows, int k, long long t_len, const float* xs) {
+__device__ __forceinline__ void store_rows(T* x, long long row0, long long rows, int k, long long t_len,
+                                           const float* xs) {
     if (t_len > 0) {
         const int r = threadIdx.x % R;
         if (row0 + r >= rows) return;
@@ -1426,7 +1424,8 @@ __device__ __forceinline__ void store_rows(T* x, long long row0, long long rows,
 // A row's labels in a group of 8 lanes: their shares q into shared memory as (class or -1, q), and
 // sum_i q_i log q_i; a share may round to zero. False when the row has none (it is then ignored), or
 // none is asked for.
-__device__ __forceinline__ bool group_labels(const LossLabels& L, long long row, bool live, int s, int2* ent, float& entropy) {
+__device__ __forceinline__ bool group_labels(const LossLabels& L, long long row, bool live, int s, int2* ent,
+                                             float& entropy) {
     entropy = 0.0f;
     if (L.target) {
         const int t = live ? L.target[row] : -1;
@@ -1526,7 +1525,8 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 3 : 1) loss_rows_kernel(const 
     const long long row0 = (long long)blockIdx.x * R;
     const int mb = (int)(row0 >> 7), l0 = (int)(row0 & 127);
     const int ns = mb < p.whole_units ? 1 : p.n_splits;
-    const size_t u0 = mb < p.whole_units ? (size_t)mb : (size_t)p.whole_units + (size_t)(mb - p.whole_units) * p.n_splits;
+    const size_t u0 = mb < p.whole_units ? (size_t)mb
+                                         : (size_t)p.whole_units + (size_t)(mb - p.whole_units) * p.n_splits;
 
     RowLoad<R, NT, T> xv;
     xv.fetch(static_cast<const T*>(p.x), row0, p.rows, p.k, p.t_len);
@@ -1806,7 +1806,8 @@ __global__ void __launch_bounds__(256) loss_reduce_kernel(const __grid_constant_
     wait_previous();
     const int j0 = (int)blockIdx.x * R, tile = j0 >> 7, l0 = j0 & 127;
     const int ns = tile < p.whole_units ? 1 : p.n_splits;
-    const size_t u0 = tile < p.whole_units ? (size_t)tile : (size_t)p.whole_units + (size_t)(tile - p.whole_units) * p.n_splits;
+    const size_t u0 = tile < p.whole_units ? (size_t)tile
+                                           : (size_t)p.whole_units + (size_t)(tile - p.whole_units) * p.n_splits;
     join_units<R, 256, false>(p.part_o, u0, ns, p.feat, l0, nullptr, sm);
     if (p.db && threadIdx.x < R && j0 + (int)threadIdx.x < p.n) {
         float a = 0.0f;
@@ -1818,7 +1819,8 @@ __global__ void __launch_bounds__(256) loss_reduce_kernel(const __grid_constant_
 #pragma unroll
     for (int r = threadIdx.x >> 5; r < R; r += 8) {
         if (j0 + r < p.n) {
-            for (int kk = threadIdx.x & 31; kk < p.k; kk += 32) dw[(long long)(j0 + r) * p.k + kk] = (T)sm[r * (p.feat + 1) + kk];
+            for (int kk = threadIdx.x & 31; kk < p.k; kk += 32)
+                dw[(long long)(j0 + r) * p.k + kk] = (T)sm[r * (p.feat + 1) + kk];
         }
     }
 }
@@ -1839,7 +1841,8 @@ template <int FORM>
 __device__ __forceinline__ void packed_row(const uint8_t* tiles, int c, int s, float2 (&v)[8]) {
     const int tile = c >> 7, r = c & 127;
     if constexpr (FORM == 1) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(tiles + (size_t)tile * kTile8Bytes + image8_offset(r, 16 * s)));
+        const uint8_t* a = tiles + (size_t)tile * kTile8Bytes + image8_offset(r, 16 * s);
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(a));
         const uint32_t x[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -1883,7 +1886,9 @@ __global__ void __launch_bounds__(256) loss_score_kernel(const __grid_constant__
     const bool live = row < p.rows;
     RowLoad<kLossRows, 256, float> xv;
     xv.fetch(p.x, row0, p.rows, p.k, p.t_len);
-    // the caller's features and labels are there already; only what the decode kernel writes is waited for
+    // The caller's features and labels are there already; only what the decode kernel writes is waited for.
+    // (That kernel has no trigger, so this one starts as its last blocks end: the reads above run beside
+    // their end and the flush after it, no earlier.)
     int2* ent = ents + r * p.lab.n_top;
     float entropy;
     const bool valid = group_labels(p.lab, row, live, s, ent, entropy);
@@ -1927,7 +1932,8 @@ __global__ void __launch_bounds__(256) loss_score_kernel(const __grid_constant__
             const int ob = __shfl_xor_sync(group, best, o);
             const float M = fmaxf(m, om);
             if (M != -CUDART_INF_F) {
-                sum = (m == -CUDART_INF_F ? 0.0f : sum * ex2_approx(m - M)) + (om == -CUDART_INF_F ? 0.0f : os * ex2_approx(om - M));
+                sum = (m == -CUDART_INF_F ? 0.0f : sum * ex2_approx(m - M)) +
+                      (om == -CUDART_INF_F ? 0.0f : os * ex2_approx(om - M));
                 best = m == om ? min(best, ob) : m > om ? best : ob;
             } else {
                 sum += os;
@@ -2101,7 +2107,9 @@ cudaError_t launch_loss_table(const float* ctab, long long n_floats, float inv_t
 
 cudaError_t launch_loss_score(const LossScoreParams& p, cudaStream_t stream) {
     const int grid = (int)((p.rows + kLossRows - 1) / kLossRows);
-    void (*k)(LossScoreParams) = p.form == 0 ? loss_score_kernel<0> : p.form == 1 ? loss_score_kernel<1> : loss_score_kernel<2>;
+    void (*k)(LossScoreParams) = p.form == 0   ? loss_score_kernel<0>
+                                 : p.form == 1 ? loss_score_kernel<1>
+                                               : loss_score_kernel<2>;
     return launch_chained(k, grid, 256, score_smem_bytes(p.k, p.lab.n_top), stream, p);
 }
 

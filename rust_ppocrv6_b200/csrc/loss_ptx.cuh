@@ -59,7 +59,8 @@ __device__ __forceinline__ void tmem_st32x32b_x16(uint32_t taddr, const uint32_t
 // image 32 KB further); A in TMEM, 8 columns a step, the low part 64 columns further. One elect.sync
 // and immediate offsets: the tensor core queues only a few instructions, so what the issuing warp
 // spends between them is time it stands still.
-__device__ __forceinline__ void mma_scores_f32_warp(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, int steps) {
+__device__ __forceinline__ void mma_scores_f32_warp(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                                    int steps) {
     asm volatile(
         "{\n\t.reg .pred e, pf, pt, q1, q2, q3, q4, q5, q6, q7;\n\t.reg .b64 b<8>, c<8>;\n\t"
         "elect.sync _|e, 0xffffffff;\n\t"
@@ -116,7 +117,8 @@ __device__ __forceinline__ void mma_scores_f32_warp(uint32_t d_tmem, uint32_t a_
 }
 
 // Scores of a tile, bf16: up to 8 K steps, A in shared memory, an image like B's.
-__device__ __forceinline__ void mma_scores_bf16_warp(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, int steps) {
+__device__ __forceinline__ void mma_scores_bf16_warp(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                                     int steps) {
     asm volatile(
         "{\n\t.reg .pred e, pf, pt, q1, q2, q3, q4, q5, q6, q7;\n\t.reg .b64 a<8>, b<8>;\n\t"
         "elect.sync _|e, 0xffffffff;\n\t"

@@ -867,8 +867,8 @@ struct LossLayout {
     LossPlan row, cls;
     int x_tiles = 0, w_tiles = 0, feat = 0;
     bool slots = false;  // the bias rides in three spare K slots
-    size_t x_img, w_img, x_scale, w_scale, g_scale, class_e, row_tab, x_norm, w_bound, tile_top, tile_done, sp_off, sp_ent,
-        sp_pos, part_o, part_ms, total;
+    size_t x_img, w_img, x_scale, w_scale, g_scale, class_e, row_tab, x_norm, w_bound, tile_top, tile_done, sp_off,
+        sp_ent, sp_pos, part_o, part_ms, total;
 };
 // up_to: with room for every smaller number of rows as well. The plans of fewer rows may have more units
 // (a split has up to 4 sms of them), at most as many as `most` says, which grows with the rows.
@@ -1233,8 +1233,8 @@ int enqueue_score(rh_ctx* ctx, const rh_weight* w, Slot& s, const rh_weight::Per
                   int64_t t_len, const rh::LossLabels& lab, float* d_loss, float* d_lse, uint8_t* ws,
                   const ScoreLayout& L, cudaStream_t st) {
     int grid;
-    rh::HeadParams p = head_params(ctx, w, s, pw, d_a, rows, t_len, (int32_t*)(ws + L.idx), (float*)(ws + L.prob), nullptr,
-                                   grid);
+    rh::HeadParams p = head_params(ctx, w, s, pw, d_a, rows, t_len, (int32_t*)(ws + L.idx), (float*)(ws + L.prob),
+                                   nullptr, grid);
     p.partial = (float4*)(ws + L.partial);
     if (lab.temp != 1.0f) {
         RH_CUDA(rh::launch_loss_table(pw.ctab, (long long)w->g.n_chunks * rh::kCtabFloats, lab.inv_temp,
@@ -2064,8 +2064,8 @@ int rh_head_distill_device(rh_ctx* ctx, const rh_weight* w, int slot, const floa
                            const int32_t* d_top_idx, const float* d_top_logits, int64_t n_top, float temperature,
                            float* d_loss, float* d_lse, void* d_workspace, int64_t workspace_bytes, void* stream) {
     return guarded([&]() -> int {
-        return score_device(ctx, w, slot, d_a, rows, t_len, nullptr, d_top_idx, d_top_logits, n_top, temperature, d_loss,
-                            d_lse, d_workspace, workspace_bytes, stream);
+        return score_device(ctx, w, slot, d_a, rows, t_len, nullptr, d_top_idx, d_top_logits, n_top, temperature,
+                            d_loss, d_lse, d_workspace, workspace_bytes, stream);
     });
 }
 
@@ -2078,8 +2078,8 @@ int64_t rh_head_grad_workspace_bytes(rh_ctx* ctx, int slot, int dtype, int64_t r
         if (int rc = check_grad_shape(dtype, rows, k, n)) return rc;
         if (n_top < 0 || n_top > rh::kLossMaxTop)
             return fail(RH_ERR_INVALID_ARG, "n_top = " + std::to_string(n_top) + " is outside [0, 64]");
-        bytes = (int64_t)loss_layout(dtype == RH_DTYPE_F32, rows, k, n, std::max<int64_t>(n_top, 1), ctx->slots[slot]->sms,
-                                     true)
+        bytes = (int64_t)loss_layout(dtype == RH_DTYPE_F32, rows, k, n, std::max<int64_t>(n_top, 1),
+                                     ctx->slots[slot]->sms, true)
                     .total;
         return RH_OK;
     });
@@ -2124,9 +2124,9 @@ int rh_head_distill_grad_device(rh_ctx* ctx, int slot, int dtype, const void* d_
                                 const float* d_row_grad, float* d_loss, float* d_lse, void* d_da, void* d_dw,
                                 float* d_dbias, void* d_workspace, int64_t workspace_bytes, void* stream) {
     return guarded([&]() -> int {
-        return grad_device(ctx, slot, dtype, d_a, rows, k, t_len, d_w, n, d_bias, nullptr, d_top_idx, d_top_logits, n_top,
-                           temperature, d_row_grad, d_loss, d_lse, d_da, d_dw, d_dbias, d_workspace, workspace_bytes,
-                           stream);
+        return grad_device(ctx, slot, dtype, d_a, rows, k, t_len, d_w, n, d_bias, nullptr, d_top_idx, d_top_logits,
+                           n_top, temperature, d_row_grad, d_loss, d_lse, d_da, d_dw, d_dbias, d_workspace,
+                           workspace_bytes, stream);
     });
 }
 

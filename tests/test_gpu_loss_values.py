@@ -246,7 +246,7 @@ def test_score_losses_are_as_near_as_f32_arithmetic(rh, ctx, form):
 
 
 @pytest.mark.parametrize("form", ["int8", "compact", "f32"])
-@pytest.mark.parametrize("rows", [1, 200])
+@pytest.mark.parametrize("rows", [1, 200, 19_000])  # the last with rows whose classes one unit has
 def test_score_with_every_class_masked(rh, ctx, form, rows):
     d = make(rows, 40, 300, seed=14, ignored=0.0)
     d["b"][:] = -np.inf
