@@ -951,15 +951,8 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                 // (not below the least normal: a named column's -inf must stay one)
                 const float mul1 = fmaxf(own_mul * str_s, 1.17549435e-38f);
                 const float2 mul = make_float2(mul1, mul1);
-                const uint32_t buf = (cc + i) % Ring<F32>::kBufs;
-                const uint32_t t_s = t_bufs + 128u * buf;
-                ok = loss_wait(bar(kLBarSFull + (int)buf), ((cc + i) / Ring<F32>::kBufs) & 1u, wt, 107);
-                // the column table came with the tile: its barrier has passed, but this warp has to
-                // observe it before it reads what the copy wrote
-                ok = ok && loss_wait(bar(kLBarFull + s), ((cc + i) / kStages) & 1u, wt, 108);
-                if (!ok) break;
-                tc_fence_after();
-                // the named columns of the warp's rows, a row a lane: their scores become -inf
+                // the named columns of the warp's rows, a row a lane: their scores become -inf.
+                // Gathered while the scores are on their way.
                 uint32_t bits0 = 0, bits1 = 0, chunks = 0;
                 if (!WPASS && nr.next < nr.end) {
                     bool hit = false;
@@ -981,6 +974,14 @@ __global__ void __launch_bounds__(kMainThreads, 1) loss_main_kernel(const __grid
                                  ((all1 & 0xffffu) ? 4u : 0u) | ((all1 >> 16) ? 8u : 0u);
                     }
                 }
+                const uint32_t buf = (cc + i) % Ring<F32>::kBufs;
+                const uint32_t t_s = t_bufs + 128u * buf;
+                ok = loss_wait(bar(kLBarSFull + (int)buf), ((cc + i) / Ring<F32>::kBufs) & 1u, wt, 107);
+                // the column table came with the tile: its barrier has passed, but this warp has to
+                // observe it before it reads what the copy wrote
+                ok = ok && loss_wait(bar(kLBarFull + s), ((cc + i) / kStages) & 1u, wt, 108);
+                if (!ok) break;
+                tc_fence_after();
                 // (a chunk of 16 columns in which no row of the warp names one passes by)
                 auto drop_named = [&](uint32_t (&x)[16], int q) {
                     if ((chunks >> q) & 1u) {
